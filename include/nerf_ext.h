@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-enum { NERF_EXT_F32 = 0, NERF_EXT_F16 = 1 };
+enum { NERF_EXT_F32 = 0, NERF_EXT_F16 = 1, NERF_EXT_BF16 = 2 /* linear layers and the optimiser only */ };
 enum { NERF_EXT_H2D = 1, NERF_EXT_D2H = 2, NERF_EXT_D2D = 3 };
 enum { NERF_EXT_DENSITY_PARAMS = 3072, NERF_EXT_COLOR_PARAMS = 7168 };
 /* Parameter counts of the reference's own network (reference-model mode):
@@ -195,6 +195,95 @@ NERF_API NerfStatus nerf_ext_ref_composite_backward(const uint32_t* counts, cons
  * features fp16 [n][32], unit directions [n][3] -> out [n][4] = (sigma, r, g, b).
  * The fused fp16-MFMA MLP pass on its own (no table gathers). */
 NERF_API NerfStatus nerf_ext_field_mlp(const uint16_t* density_params, const uint16_t* color_params, const uint16_t* features, const float* directions, uint32_t n, float* out, void* stream);
+
+/* ------------------------------------- linear layers, gradients, optimiser */
+/* Operators for a host's own network next to the hash grid and the frequency
+ * encoding (no counterpart in the reference, whose layers are fixed at compile
+ * time, backend-cuda.cu:23-54).  Rows are samples.  All arrays are on the
+ * device; nothing is allocated and nothing synchronises, so the calls may be
+ * recorded into a graph.  Arrays need only be aligned to their elements and
+ * strides may be odd; arrays aligned to 16 bytes with strides and widths that
+ * are multiples of 8 are the fast ones.
+ *
+ * workspace: device memory aligned to 16 bytes that no other call uses at the
+ * same time.  A linear layer's calls split a long sum over workgroups as far
+ * as it holds the parts (NERF_EXT_LINEAR_WORKSPACE is enough for every split
+ * they take) and need none to be right: NULL and 0 serve, slower.  Results
+ * are the same every time for the same arguments and workspace size. */
+enum { NERF_EXT_ACT_NONE = 0, NERF_EXT_ACT_RELU = 1, NERF_EXT_ACT_SOFTPLUS = 2, NERF_EXT_ACT_SIGMOID = 3, NERF_EXT_ACT_SILU = 4, NERF_EXT_ACT_GELU = 5 /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */ };
+enum { NERF_EXT_LINEAR_WORKSPACE = 64 << 20, NERF_EXT_NORM_WORKSPACE = 64 << 10 };
+
+typedef struct NerfExtLinearDesc {
+    uint32_t rows;            /* at most 2^30; 0: gradients of weight and bias are 0 */
+    uint32_t in_features;     /* 1..65536 */
+    uint32_t out_features;    /* 1..65536 */
+    uint32_t dtype;           /* NERF_EXT_F16 or NERF_EXT_BF16: every 16-bit array */
+    uint32_t out_dtype;       /* of y: dtype or NERF_EXT_F32 */
+    uint32_t activation;      /* NERF_EXT_ACT_*; forward: on this layer's output;
+                                 backward: the one that made this layer's input */
+    uint32_t x_stride;        /* elements between rows of x, add and dx; 0: in_features */
+    uint32_t y_stride;        /* of y and delta; 0: out_features */
+    uint32_t residual_stride; /* of residual; 0: out_features */
+    uint32_t reserved;        /* 0 */
+} NerfExtLinearDesc;
+
+/* z = x weight^T + bias, y = act(z) + residual: x [rows][in], weight
+ * [out][in] (dense), bias fp32 [out] or NULL, residual [rows][out] of dtype or
+ * NULL, y [rows][out] of out_dtype; pre (dense [rows][out] of dtype, or NULL)
+ * gets z, which the backward pass of the next layer reads.  y may be residual
+ * itself; no other two arrays may overlap.  Sums in 32 bits, one rounding of
+ * each output. */
+NERF_API NerfStatus nerf_ext_linear_forward(const NerfExtLinearDesc* desc, const void* x, const void* weight, const float* bias, const void* residual, void* y, void* pre, void* workspace, uint64_t workspace_bytes, void* stream);
+/* Gradients of the layer from delta [rows][out] = d loss / d z:
+ *   g = delta weight + add     add [rows][in] or NULL: what reaches x on other ways,
+ *                              such as a residual around the layer
+ *   dx = g                     [rows][in] or NULL
+ *   dpre = g act'(pre)         dense [rows][in] or NULL, with pre [rows][in] (dense) the
+ *                              z that made x = act(z) (+ residual): the delta of the layer
+ *                              before, so each derivative is taken where its
+ *                              gradient is made
+ *   dweight = delta^T x        fp32 [out][in] or NULL, overwritten
+ *   dbias = sum over rows of delta   fp32 [out] or NULL; with dweight only
+ * The relu's derivative at 0 is 0.  dx may be add itself, dpre may be pre
+ * itself; no other two arrays may overlap.  What an output does not need may be
+ * NULL (weight, x, pre). */
+NERF_API NerfStatus nerf_ext_linear_backward(const NerfExtLinearDesc* desc, const void* x, const void* weight, const void* delta, const void* pre, const void* add, void* dx, void* dpre, float* dweight, float* dbias, void* workspace,
+                                            uint64_t workspace_bytes, void* stream);
+
+typedef struct NerfExtGradTensor {
+    const void* grad; /* device, count elements of dtype */
+    void* out;        /* nerf_ext_grad_clip: the clipped gradient, of dtype; may be grad */
+    uint64_t count;   /* at most 2^36; 0: nothing is read or written */
+    uint32_t dtype;   /* NERF_EXT_F32, _F16 or _BF16 */
+    uint32_t reserved; /* 0 */
+} NerfExtGradTensor;
+
+typedef struct NerfExtAdamTensor {
+    float* param;      /* fp32 master weights */
+    const float* grad; /* times loss_scale */
+    float* m;
+    float* v;
+    void* copy;        /* working copy in copy_dtype, or NULL */
+    uint64_t count;
+    uint32_t copy_dtype; /* NERF_EXT_F16 or NERF_EXT_BF16 */
+    uint32_t reserved;   /* 0 */
+} NerfExtAdamTensor;
+
+/* The lists are host arrays and are read during the call.  workspace:
+ * NERF_EXT_NORM_WORKSPACE bytes at least.  norm (device) = the Euclidean norm
+ * of all tensors' elements together, squares summed in 64 bits. */
+NERF_API NerfStatus nerf_ext_grad_norm(const NerfExtGradTensor* tensors, uint32_t count, float* norm, void* workspace, uint64_t workspace_bytes, void* stream);
+/* out = grad * (max_norm / norm if norm > max_norm, else 1).  A norm that is
+ * not finite (it is reported) leaves the values as they are.  A tensor's out
+ * may be its grad; it may overlap no other tensor. */
+NERF_API NerfStatus nerf_ext_grad_clip(const NerfExtGradTensor* tensors, uint32_t count, float max_norm, float* norm, void* workspace, uint64_t workspace_bytes, void* stream);
+/* The trainer's update (backend-cuda.cu:1513-1554) on a caller's tensors: step
+ * counts from 1, grad_norm (device) is nerf_ext_grad_norm's of the gradients as
+ * they are (times loss_scale).  Nothing changes, and *skipped (device, or NULL)
+ * is 1, where the norm / loss_scale is not finite or above
+ * update_guard_grad_norm; gradients are scaled by grad_clip_norm / norm where
+ * the norm is above it. */
+NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_t count, const NerfHyperParams* hyper, uint32_t step, const float* grad_norm, uint32_t* skipped, void* stream);
 
 /* ------------------------------------------------------- context options */
 /* Options of a nerf.h context (void* from nerf_create_context); nerf.h itself

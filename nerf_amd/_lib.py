@@ -122,6 +122,10 @@ class NerfCheckpointFileDesc(C.Structure):
 # ------------------------------------------------------------- nerf_ext.h
 NERF_EXT_F32 = 0
 NERF_EXT_F16 = 1
+NERF_EXT_BF16 = 2
+NERF_EXT_ACT_NONE, NERF_EXT_ACT_RELU, NERF_EXT_ACT_SOFTPLUS, NERF_EXT_ACT_SIGMOID, NERF_EXT_ACT_SILU, NERF_EXT_ACT_GELU = range(6)
+NERF_EXT_LINEAR_WORKSPACE = 64 << 20
+NERF_EXT_NORM_WORKSPACE = 64 << 10
 NERF_EXT_MODEL_HASHGRID = 0
 NERF_EXT_MODEL_REFERENCE = 1
 NERF_EXT_SAMPLING_DEFAULT = 0
@@ -253,6 +257,18 @@ class NerfExtRenderStats(C.Structure):
     ]
 
 
+class NerfExtLinearDesc(C.Structure):
+    _fields_ = [(k, C.c_uint32) for k in ("rows", "in_features", "out_features", "dtype", "out_dtype", "activation", "x_stride", "y_stride", "residual_stride", "reserved")]
+
+
+class NerfExtGradTensor(C.Structure):
+    _fields_ = [("grad", C.c_void_p), ("out", C.c_void_p), ("count", C.c_uint64), ("dtype", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class NerfExtAdamTensor(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("param", "grad", "m", "v", "copy")] + [("count", C.c_uint64), ("copy_dtype", C.c_uint32), ("reserved", C.c_uint32)]
+
+
 class NerfExtContextOptions(C.Structure):
     _fields_ = [("model_kind", C.c_uint32), ("inference_sampling", C.c_uint32)]
 
@@ -352,6 +368,12 @@ PROTOTYPES: dict[str, tuple] = {
     "nerf_ext_ref_composite_backward": (_S, [_P, _P, _P, _P, _P, _U32, _F, _P, _P, _P]),
     "nerf_ext_ref_backward": (_S, [_P, _P, _P, _P, _P, _U32, _F, _P, _P, _P]),
     "nerf_ext_ref_backward_rows": (_S, [_P, _P, _P, _P, _P, _U32, _F, _P, _P, _P, _P, _P]),
+    # linear layers, gradients, optimiser
+    "nerf_ext_linear_forward": (_S, [C.POINTER(NerfExtLinearDesc), _P, _P, _P, _P, _P, _P, _P, _U64, _P]),
+    "nerf_ext_linear_backward": (_S, [C.POINTER(NerfExtLinearDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P]),
+    "nerf_ext_grad_norm": (_S, [C.POINTER(NerfExtGradTensor), _U32, _P, _P, _U64, _P]),
+    "nerf_ext_grad_clip": (_S, [C.POINTER(NerfExtGradTensor), _U32, _F, _P, _P, _U64, _P]),
+    "nerf_ext_adam_step": (_S, [C.POINTER(NerfExtAdamTensor), _U32, C.POINTER(NerfHyperParams), _U32, _P, _P, _P]),
     # scene
     "nerf_ext_scene_gaussians": (_S, [C.POINTER(NerfExtSceneDesc), _P]),
     "nerf_ext_scene_density": (_S, [_P, _U32, _P, _U32, _P, _P]),

@@ -1,0 +1,303 @@
+// optimizer.hip — the norm and clipping of gradients that lie in many tensors,
+// and the trainer's Adam update on a caller's tensors (include/nerf_ext.h,
+// nerf_ext_grad_norm, nerf_ext_grad_clip, nerf_ext_adam_step).
+//
+// A launch covers many tensors: their pointers and lengths travel as kernel
+// arguments, and a workgroup finds the tensor of its piece by the pieces'
+// running count.  Squares are summed in 64 bits, per workgroup and then over
+// the workgroups in their order, so that the norm is the same every time and
+// neither overflows nor loses small gradients beside large ones.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.hpp"
+
+using namespace nerf_hip;
+
+namespace {
+
+typedef __bf16 bf16_t;
+
+constexpr uint32_t kThreads  = 256u;
+constexpr uint32_t kPiece    = 4096u;  // elements of a workgroup's turn
+constexpr uint32_t kMaxParts = NERF_EXT_NORM_WORKSPACE / sizeof(double);
+
+// Kernel arguments are kept below 4 KiB.
+constexpr uint32_t kNormListed = 128u, kAdamListed = 64u;
+struct NormList {
+    const void* data[kNormListed];
+    void* out[kNormListed];
+    uint64_t count[kNormListed];
+    uint32_t first[kNormListed];  // pieces before the tensor's
+    uint8_t dtype[kNormListed];
+    uint32_t tensors, pieces;
+};
+struct AdamList {
+    float* param[kAdamListed];
+    const float* grad[kAdamListed];
+    float* m[kAdamListed];
+    float* v[kAdamListed];
+    void* copy[kAdamListed];
+    uint64_t count[kAdamListed];
+    uint32_t first[kAdamListed];
+    uint8_t dtype[kAdamListed];
+    uint32_t tensors, pieces;
+};
+
+template <typename List>
+__device__ __forceinline__ uint32_t tensor_of(const List& l, uint32_t piece) {
+    uint32_t lo = 0u, hi = l.tensors - 1u;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi + 1u) / 2u;
+        if (l.first[mid] <= piece) lo = mid;
+        else hi = mid - 1u;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float load_as_f32(const void* p, uint64_t i, uint32_t dtype) {
+    if (dtype == NERF_EXT_F32) return ((const float*)p)[i];
+    if (dtype == NERF_EXT_F16) return (float)((const half_t*)p)[i];
+    return (float)((const bf16_t*)p)[i];
+}
+__device__ __forceinline__ void store_rounded(void* p, uint64_t i, uint32_t dtype, float v) {
+    if (dtype == NERF_EXT_F32) ((float*)p)[i] = v;
+    else if (dtype == NERF_EXT_F16) ((half_t*)p)[i] = (half_t)v;
+    else ((bf16_t*)p)[i] = (bf16_t)v;
+}
+
+// Sum over the workgroup, in thread 0.
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double ws[kThreads / 64u];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_down(v, d);
+    if ((threadIdx.x & 63u) == 0u) ws[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+    for (uint32_t w = 0; w < kThreads / 64u; ++w) s += ws[w];
+    return s;
+}
+
+// parts[b] = sum of the squares of workgroup b's pieces.
+__global__ __launch_bounds__(kThreads) void k_square_sums(NormList l, double* __restrict__ parts) {
+    double s = 0.0;
+    for (uint32_t piece = blockIdx.x; piece < l.pieces; piece += gridDim.x) {
+        const uint32_t t     = tensor_of(l, piece);
+        const uint64_t first = (uint64_t)(piece - l.first[t]) * kPiece;
+        const uint64_t end   = min(first + kPiece, l.count[t]);
+        for (uint64_t i = first + threadIdx.x; i < end; i += kThreads) {
+            const double g = (double)load_as_f32(l.data[t], i, l.dtype[t]);
+            s += g * g;
+        }
+    }
+    s = block_sum(s);
+    if (threadIdx.x == 0u) parts[blockIdx.x] = s;
+}
+
+// sqrt of the sum of all parts, the same in every workgroup and thread.
+__device__ __forceinline__ float norm_of(const double* __restrict__ parts, uint32_t n) {
+    __shared__ double total;
+    double s = 0.0;
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) s += parts[i];
+    s = block_sum(s);
+    if (threadIdx.x == 0u) total = s;
+    __syncthreads();
+    return (float)sqrt(total);
+}
+
+__global__ __launch_bounds__(kThreads) void k_norm(const double* __restrict__ parts, uint32_t n, float* __restrict__ norm) {
+    const float v = norm_of(parts, n);
+    if (threadIdx.x == 0u) *norm = v;
+}
+
+__global__ __launch_bounds__(kThreads) void k_clip(NormList l, const double* __restrict__ parts, uint32_t n, float max_norm, float* __restrict__ norm) {
+    const float v      = norm_of(parts, n);
+    const float factor = v > max_norm && isfinite(v) ? max_norm / v : 1.0f;
+    if (blockIdx.x == 0u && threadIdx.x == 0u) *norm = v;
+    for (uint32_t piece = blockIdx.x; piece < l.pieces; piece += gridDim.x) {
+        const uint32_t t     = tensor_of(l, piece);
+        const uint64_t first = (uint64_t)(piece - l.first[t]) * kPiece;
+        const uint64_t end   = min(first + kPiece, l.count[t]);
+        for (uint64_t i = first + threadIdx.x; i < end; i += kThreads) store_rounded(l.out[t], i, l.dtype[t], load_as_f32(l.data[t], i, l.dtype[t]) * factor);
+    }
+}
+
+struct AdamRule {
+    float lr, beta1, beta2, eps, bc1, bc2, clip, guard, loss_scale;
+};
+
+__global__ __launch_bounds__(kThreads) void k_adam_tensors(AdamList l, AdamRule r, const float* __restrict__ norm, uint32_t* __restrict__ skipped) {
+    const float gn  = *norm / r.loss_scale;
+    const bool skip = !isfinite(gn) || gn > r.guard;
+    if (skipped && blockIdx.x == 0u && threadIdx.x == 0u) *skipped = skip ? 1u : 0u;
+    if (skip) return;
+    const float gs = (gn > r.clip && gn > 0.0f ? r.clip / gn : 1.0f) * (1.0f / r.loss_scale);
+    for (uint32_t piece = blockIdx.x; piece < l.pieces; piece += gridDim.x) {
+        const uint32_t t     = tensor_of(l, piece);
+        const uint64_t first = (uint64_t)(piece - l.first[t]) * kPiece;
+        const uint64_t end   = min(first + kPiece, l.count[t]);
+        for (uint64_t i = first + threadIdx.x; i < end; i += kThreads) {
+            const float g = l.grad[t][i] * gs;
+            const float m = r.beta1 * l.m[t][i] + (1.0f - r.beta1) * g;
+            const float v = r.beta2 * l.v[t][i] + (1.0f - r.beta2) * g * g;
+            const float p = l.param[t][i] - r.lr * (m * r.bc1) / (sqrtf(v * r.bc2) + r.eps);
+            l.m[t][i]     = m;
+            l.v[t][i]     = v;
+            l.param[t][i] = p;
+            if (l.copy[t]) store_rounded(l.copy[t], i, l.dtype[t], p);
+        }
+    }
+}
+
+// ------------------------------------------------------------------- host
+uint64_t element_bytes(uint32_t dtype) { return dtype == NERF_EXT_F32 ? 4u : 2u; }
+bool aligned(const void* p, uint64_t bytes) { return (uintptr_t)p % bytes == 0u; }
+
+NerfStatus refuse(const char* fn, const char* why) {
+    set_error(std::string(fn) + ": " + why);
+    return NERF_STATUS_INVALID_USAGE;
+}
+
+// Pieces of a list (128 tensors at most) fit 32 bits: 2^24 each.
+constexpr uint64_t kMaxCount   = (uint64_t)kPiece << 24;
+constexpr uint32_t kMaxTensors = 1u << 20;                // a list has a part at least
+
+NerfStatus check_grads(const char* fn, const NerfExtGradTensor* tensors, uint32_t count, const float* norm, const void* workspace, uint64_t bytes, bool outputs) {
+    if (count && !tensors) return refuse(fn, "null tensor list");
+    if (count > kMaxTensors) return refuse(fn, "more than 2^20 tensors");
+    if (!norm || !aligned(norm, 4u)) return refuse(fn, "norm must be a device float");
+    if (!workspace || bytes < NERF_EXT_NORM_WORKSPACE || !aligned(workspace, 16u)) return refuse(fn, "workspace must have NERF_EXT_NORM_WORKSPACE bytes, aligned to 16");
+    for (uint32_t i = 0; i < count; ++i) {
+        const NerfExtGradTensor& t = tensors[i];
+        if (t.dtype != NERF_EXT_F32 && t.dtype != NERF_EXT_F16 && t.dtype != NERF_EXT_BF16) return refuse(fn, "unknown dtype of a tensor");
+        if (t.reserved != 0u) return refuse(fn, "reserved must be 0");
+        if (t.count > kMaxCount) return refuse(fn, "a tensor has more than 2^36 elements");
+        if (t.count && (!t.grad || (outputs && !t.out))) return refuse(fn, "null data of a tensor");
+        if (!aligned(t.grad, element_bytes(t.dtype)) || (outputs && !aligned(t.out, element_bytes(t.dtype)))) return refuse(fn, "a tensor is not aligned to its elements");
+    }
+    return NERF_STATUS_OK;
+}
+
+// f(list) for the tensors in lists of at most the arguments' size; empty
+// tensors are left out.  f also gets each list's number.
+template <typename List, uint32_t kListed, typename Tensor, typename Put, typename F>
+hipError_t each_list(const Tensor* tensors, uint32_t count, Put&& put, F&& f) {
+    uint32_t number = 0u;
+    for (uint32_t at = 0; at < count;) {
+        List l;
+        l.tensors = l.pieces = 0u;
+        for (; at < count && l.tensors < kListed; ++at) {
+            if (tensors[at].count == 0u) continue;
+            const uint64_t pieces = (tensors[at].count + kPiece - 1u) / kPiece;
+            l.count[l.tensors] = tensors[at].count;
+            l.first[l.tensors] = l.pieces;
+            put(l, l.tensors, tensors[at]);
+            l.pieces += (uint32_t)pieces;
+            ++l.tensors;
+        }
+        if (l.tensors == 0u) break;
+        const hipError_t e = f(l, number++);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+void put_grad(NormList& l, uint32_t i, const NerfExtGradTensor& t) {
+    l.data[i]  = t.grad;
+    l.out[i]   = t.out;
+    l.dtype[i] = (uint8_t)t.dtype;
+}
+
+// The parts of all tensors' squares, *n of them.
+hipError_t square_sums(const NerfExtGradTensor* tensors, uint32_t count, double* parts, uint32_t* n, hipStream_t stream) {
+    const uint32_t lists = (count + kNormListed - 1u) / kNormListed;
+    const uint32_t most  = std::max(1u, std::min(4u * device_cu_count(), kMaxParts / std::max(1u, lists)));
+    *n = 0u;
+    return each_list<NormList, kNormListed>(tensors, count, put_grad, [&](const NormList& l, uint32_t) {
+        const uint32_t blocks = std::min(l.pieces, most);
+        k_square_sums<<<blocks, kThreads, 0, stream>>>(l, parts + *n);
+        *n += blocks;
+        return hipGetLastError();
+    });
+}
+
+}  // namespace
+
+extern "C" {
+
+NERF_API NerfStatus nerf_ext_grad_norm(const NerfExtGradTensor* tensors, uint32_t count, float* norm, void* workspace, uint64_t workspace_bytes, void* stream) {
+    const NerfStatus s = check_grads("nerf_ext_grad_norm", tensors, count, norm, workspace, workspace_bytes, false);
+    if (s != NERF_STATUS_OK) return s;
+    uint32_t n = 0u;
+    NERF_HIP_TRY(square_sums(tensors, count, (double*)workspace, &n, (hipStream_t)stream));
+    k_norm<<<1, kThreads, 0, (hipStream_t)stream>>>((const double*)workspace, n, norm);
+    NERF_LAUNCH_CHECK("k_norm");
+    return NERF_STATUS_OK;
+}
+
+NERF_API NerfStatus nerf_ext_grad_clip(const NerfExtGradTensor* tensors, uint32_t count, float max_norm, float* norm, void* workspace, uint64_t workspace_bytes, void* stream) {
+    const NerfStatus s = check_grads("nerf_ext_grad_clip", tensors, count, norm, workspace, workspace_bytes, true);
+    if (s != NERF_STATUS_OK) return s;
+    NERF_CHECK_ARG(max_norm >= 0.0f, "nerf_ext_grad_clip: max_norm must not be negative or NaN");
+    uint32_t n = 0u;
+    NERF_HIP_TRY(square_sums(tensors, count, (double*)workspace, &n, (hipStream_t)stream));
+    if (n == 0u) {
+        k_norm<<<1, kThreads, 0, (hipStream_t)stream>>>((const double*)workspace, 0u, norm);
+        NERF_LAUNCH_CHECK("k_norm");
+        return NERF_STATUS_OK;
+    }
+    NERF_HIP_TRY((each_list<NormList, kNormListed>(tensors, count, put_grad, [&](const NormList& l, uint32_t) {
+        k_clip<<<std::min(l.pieces, 8u * device_cu_count()), kThreads, 0, (hipStream_t)stream>>>(l, (const double*)workspace, n, max_norm, norm);
+        return hipGetLastError();
+    })));
+    return NERF_STATUS_OK;
+}
+
+NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_t count, const NerfHyperParams* hyper, uint32_t step, const float* grad_norm, uint32_t* skipped, void* stream) {
+    const char* fn = "nerf_ext_adam_step";
+    if (count && !tensors) return refuse(fn, "null tensor list");
+    if (count > kMaxTensors) return refuse(fn, "more than 2^20 tensors");
+    if (!hyper || !grad_norm || !aligned(grad_norm, 4u) || !aligned(skipped, 4u)) return refuse(fn, "null or unaligned hyper-parameters, grad_norm or skipped");
+    if (step == 0u) return refuse(fn, "steps count from 1");
+    if (!(hyper->loss_scale > 0.0f)) return refuse(fn, "loss_scale must be positive");
+    if (!(hyper->adam_beta1 >= 0.0f && hyper->adam_beta1 < 1.0f && hyper->adam_beta2 >= 0.0f && hyper->adam_beta2 < 1.0f)) return refuse(fn, "betas must be in [0, 1)");
+    for (uint32_t i = 0; i < count; ++i) {
+        const NerfExtAdamTensor& t = tensors[i];
+        if (t.copy && t.copy_dtype != NERF_EXT_F16 && t.copy_dtype != NERF_EXT_BF16) return refuse(fn, "copy_dtype must be NERF_EXT_F16 or NERF_EXT_BF16");
+        if (t.reserved != 0u) return refuse(fn, "reserved must be 0");
+        if (t.count > kMaxCount) return refuse(fn, "a tensor has more than 2^36 elements");
+        if (t.count && (!t.param || !t.grad || !t.m || !t.v)) return refuse(fn, "null data of a tensor");
+        if (!aligned(t.param, 4u) || !aligned(t.grad, 4u) || !aligned(t.m, 4u) || !aligned(t.v, 4u) || !aligned(t.copy, 2u)) return refuse(fn, "a tensor is not aligned to its elements");
+    }
+    // The trainer's coefficients (backend-cuda.cu:1513-1536), those that do not
+    // depend on the norm computed here in 64 bits.
+    const double decay = (double)hyper->lr_decay_ksteps * 1000.0;
+    AdamRule r;
+    r.lr         = decay > 0.0 ? (float)(hyper->learning_rate * pow(0.1, step / decay)) : hyper->learning_rate;
+    r.beta1      = hyper->adam_beta1;
+    r.beta2      = hyper->adam_beta2;
+    r.eps        = hyper->adam_eps;
+    r.bc1        = (float)(1.0 / (1.0 - pow((double)hyper->adam_beta1, step)));
+    r.bc2        = (float)(1.0 / (1.0 - pow((double)hyper->adam_beta2, step)));
+    r.clip       = hyper->grad_clip_norm;
+    r.guard      = hyper->update_guard_grad_norm;
+    r.loss_scale = hyper->loss_scale;
+    NERF_HIP_TRY((each_list<AdamList, kAdamListed>(
+        tensors, count,
+        [](AdamList& l, uint32_t i, const NerfExtAdamTensor& t) {
+            l.param[i] = t.param;
+            l.grad[i]  = t.grad;
+            l.m[i]     = t.m;
+            l.v[i]     = t.v;
+            l.copy[i]  = t.copy;
+            l.dtype[i] = (uint8_t)t.copy_dtype;
+        },
+        [&](const AdamList& l, uint32_t number) {
+            k_adam_tensors<<<std::min(l.pieces, 8u * device_cu_count()), kThreads, 0, (hipStream_t)stream>>>(l, r, grad_norm, number == 0u ? skipped : nullptr);
+            return hipGetLastError();
+        })));
+    return NERF_STATUS_OK;
+}
+
+}  // extern "C"
