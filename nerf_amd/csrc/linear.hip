@@ -10,7 +10,7 @@
 //   dx       P = W (p contiguous)   Q = d (k contiguous)   k = output feature
 //   dW       P = x (p contiguous)   Q = d (q contiguous)   k = row
 // P is the matrix instruction's A operand, so that a lane ends with four
-// consecutive p of one q and stores them together.  An operand whose k is not
+// consecutive p of one q.  An operand whose k is not
 // contiguous is read from LDS through the transposing read
 // (ds_read_b64_tr_b16), four k of one p a lane, so no operand is transposed in
 // memory.  Products are of 16-bit values, exact in 32 bits, and summed in 32
@@ -25,7 +25,6 @@ namespace {
 
 typedef __bf16 bf16_t;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef short short8_t __attribute__((ext_vector_type(8)));
 
@@ -33,13 +32,11 @@ template <typename T>
 struct Vec;
 template <>
 struct Vec<half_t> {
-    using x4 = half4_t;
     using x8 = half8_t;
     static __device__ __forceinline__ floatx4 mfma(x8 a, x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Vec<bf16_t> {
-    using x4 = bf16x4_t;
     using x8 = bf16x8_t;
     static __device__ __forceinline__ floatx4 mfma(x8 a, x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
@@ -90,58 +87,97 @@ __device__ __forceinline__ float act_slope(float z) {
     return 1.0f;
 }
 
-// f(constant of the activation): one branch for a whole tile.
-template <typename F>
-__device__ __forceinline__ void with_activation(uint32_t act, F&& f) {
+// act_value / act_slope of eight values, one branch for all of them.
+typedef float floatx8 __attribute__((ext_vector_type(8)));
+
+template <uint32_t kAct>
+__device__ __forceinline__ void values8(floatx8& z) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) z[r] = act_value<kAct>(z[r]);
+}
+template <uint32_t kAct>
+__device__ __forceinline__ void slopes8(floatx8& z) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) z[r] = act_slope<kAct>(z[r]);
+}
+__device__ __forceinline__ void act_values(uint32_t act, floatx8& z) {
     switch (act) {
-    case NERF_EXT_ACT_RELU: f(std::integral_constant<uint32_t, NERF_EXT_ACT_RELU>{}); break;
-    case NERF_EXT_ACT_SOFTPLUS: f(std::integral_constant<uint32_t, NERF_EXT_ACT_SOFTPLUS>{}); break;
-    case NERF_EXT_ACT_SIGMOID: f(std::integral_constant<uint32_t, NERF_EXT_ACT_SIGMOID>{}); break;
-    case NERF_EXT_ACT_SILU: f(std::integral_constant<uint32_t, NERF_EXT_ACT_SILU>{}); break;
-    case NERF_EXT_ACT_GELU: f(std::integral_constant<uint32_t, NERF_EXT_ACT_GELU>{}); break;
-    default: f(std::integral_constant<uint32_t, NERF_EXT_ACT_NONE>{}); break;
+    case NERF_EXT_ACT_RELU: return values8<NERF_EXT_ACT_RELU>(z);
+    case NERF_EXT_ACT_SOFTPLUS: return values8<NERF_EXT_ACT_SOFTPLUS>(z);
+    case NERF_EXT_ACT_SIGMOID: return values8<NERF_EXT_ACT_SIGMOID>(z);
+    case NERF_EXT_ACT_SILU: return values8<NERF_EXT_ACT_SILU>(z);
+    case NERF_EXT_ACT_GELU: return values8<NERF_EXT_ACT_GELU>(z);
+    default: return;
+    }
+}
+__device__ __forceinline__ void act_slopes(uint32_t act, floatx8& z) {
+    switch (act) {
+    case NERF_EXT_ACT_RELU: return slopes8<NERF_EXT_ACT_RELU>(z);
+    case NERF_EXT_ACT_SOFTPLUS: return slopes8<NERF_EXT_ACT_SOFTPLUS>(z);
+    case NERF_EXT_ACT_SIGMOID: return slopes8<NERF_EXT_ACT_SIGMOID>(z);
+    case NERF_EXT_ACT_SILU: return slopes8<NERF_EXT_ACT_SILU>(z);
+    case NERF_EXT_ACT_GELU: return slopes8<NERF_EXT_ACT_GELU>(z);
+    default: return slopes8<NERF_EXT_ACT_NONE>(z);
     }
 }
 
 // ------------------------------------------------------------- epilogues
-// What becomes of a finished sum.  Each gets four consecutive p of one q at a
-// time, q < nq, p < np; vec: all four exist and every array's four are one
-// aligned access.
+// What becomes of a finished sum.  Arrays are reached through buffer
+// descriptors that start at the workgroup's first row: offsets are 32 bits,
+// and an access whose offset is kBeyond does nothing (loads give 0), which
+// takes the place of branches at the edges.
+constexpr uint32_t kBeyond = 0x80000000u;
+typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
+
+template <typename E>
+struct Rows {
+    __amdgpu_buffer_rsrc_t rsrc;
+    uint32_t ld;
+    // Row `first` of an array with rows ld elements apart.
+    __device__ __forceinline__ Rows(const void* data, uint64_t first, uint64_t ld_) : rsrc(__builtin_amdgcn_make_buffer_rsrc((void*)((const E*)data + first * ld_), (short)0, (int)0x7FFFFFFF, 0x00020000)), ld((uint32_t)ld_) {}
+    // Eight elements from (row, p), n of them inside; vec: all, aligned to 16 bytes.
+    __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t p) const { return (row * ld + p) * (uint32_t)sizeof(E); }
+    __device__ __forceinline__ uintx4 load(uint32_t row, uint32_t p, uint32_t n, bool vec) const {
+        static_assert(sizeof(E) == 2);
+        if (vec) return __builtin_bit_cast(uintx4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(n ? at(row, p) : kBeyond), 0, 0));
+        short8_t v;
+#pragma unroll
+        for (uint32_t r = 0; r < 8u; ++r) v[r] = (short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)(r < n ? at(row, p + r) : kBeyond), 0, 0);
+        return __builtin_bit_cast(uintx4, v);
+    }
+    __device__ __forceinline__ void store(uint32_t row, uint32_t p, uint32_t n, bool vec, const floatx8& v) const {
+        if constexpr (sizeof(E) == 4) {
+            if (vec) {
+                // Copies: a bit cast of part of a vector takes the vector's first part.
+                const floatx4 lo = v.lo, hi = v.hi;
+                const uint32_t o = n ? at(row, p) : kBeyond;
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, lo), rsrc, (int)o, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, hi), rsrc, (int)(o + 16u), 0, 0);
+                return;
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < 8u; ++r) {
+                const float e = v[r];
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, e), rsrc, (int)(r < n ? at(row, p + r) : kBeyond), 0, 0);
+            }
+        } else {
+            const typename Vec<E>::x8 h = __builtin_convertvector(v, typename Vec<E>::x8);
+            if (vec) return __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, h), rsrc, (int)(n ? at(row, p) : kBeyond), 0, 0);
+            const short8_t b = __builtin_bit_cast(short8_t, h);
+#pragma unroll
+            for (uint32_t r = 0; r < 8u; ++r) __builtin_amdgcn_raw_buffer_store_b16(b[r], rsrc, (int)(r < n ? at(row, p + r) : kBeyond), 0, 0);
+        }
+    }
+};
+
 template <typename T>
-__device__ __forceinline__ floatx4 load4(const T* p, uint32_t n, bool vec) {
-    if (vec) {
-        const typename Vec<T>::x4 v = *reinterpret_cast<const typename Vec<T>::x4*>(p);
-        return floatx4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
-    }
-    floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (uint32_t r = 0; r < 4u; ++r)
-        if (r < n) o[r] = (float)p[r];
-    return o;
-}
-template <typename T>
-__device__ __forceinline__ void store4(T* p, floatx4 v, uint32_t n, bool vec) {
-    if (vec) {
-        typename Vec<T>::x4 h;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) h[r] = (T)v[r];
-        *reinterpret_cast<typename Vec<T>::x4*>(p) = h;
-        return;
-    }
-#pragma unroll
-    for (uint32_t r = 0; r < 4u; ++r)
-        if (r < n) p[r] = (T)v[r];
-}
-__device__ __forceinline__ void store4(float* p, floatx4 v, uint32_t n, bool vec) {
-    if (vec) {
-        *reinterpret_cast<floatx4*>(p) = v;
-        return;
-    }
-#pragma unroll
-    for (uint32_t r = 0; r < 4u; ++r)
-        if (r < n) p[r] = v[r];
+__device__ __forceinline__ floatx8 widen(uintx4 v) {
+    return __builtin_convertvector(__builtin_bit_cast(typename Vec<T>::x8, v), floatx8);
 }
 
+// Each epilogue gets eight consecutive p of one row q0 + row at a time, n of
+// them inside the output (0 for a row outside), and first loads what it needs
+// besides the sums, so that a caller can have that under way early.
 template <typename T>
 struct ForwardOut {
     const float* bias;
@@ -151,25 +187,24 @@ struct ForwardOut {
     uint64_t ldr, ldy;
     uint32_t np, nq, act;
     bool y32, vec;
+    struct Aux {
+        uintx4 residual;
+    };
 
-    template <uint32_t kAct>
-    __device__ __forceinline__ void put(uint32_t q, uint32_t p, floatx4 z) const {
-        const uint32_t n = np - p;
+    __device__ __forceinline__ Aux load(uint32_t q0, uint32_t row, uint32_t p, uint32_t n) const {
+        return {residual ? Rows<T>(residual, q0, ldr).load(row, p, n, vec) : uintx4{0u, 0u, 0u, 0u}};
+    }
+    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 z, const Aux& a) const {
         if (bias) {
+            const Rows<float> b(bias, 0u, 0u);
 #pragma unroll
-            for (uint32_t r = 0; r < 4u; ++r)
-                if (vec || r < n) z[r] += bias[p + r];
+            for (uint32_t r = 0; r < 8u; ++r) z[r] += __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b.rsrc, (int)(r < n ? 4u * (p + r) : kBeyond), 0, 0));
         }
-        if (pre) store4(pre + (uint64_t)q * np + p, z, n, vec);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) z[r] = act_value<kAct>(z[r]);
-        if (residual) {
-            const floatx4 a = load4(residual + (uint64_t)q * ldr + p, n, vec);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) z[r] += a[r];
-        }
-        if (y32) store4((float*)y + (uint64_t)q * ldy + p, z, n, vec);
-        else store4((T*)y + (uint64_t)q * ldy + p, z, n, vec);
+        if (pre) Rows<T>(pre, q0, np).store(row, p, n, vec, z);
+        act_values(act, z);
+        if (residual) z += widen<T>(a.residual);
+        if (y32) Rows<float>(y, q0, ldy).store(row, p, n, vec, z);
+        else Rows<T>(y, q0, ldy).store(row, p, n, vec, z);
     }
 };
 
@@ -182,21 +217,23 @@ struct InputGradientOut {
     uint64_t ldx;
     uint32_t np, nq, act;
     bool vec;
+    struct Aux {
+        uintx4 add, pre;
+    };
 
-    template <uint32_t kAct>
-    __device__ __forceinline__ void put(uint32_t q, uint32_t p, floatx4 g) const {
-        const uint32_t n = np - p;
-        if (add) {
-            const floatx4 a = load4(add + (uint64_t)q * ldx + p, n, vec);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) g[r] += a[r];
-        }
-        if (dx) store4(dx + (uint64_t)q * ldx + p, g, n, vec);
+    __device__ __forceinline__ Aux load(uint32_t q0, uint32_t row, uint32_t p, uint32_t n) const {
+        Aux a{};
+        if (add) a.add = Rows<T>(add, q0, ldx).load(row, p, n, vec);
+        if (dpre) a.pre = Rows<T>(pre, q0, np).load(row, p, n, vec);
+        return a;
+    }
+    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 g, const Aux& a) const {
+        if (add) g += widen<T>(a.add);
+        if (dx) Rows<T>(dx, q0, ldx).store(row, p, n, vec, g);
         if (dpre) {
-            const floatx4 z = load4(pre + (uint64_t)q * np + p, n, vec);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) g[r] *= act_slope<kAct>(z[r]);
-            store4(dpre + (uint64_t)q * np + p, g, n, vec);
+            floatx8 s = widen<T>(a.pre);
+            act_slopes(act, s);
+            Rows<T>(dpre, q0, np).store(row, p, n, vec, g * s);
         }
     }
 };
@@ -204,17 +241,17 @@ struct InputGradientOut {
 // Plain sums in 32 bits: dW, or one part of a sum that was split over k.
 struct SumOut {
     float* out;
-    uint64_t part;  // elements from one part to the next
+    uint64_t part;    // elements from one part to the next
     float* row_sums;  // sum_k Q(q, k), or null; nq of them a part
-    uint32_t np, nq, act;
+    uint32_t np, nq;
     bool vec;
-    template <uint32_t kAct>
-    __device__ __forceinline__ void put(uint32_t q, uint32_t p, floatx4 v) const { store4(out + (uint64_t)q * np + p, v, np - p, vec); }
+    struct Aux {};
+    __device__ __forceinline__ Aux load(uint32_t, uint32_t, uint32_t, uint32_t) const { return {}; }
+    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, const floatx8& v, const Aux&) const { Rows<float>(out, q0, np).store(row, p, n, vec, v); }
 };
 
 // ----------------------------------------------------------------- product
 constexpr uint32_t kBK = 64u;  // k per tile: two matrix instructions' worth
-constexpr uint32_t kThreads = 256u;
 
 struct Operands {
     const void* p;
@@ -230,13 +267,17 @@ struct Operands {
 // read's lanes in 8 different places; kT (row contiguous), k-major [64][kB],
 // the four k of a transposing read 32 bytes apart.
 template <uint32_t kB, bool kT>
-__device__ __forceinline__ uint32_t chunk_slot(uint32_t row, uint32_t chunk) {
-    if constexpr (kT) return row * (kB / 8u) + (chunk ^ ((row & 3u) << 1));
-    else return row * 8u + (chunk ^ (row & 7u));
+__device__ __forceinline__ constexpr uint32_t chunk_key(uint32_t line) {
+    return kT ? (line & 3u) << 1 : line & 7u;
+}
+template <uint32_t kB, bool kT>
+__device__ __forceinline__ constexpr uint32_t chunk_slot(uint32_t line, uint32_t chunk) {
+    return line * (kT ? kB / 8u : 8u) + (chunk ^ chunk_key<kB, kT>(line));
 }
 
-// Tile [row0, row0 + kB) x [k0, k0 + 64) into LDS, zeros outside [0, n) x [0, nk).
-template <typename T, uint32_t kB, bool kT>
+// Tile [row0, row0 + kB) x [k0, k0 + 64) into LDS, zeros outside [0, n) x [0, nk):
+// through registers, any alignment.
+template <typename T, uint32_t kB, bool kT, uint32_t kThreads>
 __device__ __forceinline__ void stage(const T* __restrict__ src, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end, uint4* lds) {
     constexpr uint32_t kChunks = kT ? kB / 8u : 8u;
 #pragma unroll
@@ -262,6 +303,48 @@ __device__ __forceinline__ void stage(const T* __restrict__ src, uint64_t ld, ui
     }
 }
 
+// The same straight from memory into LDS, 16 bytes a lane, for chunks that are
+// whole and aligned (start, stride and the contiguous length multiples of 8):
+// a wave fills 64 slots in their order, each lane fetching the chunk whose
+// place its slot is.  Chunks outside the operand take an offset beyond the
+// descriptor's range, for which the hardware delivers zeros.
+template <typename T, uint32_t kB, bool kT, uint32_t kThreads>
+struct Loader {
+    static constexpr uint32_t kChunks = kT ? kB / 8u : 8u;
+    static constexpr uint32_t kLoads  = kB * 8u / kThreads;
+    static_assert(kB * 8u % kThreads == 0u);
+    const T* base;           // of the tile at its next k
+    uint64_t step;           // elements from one tile of k to the next
+    uint32_t offset[kLoads]; // bytes, kBeyond for rows outside
+    uint32_t minor;          // kT: unused; else the lane's first k within the tile
+
+    __device__ __forceinline__ void begin(const T* src, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0) {
+        base = src + (kT ? (uint64_t)k0 * ld + row0 : (uint64_t)row0 * ld + k0);
+        step = kT ? kBK * ld : kBK;
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            const uint32_t s = i * kThreads + threadIdx.x, line = s / kChunks, chunk = (s % kChunks) ^ chunk_key<kB, kT>(line);
+            const bool inside = kT ? row0 + 8u * chunk < n : row0 + line < n;
+            offset[i]         = inside ? (line * (uint32_t)ld + 8u * chunk) * 2u : kBeyond;
+        }
+    }
+    // left: k from the tile's start to the end of the part.
+    __device__ __forceinline__ void issue(uint4* lds, int left) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)0x7FFFFFFF, 0x00020000);
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            uint32_t at = offset[i];
+            if (left < (int)kBK) {
+                const uint32_t s = i * kThreads + threadIdx.x, line = s / kChunks, chunk = (s % kChunks) ^ chunk_key<kB, kT>(line);
+                if ((int)(kT ? line : 8u * chunk) >= left) at = kBeyond;
+            }
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + i * kThreads + wave * 64u), 16, (int)at, 0, 0, 0);
+        }
+        base += step;
+    }
+};
+
 // The 8 k of rows [row0, row0 + 16) that a lane feeds to one 16x16x32 matrix
 // instruction: k = 32 step + 8 (lane / 16) + 0..7 of row row0 + lane % 16.
 template <typename T, uint32_t kB, bool kT>
@@ -283,12 +366,23 @@ __device__ __forceinline__ typename Vec<T>::x8 fragment(const uint4* lds, uint32
     }
 }
 
-template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, bool kPT, bool kQT, typename Out>
-__global__ __launch_bounds__(kThreads) void k_product(Operands A, Out out) {
-    static_assert(kWP * kWQ * 64u == kThreads);
+// Waits for the wave's own loads into LDS and then for the workgroup.
+__device__ __forceinline__ void arrived() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// kBP x kBQ outputs a workgroup, kWP x kWQ waves.  kAligned: both operands go
+// straight into LDS, the next 64 k while this one is multiplied.
+template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, bool kPT, bool kQT, bool kAligned, typename Out>
+__global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out) {
+    constexpr uint32_t kThreads = kWP * kWQ * 64u;
     constexpr uint32_t kFP = kBP / kWP / 16u, kFQ = kBQ / kWQ / 16u;
-    __shared__ uint4 lds_p[kBP * 8u];
-    __shared__ uint4 lds_q[kBQ * 8u];
+    // Variables of their own, so that the compiler sees that a read of one is no
+    // read of what is on its way into another.
+    __shared__ uint4 lds_p0[kBP * 8u], lds_q0[kBQ * 8u], lds_p1[kAligned ? kBP * 8u : 1u], lds_q1[kAligned ? kBQ * 8u : 1u];
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
     const uint32_t wp = (wave % kWP) * (kBP / kWP), wq = (wave / kWP) * (kBQ / kWQ);
     const uint32_t p0 = blockIdx.x * kBP, q0 = blockIdx.y * kBQ;
@@ -307,17 +401,14 @@ __global__ __launch_bounds__(kThreads) void k_product(Operands A, Out out) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = (T)1.0f;
 
-    for (uint32_t k = k0; k < k_end; k += kBK) {
-        stage<T, kBP, kPT>((const T*)A.p, A.ldp, A.np, p0, k, k_end, lds_p);
-        stage<T, kBQ, kQT>((const T*)A.q, A.ldq, A.nq, q0, k, k_end, lds_q);
-        __syncthreads();
+    auto multiply = [&](const uint4* lp, const uint4* lq) {
 #pragma unroll
         for (uint32_t step = 0; step < 2u; ++step) {
             typename Vec<T>::x8 fp[kFP], fq[kFQ];
 #pragma unroll
-            for (uint32_t i = 0; i < kFP; ++i) fp[i] = fragment<T, kBP, kPT>(lds_p, wp + 16u * i, step);
+            for (uint32_t i = 0; i < kFP; ++i) fp[i] = fragment<T, kBP, kPT>(lp, wp + 16u * i, step);
 #pragma unroll
-            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = fragment<T, kBQ, kQT>(lds_q, wq + 16u * j, step);
+            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = fragment<T, kBQ, kQT>(lq, wq + 16u * j, step);
 #pragma unroll
             for (uint32_t i = 0; i < kFP; ++i)
 #pragma unroll
@@ -328,8 +419,42 @@ __global__ __launch_bounds__(kThreads) void k_product(Operands A, Out out) {
                     for (uint32_t j = 0; j < kFQ; ++j) sums[j] = Vec<T>::mfma(ones, fq[j], sums[j]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);  // the fragments of one step at a time in registers
         }
-        __syncthreads();
+    };
+
+    if constexpr (kAligned) {
+        Loader<T, kBP, kPT, kThreads> load_p;
+        Loader<T, kBQ, kQT, kThreads> load_q;
+        load_p.begin((const T*)A.p, A.ldp, A.np, p0, k0);
+        load_q.begin((const T*)A.q, A.ldq, A.nq, q0, k0);
+        // Two tiles a turn, one from each pair of buffers; a last odd tile is
+        // followed by one of zeros (a way out between the two would keep a second
+        // copy of the sums alive).
+        load_p.issue(lds_p0, (int)(k_end - k0));
+        load_q.issue(lds_q0, (int)(k_end - k0));
+        for (int left = (int)(k_end - k0); left > 0; left -= (int)(2u * kBK)) {
+            // Everyone's part of this tile has come, and everyone is done with the
+            // other buffers.
+            arrived();
+            load_p.issue(lds_p1, left - (int)kBK);
+            load_q.issue(lds_q1, left - (int)kBK);
+            multiply(lds_p0, lds_q0);
+            arrived();
+            if (left > (int)(2u * kBK)) {
+                load_p.issue(lds_p0, left - (int)(2u * kBK));
+                load_q.issue(lds_q0, left - (int)(2u * kBK));
+            }
+            multiply(lds_p1, lds_q1);
+        }
+    } else {
+        for (uint32_t k = k0; k < k_end; k += kBK) {
+            stage<T, kBP, kPT, kThreads>((const T*)A.p, A.ldp, A.np, p0, k, k_end, lds_p0);
+            stage<T, kBQ, kQT, kThreads>((const T*)A.q, A.ldq, A.nq, q0, k, k_end, lds_q0);
+            __syncthreads();
+            multiply(lds_p0, lds_q0);
+            __syncthreads();
+        }
     }
 
     if constexpr (std::is_same_v<Out, SumOut>) {
@@ -342,41 +467,69 @@ __global__ __launch_bounds__(kThreads) void k_product(Operands A, Out out) {
             }
         }
     }
-    with_activation(out.act, [&](auto act) {
+
+    // The wave's sums, 16 q x kSP p at a time, through LDS of its own into rows:
+    // a lane then has eight consecutive p, and eight lanes one 128-byte line
+    // (16-bit outputs).  Chunks of four p, their place xor-ed with the row.
+    constexpr uint32_t kSP = kBP / kWP < 64u ? kBP / kWP : 64u, kStrips = kFQ * (kBP / kWP / kSP);
+    constexpr uint32_t kLanes = kSP / 8u, kPasses = 16u * kLanes / 64u;
+    static_assert(kWP * kWQ * kSP <= 8u * kBP);
+    __syncthreads();
+    floatx4* strip = reinterpret_cast<floatx4*>(lds_p0) + wave * (kSP * 4u);
+    const uint32_t row = lane / kLanes, col = 8u * (lane % kLanes);
+    auto row_of = [&](uint32_t s, uint32_t pass) { return wq + 16u * (s % kFQ) + (64u / kLanes) * pass + row; };
+    auto p_of = [&](uint32_t s) { return p0 + wp + kSP * (s / kFQ) + col; };
+    auto inside = [&](uint32_t s, uint32_t pass) { return q0 + row_of(s, pass) < out.nq && p_of(s) < out.np ? min(8u, out.np - p_of(s)) : 0u; };
+    typename Out::Aux aux[2][kPasses];
+    auto prefetch = [&](uint32_t s) {
 #pragma unroll
-        for (uint32_t j = 0; j < kFQ; ++j) {
-            const uint32_t q = q0 + wq + 16u * j + (lane & 15u);
+        for (uint32_t t = 0; t < kPasses; ++t) aux[s & 1u][t] = out.load(q0, row_of(s, t), p_of(s), inside(s, t));
+    };
+    prefetch(0u);
 #pragma unroll
-            for (uint32_t i = 0; i < kFP; ++i) {
-                const uint32_t p = p0 + wp + 16u * i + 4u * (lane >> 4);
-                if (q < out.nq && p < out.np) out.template put<act()>(q, p, acc[i][j]);
-            }
+    for (uint32_t s = 0; s < kStrips; ++s) {
+#pragma unroll
+        for (uint32_t f = 0; f < kSP / 16u; ++f) strip[(lane & 15u) * (kSP / 4u) + ((4u * f + (lane >> 4)) ^ (lane & 7u))] = acc[kSP / 16u * (s / kFQ) + f][s % kFQ];
+        if (s + 1u < kStrips) prefetch(s + 1u);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (uint32_t t = 0; t < kPasses; ++t) {
+            const uint32_t r = (64u / kLanes) * t + row;
+            floatx8 v;
+            v.lo = strip[r * (kSP / 4u) + ((col / 4u) ^ (r & 7u))];
+            v.hi = strip[r * (kSP / 4u) + ((col / 4u + 1u) ^ (r & 7u))];
+            out.put(q0, row_of(s, t), p_of(s), inside(s, t), v, aux[s & 1u][t]);
         }
-    });
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // Joins the parts of a sum that was split over k, in their order.
 template <typename Out>
 __global__ __launch_bounds__(256) void k_join(const float* __restrict__ parts, uint64_t part, uint32_t count, const float* __restrict__ sums, float* __restrict__ row_sums, Out out) {
-    const uint32_t quads = (out.np + 3u) / 4u;
-    const uint64_t total = (uint64_t)quads * out.nq, step = (uint64_t)gridDim.x * blockDim.x, first = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    with_activation(out.act, [&](auto act) {
-        for (uint64_t at = first; at < total; at += step) {
-            const uint32_t q = (uint32_t)(at / quads), p = 4u * (uint32_t)(at % quads);
-            floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (uint32_t c = 0; c < count; ++c) {
-                const float* src = parts + c * part + (uint64_t)q * out.np + p;
-                if (out.vec) {
-                    v += *reinterpret_cast<const floatx4*>(src);
-                } else {
+    const uint32_t eights = (out.np + 7u) / 8u;
+    const uint64_t total = (uint64_t)eights * out.nq, step = (uint64_t)gridDim.x * blockDim.x, first = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const bool vec = out.np % 4u == 0u;
+    for (uint64_t at = first; at < total; at += step) {
+        const uint32_t q = (uint32_t)(at / eights), p = 8u * (uint32_t)(at % eights), n = min(8u, out.np - p);
+        // The epilogues count rows from a uniform one: the first that the
+        // workgroup's threads have in this turn.
+        const uint32_t q0 = (uint32_t)((at - threadIdx.x) / eights);
+        const typename Out::Aux aux = out.load(q0, q - q0, p, n);
+        floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t c = 0; c < count; ++c) {
+            const float* src = parts + c * part + (uint64_t)q * out.np + p;
+            if (vec && n == 8u) {
+                v.lo += reinterpret_cast<const floatx4*>(src)[0];
+                v.hi += reinterpret_cast<const floatx4*>(src)[1];
+            } else {
 #pragma unroll
-                    for (uint32_t r = 0; r < 4u; ++r)
-                        if (p + r < out.np) v[r] += src[r];
-                }
+                for (uint32_t r = 0; r < 8u; ++r)
+                    if (r < n) v[r] += src[r];
             }
-            out.template put<act()>(q, p, v);
         }
-    });
+        out.put(q0, q - q0, p, n, v, aux);
+    }
     if (row_sums) {
         for (uint64_t q = first; q < out.nq; q += step) {
             float s = 0.0f;
@@ -387,7 +540,7 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ parts, u
 }
 
 // ------------------------------------------------------------------- host
-constexpr uint32_t kMaxFeatures = 1u << 16, kMaxStride = 1u << 22, kMaxRows = 1u << 30;
+constexpr uint32_t kMaxFeatures = 1u << 16, kMaxStride = 1u << 20, kMaxRows = 1u << 30;
 
 bool aligned(const void* p, uint64_t bytes) { return ((uintptr_t)p & (bytes - 1u)) == 0u; }
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1u) / b); }
@@ -397,15 +550,17 @@ struct Workspace {
     uint64_t bytes;
 };
 
-template <typename T, bool kPT, bool kQT, typename Out>
-hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hipStream_t stream) {
-    constexpr uint32_t kBP = 64u, kBQ = 64u;
+// Whether an operand's chunks of 8 along its contiguous length are whole and aligned.
+bool whole_chunks(const void* p, uint64_t ld, uint32_t contiguous) { return aligned(p, 16u) && ld % 8u == 0u && contiguous % 8u == 0u; }
+
+template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, bool kPT, bool kQT, bool kAligned, bool kSplit = true, typename Out>
+hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipStream_t stream) {
     const uint32_t tp = ceil_div(A.np, kBP), tq = ceil_div(A.nq, kBQ);
     // Split over k until every CU has two workgroups, with four tiles of k a
     // part at least, as far as the workspace holds the parts.
     const uint64_t part = (uint64_t)A.np * A.nq;
     const uint64_t per = 4u * (part + (row_sums ? A.nq : 0u));
-    uint64_t splits = (2ull * device_cu_count()) / ((uint64_t)tp * tq);
+    uint64_t splits = kSplit ? (2ull * device_cu_count()) / ((uint64_t)tp * tq) : 1u;
     splits = std::min<uint64_t>({splits, ceil_div(A.nk, 4u * kBK), ws.data ? ws.bytes / per : 0u, 65535u});
     const bool split = splits > 1u;
     if (!split) splits = 1u;
@@ -413,18 +568,30 @@ hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hi
     if (A.k_split == 0u) A.k_split = kBK;
     const uint32_t parts = std::max(1u, ceil_div(A.nk, A.k_split));
     const dim3 grid(tp, tq, parts);
-    if (parts > 1u) {
-        float* sums = row_sums ? ws.data + parts * part : nullptr;
-        const SumOut so{ws.data, part, sums, A.np, A.nq, NERF_EXT_ACT_NONE, A.np % 4u == 0u};
-        k_product<T, kBP, kBQ, 2, 2, kPT, kQT, SumOut><<<grid, kThreads, 0, stream>>>(A, so);
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        const uint64_t quads = (uint64_t)ceil_div(A.np, 4u) * A.nq;
-        k_join<Out><<<(uint32_t)std::min<uint64_t>(ceil_div(quads, 256u), 4096u), 256, 0, stream>>>(ws.data, part, parts, sums, row_sums, out);
-        return hipGetLastError();
+    constexpr uint32_t kThreads = kWP * kWQ * 64u;
+    if constexpr (kSplit) {
+        if (parts > 1u) {
+            float* sums = row_sums ? ws.data + parts * part : nullptr;
+            const SumOut so{ws.data, part, sums, A.np, A.nq, A.np % 8u == 0u};
+            k_product<T, kBP, kBQ, kWP, kWQ, kPT, kQT, kAligned, SumOut><<<grid, kThreads, 0, stream>>>(A, so);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+            const uint64_t eights = (uint64_t)ceil_div(A.np, 8u) * A.nq;
+            k_join<Out><<<(uint32_t)std::min<uint64_t>(ceil_div(eights, 256u), 4096u), 256, 0, stream>>>(ws.data, part, parts, sums, row_sums, out);
+            return hipGetLastError();
+        }
     }
-    k_product<T, kBP, kBQ, 2, 2, kPT, kQT, Out><<<grid, kThreads, 0, stream>>>(A, out);
+    k_product<T, kBP, kBQ, kWP, kWQ, kPT, kQT, kAligned, Out><<<grid, kThreads, 0, stream>>>(A, out);
     return hipGetLastError();
+}
+
+template <typename T, bool kPT, bool kQT, typename Out>
+hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hipStream_t stream) {
+    if (!whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, kQT ? A.nq : A.nk)) return launch_tiles<T, 64, 64, 2, 2, kPT, kQT, false>(A, out, row_sums, ws, stream);
+    const uint32_t cus = device_cu_count();
+    if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) >= cus / 2u && A.np > 128u && A.nk >= 512u) return launch_tiles<T, 256, 256, 2, 4, kPT, kQT, true, false>(A, out, row_sums, ws, stream);
+    if ((uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u) >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u)) return launch_tiles<T, 128, 128, 2, 2, kPT, kQT, true>(A, out, row_sums, ws, stream);
+    return launch_tiles<T, 64, 64, 2, 2, kPT, kQT, true>(A, out, row_sums, ws, stream);
 }
 
 // rows beyond gridDim's range of 64-row tiles are taken in launches of this many.
@@ -433,7 +600,7 @@ constexpr uint32_t kRowsPerLaunch = 65535u * 64u;
 template <typename T>
 NerfStatus forward(const NerfExtLinearDesc& d, const void* x, const void* w, const float* bias, const void* residual, void* y, void* pre, Workspace ws, hipStream_t stream) {
     const bool y32 = d.out_dtype == NERF_EXT_F32;
-    const bool vec = d.out_features % 4u == 0u && d.y_stride % 4u == 0u && aligned(y, y32 ? 16u : 8u) && aligned(bias, 16u) && (!pre || aligned(pre, 8u)) && (!residual || (d.residual_stride % 4u == 0u && aligned(residual, 8u)));
+    const bool vec = d.out_features % 8u == 0u && d.y_stride % 8u == 0u && aligned(y, 16u) && aligned(pre, 16u) && (!residual || (d.residual_stride % 8u == 0u && aligned(residual, 16u)));
     for (uint64_t r0 = 0; r0 < d.rows; r0 += kRowsPerLaunch) {
         const uint32_t n = (uint32_t)std::min<uint64_t>(kRowsPerLaunch, d.rows - r0);
         const Operands A{w, (const T*)x + r0 * d.x_stride, d.in_features, d.x_stride, d.out_features, n, d.in_features, 0u};
@@ -447,7 +614,7 @@ NerfStatus forward(const NerfExtLinearDesc& d, const void* x, const void* w, con
 template <typename T>
 NerfStatus backward(const NerfExtLinearDesc& d, const void* x, const void* w, const void* delta, const void* pre, const void* add, void* dx, void* dpre, float* dw, float* db, Workspace ws, hipStream_t stream) {
     if (dx || dpre) {
-        const bool vec = d.in_features % 4u == 0u && (!(add || dx) || d.x_stride % 4u == 0u) && aligned(add, 8u) && aligned(dx, 8u) && aligned(pre, 8u) && aligned(dpre, 8u);
+        const bool vec = d.in_features % 8u == 0u && (!(add || dx) || d.x_stride % 8u == 0u) && aligned(add, 16u) && aligned(dx, 16u) && aligned(pre, 16u) && aligned(dpre, 16u);
         for (uint64_t r0 = 0; r0 < d.rows; r0 += kRowsPerLaunch) {
             const uint32_t n = (uint32_t)std::min<uint64_t>(kRowsPerLaunch, d.rows - r0);
             const Operands A{w, (const T*)delta + r0 * d.y_stride, d.in_features, d.y_stride, d.in_features, n, d.out_features, 0u};
@@ -458,7 +625,7 @@ NerfStatus backward(const NerfExtLinearDesc& d, const void* x, const void* w, co
     }
     if (dw) {
         const Operands A{x, delta, d.x_stride, d.y_stride, d.in_features, d.out_features, d.rows, 0u};
-        const SumOut out{dw, 0u, db, d.in_features, d.out_features, NERF_EXT_ACT_NONE, d.in_features % 4u == 0u && aligned(dw, 16u)};
+        const SumOut out{dw, 0u, db, d.in_features, d.out_features, d.in_features % 8u == 0u && aligned(dw, 16u)};
         NERF_HIP_TRY((launch_product<T, true, true>(A, out, db, ws, stream)));
     }
     return NERF_STATUS_OK;
@@ -481,7 +648,7 @@ NerfStatus check_desc(const NerfExtLinearDesc* desc, NerfExtLinearDesc& d, const
     if (d.y_stride == 0u) d.y_stride = d.out_features;
     if (d.residual_stride == 0u) d.residual_stride = d.out_features;
     if (d.x_stride < d.in_features || d.y_stride < d.out_features || d.residual_stride < d.out_features) return refuse("a row stride is smaller than the row");
-    if (d.x_stride > kMaxStride || d.y_stride > kMaxStride || d.residual_stride > kMaxStride) return refuse("a row stride is above 2^22");
+    if (d.x_stride > kMaxStride || d.y_stride > kMaxStride || d.residual_stride > kMaxStride) return refuse("a row stride is above 2^20");
     return NERF_STATUS_OK;
 }
 

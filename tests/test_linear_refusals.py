@@ -30,7 +30,7 @@ def bwd(d, x=A, w=A, g=A, z=A, a=A, dx=A, dz=A, dw=A, db=A, ws=A, nb=1 << 20):
 
 @pytest.mark.parametrize("change,word", [(dict(in_features=0), "features"), (dict(out_features=0), "features"), (dict(in_features=65537), "features"), (dict(out_features=1 << 31), "features"), (dict(rows=(1 << 30) + 1), "rows"),
                                          (dict(dtype=L.NERF_EXT_F32), "dtype"), (dict(dtype=3), "dtype"), (dict(out_dtype=L.NERF_EXT_BF16), "out_dtype"), (dict(activation=6), "activation"), (dict(x_stride=7), "stride"),
-                                         (dict(y_stride=15), "stride"), (dict(residual_stride=15), "stride"), (dict(x_stride=(1 << 22) + 1), "stride"), (dict(reserved=1), "reserved")])
+                                         (dict(y_stride=15), "stride"), (dict(residual_stride=15), "stride"), (dict(x_stride=(1 << 20) + 1), "stride"), (dict(reserved=1), "reserved")])
 def test_descriptors(lib, change, word):
     for call in (fwd, bwd):
         assert call(desc(**change)) == BAD
