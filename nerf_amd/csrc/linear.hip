@@ -275,33 +275,56 @@ __device__ __forceinline__ constexpr uint32_t chunk_slot(uint32_t line, uint32_t
     return line * (kT ? kB / 8u : 8u) + (chunk ^ chunk_key<kB, kT>(line));
 }
 
-// Tile [row0, row0 + kB) x [k0, k0 + 64) into LDS, zeros outside [0, n) x [0, nk):
-// through registers, any alignment.
+// Tile [row0, row0 + kB) x [k0, k0 + 64) into LDS, zeros outside [0, n) x [0, nk),
+// through registers and at any alignment: fetch() asks for a tile, keep() writes
+// it to LDS.
 template <typename T, uint32_t kB, bool kT, uint32_t kThreads>
-__device__ __forceinline__ void stage(const T* __restrict__ src, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end, uint4* lds) {
-    constexpr uint32_t kChunks = kT ? kB / 8u : 8u;
+struct Stager {
+    static constexpr uint32_t kChunks = kT ? kB / 8u : 8u;
+    static constexpr uint32_t kLoads  = (kB * 8u + kThreads - 1u) / kThreads;
+    uint4 held[kLoads];
+
+    __device__ __forceinline__ void fetch(const T* __restrict__ src, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) {
 #pragma unroll
-    for (uint32_t s = threadIdx.x; s < kB * 8u; s += kThreads) {
-        const uint32_t line = s / kChunks;
-        const uint32_t chunk = s % kChunks;
-        const uint32_t major = (kT ? k0 : row0) + line, minor = (kT ? row0 : k0) + 8u * chunk;
-        const uint32_t major_end = kT ? k_end : n, minor_end = kT ? n : k_end;
-        uint4 v = {0u, 0u, 0u, 0u};
-        if (major < major_end && minor < minor_end) {
-            const T* at = src + (uint64_t)major * ld + minor;
-            if (minor + 8u <= minor_end) {
-                __builtin_memcpy(&v, at, 16);
-            } else {
-                short8_t h = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            const uint32_t s = i * kThreads + threadIdx.x, line = s / kChunks, chunk = s % kChunks;
+            const uint32_t major = (kT ? k0 : row0) + line, minor = (kT ? row0 : k0) + 8u * chunk;
+            const uint32_t major_end = kT ? k_end : n, minor_end = kT ? n : k_end;
+            held[i] = uint4{0u, 0u, 0u, 0u};
+            if (s < kB * 8u && major < major_end && minor < minor_end) {
+                const T* line_at = src + (uint64_t)major * ld;
+                if (minor_end >= 8u) {
+                    // A chunk that the line's end cuts is fetched so that it ends there,
+                    // and moved down; what moves in is zero.
+                    const uint32_t over = minor + 8u > minor_end ? minor + 8u - minor_end : 0u;
+                    unsigned long long v[2];
+                    __builtin_memcpy(v, line_at + minor - over, 16);
+                    if (over >= 4u) {
+                        v[0] = v[1] >> (16u * (over - 4u));
+                        v[1] = 0ull;
+                    } else if (over) {
+                        v[0] = v[0] >> (16u * over) | v[1] << (64u - 16u * over);
+                        v[1] >>= 16u * over;
+                    }
+                    __builtin_memcpy(&held[i], v, 16);
+                } else {
+                    short8_t h = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                for (uint32_t j = 0; j < 7u; ++j)
-                    if (minor + j < minor_end) h[j] = __builtin_bit_cast(short, at[j]);
-                v = __builtin_bit_cast(uint4, h);
+                    for (uint32_t j = 0; j < 7u; ++j)
+                        if (minor + j < minor_end) h[j] = __builtin_bit_cast(short, line_at[minor + j]);
+                    held[i] = __builtin_bit_cast(uint4, h);
+                }
             }
         }
-        lds[chunk_slot<kB, kT>(line, chunk)] = v;
     }
-}
+    __device__ __forceinline__ void keep(uint4* lds) const {
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            const uint32_t s = i * kThreads + threadIdx.x;
+            if (kB * 8u % kThreads == 0u || s < kB * 8u) lds[chunk_slot<kB, kT>(s / kChunks, s % kChunks)] = held[i];
+        }
+    }
+};
 
 // The same straight from memory into LDS, 16 bytes a lane, for chunks that are
 // whole and aligned (start, stride and the contiguous length multiples of 8):
@@ -448,10 +471,19 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
             multiply(lds_p1, lds_q1);
         }
     } else {
+        // One pair of buffers; the next tile waits in registers meanwhile.
+        Stager<T, kBP, kPT, kThreads> stage_p;
+        Stager<T, kBQ, kQT, kThreads> stage_q;
+        stage_p.fetch((const T*)A.p, A.ldp, A.np, p0, k0, k_end);
+        stage_q.fetch((const T*)A.q, A.ldq, A.nq, q0, k0, k_end);
         for (uint32_t k = k0; k < k_end; k += kBK) {
-            stage<T, kBP, kPT, kThreads>((const T*)A.p, A.ldp, A.np, p0, k, k_end, lds_p0);
-            stage<T, kBQ, kQT, kThreads>((const T*)A.q, A.ldq, A.nq, q0, k, k_end, lds_q0);
+            stage_p.keep(lds_p0);
+            stage_q.keep(lds_q0);
             __syncthreads();
+            if (k + kBK < k_end) {
+                stage_p.fetch((const T*)A.p, A.ldp, A.np, p0, k + kBK, k_end);
+                stage_q.fetch((const T*)A.q, A.ldq, A.nq, q0, k + kBK, k_end);
+            }
             multiply(lds_p0, lds_q0);
             __syncthreads();
         }
@@ -504,35 +536,54 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     }
 }
 
-// Joins the parts of a sum that was split over k, in their order.
+// Joins the parts of a sum that was split over k: 16 slices of a workgroup take
+// every 16th part each, in order, and the slices are added in theirs, so the
+// result is the same every time.  (With one thread an output the reads of 128
+// parts of 256 x 256 sums, one after another, took 73 us.)
+constexpr uint32_t kSlices = 16u, kJoined = 256u / kSlices;
 template <typename Out>
 __global__ __launch_bounds__(256) void k_join(const float* __restrict__ parts, uint64_t part, uint32_t count, const float* __restrict__ sums, float* __restrict__ row_sums, Out out) {
-    const uint32_t eights = (out.np + 7u) / 8u;
-    const uint64_t total = (uint64_t)eights * out.nq, step = (uint64_t)gridDim.x * blockDim.x, first = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const bool vec = out.np % 4u == 0u;
-    for (uint64_t at = first; at < total; at += step) {
-        const uint32_t q = (uint32_t)(at / eights), p = 8u * (uint32_t)(at % eights), n = min(8u, out.np - p);
-        // The epilogues count rows from a uniform one: the first that the
-        // workgroup's threads have in this turn.
-        const uint32_t q0 = (uint32_t)((at - threadIdx.x) / eights);
-        const typename Out::Aux aux = out.load(q0, q - q0, p, n);
+    __shared__ floatx4 slice_sum[2][kSlices][kJoined];
+    const uint32_t eights = (out.np + 7u) / 8u, slice = threadIdx.x / kJoined, mine = threadIdx.x % kJoined;
+    const uint64_t total = (uint64_t)eights * out.nq;
+    const bool vec = out.np % 8u == 0u;
+    for (uint64_t base = (uint64_t)blockIdx.x * kJoined; base < total; base += (uint64_t)gridDim.x * kJoined) {
+        const uint64_t at = base + mine;
+        const uint32_t q = (uint32_t)(at / eights), p = 8u * (uint32_t)(at % eights), n = at < total ? min(8u, out.np - p) : 0u;
         floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t c = 0; c < count; ++c) {
-            const float* src = parts + c * part + (uint64_t)q * out.np + p;
-            if (vec && n == 8u) {
-                v.lo += reinterpret_cast<const floatx4*>(src)[0];
-                v.hi += reinterpret_cast<const floatx4*>(src)[1];
-            } else {
+        if (n) {
+#pragma unroll 4
+            for (uint32_t c = slice; c < count; c += kSlices) {
+                const float* src = parts + c * part + (uint64_t)q * out.np + p;
+                if (vec) {
+                    v.lo += reinterpret_cast<const floatx4*>(src)[0];
+                    v.hi += reinterpret_cast<const floatx4*>(src)[1];
+                } else {
 #pragma unroll
-                for (uint32_t r = 0; r < 8u; ++r)
-                    if (r < n) v[r] += src[r];
+                    for (uint32_t r = 0; r < 8u; ++r) v[r] += r < n ? src[r] : 0.0f;
+                }
             }
         }
-        out.put(q0, q - q0, p, n, v, aux);
+        __syncthreads();
+        slice_sum[0][slice][mine] = v.lo;
+        slice_sum[1][slice][mine] = v.hi;
+        __syncthreads();
+        if (slice == 0u) {
+            // The epilogues count rows from a uniform one: the workgroup's first.
+            const uint32_t q0 = (uint32_t)(base / eights);
+            const typename Out::Aux aux = out.load(q0, q - q0, p, n);
+#pragma unroll
+            for (uint32_t c = 1; c < kSlices; ++c) {
+                v.lo += slice_sum[0][c][mine];
+                v.hi += slice_sum[1][c][mine];
+            }
+            out.put(q0, q - q0, p, n, v, aux);
+        }
     }
     if (row_sums) {
-        for (uint64_t q = first; q < out.nq; q += step) {
+        for (uint32_t q = blockIdx.x * 256u + threadIdx.x; q < out.nq; q += gridDim.x * 256u) {
             float s = 0.0f;
+#pragma unroll 8
             for (uint32_t c = 0; c < count; ++c) s += sums[(uint64_t)c * out.nq + q];
             row_sums[q] = s;
         }
@@ -556,11 +607,13 @@ bool whole_chunks(const void* p, uint64_t ld, uint32_t contiguous) { return alig
 template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, bool kPT, bool kQT, bool kAligned, bool kSplit = true, typename Out>
 hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipStream_t stream) {
     const uint32_t tp = ceil_div(A.np, kBP), tq = ceil_div(A.nq, kBQ);
-    // Split over k until every CU has two workgroups, with four tiles of k a
-    // part at least, as far as the workspace holds the parts.
+    // Split over k until every CU has its workgroups (two; one of the widest
+    // tile, whose buffers take the LDS of a CU), with four tiles of k a part at
+    // least, as far as the workspace holds the parts.
     const uint64_t part = (uint64_t)A.np * A.nq;
     const uint64_t per = 4u * (part + (row_sums ? A.nq : 0u));
-    uint64_t splits = kSplit ? (2ull * device_cu_count()) / ((uint64_t)tp * tq) : 1u;
+    const uint64_t fill = (kBP == 256u ? 1u : 2u) * device_cu_count();
+    uint64_t splits = kSplit ? fill / ((uint64_t)tp * tq) : 1u;
     splits = std::min<uint64_t>({splits, ceil_div(A.nk, 4u * kBK), ws.data ? ws.bytes / per : 0u, 65535u});
     const bool split = splits > 1u;
     if (!split) splits = 1u;
@@ -577,7 +630,7 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
             const uint64_t eights = (uint64_t)ceil_div(A.np, 8u) * A.nq;
-            k_join<Out><<<(uint32_t)std::min<uint64_t>(ceil_div(eights, 256u), 4096u), 256, 0, stream>>>(ws.data, part, parts, sums, row_sums, out);
+            k_join<Out><<<(uint32_t)std::min<uint64_t>(ceil_div(eights, kJoined), 4096u), 256, 0, stream>>>(ws.data, part, parts, sums, row_sums, out);
             return hipGetLastError();
         }
     }
@@ -587,9 +640,12 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
 
 template <typename T, bool kPT, bool kQT, typename Out>
 hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hipStream_t stream) {
-    if (!whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, kQT ? A.nq : A.nk)) return launch_tiles<T, 64, 64, 2, 2, kPT, kQT, false>(A, out, row_sums, ws, stream);
     const uint32_t cus = device_cu_count();
-    if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) >= cus / 2u && A.np > 128u && A.nk >= 512u) return launch_tiles<T, 256, 256, 2, 4, kPT, kQT, true, false>(A, out, row_sums, ws, stream);
+    if (!whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, kQT ? A.nq : A.nk)) {
+        if ((uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u) >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u)) return launch_tiles<T, 128, 128, 2, 2, kPT, kQT, false>(A, out, row_sums, ws, stream);
+        return launch_tiles<T, 64, 64, 2, 2, kPT, kQT, false>(A, out, row_sums, ws, stream);
+    }
+    if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) * (kPT && kQT ? ceil_div(A.nk, 1024u) : 1u) >= cus / 2u && A.np > 128u && A.nk >= 512u) return launch_tiles<T, 256, 256, 2, 4, kPT, kQT, true, kPT && kQT>(A, out, row_sums, ws, stream);
     if ((uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u) >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u)) return launch_tiles<T, 128, 128, 2, 2, kPT, kQT, true>(A, out, row_sums, ws, stream);
     return launch_tiles<T, 64, 64, 2, 2, kPT, kQT, true>(A, out, row_sums, ws, stream);
 }

@@ -21,6 +21,7 @@ typedef __bf16 bf16_t;
 
 constexpr uint32_t kThreads  = 256u;
 constexpr uint32_t kPiece    = 4096u;  // elements of a workgroup's turn
+constexpr uint32_t kTurns    = kPiece / (8u * kThreads);
 constexpr uint32_t kMaxParts = NERF_EXT_NORM_WORKSPACE / sizeof(double);
 
 // Kernel arguments are kept below 4 KiB.
@@ -28,10 +29,10 @@ constexpr uint32_t kNormListed = 128u, kAdamListed = 64u;
 struct NormList {
     const void* data[kNormListed];
     void* out[kNormListed];
-    uint64_t count[kNormListed];
-    uint32_t first[kNormListed];  // pieces before the tensor's
+    uint32_t first[kNormListed + 1u];  // pieces before the tensor's; all pieces behind the last
+    uint16_t tail[kNormListed];        // elements of its last piece
     uint8_t dtype[kNormListed];
-    uint32_t tensors, pieces;
+    uint32_t tensors, pieces, share;
 };
 struct AdamList {
     float* param[kAdamListed];
@@ -39,32 +40,60 @@ struct AdamList {
     float* m[kAdamListed];
     float* v[kAdamListed];
     void* copy[kAdamListed];
-    uint64_t count[kAdamListed];
-    uint32_t first[kAdamListed];
+    uint32_t first[kAdamListed + 1u];
+    uint16_t tail[kAdamListed];
     uint8_t dtype[kAdamListed];
-    uint32_t tensors, pieces;
+    uint32_t tensors, pieces, share;
 };
 
-template <typename List>
-__device__ __forceinline__ uint32_t tensor_of(const List& l, uint32_t piece) {
-    uint32_t lo = 0u, hi = l.tensors - 1u;
+// Workgroup b of a launch has pieces b * share and on, `share` of them, in their
+// order.  f(tensor, first element, elements).  Counts are 32-bit words: of a
+// select between 64-bit lengths (the piece's end or the tensor's) the compiler
+// kept the wrong condition here and let workgroups run past a tensor's end.
+template <typename List, typename F>
+__device__ __forceinline__ void each_piece(const List& l, F&& f) {
+    const uint32_t begin = blockIdx.x * l.share, end = min(begin + l.share, l.pieces);
+    if (begin >= end) return;
+    uint32_t lo = 0u, hi = l.tensors - 1u;  // the tensor of piece `begin`
     while (lo < hi) {
         const uint32_t mid = (lo + hi + 1u) / 2u;
-        if (l.first[mid] <= piece) lo = mid;
+        if (l.first[mid] <= begin) lo = mid;
         else hi = mid - 1u;
     }
-    return lo;
+    uint32_t t = lo;
+    for (uint32_t piece = begin; piece < end; ++piece) {
+        if (piece == l.first[t + 1u]) ++t;
+        f(t, (uint64_t)(piece - l.first[t]) * kPiece, piece + 1u == l.first[t + 1u] ? l.tail[t] : kPiece);
+    }
 }
 
-__device__ __forceinline__ float load_as_f32(const void* p, uint64_t i, uint32_t dtype) {
-    if (dtype == NERF_EXT_F32) return ((const float*)p)[i];
-    if (dtype == NERF_EXT_F16) return (float)((const half_t*)p)[i];
-    return (float)((const bf16_t*)p)[i];
+typedef float floatx8 __attribute__((ext_vector_type(8)));
+template <typename E>
+struct Eight {
+    typedef E type __attribute__((ext_vector_type(8)));
+};
+
+// Eight elements as 32-bit values, and back with one rounding.  Arrays are
+// aligned to their elements; the hardware serves wide accesses at any such
+// address.
+template <typename E>
+__device__ __forceinline__ floatx8 load8(const E* p) {
+    typename Eight<E>::type v;
+    __builtin_memcpy(&v, p, sizeof(v));
+    return __builtin_convertvector(v, floatx8);
 }
-__device__ __forceinline__ void store_rounded(void* p, uint64_t i, uint32_t dtype, float v) {
-    if (dtype == NERF_EXT_F32) ((float*)p)[i] = v;
-    else if (dtype == NERF_EXT_F16) ((half_t*)p)[i] = (half_t)v;
-    else ((bf16_t*)p)[i] = (bf16_t)v;
+template <typename E>
+__device__ __forceinline__ void store8(E* p, const floatx8& v) {
+    const typename Eight<E>::type h = __builtin_convertvector(v, typename Eight<E>::type);
+    __builtin_memcpy(p, &h, sizeof(h));
+}
+
+// f(pointer type tag) for an element type.
+template <typename F>
+__device__ __forceinline__ void with_type(uint32_t dtype, F&& f) {
+    if (dtype == NERF_EXT_F32) f((float*)nullptr);
+    else if (dtype == NERF_EXT_F16) f((half_t*)nullptr);
+    else f((bf16_t*)nullptr);
 }
 
 // Sum over the workgroup, in thread 0.
@@ -82,15 +111,26 @@ __device__ __forceinline__ double block_sum(double v) {
 // parts[b] = sum of the squares of workgroup b's pieces.
 __global__ __launch_bounds__(kThreads) void k_square_sums(NormList l, double* __restrict__ parts) {
     double s = 0.0;
-    for (uint32_t piece = blockIdx.x; piece < l.pieces; piece += gridDim.x) {
-        const uint32_t t     = tensor_of(l, piece);
-        const uint64_t first = (uint64_t)(piece - l.first[t]) * kPiece;
-        const uint64_t end   = min(first + kPiece, l.count[t]);
-        for (uint64_t i = first + threadIdx.x; i < end; i += kThreads) {
-            const double g = (double)load_as_f32(l.data[t], i, l.dtype[t]);
-            s += g * g;
-        }
-    }
+    each_piece(l, [&](uint32_t t, uint64_t first, uint32_t n) {
+        with_type(l.dtype[t], [&](auto* tag) {
+            using E       = std::remove_pointer_t<decltype(tag)>;
+            const E* data = (const E*)l.data[t] + first;
+            if (n == kPiece) {
+                floatx8 g[kTurns];
+#pragma unroll
+                for (uint32_t k = 0; k < kTurns; ++k) g[k] = load8(data + 8u * (k * kThreads + threadIdx.x));
+#pragma unroll
+                for (uint32_t k = 0; k < kTurns; ++k)
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) s += (double)g[k][r] * (double)g[k][r];
+            } else {
+                for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+                    const double g = (double)(float)data[i];
+                    s += g * g;
+                }
+            }
+        });
+    });
     s = block_sum(s);
     if (threadIdx.x == 0u) parts[blockIdx.x] = s;
 }
@@ -115,12 +155,22 @@ __global__ __launch_bounds__(kThreads) void k_clip(NormList l, const double* __r
     const float v      = norm_of(parts, n);
     const float factor = v > max_norm && isfinite(v) ? max_norm / v : 1.0f;
     if (blockIdx.x == 0u && threadIdx.x == 0u) *norm = v;
-    for (uint32_t piece = blockIdx.x; piece < l.pieces; piece += gridDim.x) {
-        const uint32_t t     = tensor_of(l, piece);
-        const uint64_t first = (uint64_t)(piece - l.first[t]) * kPiece;
-        const uint64_t end   = min(first + kPiece, l.count[t]);
-        for (uint64_t i = first + threadIdx.x; i < end; i += kThreads) store_rounded(l.out[t], i, l.dtype[t], load_as_f32(l.data[t], i, l.dtype[t]) * factor);
-    }
+    each_piece(l, [&](uint32_t t, uint64_t first, uint32_t n) {
+        with_type(l.dtype[t], [&](auto* tag) {
+            using E       = std::remove_pointer_t<decltype(tag)>;
+            const E* data = (const E*)l.data[t] + first;
+            E* out        = (E*)l.out[t] + first;
+            if (n == kPiece) {
+                floatx8 g[kTurns];
+#pragma unroll
+                for (uint32_t k = 0; k < kTurns; ++k) g[k] = load8(data + 8u * (k * kThreads + threadIdx.x));
+#pragma unroll
+                for (uint32_t k = 0; k < kTurns; ++k) store8(out + 8u * (k * kThreads + threadIdx.x), g[k] * factor);
+            } else {
+                for (uint32_t i = threadIdx.x; i < n; i += kThreads) out[i] = (E)((float)data[i] * factor);
+            }
+        });
+    });
 }
 
 struct AdamRule {
@@ -133,21 +183,48 @@ __global__ __launch_bounds__(kThreads) void k_adam_tensors(AdamList l, AdamRule 
     if (skipped && blockIdx.x == 0u && threadIdx.x == 0u) *skipped = skip ? 1u : 0u;
     if (skip) return;
     const float gs = (gn > r.clip && gn > 0.0f ? r.clip / gn : 1.0f) * (1.0f / r.loss_scale);
-    for (uint32_t piece = blockIdx.x; piece < l.pieces; piece += gridDim.x) {
-        const uint32_t t     = tensor_of(l, piece);
-        const uint64_t first = (uint64_t)(piece - l.first[t]) * kPiece;
-        const uint64_t end   = min(first + kPiece, l.count[t]);
-        for (uint64_t i = first + threadIdx.x; i < end; i += kThreads) {
-            const float g = l.grad[t][i] * gs;
-            const float m = r.beta1 * l.m[t][i] + (1.0f - r.beta1) * g;
-            const float v = r.beta2 * l.v[t][i] + (1.0f - r.beta2) * g * g;
-            const float p = l.param[t][i] - r.lr * (m * r.bc1) / (sqrtf(v * r.bc2) + r.eps);
-            l.m[t][i]     = m;
-            l.v[t][i]     = v;
-            l.param[t][i] = p;
-            if (l.copy[t]) store_rounded(l.copy[t], i, l.dtype[t], p);
+    each_piece(l, [&](uint32_t t, uint64_t first, uint32_t n) {
+        float *param = l.param[t] + first, *ms = l.m[t] + first, *vs = l.v[t] + first;
+        const float* grad = l.grad[t] + first;
+        void* copy        = l.copy[t];
+        const auto one = [&](float& p, float g, float& m, float& v) {
+            g *= gs;
+            m = r.beta1 * m + (1.0f - r.beta1) * g;
+            v = r.beta2 * v + (1.0f - r.beta2) * g * g;
+            p = p - r.lr * (m * r.bc1) / (sqrtf(v * r.bc2) + r.eps);
+        };
+        if (n == kPiece) {
+#pragma unroll
+            for (uint32_t k = 0; k < kTurns; ++k) {
+                const uint32_t i = 8u * (k * kThreads + threadIdx.x);
+                floatx8 p = load8(param + i), m = load8(ms + i), v = load8(vs + i);
+                const floatx8 g = load8(grad + i);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float pe = p[e], me = m[e], ve = v[e];
+                    one(pe, g[e], me, ve);
+                    p[e] = pe;
+                    m[e] = me;
+                    v[e] = ve;
+                }
+                store8(param + i, p);
+                store8(ms + i, m);
+                store8(vs + i, v);
+                if (copy && l.dtype[t] == NERF_EXT_F16) store8((half_t*)copy + first + i, p);
+                else if (copy) store8((bf16_t*)copy + first + i, p);
+            }
+        } else {
+            for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+                float p = param[i], m = ms[i], v = vs[i];
+                one(p, grad[i], m, v);
+                param[i] = p;
+                ms[i]    = m;
+                vs[i]    = v;
+                if (copy && l.dtype[t] == NERF_EXT_F16) ((half_t*)copy)[first + i] = (half_t)p;
+                else if (copy) ((bf16_t*)copy)[first + i] = (bf16_t)p;
+            }
         }
-    }
+    });
 }
 
 // ------------------------------------------------------------------- host
@@ -159,7 +236,8 @@ NerfStatus refuse(const char* fn, const char* why) {
     return NERF_STATUS_INVALID_USAGE;
 }
 
-// Pieces of a list (128 tensors at most) fit 32 bits: 2^24 each.
+// Pieces of a list (128 tensors at most) fit 32 bits: 2^24 each, and so does
+// their number rounded up to whole shares.
 constexpr uint64_t kMaxCount   = (uint64_t)kPiece << 24;
 constexpr uint32_t kMaxTensors = 1u << 20;                // a list has a part at least
 
@@ -179,25 +257,26 @@ NerfStatus check_grads(const char* fn, const NerfExtGradTensor* tensors, uint32_
     return NERF_STATUS_OK;
 }
 
-// f(list) for the tensors in lists of at most the arguments' size; empty
-// tensors are left out.  f also gets each list's number.
+// f(list, workgroups) for the tensors, in lists of at most the arguments' size
+// and with at most `most` workgroups a list; empty tensors are left out.
 template <typename List, uint32_t kListed, typename Tensor, typename Put, typename F>
-hipError_t each_list(const Tensor* tensors, uint32_t count, Put&& put, F&& f) {
-    uint32_t number = 0u;
+hipError_t each_list(const Tensor* tensors, uint32_t count, uint32_t most, Put&& put, F&& f) {
     for (uint32_t at = 0; at < count;) {
         List l;
         l.tensors = l.pieces = 0u;
         for (; at < count && l.tensors < kListed; ++at) {
-            if (tensors[at].count == 0u) continue;
-            const uint64_t pieces = (tensors[at].count + kPiece - 1u) / kPiece;
-            l.count[l.tensors] = tensors[at].count;
+            const uint64_t n = tensors[at].count;
+            if (n == 0u) continue;
             l.first[l.tensors] = l.pieces;
+            l.tail[l.tensors]  = (uint16_t)((n - 1u) % kPiece + 1u);
             put(l, l.tensors, tensors[at]);
-            l.pieces += (uint32_t)pieces;
+            l.pieces += (uint32_t)((n + kPiece - 1u) / kPiece);
             ++l.tensors;
         }
         if (l.tensors == 0u) break;
-        const hipError_t e = f(l, number++);
+        l.first[l.tensors] = l.pieces;
+        l.share            = (l.pieces + most - 1u) / most;
+        const hipError_t e = f(l, (l.pieces + l.share - 1u) / l.share);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -214,8 +293,7 @@ hipError_t square_sums(const NerfExtGradTensor* tensors, uint32_t count, double*
     const uint32_t lists = (count + kNormListed - 1u) / kNormListed;
     const uint32_t most  = std::max(1u, std::min(4u * device_cu_count(), kMaxParts / std::max(1u, lists)));
     *n = 0u;
-    return each_list<NormList, kNormListed>(tensors, count, put_grad, [&](const NormList& l, uint32_t) {
-        const uint32_t blocks = std::min(l.pieces, most);
+    return each_list<NormList, kNormListed>(tensors, count, most, put_grad, [&](const NormList& l, uint32_t blocks) {
         k_square_sums<<<blocks, kThreads, 0, stream>>>(l, parts + *n);
         *n += blocks;
         return hipGetLastError();
@@ -247,8 +325,8 @@ NERF_API NerfStatus nerf_ext_grad_clip(const NerfExtGradTensor* tensors, uint32_
         NERF_LAUNCH_CHECK("k_norm");
         return NERF_STATUS_OK;
     }
-    NERF_HIP_TRY((each_list<NormList, kNormListed>(tensors, count, put_grad, [&](const NormList& l, uint32_t) {
-        k_clip<<<std::min(l.pieces, 8u * device_cu_count()), kThreads, 0, (hipStream_t)stream>>>(l, (const double*)workspace, n, max_norm, norm);
+    NERF_HIP_TRY((each_list<NormList, kNormListed>(tensors, count, 8u * device_cu_count(), put_grad, [&](const NormList& l, uint32_t blocks) {
+        k_clip<<<blocks, kThreads, 0, (hipStream_t)stream>>>(l, (const double*)workspace, n, max_norm, norm);
         return hipGetLastError();
     })));
     return NERF_STATUS_OK;
@@ -283,8 +361,9 @@ NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_
     r.clip       = hyper->grad_clip_norm;
     r.guard      = hyper->update_guard_grad_norm;
     r.loss_scale = hyper->loss_scale;
+    bool first = true;
     NERF_HIP_TRY((each_list<AdamList, kAdamListed>(
-        tensors, count,
+        tensors, count, 8u * device_cu_count(),
         [](AdamList& l, uint32_t i, const NerfExtAdamTensor& t) {
             l.param[i] = t.param;
             l.grad[i]  = t.grad;
@@ -293,8 +372,9 @@ NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_
             l.copy[i]  = t.copy;
             l.dtype[i] = (uint8_t)t.copy_dtype;
         },
-        [&](const AdamList& l, uint32_t number) {
-            k_adam_tensors<<<std::min(l.pieces, 8u * device_cu_count()), kThreads, 0, (hipStream_t)stream>>>(l, r, grad_norm, number == 0u ? skipped : nullptr);
+        [&](const AdamList& l, uint32_t blocks) {
+            k_adam_tensors<<<blocks, kThreads, 0, (hipStream_t)stream>>>(l, r, grad_norm, first ? skipped : nullptr);
+            first = false;
             return hipGetLastError();
         })));
     return NERF_STATUS_OK;
