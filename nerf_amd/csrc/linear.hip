@@ -240,8 +240,9 @@ struct InputGradientOut {
 
 // Plain sums in 32 bits: dW, or one part of a sum that was split over k.
 struct SumOut {
-    float* out;
-    uint64_t part;    // elements from one part to the next
+    float* out;       // the first part, or all of it
+    float* parts;     // the others
+    uint64_t part;    // elements from one of them to the next
     float* row_sums;  // sum_k Q(q, k), or null; nq of them a part
     uint32_t np, nq;
     bool vec;
@@ -262,13 +263,19 @@ struct Operands {
 };
 
 // A tile of kB rows x 64 k lies in LDS in 16-byte chunks of 8 values, the
-// chunk's place xor-ed with bits of its row so that the lanes of one read
-// fall on different banks: k contiguous, row-major [kB][64], the 8 rows of a
-// read's lanes in 8 different places; kT (row contiguous), k-major [64][kB],
-// the four k of a transposing read 32 bytes apart.
+// chunk's place xor-ed with bits of its line so that the lanes that the LDS
+// serves together fall on different banks.  k contiguous: row-major [kB][64],
+// 8 lanes a turn, the 8 rows in 8 different places.  kT (row contiguous):
+// k-major [64][kB]; 32 lanes of a transposing read are served together, k 0..3
+// and 8..11 of 32 bytes each, which go to the 8 different places of 256 bytes
+// (with kB = 64 the line's parity is one of the place's bits already).  With
+// both groups of four k in the same four places half of the LDS' cycles were
+// conflicts.
 template <uint32_t kB, bool kT>
 __device__ __forceinline__ constexpr uint32_t chunk_key(uint32_t line) {
-    return kT ? (line & 3u) << 1 : line & 7u;
+    if (!kT) return line & 7u;
+    if (kB >= 128u) return ((line & 3u) | ((line >> 3) & 1u) << 2) << 1;
+    return (((line >> 1) & 1u) | ((line >> 3) & 1u) << 1) << 1;
 }
 template <uint32_t kB, bool kT>
 __device__ __forceinline__ constexpr uint32_t chunk_slot(uint32_t line, uint32_t chunk) {
@@ -368,23 +375,29 @@ struct Loader {
     }
 };
 
-// The 8 k of rows [row0, row0 + 16) that a lane feeds to one 16x16x32 matrix
-// instruction: k = 32 step + 8 (lane / 16) + 0..7 of row row0 + lane % 16.
+// The 8 k of 16 rows that a lane feeds to one 16x16x32 matrix instruction:
+// k = 32 step + 8 (lane / 16) + 0..7 of row wave0 + 16 i + lane % 16.  A lane
+// keeps one place in a tile (fragment_base: i = step = 0); the others differ
+// from it by constants and by single bits, which are put in as they are used
+// (held in registers, the places of all fragments left too few for the sums).
+template <uint32_t kB, bool kT>
+__device__ __forceinline__ uint32_t fragment_base(uint32_t wave0) {
+    const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, g = lane >> 4;
+    if (!kT) return 16u * chunk_slot<kB, false>(wave0 + l, g);
+    const uint32_t row = wave0 + 4u * (l & 3u);
+    return 16u * chunk_slot<kB, true>(8u * g + (l >> 2), row >> 3) + 2u * (row & 7u);
+}
 template <typename T, uint32_t kB, bool kT>
-__device__ __forceinline__ typename Vec<T>::x8 fragment(const uint4* lds, uint32_t row0, uint32_t step) {
-    const uint32_t lane = threadIdx.x & 63u, i = lane & 15u, g = lane >> 4;
+__device__ __forceinline__ typename Vec<T>::x8 fragment(const uint4* lds, uint32_t base, uint32_t i, uint32_t step) {
+    const char* tile = reinterpret_cast<const char*>(lds);
     if constexpr (!kT) {
-        return __builtin_bit_cast(typename Vec<T>::x8, lds[chunk_slot<kB, false>(row0 + i, 4u * step + g)]);
+        return *reinterpret_cast<const typename Vec<T>::x8*>(tile + (base ^ (64u * step)) + 2048u * i);
     } else {
-        // Lane 4 r + c of 16 reads rows row0 + 4 c .. + 3 at k = r; the read hands
-        // lane i the four k of row row0 + i.
+        // Lane 4 r + c of 16 reads rows 4 c .. 4 c + 3 at k = r; the read hands lane
+        // l the four k of row l.
         short4_t h[2];
 #pragma unroll
-        for (uint32_t half = 0; half < 2u; ++half) {
-            const uint32_t k = 32u * step + 8u * g + 4u * half + (i >> 2), row = row0 + 4u * (i & 3u);
-            const char* at = reinterpret_cast<const char*>(lds) + 16u * chunk_slot<kB, true>(k, row >> 3) + 2u * (row & 7u);
-            h[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(at));
-        }
+        for (uint32_t half = 0; half < 2u; ++half) h[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(tile + (base ^ (32u * i)) + 2u * kB * (32u * step + 4u * half)));
         return __builtin_bit_cast(typename Vec<T>::x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }
@@ -406,43 +419,69 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     // Variables of their own, so that the compiler sees that a read of one is no
     // read of what is on its way into another.
     __shared__ uint4 lds_p0[kBP * 8u], lds_q0[kBQ * 8u], lds_p1[kAligned ? kBP * 8u : 1u], lds_q1[kAligned ? kBQ * 8u : 1u];
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t wp = (wave % kWP) * (kBP / kWP), wq = (wave / kWP) * (kBQ / kWQ);
     const uint32_t p0 = blockIdx.x * kBP, q0 = blockIdx.y * kBQ;
     const uint32_t k0 = blockIdx.z * A.k_split, k_end = min(A.nk, k0 + A.k_split);
 
-    floatx4 acc[kFP][kFQ], sums[kFQ];
+    // Sums of Q over k, for out.row_sums: a product with ones, the fragments of Q
+    // shared out among the waves that hold the same.
+    constexpr bool kSums = std::is_same_v<Out, SumOut>;
+    constexpr uint32_t kSumsQ = kSums ? kFQ / kWP : 1u;
+    floatx4 acc[kFP][kFQ], sums[kSumsQ];
+#pragma unroll
+    for (uint32_t j = 0; j < kSumsQ; ++j) sums[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (uint32_t j = 0; j < kFQ; ++j) {
-        sums[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t i = 0; i < kFP; ++i) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     bool take_sums = false;
-    if constexpr (std::is_same_v<Out, SumOut>) take_sums = out.row_sums && blockIdx.x == 0u && wp == 0u;
+    if constexpr (kSums) take_sums = out.row_sums && blockIdx.x == 0u;
     typename Vec<T>::x8 ones;
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = (T)1.0f;
 
+    const uint32_t base_p = fragment_base<kBP, kPT>(wp), base_q = fragment_base<kBQ, kQT>(wq);
+    // One tile of 64 k: kG fragments of P against all of Q at a time, the next
+    // fragments on their way from LDS meanwhile.
+    constexpr uint32_t kG = kFP < 2u ? 1u : 2u, kPhases = kFP / kG;
     auto multiply = [&](const uint4* lp, const uint4* lq) {
+        typename Vec<T>::x8 fp[2][kG], fq[2][kFQ];
+        uint32_t bp = base_p, bq = base_q;
+        asm volatile("" : "+v"(bp), "+v"(bq));
+        auto fetch_p = [&](uint32_t phase) {
 #pragma unroll
-        for (uint32_t step = 0; step < 2u; ++step) {
-            typename Vec<T>::x8 fp[kFP], fq[kFQ];
+            for (uint32_t g = 0; g < kG; ++g) fp[phase & 1u][g] = fragment<T, kBP, kPT>(lp, bp, phase % kPhases * kG + g, phase / kPhases);
+        };
+        auto fetch_q = [&](uint32_t step) {
 #pragma unroll
-            for (uint32_t i = 0; i < kFP; ++i) fp[i] = fragment<T, kBP, kPT>(lp, wp + 16u * i, step);
+            for (uint32_t j = 0; j < kFQ; ++j) fq[step][j] = fragment<T, kBQ, kQT>(lq, bq, j, step);
+        };
+        fetch_q(0u);
+        fetch_p(0u);
 #pragma unroll
-            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = fragment<T, kBQ, kQT>(lq, wq + 16u * j, step);
+        for (uint32_t phase = 0; phase < 2u * kPhases; ++phase) {
+            const uint32_t step = phase / kPhases;
+            if (phase + 1u < 2u * kPhases) {
+                if ((phase + 1u) % kPhases == 0u) fetch_q(step + 1u);
+                fetch_p(phase + 1u);
+            }
 #pragma unroll
-            for (uint32_t i = 0; i < kFP; ++i)
+            for (uint32_t g = 0; g < kG; ++g)
 #pragma unroll
-                for (uint32_t j = 0; j < kFQ; ++j) acc[i][j] = Vec<T>::mfma(fp[i], fq[j], acc[i][j]);
-            if constexpr (std::is_same_v<Out, SumOut>) {
-                if (take_sums) {
+                for (uint32_t j = 0; j < kFQ; ++j) acc[phase % kPhases * kG + g][j] = Vec<T>::mfma(fp[phase & 1u][g], fq[step][j], acc[phase % kPhases * kG + g][j]);
+            if constexpr (kSums) {
+                if (take_sums && phase % kPhases == 0u) {
 #pragma unroll
-                    for (uint32_t j = 0; j < kFQ; ++j) sums[j] = Vec<T>::mfma(ones, fq[j], sums[j]);
+                    for (uint32_t c = 0; c < kWP; ++c)
+                        if (wave % kWP == c) {
+#pragma unroll
+                            for (uint32_t j = 0; j < kSumsQ; ++j) sums[j] = Vec<T>::mfma(ones, fq[step][c * kSumsQ + j], sums[j]);
+                        }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);  // the fragments of one step at a time in registers
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
@@ -490,11 +529,11 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     }
 
     if constexpr (std::is_same_v<Out, SumOut>) {
-        out.out += blockIdx.z * out.part;
+        if (blockIdx.z) out.out = out.parts + (blockIdx.z - 1u) * out.part;
         if (take_sums && lane < 16u) {  // every p of the product with ones holds the sum
 #pragma unroll
-            for (uint32_t j = 0; j < kFQ; ++j) {
-                const uint32_t q = q0 + wq + 16u * j + lane;
+            for (uint32_t j = 0; j < kSumsQ; ++j) {
+                const uint32_t q = q0 + wq + 16u * (wave % kWP * kSumsQ + j) + lane;
                 if (q < out.nq) out.row_sums[(uint64_t)blockIdx.z * out.nq + q] = sums[j][0];
             }
         }
@@ -542,11 +581,11 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
 // parts of 256 x 256 sums, one after another, took 73 us.)
 constexpr uint32_t kSlices = 16u, kJoined = 256u / kSlices;
 template <typename Out>
-__global__ __launch_bounds__(256) void k_join(const float* __restrict__ parts, uint64_t part, uint32_t count, const float* __restrict__ sums, float* __restrict__ row_sums, Out out) {
+__global__ __launch_bounds__(256) void k_join(const float* first_part, const float* __restrict__ parts, uint64_t part, uint32_t count, const float* __restrict__ sums, float* __restrict__ row_sums, Out out) {
     __shared__ floatx4 slice_sum[2][kSlices][kJoined];
     const uint32_t eights = (out.np + 7u) / 8u, slice = threadIdx.x / kJoined, mine = threadIdx.x % kJoined;
     const uint64_t total = (uint64_t)eights * out.nq;
-    const bool vec = out.np % 8u == 0u;
+    const bool vec = out.np % 8u == 0u && ((uintptr_t)first_part & 15u) == 0u;
     for (uint64_t base = (uint64_t)blockIdx.x * kJoined; base < total; base += (uint64_t)gridDim.x * kJoined) {
         const uint64_t at = base + mine;
         const uint32_t q = (uint32_t)(at / eights), p = 8u * (uint32_t)(at % eights), n = at < total ? min(8u, out.np - p) : 0u;
@@ -554,7 +593,7 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ parts, u
         if (n) {
 #pragma unroll 4
             for (uint32_t c = slice; c < count; c += kSlices) {
-                const float* src = parts + c * part + (uint64_t)q * out.np + p;
+                const float* src = (c ? parts + (c - 1u) * part : first_part) + (uint64_t)q * out.np + p;
                 if (vec) {
                     v.lo += reinterpret_cast<const floatx4*>(src)[0];
                     v.hi += reinterpret_cast<const floatx4*>(src)[1];
@@ -610,11 +649,13 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
     // Split over k until every CU has its workgroups (two; one of the widest
     // tile, whose buffers take the LDS of a CU), with four tiles of k a part at
     // least, as far as the workspace holds the parts.
-    const uint64_t part = (uint64_t)A.np * A.nq;
-    const uint64_t per = 4u * (part + (row_sums ? A.nq : 0u));
+    // The first part of a plain sum is kept where the sum will be.
+    const uint64_t part = (uint64_t)A.np * A.nq, words = ws.bytes / 4u;
+    constexpr bool kSums = std::is_same_v<Out, SumOut>;
+    const uint64_t held = kSums ? (words + part) / (part + (row_sums ? A.nq : 0u)) : words / part;
     const uint64_t fill = (kBP == 256u ? 1u : 2u) * device_cu_count();
     uint64_t splits = kSplit ? fill / ((uint64_t)tp * tq) : 1u;
-    splits = std::min<uint64_t>({splits, ceil_div(A.nk, 4u * kBK), ws.data ? ws.bytes / per : 0u, 65535u});
+    splits = std::min<uint64_t>({splits, ceil_div(A.nk, 4u * kBK), held, 65535u});
     const bool split = splits > 1u;
     if (!split) splits = 1u;
     A.k_split = ceil_div(ceil_div(A.nk, kBK), splits) * kBK;
@@ -624,13 +665,26 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
     constexpr uint32_t kThreads = kWP * kWQ * 64u;
     if constexpr (kSplit) {
         if (parts > 1u) {
-            float* sums = row_sums ? ws.data + parts * part : nullptr;
-            const SumOut so{ws.data, part, sums, A.np, A.nq, A.np % 8u == 0u};
+            SumOut so{};
+            float* rest = ws.data;
+            if constexpr (kSums) {
+                so = out;
+            } else {
+                so.out = ws.data;
+                so.np  = A.np;
+                so.nq  = A.nq;
+                so.vec = A.np % 8u == 0u;
+                rest += part;
+            }
+            so.parts    = rest;
+            so.part     = part;
+            float* sums = row_sums ? rest + (parts - 1u) * part : nullptr;
+            so.row_sums = sums;
             k_product<T, kBP, kBQ, kWP, kWQ, kPT, kQT, kAligned, SumOut><<<grid, kThreads, 0, stream>>>(A, so);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
             const uint64_t eights = (uint64_t)ceil_div(A.np, 8u) * A.nq;
-            k_join<Out><<<(uint32_t)std::min<uint64_t>(ceil_div(eights, kJoined), 4096u), 256, 0, stream>>>(ws.data, part, parts, sums, row_sums, out);
+            k_join<Out><<<(uint32_t)std::min<uint64_t>(ceil_div(eights, kJoined), 4096u), 256, 0, stream>>>(so.out, rest, part, parts, sums, row_sums, out);
             return hipGetLastError();
         }
     }
@@ -681,7 +735,7 @@ NerfStatus backward(const NerfExtLinearDesc& d, const void* x, const void* w, co
     }
     if (dw) {
         const Operands A{x, delta, d.x_stride, d.y_stride, d.in_features, d.out_features, d.rows, 0u};
-        const SumOut out{dw, 0u, db, d.in_features, d.out_features, d.in_features % 8u == 0u && aligned(dw, 16u)};
+        const SumOut out{dw, nullptr, 0u, db, d.in_features, d.out_features, d.in_features % 8u == 0u && aligned(dw, 16u)};
         NERF_HIP_TRY((launch_product<T, true, true>(A, out, db, ws, stream)));
     }
     return NERF_STATUS_OK;
