@@ -175,9 +175,28 @@ __device__ __forceinline__ floatx8 widen(uintx4 v) {
     return __builtin_convertvector(__builtin_bit_cast(typename Vec<T>::x8, v), floatx8);
 }
 
+// The biases of p0 .. p0 + kB in LDS, zeros where there are none, and eight of
+// them.  Loads return in their order: a bias loaded from memory as it is used
+// is waited for with everything that was asked for before it, which was the
+// next rows' operands (2^18 x 256 -> 256: 169 us with it, 114 us without).
+template <uint32_t kB, typename Out>
+__device__ __forceinline__ void keep_bias(const Out& out, uint32_t p0, float* lds) {
+    if constexpr (Out::kBias)
+        for (uint32_t i = threadIdx.x; i < kB; i += blockDim.x) lds[i] = out.bias && p0 + i < out.np ? out.bias[p0 + i] : 0.0f;
+}
+template <typename Out>
+__device__ __forceinline__ floatx8 bias8(const float* lds, uint32_t at) {
+    floatx8 b = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (Out::kBias) {
+        b.lo = *reinterpret_cast<const floatx4*>(lds + at);
+        b.hi = *reinterpret_cast<const floatx4*>(lds + at + 4u);
+    }
+    return b;
+}
+
 // Each epilogue gets eight consecutive p of one row q0 + row at a time, n of
-// them inside the output (0 for a row outside), and first loads what it needs
-// besides the sums, so that a caller can have that under way early.
+// them inside the output (0 for a row outside), with their biases, and first
+// loads what else it needs, so that a caller can have that under way early.
 template <typename T>
 struct ForwardOut {
     const float* bias;
@@ -190,16 +209,13 @@ struct ForwardOut {
     struct Aux {
         uintx4 residual;
     };
+    static constexpr bool kBias = true;
 
     __device__ __forceinline__ Aux load(uint32_t q0, uint32_t row, uint32_t p, uint32_t n) const {
         return {residual ? Rows<T>(residual, q0, ldr).load(row, p, n, vec) : uintx4{0u, 0u, 0u, 0u}};
     }
-    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 z, const Aux& a) const {
-        if (bias) {
-            const Rows<float> b(bias, 0u, 0u);
-#pragma unroll
-            for (uint32_t r = 0; r < 8u; ++r) z[r] += __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b.rsrc, (int)(r < n ? 4u * (p + r) : kBeyond), 0, 0));
-        }
+    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 z, const floatx8& b, const Aux& a) const {
+        z += b;
         if (pre) Rows<T>(pre, q0, np).store(row, p, n, vec, z);
         act_values(act, z);
         if (residual) z += widen<T>(a.residual);
@@ -220,6 +236,7 @@ struct InputGradientOut {
     struct Aux {
         uintx4 add, pre;
     };
+    static constexpr bool kBias = false;
 
     __device__ __forceinline__ Aux load(uint32_t q0, uint32_t row, uint32_t p, uint32_t n) const {
         Aux a{};
@@ -227,7 +244,7 @@ struct InputGradientOut {
         if (dpre) a.pre = Rows<T>(pre, q0, np).load(row, p, n, vec);
         return a;
     }
-    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 g, const Aux& a) const {
+    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 g, const floatx8&, const Aux& a) const {
         if (add) g += widen<T>(a.add);
         if (dx) Rows<T>(dx, q0, ldx).store(row, p, n, vec, g);
         if (dpre) {
@@ -247,8 +264,9 @@ struct SumOut {
     uint32_t np, nq;
     bool vec;
     struct Aux {};
+    static constexpr bool kBias = false;
     __device__ __forceinline__ Aux load(uint32_t, uint32_t, uint32_t, uint32_t) const { return {}; }
-    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, const floatx8& v, const Aux&) const { Rows<float>(out, q0, np).store(row, p, n, vec, v); }
+    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, const floatx8& v, const floatx8&, const Aux&) const { Rows<float>(out, q0, np).store(row, p, n, vec, v); }
 };
 
 // ----------------------------------------------------------------- product
@@ -419,6 +437,7 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     // Variables of their own, so that the compiler sees that a read of one is no
     // read of what is on its way into another.
     __shared__ uint4 lds_p0[kBP * 8u], lds_q0[kBQ * 8u], lds_p1[kAligned ? kBP * 8u : 1u], lds_q1[kAligned ? kBQ * 8u : 1u];
+    __shared__ floatx4 lds_bias[Out::kBias ? kBP / 4u : 1u];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t wp = (wave % kWP) * (kBP / kWP), wq = (wave / kWP) * (kBQ / kWQ);
     const uint32_t p0 = blockIdx.x * kBP, q0 = blockIdx.y * kBQ;
@@ -428,6 +447,7 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     // shared out among the waves that hold the same.
     constexpr bool kSums = std::is_same_v<Out, SumOut>;
     constexpr uint32_t kSumsQ = kSums ? kFQ / kWP : 1u;
+    keep_bias<kBP>(out, p0, reinterpret_cast<float*>(lds_bias));
     floatx4 acc[kFP][kFQ], sums[kSumsQ];
 #pragma unroll
     for (uint32_t j = 0; j < kSumsQ; ++j) sums[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -569,9 +589,134 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
             floatx8 v;
             v.lo = strip[r * (kSP / 4u) + ((col / 4u) ^ (r & 7u))];
             v.hi = strip[r * (kSP / 4u) + ((col / 4u + 1u) ^ (r & 7u))];
-            out.put(q0, row_of(s, t), p_of(s), inside(s, t), v, aux[s & 1u][t]);
+            out.put(q0, row_of(s, t), p_of(s), inside(s, t), v, bias8<Out>(reinterpret_cast<const float*>(lds_bias), p_of(s) - p0), aux[s & 1u][t]);
         }
         __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// ------------------------------------------------------------ short sums
+// Many rows and at most 32 kKS <= 256 k: memory bound.  A wave keeps its
+// 16 kFP p of P in registers for all k (at most 128 of them) and goes through
+// the rows 16 at a time: it reads Q as the matrix instruction takes it, straight
+// from memory, the next rows' Q and epilogue inputs being on their way while
+// these rows' outputs leave.  Waves do not wait for each other.  Waves of a
+// workgroup that hold other p read the same Q at about the same time, from the
+// CU's cache.
+constexpr uint32_t kStreamWaves = 8u;
+template <typename T, uint32_t kKS, uint32_t kFP, bool kPT, typename Out>
+__global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out out, uint32_t p_waves) {
+    constexpr uint32_t kThreads = kStreamWaves * 64u, kSP = 16u * kFP, kBP = 256u;
+    constexpr uint32_t kLanes = kSP / 8u, kPasses = 16u * kLanes / 64u;
+    using x8 = typename Vec<T>::x8;
+    __shared__ uint4 lds[kBP * 8u];
+    __shared__ floatx4 lds_bias[Out::kBias ? kBP / 4u : 1u];
+    static_assert(kStreamWaves * kSP * 4u <= kBP * 8u);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
+    const uint32_t wp = wave % p_waves * kSP, p0 = blockIdx.y * p_waves * kSP;
+
+    keep_bias<kBP>(out, p0, reinterpret_cast<float*>(lds_bias));
+    x8 fp[kKS][kFP];
+    {
+        Stager<T, kBP, kPT, kThreads> stager;
+        stager.fetch((const T*)A.p, A.ldp, A.np, p0, 0u, A.nk);
+        const uint32_t base = fragment_base<kBP, kPT>(wp & ~127u);
+#pragma unroll
+        for (uint32_t s = 0; s < kKS; s += 2u) {
+            stager.keep(lds);
+            __syncthreads();
+            if (s + 2u < kKS) stager.fetch((const T*)A.p, A.ldp, A.np, p0, 32u * (s + 2u), A.nk);
+#pragma unroll
+            for (uint32_t i = 0; i < kFP; ++i)
+#pragma unroll
+                for (uint32_t h = 0; h < 2u; ++h)
+                    if (s + h < kKS) fp[s + h][i] = fragment<T, kBP, kPT>(lds, base, (wp & 127u) / 16u + i, h);
+            __syncthreads();
+        }
+    }
+
+    // Rows: lane l has k 8 (l / 16) + 0..7 of every 32 of row l % 16.
+    const uint32_t groups = kStreamWaves / p_waves, tiles = (A.nq + 15u) / 16u, stride = gridDim.x * groups;
+    const uint32_t l = lane & 15u, g = lane >> 4;
+    const uint32_t whole = A.nk / 32u;  // steps of 32 k that every row has in full
+    const bool ragged    = A.nk % 32u != 0u;
+    // The step after them: `some` of the lane's 8 k are left.  They are fetched
+    // as 8 values that end with the row (or begin with the array, in its first
+    // rows), and moved down by `down` values when they are used.
+    const uint32_t left = A.nk % 32u, some = left > 8u * g ? min(8u, left - 8u * g) : 0u;
+    uint32_t down = 0u;
+    x8 fq[kKS];
+#pragma unroll
+    for (uint32_t s = 0; s < kKS; ++s) fq[s] = x8{};
+    auto fetch_q = [&](uint32_t tile) {
+        const uint64_t first = (uint64_t)min(tile * 16u + l, A.nq - 1u) * A.ldq + 8u * g;
+        const T* at          = (const T*)A.q + first;
+#pragma unroll
+        for (uint32_t s = 0; s < kKS; ++s) {
+            if (s < whole) __builtin_memcpy(&fq[s], at + 32u * s, 16);
+            if (s == whole && ragged) {
+                const uint64_t end = first + 32u * s + some, from = end > 8u ? end - 8u : 0ull;
+                down               = some ? (uint32_t)(first + 32u * s - from) : 0u;
+                __builtin_memcpy(&fq[s], (const T*)A.q + (some ? from : 0ull), 16);
+            }
+        }
+    };
+    auto settle = [&](x8& v) {
+        unsigned long long w[2];
+        __builtin_memcpy(w, &v, 16);
+        const uint32_t bits = 16u * (down & 3u);
+        if (down >= 4u) {
+            w[0] = w[1];
+            w[1] = 0ull;
+        }
+        if (bits) {
+            w[0] = w[0] >> bits | w[1] << (64u - bits);
+            w[1] >>= bits;
+        }
+        const unsigned long long ones = ~0ull;
+        w[0] &= some >= 4u ? ones : ~(ones << (16u * some));
+        w[1] &= some >= 8u ? ones : some > 4u ? ~(ones << (16u * (some - 4u))) : 0ull;
+        __builtin_memcpy(&v, w, 16);
+    };
+    floatx4* strip = reinterpret_cast<floatx4*>(lds) + wave * (kSP * 4u);
+    const uint32_t row = lane / kLanes, col = 8u * (lane % kLanes), p = p0 + wp + col;
+    const uint32_t n = p < out.np ? min(8u, out.np - p) : 0u;
+    auto inside = [&](uint32_t tile, uint32_t pass) { return tile < tiles && tile * 16u + (64u / kLanes) * pass + row < out.nq ? n : 0u; };
+    typename Out::Aux aux[kPasses], next[kPasses];
+    uint32_t tile = __builtin_amdgcn_readfirstlane(blockIdx.x * groups + wave / p_waves);
+    if (tile >= tiles) return;
+    fetch_q(tile);
+#pragma unroll
+    for (uint32_t t = 0; t < kPasses; ++t) next[t] = out.load(tile * 16u, (64u / kLanes) * t + row, p, inside(tile, t));
+    for (; tile < tiles; tile += stride) {
+#pragma unroll
+        for (uint32_t t = 0; t < kPasses; ++t) aux[t] = next[t];
+        floatx4 acc[kFP];
+#pragma unroll
+        for (uint32_t i = 0; i < kFP; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t s = 0; s < kKS; ++s) {
+            if (ragged && s == whole) settle(fq[s]);
+#pragma unroll
+            for (uint32_t i = 0; i < kFP; ++i) acc[i] = Vec<T>::mfma(fp[s][i], fq[s], acc[i]);
+        }
+        if (tile + stride < tiles) {
+            fetch_q(tile + stride);
+#pragma unroll
+            for (uint32_t t = 0; t < kPasses; ++t) next[t] = out.load((tile + stride) * 16u, (64u / kLanes) * t + row, p, inside(tile + stride, t));
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kFP; ++i) strip[l * (kSP / 4u) + ((4u * i + g) ^ (l & 7u))] = acc[i];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (uint32_t t = 0; t < kPasses; ++t) {
+            const uint32_t r = (64u / kLanes) * t + row;
+            floatx8 v;
+            v.lo = strip[r * (kSP / 4u) + ((col / 4u) ^ (r & 7u))];
+            v.hi = strip[r * (kSP / 4u) + ((col / 4u + 1u) ^ (r & 7u))];
+            out.put(tile * 16u, r, p, inside(tile, t), v, bias8<Out>(reinterpret_cast<const float*>(lds_bias), wp + col), aux[t]);
+        }
+        asm volatile("" ::: "memory");
     }
 }
 
@@ -616,7 +761,14 @@ __global__ __launch_bounds__(256) void k_join(const float* first_part, const flo
                 v.lo += slice_sum[0][c][mine];
                 v.hi += slice_sum[1][c][mine];
             }
-            out.put(q0, q - q0, p, n, v, aux);
+            floatx8 b = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (Out::kBias) {
+                if (out.bias) {
+#pragma unroll
+                    for (uint32_t r = 0; r < 8u; ++r) b[r] = r < n ? out.bias[p + r] : 0.0f;
+                }
+            }
+            out.put(q0, q - q0, p, n, v, b, aux);
         }
     }
     if (row_sums) {
@@ -692,9 +844,29 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
     return hipGetLastError();
 }
 
+template <typename T, uint32_t kKS, bool kPT, typename Out>
+hipError_t launch_stream(const Operands& A, const Out& out, hipStream_t stream) {
+    const uint32_t wide = A.np <= 32u ? 32u : 64u;  // p a wave holds
+    const uint32_t held = ceil_div(A.np, wide), p_waves = held >= 4u ? 4u : held >= 2u ? 2u : 1u;
+    const uint32_t across = ceil_div(A.np, wide * p_waves), tiles = ceil_div(A.nq, 16u), groups = kStreamWaves / p_waves;
+    // One workgroup fills a CU's registers; every one goes through as many rows.
+    const dim3 grid(std::min(ceil_div(tiles, groups), std::max(1u, device_cu_count() / across)), across);
+    if (wide == 32u) k_stream<T, kKS, 2u, kPT, Out><<<grid, kStreamWaves * 64u, 0, stream>>>(A, out, p_waves);
+    else k_stream<T, kKS, 4u, kPT, Out><<<grid, kStreamWaves * 64u, 0, stream>>>(A, out, p_waves);
+    return hipGetLastError();
+}
+
 template <typename T, bool kPT, bool kQT, typename Out>
 hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hipStream_t stream) {
     const uint32_t cus = device_cu_count();
+    if constexpr (!kQT) {
+        if (A.nk <= 256u && A.np <= 1024u && A.nq >= 16384u) {
+            if (A.nk <= 32u) return launch_stream<T, 1u, kPT>(A, out, stream);
+            if (A.nk <= 64u) return launch_stream<T, 2u, kPT>(A, out, stream);
+            if (A.nk <= 128u) return launch_stream<T, 4u, kPT>(A, out, stream);
+            return launch_stream<T, 8u, kPT>(A, out, stream);
+        }
+    }
     if (!whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, kQT ? A.nq : A.nk)) {
         if ((uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u) >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u)) return launch_tiles<T, 128, 128, 2, 2, kPT, kQT, false>(A, out, row_sums, ws, stream);
         return launch_tiles<T, 64, 64, 2, 2, kPT, kQT, false>(A, out, row_sums, ws, stream);

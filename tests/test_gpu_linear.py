@@ -186,6 +186,21 @@ def test_rows_over_many_tiles():
     check_backward(33001, 256, 256, "f16", "relu")
 
 
+# Many rows and few k: every step of 32 k, whole and cut rows, narrow and wide
+# outputs, a last tile of rows that is not whole.
+@pytest.mark.parametrize("n,k,p", [(16384, 1, 3), (16385, 7, 40), (16400, 8, 33), (20011, 31, 64), (20011, 33, 200), (16397, 63, 256), (17001, 96, 129), (16999, 130, 70), (16384, 255, 300), (20000, 256, 16), (16401, 250, 257), (16411, 200, 96)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_many_rows(n, k, p, kind):
+    check_forward(n, k, p, kind, kind if p % 2 else "f32", "relu")
+    check_backward(n, p, k, kind, "relu", dw=False, db=False)
+
+
+def test_many_rows_with_strides():
+    for strides, shift in (((272, 136, 144), 0), ((257, 131, 133), 1)):
+        check_forward(17003, 256, 130, "f16", "f16", "silu", strides=strides, shift=shift)
+        check_backward(17003, 256, 130, "f16", "silu", strides=strides[:2], shift=shift, dw=False, db=False)
+
+
 def test_wide_layers():
     check_forward(700, 1024, 2056, "bf16", "bf16", "gelu")
     check_backward(700, 1032, 1024, "bf16", "gelu")
