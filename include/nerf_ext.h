@@ -253,7 +253,7 @@ NERF_API NerfStatus nerf_ext_linear_backward(const NerfExtLinearDesc* desc, cons
 typedef struct NerfExtGradTensor {
     const void* grad; /* device, count elements of dtype */
     void* out;        /* nerf_ext_grad_clip: the clipped gradient, of dtype; may be grad */
-    uint64_t count;   /* at most 2^36; 0: nothing is read or written */
+    uint64_t count;   /* at most 2^34; 0: nothing is read or written */
     uint32_t dtype;   /* NERF_EXT_F32, _F16 or _BF16 */
     uint32_t reserved; /* 0 */
 } NerfExtGradTensor;
@@ -264,7 +264,7 @@ typedef struct NerfExtAdamTensor {
     float* m;
     float* v;
     void* copy;        /* working copy in copy_dtype, or NULL */
-    uint64_t count;
+    uint64_t count;    /* at most 2^34 */
     uint32_t copy_dtype; /* NERF_EXT_F16 or NERF_EXT_BF16 */
     uint32_t reserved;   /* 0 */
 } NerfExtAdamTensor;

@@ -178,11 +178,13 @@ __device__ __forceinline__ floatx8 widen(uintx4 v) {
 // The biases of p0 .. p0 + kB in LDS, zeros where there are none, and eight of
 // them.  Loads return in their order: a bias loaded from memory as it is used
 // is waited for with everything that was asked for before it, which was the
-// next rows' operands (2^18 x 256 -> 256: 169 us with it, 114 us without).
+// next rows' operands (2^18 x 256 -> 256: 169 us with it, 117 us without).
+// One bias a thread: asked for first and kept once the operands are asked for.
 template <uint32_t kB, typename Out>
-__device__ __forceinline__ void keep_bias(const Out& out, uint32_t p0, float* lds) {
+__device__ __forceinline__ float thread_bias(const Out& out, uint32_t p0) {
     if constexpr (Out::kBias)
-        for (uint32_t i = threadIdx.x; i < kB; i += blockDim.x) lds[i] = out.bias && p0 + i < out.np ? out.bias[p0 + i] : 0.0f;
+        if (out.bias && threadIdx.x < kB && p0 + threadIdx.x < out.np) return out.bias[p0 + threadIdx.x];
+    return 0.0f;
 }
 template <typename Out>
 __device__ __forceinline__ floatx8 bias8(const float* lds, uint32_t at) {
@@ -300,53 +302,92 @@ __device__ __forceinline__ constexpr uint32_t chunk_slot(uint32_t line, uint32_t
     return line * (kT ? kB / 8u : 8u) + (chunk ^ chunk_key<kB, kT>(line));
 }
 
-// Tile [row0, row0 + kB) x [k0, k0 + 64) into LDS, zeros outside [0, n) x [0, nk),
+// Eight values of which `some` are an operand's, fetched from `down` values
+// ahead of them: those moved to the front, zeros behind them.
+__device__ __forceinline__ uint4 settled(uint4 v, uint32_t down, uint32_t some) {
+    unsigned long long w[2];
+    __builtin_memcpy(w, &v, 16);
+    const uint32_t bits = 16u * (down & 3u);
+    if (down >= 4u) {
+        w[0] = w[1];
+        w[1] = 0ull;
+    }
+    if (bits) {
+        w[0] = w[0] >> bits | w[1] << (64u - bits);
+        w[1] >>= bits;
+    }
+    const unsigned long long ones = ~0ull;
+    w[0] &= some >= 4u ? ones : ~(ones << (16u * some));
+    w[1] &= some >= 8u ? ones : some > 4u ? ~(ones << (16u * (some - 4u))) : 0ull;
+    __builtin_memcpy(&v, w, 16);
+    return v;
+}
+
+// Tile [row0, row0 + kB) x [k0, k0 + 64) into LDS, zeros outside [0, n) x [0, k_end),
 // through registers and at any alignment: fetch() asks for a tile, keep() writes
-// it to LDS.
+// it to LDS.  Every chunk is fetched as 16 bytes inside the array, in a tile at
+// an edge from a place that ends with the line (or begins with the array), and
+// put right in keep(): nothing waits for a load between the loads (with the
+// edges' work between them, one wait each, 20011 x 1209 -> 487 took 112 us).
 template <typename T, uint32_t kB, bool kT, uint32_t kThreads>
 struct Stager {
     static constexpr uint32_t kChunks = kT ? kB / 8u : 8u;
     static constexpr uint32_t kLoads  = (kB * 8u + kThreads - 1u) / kThreads;
     uint4 held[kLoads];
 
+    struct Place {
+        uint32_t line, chunk, major, minor, some;  // some: values of the chunk inside
+    };
+    static __device__ __forceinline__ Place place(uint32_t i, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) {
+        const uint32_t s = i * kThreads + threadIdx.x;
+        Place o;
+        o.line  = s / kChunks;
+        o.chunk = s % kChunks;
+        o.major = (kT ? k0 : row0) + o.line;
+        o.minor = (kT ? row0 : k0) + 8u * o.chunk;
+        const uint32_t major_end = kT ? k_end : n, minor_end = kT ? n : k_end;
+        o.some = s < kB * 8u && o.major < major_end && o.minor < minor_end ? min(8u, minor_end - o.minor) : 0u;
+        return o;
+    }
+    static __device__ __forceinline__ bool inner(uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) { return kB * 8u % kThreads == 0u && row0 + kB <= n && k0 + kBK <= k_end; }
+
     __device__ __forceinline__ void fetch(const T* __restrict__ src, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) {
+        if (inner(n, row0, k0, k_end)) {
 #pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i) {
-            const uint32_t s = i * kThreads + threadIdx.x, line = s / kChunks, chunk = s % kChunks;
-            const uint32_t major = (kT ? k0 : row0) + line, minor = (kT ? row0 : k0) + 8u * chunk;
-            const uint32_t major_end = kT ? k_end : n, minor_end = kT ? n : k_end;
-            held[i] = uint4{0u, 0u, 0u, 0u};
-            if (s < kB * 8u && major < major_end && minor < minor_end) {
-                const T* line_at = src + (uint64_t)major * ld;
-                if (minor_end >= 8u) {
-                    // A chunk that the line's end cuts is fetched so that it ends there,
-                    // and moved down; what moves in is zero.
-                    const uint32_t over = minor + 8u > minor_end ? minor + 8u - minor_end : 0u;
-                    unsigned long long v[2];
-                    __builtin_memcpy(v, line_at + minor - over, 16);
-                    if (over >= 4u) {
-                        v[0] = v[1] >> (16u * (over - 4u));
-                        v[1] = 0ull;
-                    } else if (over) {
-                        v[0] = v[0] >> (16u * over) | v[1] << (64u - 16u * over);
-                        v[1] >>= 16u * over;
-                    }
-                    __builtin_memcpy(&held[i], v, 16);
-                } else {
-                    short8_t h = {0, 0, 0, 0, 0, 0, 0, 0};
+            for (uint32_t i = 0; i < kLoads; ++i) {
+                const Place o = place(i, n, row0, k0, k_end);
+                __builtin_memcpy(&held[i], src + (uint64_t)o.major * ld + o.minor, 16);
+            }
+        } else if ((uint64_t)((kT ? k_end : n) - 1u) * ld + (kT ? n : k_end) >= 8u) {
 #pragma unroll
-                    for (uint32_t j = 0; j < 7u; ++j)
-                        if (minor + j < minor_end) h[j] = __builtin_bit_cast(short, line_at[minor + j]);
-                    held[i] = __builtin_bit_cast(uint4, h);
-                }
+            for (uint32_t i = 0; i < kLoads; ++i) {
+                const Place o      = place(i, n, row0, k0, k_end);
+                const uint64_t end = (uint64_t)o.major * ld + o.minor + o.some;
+                __builtin_memcpy(&held[i], src + (o.some && end > 8u ? end - 8u : 0ull), 16);
+            }
+        } else {  // an array of fewer than eight values
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) {
+                const Place o = place(i, n, row0, k0, k_end);
+                short8_t h    = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (uint32_t j = 0; j < 7u; ++j)
+                    if (j < o.some) h[j] = __builtin_bit_cast(short, src[(uint64_t)o.major * ld + o.minor + j]);
+                held[i] = __builtin_bit_cast(uint4, h);
             }
         }
     }
-    __device__ __forceinline__ void keep(uint4* lds) const {
+    __device__ __forceinline__ void keep(uint4* lds, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) const {
+        const bool settle = !inner(n, row0, k0, k_end) && (uint64_t)((kT ? k_end : n) - 1u) * ld + (kT ? n : k_end) >= 8u;
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
-            const uint32_t s = i * kThreads + threadIdx.x;
-            if (kB * 8u % kThreads == 0u || s < kB * 8u) lds[chunk_slot<kB, kT>(s / kChunks, s % kChunks)] = held[i];
+            const Place o = place(i, n, row0, k0, k_end);
+            uint4 v       = held[i];
+            if (settle) {
+                const uint64_t at = (uint64_t)o.major * ld + o.minor;
+                v                 = settled(v, o.some ? (at + o.some >= 8u ? 8u - o.some : (uint32_t)at) : 0u, o.some);
+            }
+            if (kB * 8u % kThreads == 0u || i * kThreads + threadIdx.x < kB * 8u) lds[chunk_slot<kB, kT>(o.line, o.chunk)] = v;
         }
     }
 };
@@ -420,23 +461,28 @@ __device__ __forceinline__ typename Vec<T>::x8 fragment(const uint4* lds, uint32
     }
 }
 
-// Waits for the wave's own loads into LDS and then for the workgroup.
+// Waits until at most `kLater` of the wave's own loads are on their way, and
+// then for the workgroup.
+template <uint32_t kLater>
 __device__ __forceinline__ void arrived() {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (kLater & 15u) | (kLater >> 4) << 14);  // vmcnt
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
 
-// kBP x kBQ outputs a workgroup, kWP x kWQ waves.  kAligned: both operands go
-// straight into LDS, the next 64 k while this one is multiplied.
-template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, bool kPT, bool kQT, bool kAligned, typename Out>
+// kBP x kBQ outputs a workgroup, kWP x kWQ waves, kDepth tiles of 64 k at a time
+// in LDS or on their way there.  kAligned: both operands go straight into LDS;
+// else the tiles on their way wait in registers.
+template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, bool kQT, bool kAligned, typename Out>
 __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out) {
     constexpr uint32_t kThreads = kWP * kWQ * 64u;
     constexpr uint32_t kFP = kBP / kWP / 16u, kFQ = kBQ / kWQ / 16u;
     // Variables of their own, so that the compiler sees that a read of one is no
     // read of what is on its way into another.
-    __shared__ uint4 lds_p0[kBP * 8u], lds_q0[kBQ * 8u], lds_p1[kAligned ? kBP * 8u : 1u], lds_q1[kAligned ? kBQ * 8u : 1u];
+    constexpr uint32_t kTile = (kBP + kBQ) * 8u;
+    static_assert(kDepth == 2u || kDepth == 4u);
+    __shared__ uint4 lds0[kTile], lds1[kAligned ? kTile : 1u], lds2[kAligned && kDepth == 4u ? kTile : 1u], lds3[kAligned && kDepth == 4u ? kTile : 1u];
     __shared__ floatx4 lds_bias[Out::kBias ? kBP / 4u : 1u];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t wp = (wave % kWP) * (kBP / kWP), wq = (wave / kWP) * (kBQ / kWQ);
@@ -447,7 +493,11 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     // shared out among the waves that hold the same.
     constexpr bool kSums = std::is_same_v<Out, SumOut>;
     constexpr uint32_t kSumsQ = kSums ? kFQ / kWP : 1u;
-    keep_bias<kBP>(out, p0, reinterpret_cast<float*>(lds_bias));
+    static_assert(kBP <= kThreads);
+    const float bias = thread_bias<kBP>(out, p0);
+    auto keep_bias   = [&] {
+        if (Out::kBias && threadIdx.x < kBP) reinterpret_cast<float*>(lds_bias)[threadIdx.x] = bias;
+    };
     floatx4 acc[kFP][kFQ], sums[kSumsQ];
 #pragma unroll
     for (uint32_t j = 0; j < kSumsQ; ++j) sums[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -466,7 +516,8 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     // One tile of 64 k: kG fragments of P against all of Q at a time, the next
     // fragments on their way from LDS meanwhile.
     constexpr uint32_t kG = kFP < 2u ? 1u : 2u, kPhases = kFP / kG;
-    auto multiply = [&](const uint4* lp, const uint4* lq) {
+    auto multiply = [&](const uint4* lp) {
+        const uint4* lq = lp + kBP * 8u;
         typename Vec<T>::x8 fp[2][kG], fq[2][kFQ];
         uint32_t bp = base_p, bq = base_q;
         asm volatile("" : "+v"(bp), "+v"(bq));
@@ -510,41 +561,74 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
         Loader<T, kBQ, kQT, kThreads> load_q;
         load_p.begin((const T*)A.p, A.ldp, A.np, p0, k0);
         load_q.begin((const T*)A.q, A.ldq, A.nq, q0, k0);
-        // Two tiles a turn, one from each pair of buffers; a last odd tile is
-        // followed by one of zeros (a way out between the two would keep a second
-        // copy of the sums alive).
-        load_p.issue(lds_p0, (int)(k_end - k0));
-        load_q.issue(lds_q0, (int)(k_end - k0));
-        for (int left = (int)(k_end - k0); left > 0; left -= (int)(2u * kBK)) {
-            // Everyone's part of this tile has come, and everyone is done with the
-            // other buffers.
-            arrived();
-            load_p.issue(lds_p1, left - (int)kBK);
-            load_q.issue(lds_q1, left - (int)kBK);
-            multiply(lds_p0, lds_q0);
-            arrived();
-            if (left > (int)(2u * kBK)) {
-                load_p.issue(lds_p0, left - (int)(2u * kBK));
-                load_q.issue(lds_q0, left - (int)(2u * kBK));
+        constexpr uint32_t kLoads = kBP * 8u / kThreads + kBQ * 8u / kThreads;
+        auto issue = [&](uint4* lds, int left) {
+            load_p.issue(lds, left);
+            load_q.issue(lds + kBP * 8u, left);
+        };
+        constexpr int kStep = (int)kBK;
+        int left            = (int)(k_end - k0);
+        if constexpr (kDepth == 2u) {
+            // Two tiles a turn; a last odd tile is followed by one of zeros (a way out
+            // between the two would keep a second copy of the sums alive).  arrived():
+            // everyone's part of the tile has come, and everyone is done with the
+            // other buffer.
+            issue(lds0, left);
+            keep_bias();
+            for (; left > 0; left -= 2 * kStep) {
+                arrived<0u>();
+                issue(lds1, left - kStep);
+                multiply(lds0);
+                arrived<0u>();
+                if (left > 2 * kStep) issue(lds0, left - 2 * kStep);
+                multiply(lds1);
             }
-            multiply(lds_p1, lds_q1);
+        } else {
+            // Three tiles on their way: few k are asked for all at once.
+            issue(lds0, left);
+            issue(lds1, left - kStep);
+            issue(lds2, left - 2 * kStep);
+            keep_bias();
+            for (; left > 0; left -= 4 * kStep) {
+                arrived<2u * kLoads>();
+                issue(lds3, left - 3 * kStep);
+                multiply(lds0);
+                arrived<2u * kLoads>();
+                issue(lds0, left - 4 * kStep);
+                if (left > kStep) multiply(lds1);
+                arrived<2u * kLoads>();
+                issue(lds1, left - 5 * kStep);
+                if (left > 2 * kStep) multiply(lds2);
+                arrived<2u * kLoads>();
+                issue(lds2, left - 6 * kStep);
+                if (left > 3 * kStep) multiply(lds3);
+            }
         }
     } else {
-        // One pair of buffers; the next tile waits in registers meanwhile.
-        Stager<T, kBP, kPT, kThreads> stage_p;
-        Stager<T, kBQ, kQT, kThreads> stage_q;
-        stage_p.fetch((const T*)A.p, A.ldp, A.np, p0, k0, k_end);
-        stage_q.fetch((const T*)A.q, A.ldq, A.nq, q0, k0, k_end);
-        for (uint32_t k = k0; k < k_end; k += kBK) {
-            stage_p.keep(lds_p0);
-            stage_q.keep(lds_q0);
-            __syncthreads();
-            if (k + kBK < k_end) {
-                stage_p.fetch((const T*)A.p, A.ldp, A.np, p0, k + kBK, k_end);
-                stage_q.fetch((const T*)A.q, A.ldq, A.nq, q0, k + kBK, k_end);
+        // The next kDepth - 1 tiles wait in registers.
+        Stager<T, kBP, kPT, kThreads> stage_p[kDepth - 1u];
+        Stager<T, kBQ, kQT, kThreads> stage_q[kDepth - 1u];
+        auto fetch = [&](uint32_t d, uint32_t k) {
+            stage_p[d].fetch((const T*)A.p, A.ldp, A.np, p0, k, k_end);
+            stage_q[d].fetch((const T*)A.q, A.ldq, A.nq, q0, k, k_end);
+        };
+#pragma unroll
+        for (uint32_t d = 0; d < kDepth - 1u; ++d)
+            if (k0 + kBK * d < k_end) fetch(d, k0 + kBK * d);
+        keep_bias();
+        for (uint32_t k = k0; k < k_end; k += kBK * (kDepth - 1u)) {
+#pragma unroll
+            for (uint32_t d = 0; d < kDepth - 1u; ++d) {
+                const uint32_t kd = k + kBK * d;
+                if (kd < k_end) {
+                    stage_p[d].keep(lds0, A.ldp, A.np, p0, kd, k_end);
+                    stage_q[d].keep(lds0 + kBP * 8u, A.ldq, A.nq, q0, kd, k_end);
+                    __syncthreads();
+                    if (kd + kBK * (kDepth - 1u) < k_end) fetch(d, kd + kBK * (kDepth - 1u));
+                    multiply(lds0);
+                    __syncthreads();
+                }
             }
-            multiply(lds_p0, lds_q0);
-            __syncthreads();
         }
     }
 
@@ -564,9 +648,10 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     // (16-bit outputs).  Chunks of four p, their place xor-ed with the row.
     constexpr uint32_t kSP = kBP / kWP < 64u ? kBP / kWP : 64u, kStrips = kFQ * (kBP / kWP / kSP);
     constexpr uint32_t kLanes = kSP / 8u, kPasses = 16u * kLanes / 64u;
-    static_assert(kWP * kWQ * kSP <= 8u * kBP);
+    static_assert(kWP * kWQ * kSP * 4u <= kTile);
     __syncthreads();
-    floatx4* strip = reinterpret_cast<floatx4*>(lds_p0) + wave * (kSP * 4u);
+    arrived<0u>();  // the zeros behind the last tile too
+    floatx4* strip = reinterpret_cast<floatx4*>(lds0) + wave * (kSP * 4u);
     const uint32_t row = lane / kLanes, col = 8u * (lane % kLanes);
     auto row_of = [&](uint32_t s, uint32_t pass) { return wq + 16u * (s % kFQ) + (64u / kLanes) * pass + row; };
     auto p_of = [&](uint32_t s) { return p0 + wp + kSP * (s / kFQ) + col; };
@@ -604,7 +689,7 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
 // workgroup that hold other p read the same Q at about the same time, from the
 // CU's cache.
 constexpr uint32_t kStreamWaves = 8u;
-template <typename T, uint32_t kKS, uint32_t kFP, bool kPT, typename Out>
+template <typename T, uint32_t kKS, uint32_t kFP, bool kPT, bool kRagged, typename Out>
 __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out out, uint32_t p_waves) {
     constexpr uint32_t kThreads = kStreamWaves * 64u, kSP = 16u * kFP, kBP = 256u;
     constexpr uint32_t kLanes = kSP / 8u, kPasses = 16u * kLanes / 64u;
@@ -615,15 +700,16 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t wp = wave % p_waves * kSP, p0 = blockIdx.y * p_waves * kSP;
 
-    keep_bias<kBP>(out, p0, reinterpret_cast<float*>(lds_bias));
     x8 fp[kKS][kFP];
     {
+        const float bias = thread_bias<kBP>(out, p0);
         Stager<T, kBP, kPT, kThreads> stager;
         stager.fetch((const T*)A.p, A.ldp, A.np, p0, 0u, A.nk);
+        if (Out::kBias && threadIdx.x < kBP) reinterpret_cast<float*>(lds_bias)[threadIdx.x] = bias;
         const uint32_t base = fragment_base<kBP, kPT>(wp & ~127u);
 #pragma unroll
         for (uint32_t s = 0; s < kKS; s += 2u) {
-            stager.keep(lds);
+            stager.keep(lds, A.ldp, A.np, p0, 32u * s, A.nk);
             __syncthreads();
             if (s + 2u < kKS) stager.fetch((const T*)A.p, A.ldp, A.np, p0, 32u * (s + 2u), A.nk);
 #pragma unroll
@@ -639,8 +725,7 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
     const uint32_t groups = kStreamWaves / p_waves, tiles = (A.nq + 15u) / 16u, stride = gridDim.x * groups;
     const uint32_t l = lane & 15u, g = lane >> 4;
     const uint32_t whole = A.nk / 32u;  // steps of 32 k that every row has in full
-    const bool ragged    = A.nk % 32u != 0u;
-    // The step after them: `some` of the lane's 8 k are left.  They are fetched
+    // kRagged, the step after them: `some` of the lane's 8 k are left.  They are fetched
     // as 8 values that end with the row (or begin with the array, in its first
     // rows), and moved down by `down` values when they are used.
     const uint32_t left = A.nk % 32u, some = left > 8u * g ? min(8u, left - 8u * g) : 0u;
@@ -654,34 +739,20 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
 #pragma unroll
         for (uint32_t s = 0; s < kKS; ++s) {
             if (s < whole) __builtin_memcpy(&fq[s], at + 32u * s, 16);
-            if (s == whole && ragged) {
+            if (kRagged && s == whole) {
                 const uint64_t end = first + 32u * s + some, from = end > 8u ? end - 8u : 0ull;
                 down               = some ? (uint32_t)(first + 32u * s - from) : 0u;
                 __builtin_memcpy(&fq[s], (const T*)A.q + (some ? from : 0ull), 16);
             }
         }
     };
-    auto settle = [&](x8& v) {
-        unsigned long long w[2];
-        __builtin_memcpy(w, &v, 16);
-        const uint32_t bits = 16u * (down & 3u);
-        if (down >= 4u) {
-            w[0] = w[1];
-            w[1] = 0ull;
-        }
-        if (bits) {
-            w[0] = w[0] >> bits | w[1] << (64u - bits);
-            w[1] >>= bits;
-        }
-        const unsigned long long ones = ~0ull;
-        w[0] &= some >= 4u ? ones : ~(ones << (16u * some));
-        w[1] &= some >= 8u ? ones : some > 4u ? ~(ones << (16u * (some - 4u))) : 0ull;
-        __builtin_memcpy(&v, w, 16);
-    };
     floatx4* strip = reinterpret_cast<floatx4*>(lds) + wave * (kSP * 4u);
     const uint32_t row = lane / kLanes, col = 8u * (lane % kLanes), p = p0 + wp + col;
     const uint32_t n = p < out.np ? min(8u, out.np - p) : 0u;
     auto inside = [&](uint32_t tile, uint32_t pass) { return tile < tiles && tile * 16u + (64u / kLanes) * pass + row < out.nq ? n : 0u; };
+    // The next rows' epilogue inputs: beside this rows', or where that takes more
+    // registers than there are, in their place as they are used.
+    constexpr bool kLate = kKS * kFP == 32u && sizeof(typename Out::Aux) > 16u;
     typename Out::Aux aux[kPasses], next[kPasses];
     uint32_t tile = __builtin_amdgcn_readfirstlane(blockIdx.x * groups + wave / p_waves);
     if (tile >= tiles) return;
@@ -696,14 +767,15 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
         for (uint32_t i = 0; i < kFP; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t s = 0; s < kKS; ++s) {
-            if (ragged && s == whole) settle(fq[s]);
+            if (kRagged && s == whole) fq[s] = __builtin_bit_cast(x8, settled(__builtin_bit_cast(uint4, fq[s]), down, some));
 #pragma unroll
             for (uint32_t i = 0; i < kFP; ++i) acc[i] = Vec<T>::mfma(fp[s][i], fq[s], acc[i]);
         }
         if (tile + stride < tiles) {
             fetch_q(tile + stride);
 #pragma unroll
-            for (uint32_t t = 0; t < kPasses; ++t) next[t] = out.load((tile + stride) * 16u, (64u / kLanes) * t + row, p, inside(tile + stride, t));
+            for (uint32_t t = 0; t < kPasses; ++t)
+                if (!kLate) next[t] = out.load((tile + stride) * 16u, (64u / kLanes) * t + row, p, inside(tile + stride, t));
         }
 #pragma unroll
         for (uint32_t i = 0; i < kFP; ++i) strip[l * (kSP / 4u) + ((4u * i + g) ^ (l & 7u))] = acc[i];
@@ -715,6 +787,7 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
             v.lo = strip[r * (kSP / 4u) + ((col / 4u) ^ (r & 7u))];
             v.hi = strip[r * (kSP / 4u) + ((col / 4u + 1u) ^ (r & 7u))];
             out.put(tile * 16u, r, p, inside(tile, t), v, bias8<Out>(reinterpret_cast<const float*>(lds_bias), wp + col), aux[t]);
+            if (kLate) next[t] = out.load((tile + stride) * 16u, r, p, inside(tile + stride, t));
         }
         asm volatile("" ::: "memory");
     }
@@ -736,7 +809,7 @@ __global__ __launch_bounds__(256) void k_join(const float* first_part, const flo
         const uint32_t q = (uint32_t)(at / eights), p = 8u * (uint32_t)(at % eights), n = at < total ? min(8u, out.np - p) : 0u;
         floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (n) {
-#pragma unroll 4
+#pragma unroll 8
             for (uint32_t c = slice; c < count; c += kSlices) {
                 const float* src = (c ? parts + (c - 1u) * part : first_part) + (uint64_t)q * out.np + p;
                 if (vec) {
@@ -795,7 +868,7 @@ struct Workspace {
 // Whether an operand's chunks of 8 along its contiguous length are whole and aligned.
 bool whole_chunks(const void* p, uint64_t ld, uint32_t contiguous) { return aligned(p, 16u) && ld % 8u == 0u && contiguous % 8u == 0u; }
 
-template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, bool kPT, bool kQT, bool kAligned, bool kSplit = true, typename Out>
+template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, bool kQT, bool kAligned, bool kSplit = true, typename Out>
 hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipStream_t stream) {
     const uint32_t tp = ceil_div(A.np, kBP), tq = ceil_div(A.nq, kBQ);
     // Split over k until every CU has its workgroups (two; one of the widest
@@ -832,7 +905,7 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
             so.part     = part;
             float* sums = row_sums ? rest + (parts - 1u) * part : nullptr;
             so.row_sums = sums;
-            k_product<T, kBP, kBQ, kWP, kWQ, kPT, kQT, kAligned, SumOut><<<grid, kThreads, 0, stream>>>(A, so);
+            k_product<T, kBP, kBQ, kWP, kWQ, kDepth, kPT, kQT, kAligned, SumOut><<<grid, kThreads, 0, stream>>>(A, so);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
             const uint64_t eights = (uint64_t)ceil_div(A.np, 8u) * A.nq;
@@ -840,19 +913,31 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
             return hipGetLastError();
         }
     }
-    k_product<T, kBP, kBQ, kWP, kWQ, kPT, kQT, kAligned, Out><<<grid, kThreads, 0, stream>>>(A, out);
+    k_product<T, kBP, kBQ, kWP, kWQ, kDepth, kPT, kQT, kAligned, Out><<<grid, kThreads, 0, stream>>>(A, out);
     return hipGetLastError();
 }
 
 template <typename T, uint32_t kKS, bool kPT, typename Out>
 hipError_t launch_stream(const Operands& A, const Out& out, hipStream_t stream) {
-    const uint32_t wide = A.np <= 32u ? 32u : 64u;  // p a wave holds
-    const uint32_t held = ceil_div(A.np, wide), p_waves = held >= 4u ? 4u : held >= 2u ? 2u : 1u;
+    // p a wave holds: 64, whose 16-bit outputs are whole lines; 32 where there are
+    // no more, or where 64 with the cut rows' work take more registers than there are.
+    const bool ragged = A.nk % 32u != 0u, narrow = A.np <= 32u || (ragged && kKS == 8u);
+    const uint32_t wide = narrow ? 32u : 64u, most = 256u / wide;
+    uint32_t p_waves = 1u;
+    while (p_waves < most && wide * p_waves < A.np) p_waves *= 2u;
     const uint32_t across = ceil_div(A.np, wide * p_waves), tiles = ceil_div(A.nq, 16u), groups = kStreamWaves / p_waves;
     // One workgroup fills a CU's registers; every one goes through as many rows.
     const dim3 grid(std::min(ceil_div(tiles, groups), std::max(1u, device_cu_count() / across)), across);
-    if (wide == 32u) k_stream<T, kKS, 2u, kPT, Out><<<grid, kStreamWaves * 64u, 0, stream>>>(A, out, p_waves);
-    else k_stream<T, kKS, 4u, kPT, Out><<<grid, kStreamWaves * 64u, 0, stream>>>(A, out, p_waves);
+    constexpr uint32_t kThreads = kStreamWaves * 64u;
+    if (narrow) {
+        if (ragged) k_stream<T, kKS, 2u, kPT, true, Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves);
+        else k_stream<T, kKS, 2u, kPT, false, Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves);
+    } else if constexpr (kKS < 8u) {
+        if (ragged) k_stream<T, kKS, 4u, kPT, true, Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves);
+        else k_stream<T, kKS, 4u, kPT, false, Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves);
+    } else {
+        k_stream<T, kKS, 4u, kPT, false, Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves);
+    }
     return hipGetLastError();
 }
 
@@ -868,12 +953,12 @@ hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hi
         }
     }
     if (!whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, kQT ? A.nq : A.nk)) {
-        if ((uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u) >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u)) return launch_tiles<T, 128, 128, 2, 2, kPT, kQT, false>(A, out, row_sums, ws, stream);
-        return launch_tiles<T, 64, 64, 2, 2, kPT, kQT, false>(A, out, row_sums, ws, stream);
+        if ((uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u) >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u && A.nk > 2048u)) return launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, false>(A, out, row_sums, ws, stream);
+        return launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, false>(A, out, row_sums, ws, stream);
     }
-    if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) * (kPT && kQT ? ceil_div(A.nk, 1024u) : 1u) >= cus / 2u && A.np > 128u && A.nk >= 512u) return launch_tiles<T, 256, 256, 2, 4, kPT, kQT, true, kPT && kQT>(A, out, row_sums, ws, stream);
-    if ((uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u) >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u)) return launch_tiles<T, 128, 128, 2, 2, kPT, kQT, true>(A, out, row_sums, ws, stream);
-    return launch_tiles<T, 64, 64, 2, 2, kPT, kQT, true>(A, out, row_sums, ws, stream);
+    if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) * (kPT && kQT ? ceil_div(A.nk, 1024u) : 1u) >= cus / 2u && A.np > 128u && A.nk >= 512u) return launch_tiles<T, 256, 256, 2, 4, 2, kPT, kQT, true, kPT && kQT>(A, out, row_sums, ws, stream);
+    if ((uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u) >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u && A.nk > 2048u)) return launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, true>(A, out, row_sums, ws, stream);
+    return launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, true>(A, out, row_sums, ws, stream);
 }
 
 // rows beyond gridDim's range of 64-row tiles are taken in launches of this many.

@@ -20,8 +20,7 @@ namespace {
 typedef __bf16 bf16_t;
 
 constexpr uint32_t kThreads  = 256u;
-constexpr uint32_t kPiece    = 4096u;  // elements of a workgroup's turn
-constexpr uint32_t kTurns    = kPiece / (8u * kThreads);
+constexpr uint32_t kPiece    = 2048u;  // elements of a workgroup's turn
 constexpr uint32_t kMaxParts = NERF_EXT_NORM_WORKSPACE / sizeof(double);
 
 // Kernel arguments are kept below 4 KiB.
@@ -47,46 +46,57 @@ struct AdamList {
 };
 
 // Workgroup b of a launch has pieces b * share and on, `share` of them, in their
-// order.  f(tensor, first element, elements).  Counts are 32-bit words: of a
-// select between 64-bit lengths (the piece's end or the tensor's) the compiler
-// kept the wrong condition here and let workgroups run past a tensor's end.
-template <typename List, typename F>
+// order or (kBack) from the last: a pass after another over the same tensors
+// begins with what the one before read last, which the memory-side cache (256
+// MiB) still holds.  f(tensor, first element, elements).  Counts are 32-bit
+// words: of a select between 64-bit lengths (the piece's end or the tensor's)
+// the compiler kept the wrong condition here and let workgroups run past a
+// tensor's end.
+template <bool kBack, typename List, typename F>
 __device__ __forceinline__ void each_piece(const List& l, F&& f) {
     const uint32_t begin = blockIdx.x * l.share, end = min(begin + l.share, l.pieces);
     if (begin >= end) return;
-    uint32_t lo = 0u, hi = l.tensors - 1u;  // the tensor of piece `begin`
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1u) / 2u;
-        if (l.first[mid] <= begin) lo = mid;
-        else hi = mid - 1u;
+    // The tensor of the first piece to come: one less than those that start at
+    // or before it, each lane asking for its own (a search by halves waited for
+    // one load after another).
+    uint32_t piece = kBack ? end - 1u : begin, t = 0u;
+    for (uint32_t base = 0; base < l.tensors; base += 64u) {
+        const uint32_t i = base + (threadIdx.x & 63u);
+        t += (uint32_t)__popcll(__ballot(i < l.tensors && l.first[i] <= piece));
     }
-    uint32_t t = lo;
-    for (uint32_t piece = begin; piece < end; ++piece) {
-        if (piece == l.first[t + 1u]) ++t;
-        f(t, (uint64_t)(piece - l.first[t]) * kPiece, piece + 1u == l.first[t + 1u] ? l.tail[t] : kPiece);
+    t = __builtin_amdgcn_readfirstlane(t - 1u);
+    for (uint32_t left = end - begin; left > 0u; --left) {
+        const uint32_t first = l.first[t], next = l.first[t + 1u];
+        f(t, (uint64_t)(piece - first) * kPiece, piece + 1u == next ? l.tail[t] : kPiece);
+        if (kBack) {
+            if (piece == first) --t;
+            --piece;
+        } else {
+            ++piece;
+            if (piece == next) ++t;
+        }
     }
 }
 
-typedef float floatx8 __attribute__((ext_vector_type(8)));
-template <typename E>
-struct Eight {
-    typedef E type __attribute__((ext_vector_type(8)));
+// A lane's turn: 16 consecutive bytes, as 32-bit values, and back with one
+// rounding; a wave's turn is one contiguous piece of memory (with 32 bytes a
+// lane, fetched by two instructions, Adam ran at 5.0 TB/s, with 16 at 5.6).
+// Arrays are aligned to their elements; the hardware serves wide accesses at
+// any such address.
+template <typename E, uint32_t kN>
+struct Turn {
+    typedef float Wide __attribute__((ext_vector_type(kN)));
+    typedef E Narrow __attribute__((ext_vector_type(kN)));
+    static __device__ __forceinline__ Wide load(const E* p) {
+        Narrow v;
+        __builtin_memcpy(&v, p, sizeof(v));
+        return __builtin_convertvector(v, Wide);
+    }
+    static __device__ __forceinline__ void store(E* p, const Wide& v) {
+        const Narrow h = __builtin_convertvector(v, Narrow);
+        __builtin_memcpy(p, &h, sizeof(h));
+    }
 };
-
-// Eight elements as 32-bit values, and back with one rounding.  Arrays are
-// aligned to their elements; the hardware serves wide accesses at any such
-// address.
-template <typename E>
-__device__ __forceinline__ floatx8 load8(const E* p) {
-    typename Eight<E>::type v;
-    __builtin_memcpy(&v, p, sizeof(v));
-    return __builtin_convertvector(v, floatx8);
-}
-template <typename E>
-__device__ __forceinline__ void store8(E* p, const floatx8& v) {
-    const typename Eight<E>::type h = __builtin_convertvector(v, typename Eight<E>::type);
-    __builtin_memcpy(p, &h, sizeof(h));
-}
 
 // f(pointer type tag) for an element type.
 template <typename F>
@@ -111,18 +121,19 @@ __device__ __forceinline__ double block_sum(double v) {
 // parts[b] = sum of the squares of workgroup b's pieces.
 __global__ __launch_bounds__(kThreads) void k_square_sums(NormList l, double* __restrict__ parts) {
     double s = 0.0;
-    each_piece(l, [&](uint32_t t, uint64_t first, uint32_t n) {
+    each_piece<false>(l, [&](uint32_t t, uint64_t first, uint32_t n) {
         with_type(l.dtype[t], [&](auto* tag) {
             using E       = std::remove_pointer_t<decltype(tag)>;
             const E* data = (const E*)l.data[t] + first;
+            constexpr uint32_t kN = 16u / sizeof(E), kTurns = kPiece / (kN * kThreads);
             if (n == kPiece) {
-                floatx8 g[kTurns];
+                typename Turn<E, kN>::Wide g[kTurns];
 #pragma unroll
-                for (uint32_t k = 0; k < kTurns; ++k) g[k] = load8(data + 8u * (k * kThreads + threadIdx.x));
+                for (uint32_t k = 0; k < kTurns; ++k) g[k] = Turn<E, kN>::load(data + kN * (k * kThreads + threadIdx.x));
 #pragma unroll
                 for (uint32_t k = 0; k < kTurns; ++k)
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) s += (double)g[k][r] * (double)g[k][r];
+                    for (uint32_t r = 0; r < kN; ++r) s += (double)g[k][r] * (double)g[k][r];
             } else {
                 for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
                     const double g = (double)(float)data[i];
@@ -155,17 +166,18 @@ __global__ __launch_bounds__(kThreads) void k_clip(NormList l, const double* __r
     const float v      = norm_of(parts, n);
     const float factor = v > max_norm && isfinite(v) ? max_norm / v : 1.0f;
     if (blockIdx.x == 0u && threadIdx.x == 0u) *norm = v;
-    each_piece(l, [&](uint32_t t, uint64_t first, uint32_t n) {
+    each_piece<true>(l, [&](uint32_t t, uint64_t first, uint32_t n) {
         with_type(l.dtype[t], [&](auto* tag) {
             using E       = std::remove_pointer_t<decltype(tag)>;
             const E* data = (const E*)l.data[t] + first;
             E* out        = (E*)l.out[t] + first;
+            constexpr uint32_t kN = 16u / sizeof(E), kTurns = kPiece / (kN * kThreads);
             if (n == kPiece) {
-                floatx8 g[kTurns];
+                typename Turn<E, kN>::Wide g[kTurns];
 #pragma unroll
-                for (uint32_t k = 0; k < kTurns; ++k) g[k] = load8(data + 8u * (k * kThreads + threadIdx.x));
+                for (uint32_t k = 0; k < kTurns; ++k) g[k] = Turn<E, kN>::load(data + kN * (k * kThreads + threadIdx.x));
 #pragma unroll
-                for (uint32_t k = 0; k < kTurns; ++k) store8(out + 8u * (k * kThreads + threadIdx.x), g[k] * factor);
+                for (uint32_t k = 0; k < kTurns; ++k) Turn<E, kN>::store(out + kN * (k * kThreads + threadIdx.x), g[k] * factor);
             } else {
                 for (uint32_t i = threadIdx.x; i < n; i += kThreads) out[i] = (E)((float)data[i] * factor);
             }
@@ -183,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void k_adam_tensors(AdamList l, AdamRule 
     if (skipped && blockIdx.x == 0u && threadIdx.x == 0u) *skipped = skip ? 1u : 0u;
     if (skip) return;
     const float gs = (gn > r.clip && gn > 0.0f ? r.clip / gn : 1.0f) * (1.0f / r.loss_scale);
-    each_piece(l, [&](uint32_t t, uint64_t first, uint32_t n) {
+    each_piece<true>(l, [&](uint32_t t, uint64_t first, uint32_t n) {
         float *param = l.param[t] + first, *ms = l.m[t] + first, *vs = l.v[t] + first;
         const float* grad = l.grad[t] + first;
         void* copy        = l.copy[t];
@@ -194,24 +206,35 @@ __global__ __launch_bounds__(kThreads) void k_adam_tensors(AdamList l, AdamRule 
             p = p - r.lr * (m * r.bc1) / (sqrtf(v * r.bc2) + r.eps);
         };
         if (n == kPiece) {
+            using F4 = Turn<float, 4u>;
+            // The next turn's values are on their way while this one's are written.
+            F4::Wide p[2], m[2], v[2], g[2];
+            auto fetch = [&](uint32_t k) {
+                const uint32_t i = 4u * (k * kThreads + threadIdx.x);
+                p[k & 1u] = F4::load(param + i);
+                m[k & 1u] = F4::load(ms + i);
+                v[k & 1u] = F4::load(vs + i);
+                g[k & 1u] = F4::load(grad + i);
+            };
+            constexpr uint32_t kTurns = kPiece / (4u * kThreads);
+            fetch(0u);
 #pragma unroll
             for (uint32_t k = 0; k < kTurns; ++k) {
-                const uint32_t i = 8u * (k * kThreads + threadIdx.x);
-                floatx8 p = load8(param + i), m = load8(ms + i), v = load8(vs + i);
-                const floatx8 g = load8(grad + i);
+                const uint32_t i = 4u * (k * kThreads + threadIdx.x), h = k & 1u;
+                if (k + 1u < kTurns) fetch(k + 1u);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float pe = p[e], me = m[e], ve = v[e];
-                    one(pe, g[e], me, ve);
-                    p[e] = pe;
-                    m[e] = me;
-                    v[e] = ve;
+                for (int e = 0; e < 4; ++e) {
+                    float pe = p[h][e], me = m[h][e], ve = v[h][e];
+                    one(pe, g[h][e], me, ve);
+                    p[h][e] = pe;
+                    m[h][e] = me;
+                    v[h][e] = ve;
                 }
-                store8(param + i, p);
-                store8(ms + i, m);
-                store8(vs + i, v);
-                if (copy && l.dtype[t] == NERF_EXT_F16) store8((half_t*)copy + first + i, p);
-                else if (copy) store8((bf16_t*)copy + first + i, p);
+                F4::store(param + i, p[h]);
+                F4::store(ms + i, m[h]);
+                F4::store(vs + i, v[h]);
+                if (copy && l.dtype[t] == NERF_EXT_F16) Turn<half_t, 4u>::store((half_t*)copy + first + i, p[h]);
+                else if (copy) Turn<bf16_t, 4u>::store((bf16_t*)copy + first + i, p[h]);
             }
         } else {
             for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
@@ -236,9 +259,8 @@ NerfStatus refuse(const char* fn, const char* why) {
     return NERF_STATUS_INVALID_USAGE;
 }
 
-// Pieces of a list (128 tensors at most) fit 32 bits: 2^24 each, and so does
-// their number rounded up to whole shares.
-constexpr uint64_t kMaxCount   = (uint64_t)kPiece << 24;
+// Pieces of a list (128 tensors at most) fit 32 bits: 2^23 each.
+constexpr uint64_t kMaxCount   = (uint64_t)kPiece << 23;
 constexpr uint32_t kMaxTensors = 1u << 20;                // a list has a part at least
 
 NerfStatus check_grads(const char* fn, const NerfExtGradTensor* tensors, uint32_t count, const float* norm, const void* workspace, uint64_t bytes, bool outputs) {
@@ -250,7 +272,7 @@ NerfStatus check_grads(const char* fn, const NerfExtGradTensor* tensors, uint32_
         const NerfExtGradTensor& t = tensors[i];
         if (t.dtype != NERF_EXT_F32 && t.dtype != NERF_EXT_F16 && t.dtype != NERF_EXT_BF16) return refuse(fn, "unknown dtype of a tensor");
         if (t.reserved != 0u) return refuse(fn, "reserved must be 0");
-        if (t.count > kMaxCount) return refuse(fn, "a tensor has more than 2^36 elements");
+        if (t.count > kMaxCount) return refuse(fn, "a tensor has more than 2^34 elements");
         if (t.count && (!t.grad || (outputs && !t.out))) return refuse(fn, "null data of a tensor");
         if (!aligned(t.grad, element_bytes(t.dtype)) || (outputs && !aligned(t.out, element_bytes(t.dtype)))) return refuse(fn, "a tensor is not aligned to its elements");
     }
@@ -291,7 +313,7 @@ void put_grad(NormList& l, uint32_t i, const NerfExtGradTensor& t) {
 // The parts of all tensors' squares, *n of them.
 hipError_t square_sums(const NerfExtGradTensor* tensors, uint32_t count, double* parts, uint32_t* n, hipStream_t stream) {
     const uint32_t lists = (count + kNormListed - 1u) / kNormListed;
-    const uint32_t most  = std::max(1u, std::min(4u * device_cu_count(), kMaxParts / std::max(1u, lists)));
+    const uint32_t most  = std::max(1u, std::min(8u * device_cu_count(), kMaxParts / std::max(1u, lists)));
     *n = 0u;
     return each_list<NormList, kNormListed>(tensors, count, most, put_grad, [&](const NormList& l, uint32_t blocks) {
         k_square_sums<<<blocks, kThreads, 0, stream>>>(l, parts + *n);
@@ -344,7 +366,7 @@ NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_
         const NerfExtAdamTensor& t = tensors[i];
         if (t.copy && t.copy_dtype != NERF_EXT_F16 && t.copy_dtype != NERF_EXT_BF16) return refuse(fn, "copy_dtype must be NERF_EXT_F16 or NERF_EXT_BF16");
         if (t.reserved != 0u) return refuse(fn, "reserved must be 0");
-        if (t.count > kMaxCount) return refuse(fn, "a tensor has more than 2^36 elements");
+        if (t.count > kMaxCount) return refuse(fn, "a tensor has more than 2^34 elements");
         if (t.count && (!t.param || !t.grad || !t.m || !t.v)) return refuse(fn, "null data of a tensor");
         if (!aligned(t.param, 4u) || !aligned(t.grad, 4u) || !aligned(t.m, 4u) || !aligned(t.v, 4u) || !aligned(t.copy, 2u)) return refuse(fn, "a tensor is not aligned to its elements");
     }

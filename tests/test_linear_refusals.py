@@ -73,7 +73,7 @@ def test_gradient_lists(lib):
         assert call(None) == BAD
         assert call(grads(), norm=None) == BAD and call(grads(), norm=A + 1) == BAD
         assert call(grads(), ws=None) == BAD and call(grads(), ws=A + 8) == BAD and call(grads(), b=nb - 1) == BAD
-        for kw in (dict(dtype=3), dict(reserved=1), dict(grad=None), dict(grad=A + 2), dict(count=(1 << 36) + 1), dict(grad=A + 1, dtype=L.NERF_EXT_F16)):
+        for kw in (dict(dtype=3), dict(reserved=1), dict(grad=None), dict(grad=A + 2), dict(count=(1 << 34) + 1), dict(grad=A + 1, dtype=L.NERF_EXT_F16)):
             assert call(grads(**kw)) == BAD, kw
             assert fn in L.last_error()
         assert call(grads(), n=(1 << 20) + 1) == BAD
@@ -94,7 +94,7 @@ def test_adam_arguments(lib):
 
     assert L.status_of("nerf_ext_adam_step", None, 1, C.byref(hyper), 1, A, None, None) == BAD
     for kw in (dict(h=None), dict(step=0), dict(norm=None), dict(norm=A + 2), dict(skipped=A + 2), dict(n=(1 << 20) + 1), dict(param=None), dict(grad=None), dict(m=None), dict(v=None), dict(param=A + 2), dict(copy=A + 1),
-               dict(copy_dtype=L.NERF_EXT_F32), dict(reserved=1), dict(count=(1 << 36) + 1)):
+               dict(copy_dtype=L.NERF_EXT_F32), dict(reserved=1), dict(count=(1 << 34) + 1)):
         assert call(**kw) == BAD, kw
         assert "nerf_ext_adam_step" in L.last_error()
     for field, value in (("loss_scale", 0.0), ("loss_scale", float("nan")), ("adam_beta1", 1.0), ("adam_beta2", -0.1), ("adam_beta2", float("nan"))):
