@@ -131,41 +131,57 @@ typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
 
 template <typename E>
 struct Rows {
+    const E* base;
     __amdgpu_buffer_rsrc_t rsrc;
     uint32_t ld;
     // Row `first` of an array with rows ld elements apart.
-    __device__ __forceinline__ Rows(const void* data, uint64_t first, uint64_t ld_) : rsrc(__builtin_amdgcn_make_buffer_rsrc((void*)((const E*)data + first * ld_), (short)0, (int)0x7FFFFFFF, 0x00020000)), ld((uint32_t)ld_) {}
-    // Eight elements from (row, p), n of them inside; vec: all, aligned to 16 bytes.
+    __device__ __forceinline__ Rows(const void* data, uint64_t first, uint64_t ld_) : base((const E*)data + first * ld_), rsrc(__builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)0x7FFFFFFF, 0x00020000)), ld((uint32_t)ld_) {}
+    // Eight elements from (row, p), n of them inside; vec: all or none, aligned to
+    // 16 bytes.  Else eight go in one access at any alignment, fewer one by one.
     __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t p) const { return (row * ld + p) * (uint32_t)sizeof(E); }
     __device__ __forceinline__ uintx4 load(uint32_t row, uint32_t p, uint32_t n, bool vec) const {
         static_assert(sizeof(E) == 2);
         if (vec) return __builtin_bit_cast(uintx4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(n ? at(row, p) : kBeyond), 0, 0));
-        short8_t v;
+        uintx4 o = {0u, 0u, 0u, 0u};
+        if (n == 8u) {
+            __builtin_memcpy(&o, base + row * ld + p, 16);
+        } else if (n) {
+            short8_t v;
 #pragma unroll
-        for (uint32_t r = 0; r < 8u; ++r) v[r] = (short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)(r < n ? at(row, p + r) : kBeyond), 0, 0);
-        return __builtin_bit_cast(uintx4, v);
+            for (uint32_t r = 0; r < 8u; ++r) v[r] = (short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)(r < n ? at(row, p + r) : kBeyond), 0, 0);
+            o = __builtin_bit_cast(uintx4, v);
+        }
+        return o;
     }
     __device__ __forceinline__ void store(uint32_t row, uint32_t p, uint32_t n, bool vec, const floatx8& v) const {
         if constexpr (sizeof(E) == 4) {
+            // Copies: a bit cast of part of a vector takes the vector's first part.
+            const floatx4 lo = v.lo, hi = v.hi;
             if (vec) {
-                // Copies: a bit cast of part of a vector takes the vector's first part.
-                const floatx4 lo = v.lo, hi = v.hi;
                 const uint32_t o = n ? at(row, p) : kBeyond;
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, lo), rsrc, (int)o, 0, 0);
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, hi), rsrc, (int)(o + 16u), 0, 0);
-                return;
-            }
+            } else if (n == 8u) {
+                __builtin_memcpy((void*)(base + row * ld + p), &lo, 16);
+                __builtin_memcpy((void*)(base + row * ld + p + 4u), &hi, 16);
+            } else if (n) {
 #pragma unroll
-            for (uint32_t r = 0; r < 8u; ++r) {
-                const float e = v[r];
-                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, e), rsrc, (int)(r < n ? at(row, p + r) : kBeyond), 0, 0);
+                for (uint32_t r = 0; r < 8u; ++r) {
+                    const float e = v[r];
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, e), rsrc, (int)(r < n ? at(row, p + r) : kBeyond), 0, 0);
+                }
             }
         } else {
             const typename Vec<E>::x8 h = __builtin_convertvector(v, typename Vec<E>::x8);
-            if (vec) return __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, h), rsrc, (int)(n ? at(row, p) : kBeyond), 0, 0);
-            const short8_t b = __builtin_bit_cast(short8_t, h);
+            if (vec) {
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, h), rsrc, (int)(n ? at(row, p) : kBeyond), 0, 0);
+            } else if (n == 8u) {
+                __builtin_memcpy((void*)(base + row * ld + p), &h, 16);
+            } else if (n) {
+                const short8_t b = __builtin_bit_cast(short8_t, h);
 #pragma unroll
-            for (uint32_t r = 0; r < 8u; ++r) __builtin_amdgcn_raw_buffer_store_b16(b[r], rsrc, (int)(r < n ? at(row, p + r) : kBeyond), 0, 0);
+                for (uint32_t r = 0; r < 8u; ++r) __builtin_amdgcn_raw_buffer_store_b16(b[r], rsrc, (int)(r < n ? at(row, p + r) : kBeyond), 0, 0);
+            }
         }
     }
 };
@@ -302,6 +318,42 @@ __device__ __forceinline__ constexpr uint32_t chunk_slot(uint32_t line, uint32_t
     return line * (kT ? kB / 8u : 8u) + (chunk ^ chunk_key<kB, kT>(line));
 }
 
+// Eight values from any address.  The hardware serves 16 bytes that start at a
+// multiple of 4 at full rate and others slowly (7 x 1601 -> 1000: 10.2 us with
+// rows that start at odd values, 5.8 us at even ones), so operands whose rows
+// may start at odd values (kWords) are fetched as the five 32-bit words that the
+// values lie in, all of which hold some of them, and put together when they are
+// used.
+typedef uint32_t word4 __attribute__((ext_vector_type(4), aligned(4)));
+template <bool kWords>
+struct Eight {
+    uint4 v;
+    uint32_t fifth[kWords ? 1 : 0];
+
+    template <typename T>
+    __device__ __forceinline__ void fetch(const T* at) {
+        if constexpr (kWords) {
+            const uint32_t half = (uint32_t)((uintptr_t)at >> 1) & 1u;
+            const word4 w       = *reinterpret_cast<const word4*>(at - half);
+            v                   = uint4{w[0], w[1], w[2], w[3]};
+            fifth[0]            = *reinterpret_cast<const uint32_t*>(at + 6u + half);
+        } else {
+            __builtin_memcpy(&v, at, 16);
+        }
+    }
+    // place: the address' number of values, at least its last bit.
+    __device__ __forceinline__ uint4 value(uint32_t place) const {
+        if constexpr (kWords) {
+            const uint32_t s = 16u * (place & 1u);
+            return uint4{__builtin_amdgcn_alignbit(v.y, v.x, s), __builtin_amdgcn_alignbit(v.z, v.y, s), __builtin_amdgcn_alignbit(v.w, v.z, s), __builtin_amdgcn_alignbit(fifth[0], v.w, s)};
+        }
+        return v;
+    }
+};
+// Number of an address in values, for Eight::value.
+template <typename T>
+__device__ __forceinline__ uint32_t value_number(const T* p) { return (uint32_t)((uintptr_t)p >> 1); }
+
 // Eight values of which `some` are an operand's, fetched from `down` values
 // ahead of them: those moved to the front, zeros behind them.
 __device__ __forceinline__ uint4 settled(uint4 v, uint32_t down, uint32_t some) {
@@ -323,71 +375,65 @@ __device__ __forceinline__ uint4 settled(uint4 v, uint32_t down, uint32_t some) 
     return v;
 }
 
+// Where a lane finds eight values of an operand at its edges: from a place that
+// ends with the line (or begins with the array, which has eight values at
+// least), `some` of them the operand's, `down` values on.
+struct Edge {
+    uint64_t at;
+    uint32_t some, down;
+};
+// line: the values' line (row, or k where rows are contiguous) of `lines`, minor
+// their place in it, of `length`.
+__device__ __forceinline__ Edge edge(uint64_t ld, uint32_t line, uint32_t lines, uint32_t minor, uint32_t length) {
+    Edge e;
+    e.some             = line < lines && minor < length ? min(8u, length - minor) : 0u;
+    const uint64_t own = (uint64_t)line * ld + minor, end = own + e.some;
+    e.at               = e.some && end > 8u ? end - 8u : 0ull;
+    e.down             = e.some ? (uint32_t)(own - e.at) : 0u;
+    return e;
+}
+
 // Tile [row0, row0 + kB) x [k0, k0 + 64) into LDS, zeros outside [0, n) x [0, k_end),
 // through registers and at any alignment: fetch() asks for a tile, keep() writes
-// it to LDS.  Every chunk is fetched as 16 bytes inside the array, in a tile at
-// an edge from a place that ends with the line (or begins with the array), and
-// put right in keep(): nothing waits for a load between the loads (with the
-// edges' work between them, one wait each, 20011 x 1209 -> 487 took 112 us).
-template <typename T, uint32_t kB, bool kT, uint32_t kThreads>
+// it to LDS.  What differs at the edges is the addresses, before the loads, and
+// keep(): a branch with a load in it, or an edge's work right behind its load,
+// makes the loads wait for each other (20011 x 1209 -> 487 took 112 us).
+template <typename T, uint32_t kB, bool kT, uint32_t kThreads, bool kWords>
 struct Stager {
     static constexpr uint32_t kChunks = kT ? kB / 8u : 8u;
-    static constexpr uint32_t kLoads  = (kB * 8u + kThreads - 1u) / kThreads;
-    uint4 held[kLoads];
+    static constexpr uint32_t kLoads  = kB * 8u / kThreads;
+    static_assert(kB * 8u % kThreads == 0u);
+    Eight<kWords> held[kLoads];
 
-    struct Place {
-        uint32_t line, chunk, major, minor, some;  // some: values of the chunk inside
-    };
-    static __device__ __forceinline__ Place place(uint32_t i, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) {
-        const uint32_t s = i * kThreads + threadIdx.x;
-        Place o;
-        o.line  = s / kChunks;
-        o.chunk = s % kChunks;
-        o.major = (kT ? k0 : row0) + o.line;
-        o.minor = (kT ? row0 : k0) + 8u * o.chunk;
-        const uint32_t major_end = kT ? k_end : n, minor_end = kT ? n : k_end;
-        o.some = s < kB * 8u && o.major < major_end && o.minor < minor_end ? min(8u, minor_end - o.minor) : 0u;
-        return o;
+    static __device__ __forceinline__ uint32_t line(uint32_t i) { return (i * kThreads + threadIdx.x) / kChunks; }
+    static __device__ __forceinline__ uint32_t chunk(uint32_t i) { return (i * kThreads + threadIdx.x) % kChunks; }
+    static __device__ __forceinline__ bool inner(uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) { return row0 + kB <= n && k0 + kBK <= k_end; }
+    static __device__ __forceinline__ Edge place(uint32_t i, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) {
+        return kT ? edge(ld, k0 + line(i), k_end, row0 + 8u * chunk(i), n) : edge(ld, row0 + line(i), n, k0 + 8u * chunk(i), k_end);
     }
-    static __device__ __forceinline__ bool inner(uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) { return kB * 8u % kThreads == 0u && row0 + kB <= n && k0 + kBK <= k_end; }
 
     __device__ __forceinline__ void fetch(const T* __restrict__ src, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) {
+        uint64_t at[kLoads];
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) at[i] = (uint64_t)((kT ? k0 : row0) + line(i)) * ld + (kT ? row0 : k0) + 8u * chunk(i);
+        if (!inner(n, row0, k0, k_end)) {
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) at[i] = place(i, ld, n, row0, k0, k_end).at;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) held[i].fetch(src + at[i]);
+    }
+    __device__ __forceinline__ void keep(uint4* lds, const T* __restrict__ src, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) const {
+        const uint32_t first = value_number(src);
         if (inner(n, row0, k0, k_end)) {
 #pragma unroll
-            for (uint32_t i = 0; i < kLoads; ++i) {
-                const Place o = place(i, n, row0, k0, k_end);
-                __builtin_memcpy(&held[i], src + (uint64_t)o.major * ld + o.minor, 16);
-            }
-        } else if ((uint64_t)((kT ? k_end : n) - 1u) * ld + (kT ? n : k_end) >= 8u) {
+            for (uint32_t i = 0; i < kLoads; ++i) lds[chunk_slot<kB, kT>(line(i), chunk(i))] = held[i].value(first + ((kT ? k0 : row0) + line(i)) * (uint32_t)ld + (kT ? row0 : k0));
+        } else {
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
-                const Place o      = place(i, n, row0, k0, k_end);
-                const uint64_t end = (uint64_t)o.major * ld + o.minor + o.some;
-                __builtin_memcpy(&held[i], src + (o.some && end > 8u ? end - 8u : 0ull), 16);
+                const Edge e                                 = place(i, ld, n, row0, k0, k_end);
+                lds[chunk_slot<kB, kT>(line(i), chunk(i))] = settled(held[i].value(first + (uint32_t)e.at), e.down, e.some);
             }
-        } else {  // an array of fewer than eight values
-#pragma unroll
-            for (uint32_t i = 0; i < kLoads; ++i) {
-                const Place o = place(i, n, row0, k0, k_end);
-                short8_t h    = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-                for (uint32_t j = 0; j < 7u; ++j)
-                    if (j < o.some) h[j] = __builtin_bit_cast(short, src[(uint64_t)o.major * ld + o.minor + j]);
-                held[i] = __builtin_bit_cast(uint4, h);
-            }
-        }
-    }
-    __device__ __forceinline__ void keep(uint4* lds, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) const {
-        const bool settle = !inner(n, row0, k0, k_end) && (uint64_t)((kT ? k_end : n) - 1u) * ld + (kT ? n : k_end) >= 8u;
-#pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i) {
-            const Place o = place(i, n, row0, k0, k_end);
-            uint4 v       = held[i];
-            if (settle) {
-                const uint64_t at = (uint64_t)o.major * ld + o.minor;
-                v                 = settled(v, o.some ? (at + o.some >= 8u ? 8u - o.some : (uint32_t)at) : 0u, o.some);
-            }
-            if (kB * 8u % kThreads == 0u || i * kThreads + threadIdx.x < kB * 8u) lds[chunk_slot<kB, kT>(o.line, o.chunk)] = v;
         }
     }
 };
@@ -461,6 +507,13 @@ __device__ __forceinline__ typename Vec<T>::x8 fragment(const uint4* lds, uint32
     }
 }
 
+// Has a fragment in registers here.  The compiler moves a transposing read that
+// is used behind a barrier to behind it, where its LDS is written again.
+template <typename V>
+__device__ __forceinline__ void settle_here(V& v) {
+    asm volatile("" : "+v"(v)::"memory");
+}
+
 // Waits until at most `kLater` of the wave's own loads are on their way, and
 // then for the workgroup.
 template <uint32_t kLater>
@@ -472,14 +525,17 @@ __device__ __forceinline__ void arrived() {
 }
 
 // kBP x kBQ outputs a workgroup, kWP x kWQ waves, kDepth tiles of 64 k at a time
-// in LDS or on their way there.  kAligned: both operands go straight into LDS;
-// else the tiles on their way wait in registers.
-template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, bool kQT, bool kAligned, typename Out>
+// in LDS or on their way there.  kMode: both operands go straight into LDS
+// (kDirect), or the tiles on their way wait in registers, fetched by chunks or as
+// words.
+enum Mode : uint32_t { kDirect, kByChunks, kByWords };
+template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, bool kQT, Mode kMode, typename Out>
 __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out) {
     constexpr uint32_t kThreads = kWP * kWQ * 64u;
     constexpr uint32_t kFP = kBP / kWP / 16u, kFQ = kBQ / kWQ / 16u;
     // Variables of their own, so that the compiler sees that a read of one is no
     // read of what is on its way into another.
+    constexpr bool kAligned  = kMode == kDirect;
     constexpr uint32_t kTile = (kBP + kBQ) * 8u;
     static_assert(kDepth == 2u || kDepth == 4u);
     __shared__ uint4 lds0[kTile], lds1[kAligned ? kTile : 1u], lds2[kAligned && kDepth == 4u ? kTile : 1u], lds3[kAligned && kDepth == 4u ? kTile : 1u];
@@ -606,8 +662,8 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
         }
     } else {
         // The next kDepth - 1 tiles wait in registers.
-        Stager<T, kBP, kPT, kThreads> stage_p[kDepth - 1u];
-        Stager<T, kBQ, kQT, kThreads> stage_q[kDepth - 1u];
+        Stager<T, kBP, kPT, kThreads, kMode == kByWords> stage_p[kDepth - 1u];
+        Stager<T, kBQ, kQT, kThreads, kMode == kByWords> stage_q[kDepth - 1u];
         auto fetch = [&](uint32_t d, uint32_t k) {
             stage_p[d].fetch((const T*)A.p, A.ldp, A.np, p0, k, k_end);
             stage_q[d].fetch((const T*)A.q, A.ldq, A.nq, q0, k, k_end);
@@ -621,8 +677,8 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
             for (uint32_t d = 0; d < kDepth - 1u; ++d) {
                 const uint32_t kd = k + kBK * d;
                 if (kd < k_end) {
-                    stage_p[d].keep(lds0, A.ldp, A.np, p0, kd, k_end);
-                    stage_q[d].keep(lds0 + kBP * 8u, A.ldq, A.nq, q0, kd, k_end);
+                    stage_p[d].keep(lds0, (const T*)A.p, A.ldp, A.np, p0, kd, k_end);
+                    stage_q[d].keep(lds0 + kBP * 8u, (const T*)A.q, A.ldq, A.nq, q0, kd, k_end);
                     __syncthreads();
                     if (kd + kBK * (kDepth - 1u) < k_end) fetch(d, kd + kBK * (kDepth - 1u));
                     multiply(lds0);
@@ -689,8 +745,10 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
 // workgroup that hold other p read the same Q at about the same time, from the
 // CU's cache.
 constexpr uint32_t kStreamWaves = 8u;
-template <typename T, uint32_t kKS, uint32_t kFP, bool kPT, bool kRagged, typename Out>
+template <typename T, uint32_t kKS, uint32_t kFP, bool kPT, bool kRagged, bool kWords, typename Out>
 __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out out, uint32_t p_waves) {
+    // Where P takes half of the registers, the outputs' edges have to do without any.
+    if constexpr (kKS * kFP == 32u) out.vec = true;
     constexpr uint32_t kThreads = kStreamWaves * 64u, kSP = 16u * kFP, kBP = 256u;
     constexpr uint32_t kLanes = kSP / 8u, kPasses = 16u * kLanes / 64u;
     using x8 = typename Vec<T>::x8;
@@ -703,20 +761,23 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
     x8 fp[kKS][kFP];
     {
         const float bias = thread_bias<kBP>(out, p0);
-        Stager<T, kBP, kPT, kThreads> stager;
+        Stager<T, kBP, kPT, kThreads, true> stager;
         stager.fetch((const T*)A.p, A.ldp, A.np, p0, 0u, A.nk);
         if (Out::kBias && threadIdx.x < kBP) reinterpret_cast<float*>(lds_bias)[threadIdx.x] = bias;
         const uint32_t base = fragment_base<kBP, kPT>(wp & ~127u);
 #pragma unroll
         for (uint32_t s = 0; s < kKS; s += 2u) {
-            stager.keep(lds, A.ldp, A.np, p0, 32u * s, A.nk);
+            stager.keep(lds, (const T*)A.p, A.ldp, A.np, p0, 32u * s, A.nk);
             __syncthreads();
             if (s + 2u < kKS) stager.fetch((const T*)A.p, A.ldp, A.np, p0, 32u * (s + 2u), A.nk);
 #pragma unroll
             for (uint32_t i = 0; i < kFP; ++i)
 #pragma unroll
                 for (uint32_t h = 0; h < 2u; ++h)
-                    if (s + h < kKS) fp[s + h][i] = fragment<T, kBP, kPT>(lds, base, (wp & 127u) / 16u + i, h);
+                    if (s + h < kKS) {
+                        fp[s + h][i] = fragment<T, kBP, kPT>(lds, base, (wp & 127u) / 16u + i, h);
+                        settle_here(fp[s + h][i]);
+                    }
             __syncthreads();
         }
     }
@@ -729,20 +790,23 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
     // as 8 values that end with the row (or begin with the array, in its first
     // rows), and moved down by `down` values when they are used.
     const uint32_t left = A.nk % 32u, some = left > 8u * g ? min(8u, left - 8u * g) : 0u;
-    uint32_t down = 0u;
-    x8 fq[kKS];
+    uint32_t down = 0u, place = 0u, place_last = 0u;  // place: see Eight::value
+    Eight<kWords> fq[kKS];
 #pragma unroll
-    for (uint32_t s = 0; s < kKS; ++s) fq[s] = x8{};
+    for (uint32_t s = 0; s < kKS; ++s) fq[s] = Eight<kWords>{};
     auto fetch_q = [&](uint32_t tile) {
         const uint64_t first = (uint64_t)min(tile * 16u + l, A.nq - 1u) * A.ldq + 8u * g;
         const T* at          = (const T*)A.q + first;
+        place                = value_number(at);
 #pragma unroll
         for (uint32_t s = 0; s < kKS; ++s) {
-            if (s < whole) __builtin_memcpy(&fq[s], at + 32u * s, 16);
+            if (s < whole) fq[s].fetch(at + 32u * s);
             if (kRagged && s == whole) {
                 const uint64_t end = first + 32u * s + some, from = end > 8u ? end - 8u : 0ull;
                 down               = some ? (uint32_t)(first + 32u * s - from) : 0u;
-                __builtin_memcpy(&fq[s], (const T*)A.q + (some ? from : 0ull), 16);
+                const T* at_last   = (const T*)A.q + (some ? from : 0ull);
+                place_last         = value_number(at_last);
+                fq[s].fetch(at_last);
             }
         }
     };
@@ -767,9 +831,10 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
         for (uint32_t i = 0; i < kFP; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t s = 0; s < kKS; ++s) {
-            if (kRagged && s == whole) fq[s] = __builtin_bit_cast(x8, settled(__builtin_bit_cast(uint4, fq[s]), down, some));
+            uint4 v = fq[s].value(place);
+            if (kRagged && s == whole) v = settled(fq[s].value(place_last), down, some);
 #pragma unroll
-            for (uint32_t i = 0; i < kFP; ++i) acc[i] = Vec<T>::mfma(fp[s][i], fq[s], acc[i]);
+            for (uint32_t i = 0; i < kFP; ++i) acc[i] = Vec<T>::mfma(fp[s][i], __builtin_bit_cast(x8, v), acc[i]);
         }
         if (tile + stride < tiles) {
             fetch_q(tile + stride);
@@ -790,6 +855,235 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
             if (kLate) next[t] = out.load((tile + stride) * 16u, r, p, inside(tile + stride, t));
         }
         asm volatile("" ::: "memory");
+    }
+}
+
+// --------------------------------------------------------------- few tiles
+// Products of too few outputs to occupy the card by tiles: what counts is the
+// time of one workgroup and the number of launches.  A workgroup has a tile of
+// 16 kF x 16 kF outputs, its eight waves every eighth 32 k each; a wave fetches
+// its operands from memory itself, several steps at a time and without waiting
+// for the others, and the eight sums are added in LDS in their order.  (A
+// launch costs the host 3.5 us, about what such a kernel takes; one with 64 x 64
+// tiles whose k were split over workgroups and a second one to join them took
+// 12 us for 7 x 1601 -> 999, this one 6 us.)
+constexpr uint32_t kFewWaves = 8u;
+
+// 16 kF rows x 32 k of an operand, any alignment, on its way to one wave; the
+// edges as Stager has them.  Rows outside are other rows: their products are in
+// outputs that nothing reads.
+template <typename T, uint32_t kF, bool kT, bool kWords>
+struct FewOperand {
+    using x8 = typename Vec<T>::x8;
+    static constexpr uint32_t kChunks = 2u * kF;  // of a line of 16 kF rows (kT)
+    Eight<kWords> held[kF];
+
+    static __device__ __forceinline__ uint64_t own(uint32_t i, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0) {
+        const uint32_t lane = threadIdx.x & 63u;
+        if (kT) return (uint64_t)(k0 + (i * 64u + lane) / kChunks) * ld + row0 + 8u * ((i * 64u + lane) % kChunks);
+        return (uint64_t)min(row0 + 16u * i + (lane & 15u), n - 1u) * ld + k0 + 8u * (lane >> 4);
+    }
+    static __device__ __forceinline__ Edge place(uint32_t i, uint64_t ld, uint32_t n, uint32_t nk, uint32_t row0, uint32_t k0) {
+        const uint32_t lane = threadIdx.x & 63u;
+        if (kT) return edge(ld, k0 + (i * 64u + lane) / kChunks, nk, row0 + 8u * ((i * 64u + lane) % kChunks), n);
+        return edge(ld, min(row0 + 16u * i + (lane & 15u), n - 1u), n, k0 + 8u * (lane >> 4), nk);
+    }
+    static __device__ __forceinline__ bool inner(uint32_t n, uint32_t nk, uint32_t row0, uint32_t k0) { return k0 + 32u <= nk && (!kT || row0 + 16u * kF <= n); }
+
+    __device__ __forceinline__ void fetch(const Operands& A, const T* __restrict__ src, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0) {
+        uint64_t at[kF];
+#pragma unroll
+        for (uint32_t i = 0; i < kF; ++i) at[i] = own(i, ld, n, row0, k0);
+        if (!inner(n, A.nk, row0, k0)) {
+#pragma unroll
+            for (uint32_t i = 0; i < kF; ++i) at[i] = place(i, ld, n, A.nk, row0, k0).at;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kF; ++i) held[i].fetch(src + at[i]);
+    }
+    // The fragments of what was fetched; lds: 1024 kF bytes of the wave's own (kT).
+    __device__ __forceinline__ void take(const Operands& A, const T* __restrict__ src, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, char* lds, x8 out[kF]) {
+        const uint32_t first = value_number(src);
+        uint4 v[kF];
+        if (inner(n, A.nk, row0, k0)) {
+#pragma unroll
+            for (uint32_t i = 0; i < kF; ++i) v[i] = held[i].value(first + (uint32_t)own(i, ld, n, row0, k0));
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kF; ++i) {
+                const Edge e = place(i, ld, n, A.nk, row0, k0);
+                v[i]         = settled(held[i].value(first + (uint32_t)e.at), e.down, e.some);
+            }
+        }
+        if constexpr (!kT) {
+#pragma unroll
+            for (uint32_t i = 0; i < kF; ++i) out[i] = __builtin_bit_cast(x8, v[i]);
+        } else {
+            const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, g = lane >> 4;
+            auto slot = [](uint32_t line, uint32_t chunk) { return line * kChunks + (chunk ^ (kF == 4u ? chunk_key<64u, true>(line) : 0u)); };
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (uint32_t i = 0; i < kF; ++i) reinterpret_cast<uint4*>(lds)[slot((i * 64u + lane) / kChunks, (i * 64u + lane) % kChunks)] = v[i];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (uint32_t i = 0; i < kF; ++i) {
+                short4_t h[2];
+#pragma unroll
+                for (uint32_t half = 0; half < 2u; ++half) {
+                    const uint32_t row = 16u * i + 4u * (l & 3u);
+                    h[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(lds + 16u * slot(8u * g + 4u * half + (l >> 2), row >> 3) + 2u * (row & 7u)));
+                }
+                out[i] = __builtin_bit_cast(x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kF; ++i) settle_here(out[i]);
+        }
+    }
+};
+
+constexpr uint32_t few_lds(uint32_t f) { return kFewWaves * std::max(16u * f * 16u * f * 4u, 2048u * f); }
+
+template <typename T, uint32_t kF, bool kPT, bool kQT, bool kWords, typename Out>
+__device__ __forceinline__ void few_tile(const Operands& A, const Out& out, uint32_t p0, uint32_t q0, char* lds, float* lds_sums) {
+    constexpr bool kSums = std::is_same_v<Out, SumOut>;
+    constexpr uint32_t kDepth = kF == 1u ? 8u : kF == 2u ? 3u : 2u;  // steps on their way
+    constexpr uint32_t kSP = 16u * kF, kEights = 16u * kF * kSP / 8u;
+    using x8 = typename Vec<T>::x8;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
+
+    // What the outputs need besides the sums: the thread's eight outputs.
+    const uint32_t row = threadIdx.x / (kSP / 8u), col = 8u * (threadIdx.x % (kSP / 8u)), p = p0 + col;
+    const uint32_t n = threadIdx.x < kEights && q0 + row < out.nq && p < out.np ? min(8u, out.np - p) : 0u;
+    floatx8 bias = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (Out::kBias) {
+        if (out.bias) {
+#pragma unroll
+            for (uint32_t r = 0; r < 8u; ++r) bias[r] = r < n ? out.bias[p + r] : 0.0f;
+        }
+    }
+    const typename Out::Aux aux = out.load(q0, row, p, n);
+
+    floatx4 acc[kF][kF], sums[kF];
+#pragma unroll
+    for (uint32_t j = 0; j < kF; ++j) {
+        sums[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t i = 0; i < kF; ++i) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const bool take_sums = kSums && p0 == 0u;
+    x8 ones;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ones[j] = (T)1.0f;
+    FewOperand<T, kF, kPT, kWords> op[kDepth];
+    FewOperand<T, kF, kQT, kWords> oq[kDepth];
+    char* mine = lds + wave * 2048u * kF;
+    auto fetch = [&](uint32_t d, uint32_t k) {
+        op[d].fetch(A, (const T*)A.p, A.ldp, A.np, p0, k);
+        oq[d].fetch(A, (const T*)A.q, A.ldq, A.nq, q0, k);
+    };
+    constexpr uint32_t kStride = 32u * kFewWaves;
+#pragma unroll
+    for (uint32_t d = 0; d < kDepth; ++d)
+        if (32u * wave + kStride * d < A.nk) fetch(d, 32u * wave + kStride * d);
+    for (uint32_t k = 32u * wave; k < A.nk; k += kStride * kDepth) {
+#pragma unroll
+        for (uint32_t d = 0; d < kDepth; ++d) {
+            const uint32_t kd = k + kStride * d;
+            if (kd < A.nk) {
+                x8 fp[kF], fq[kF];
+                op[d].take(A, (const T*)A.p, A.ldp, A.np, p0, kd, mine, fp);
+                oq[d].take(A, (const T*)A.q, A.ldq, A.nq, q0, kd, mine + 1024u * kF, fq);
+                if (kd + kStride * kDepth < A.nk) fetch(d, kd + kStride * kDepth);
+#pragma unroll
+                for (uint32_t i = 0; i < kF; ++i)
+#pragma unroll
+                    for (uint32_t j = 0; j < kF; ++j) acc[i][j] = Vec<T>::mfma(fp[i], fq[j], acc[i][j]);
+                if (take_sums) {
+#pragma unroll
+                    for (uint32_t j = 0; j < kF; ++j) sums[j] = Vec<T>::mfma(ones, fq[j], sums[j]);
+                }
+            }
+        }
+    }
+
+    __syncthreads();  // the waves' own pieces become those of the sums
+    floatx4* strips = reinterpret_cast<floatx4*>(lds);
+    constexpr uint32_t kStrip = 16u * kF * kSP / 4u;
+#pragma unroll
+    for (uint32_t j = 0; j < kF; ++j) {
+        const uint32_t r = 16u * j + (lane & 15u);
+#pragma unroll
+        for (uint32_t i = 0; i < kF; ++i) strips[wave * kStrip + r * (kSP / 4u) + ((4u * i + (lane >> 4)) ^ (r & 3u))] = acc[i][j];
+        if (take_sums && lane < 16u) lds_sums[wave * 16u * kF + r] = sums[j][0];
+    }
+    __syncthreads();
+    if (threadIdx.x < kEights) {
+        floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t w = 0; w < kFewWaves; ++w) {
+            v.lo += strips[w * kStrip + row * (kSP / 4u) + ((col / 4u) ^ (row & 3u))];
+            v.hi += strips[w * kStrip + row * (kSP / 4u) + ((col / 4u + 1u) ^ (row & 3u))];
+        }
+        out.put(q0, row, p, n, v, bias, aux);
+    }
+    if constexpr (kSums) {
+        if (take_sums && out.row_sums && threadIdx.x < 16u * kF && q0 + threadIdx.x < out.nq) {
+            float v = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kFewWaves; ++w) v += lds_sums[w * 16u * kF + threadIdx.x];
+            out.row_sums[q0 + threadIdx.x] = v;
+        }
+    }
+}
+
+template <typename T, uint32_t kF, bool kWords>
+__global__ __launch_bounds__(kFewWaves * 64u) void k_few_forward(Operands A, ForwardOut<T> out) {
+    __shared__ floatx4 lds[few_lds(kF) / 16u];
+    few_tile<T, kF, false, false, kWords>(A, out, blockIdx.x * 16u * kF, blockIdx.y * 16u * kF, reinterpret_cast<char*>(lds), nullptr);
+}
+
+// Both gradients in one launch: first the tiles of dx, x_tiles across and
+// x_blocks in all, then those of dW.
+template <typename T, uint32_t kF, bool kWords>
+__global__ __launch_bounds__(kFewWaves * 64u) void k_few_backward(Operands X, InputGradientOut<T> x_out, uint32_t x_tiles, uint32_t x_blocks, Operands W, SumOut w_out, uint32_t w_tiles) {
+    __shared__ floatx4 lds[few_lds(kF) / 16u];
+    __shared__ float lds_sums[kFewWaves * 16u * kF];
+    if (blockIdx.x < x_blocks) {
+        few_tile<T, kF, true, false, kWords>(X, x_out, blockIdx.x % x_tiles * 16u * kF, blockIdx.x / x_tiles * 16u * kF, reinterpret_cast<char*>(lds), nullptr);
+    } else {
+        const uint32_t b = blockIdx.x - x_blocks;
+        few_tile<T, kF, true, true, kWords>(W, w_out, b % w_tiles * 16u * kF, b / w_tiles * 16u * kF, reinterpret_cast<char*>(lds), lds_sums);
+    }
+}
+
+// Operands of fewer than eight values in all (at most eight k then): a thread
+// computes eight outputs from memory.
+template <typename T, bool kPT, bool kQT, typename Out>
+__global__ __launch_bounds__(256) void k_tiny(Operands A, Out out) {
+    const uint32_t eights = (out.np + 7u) / 8u;
+    const uint64_t total = (uint64_t)eights * out.nq;
+    for (uint64_t base = (uint64_t)blockIdx.x * 256u; base < total; base += (uint64_t)gridDim.x * 256u) {
+        const uint64_t at = base + threadIdx.x;
+        const uint32_t q0 = (uint32_t)(base / eights), q = (uint32_t)(at / eights), p = 8u * (uint32_t)(at % eights), n = at < total ? min(8u, out.np - p) : 0u;
+        const typename Out::Aux aux = out.load(q0, q - q0, p, n);
+        floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, b = v;
+        float sum = 0.0f;
+        for (uint32_t k = 0; n && k < A.nk; ++k) {
+            const float x = (float)((const T*)A.q)[kQT ? k * A.ldq + q : q * A.ldq + k];
+            sum += x;
+#pragma unroll
+            for (uint32_t r = 0; r < 8u; ++r) v[r] += r < n ? x * (float)((const T*)A.p)[kPT ? k * A.ldp + p + r : (uint64_t)(p + r) * A.ldp + k] : 0.0f;
+        }
+        if constexpr (Out::kBias) {
+            if (out.bias) {
+#pragma unroll
+                for (uint32_t r = 0; r < 8u; ++r) b[r] = r < n ? out.bias[p + r] : 0.0f;
+            }
+        }
+        out.put(q0, q - q0, p, n, v, b, aux);
+        if constexpr (std::is_same_v<Out, SumOut>) {
+            if (out.row_sums && n && p == 0u) out.row_sums[q] = sum;
+        }
     }
 }
 
@@ -865,10 +1159,12 @@ struct Workspace {
     uint64_t bytes;
 };
 
+// Whether an operand's rows may start at odd values.
+bool odd_rows(const void* p, uint64_t ld) { return (((uintptr_t)p >> 1 | ld) & 1u) != 0u; }
 // Whether an operand's chunks of 8 along its contiguous length are whole and aligned.
 bool whole_chunks(const void* p, uint64_t ld, uint32_t contiguous) { return aligned(p, 16u) && ld % 8u == 0u && contiguous % 8u == 0u; }
 
-template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, bool kQT, bool kAligned, bool kSplit = true, typename Out>
+template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, bool kQT, Mode kMode, bool kSplit = true, typename Out>
 hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipStream_t stream) {
     const uint32_t tp = ceil_div(A.np, kBP), tq = ceil_div(A.nq, kBQ);
     // Split over k until every CU has its workgroups (two; one of the widest
@@ -905,7 +1201,7 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
             so.part     = part;
             float* sums = row_sums ? rest + (parts - 1u) * part : nullptr;
             so.row_sums = sums;
-            k_product<T, kBP, kBQ, kWP, kWQ, kDepth, kPT, kQT, kAligned, SumOut><<<grid, kThreads, 0, stream>>>(A, so);
+            k_product<T, kBP, kBQ, kWP, kWQ, kDepth, kPT, kQT, kMode, SumOut><<<grid, kThreads, 0, stream>>>(A, so);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
             const uint64_t eights = (uint64_t)ceil_div(A.np, 8u) * A.nq;
@@ -913,15 +1209,22 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
             return hipGetLastError();
         }
     }
-    k_product<T, kBP, kBQ, kWP, kWQ, kDepth, kPT, kQT, kAligned, Out><<<grid, kThreads, 0, stream>>>(A, out);
+    k_product<T, kBP, kBQ, kWP, kWQ, kDepth, kPT, kQT, kMode, Out><<<grid, kThreads, 0, stream>>>(A, out);
     return hipGetLastError();
+}
+
+// Whether an operand has fewer than eight values from its first to its last.
+bool few_values(const Operands& A, bool pt, bool qt) {
+    auto values = [](uint64_t ld, uint32_t n, uint32_t nk, bool t) { return t ? (uint64_t)(nk - 1u) * ld + n : (uint64_t)(n - 1u) * ld + nk; };
+    return A.nk == 0u || values(A.ldp, A.np, A.nk, pt) < 8u || values(A.ldq, A.nq, A.nk, qt) < 8u;
 }
 
 template <typename T, uint32_t kKS, bool kPT, typename Out>
 hipError_t launch_stream(const Operands& A, const Out& out, hipStream_t stream) {
     // p a wave holds: 64, whose 16-bit outputs are whole lines; 32 where there are
-    // no more, or where 64 with the cut rows' work take more registers than there are.
-    const bool ragged = A.nk % 32u != 0u, narrow = A.np <= 32u || (ragged && kKS == 8u);
+    // no more, or where 64 and the work for cut rows take more registers than there
+    // are.
+    const bool ragged = A.nk % 32u != 0u, odd = odd_rows(A.q, A.ldq), narrow = A.np <= 32u || (kKS == 8u && (ragged || !out.vec || odd));
     const uint32_t wide = narrow ? 32u : 64u, most = 256u / wide;
     uint32_t p_waves = 1u;
     while (p_waves < most && wide * p_waves < A.np) p_waves *= 2u;
@@ -929,14 +1232,21 @@ hipError_t launch_stream(const Operands& A, const Out& out, hipStream_t stream) 
     // One workgroup fills a CU's registers; every one goes through as many rows.
     const dim3 grid(std::min(ceil_div(tiles, groups), std::max(1u, device_cu_count() / across)), across);
     constexpr uint32_t kThreads = kStreamWaves * 64u;
+    auto launch = [&](auto p, auto cut, auto words) { k_stream<T, kKS, p(), kPT, cut(), words(), Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves); };
+    const std::integral_constant<uint32_t, 2u> two{};
+    const std::integral_constant<uint32_t, 4u> four{};
+    const std::true_type yes{};
+    const std::false_type no{};
     if (narrow) {
-        if (ragged) k_stream<T, kKS, 2u, kPT, true, Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves);
-        else k_stream<T, kKS, 2u, kPT, false, Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves);
+        if (odd) launch(two, yes, yes);
+        else if (ragged) launch(two, yes, no);
+        else launch(two, no, no);
     } else if constexpr (kKS < 8u) {
-        if (ragged) k_stream<T, kKS, 4u, kPT, true, Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves);
-        else k_stream<T, kKS, 4u, kPT, false, Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves);
+        if (odd) launch(four, yes, yes);
+        else if (ragged) launch(four, yes, no);
+        else launch(four, no, no);
     } else {
-        k_stream<T, kKS, 4u, kPT, false, Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves);
+        launch(four, no, no);
     }
     return hipGetLastError();
 }
@@ -944,6 +1254,11 @@ hipError_t launch_stream(const Operands& A, const Out& out, hipStream_t stream) 
 template <typename T, bool kPT, bool kQT, typename Out>
 hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hipStream_t stream) {
     const uint32_t cus = device_cu_count();
+    if (few_values(A, kPT, kQT)) {
+        const uint64_t threads = (uint64_t)ceil_div(A.np, 8u) * A.nq;
+        k_tiny<T, kPT, kQT, Out><<<(uint32_t)std::min<uint64_t>(ceil_div(threads, 256u), 8u * cus), 256, 0, stream>>>(A, out);
+        return hipGetLastError();
+    }
     if constexpr (!kQT) {
         if (A.nk <= 256u && A.np <= 1024u && A.nq >= 16384u) {
             if (A.nk <= 32u) return launch_stream<T, 1u, kPT>(A, out, stream);
@@ -952,14 +1267,25 @@ hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hi
             return launch_stream<T, 8u, kPT>(A, out, stream);
         }
     }
+    const uint64_t wide = (uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u);
+    const bool wider    = wide >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u && A.nk > 2048u);
     if (!whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, kQT ? A.nq : A.nk)) {
-        if ((uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u) >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u && A.nk > 2048u)) return launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, false>(A, out, row_sums, ws, stream);
-        return launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, false>(A, out, row_sums, ws, stream);
+        const bool odd = odd_rows(A.p, A.ldp) || odd_rows(A.q, A.ldq);
+        if (wider) return odd ? launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
+        return odd ? launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
     }
-    if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) * (kPT && kQT ? ceil_div(A.nk, 1024u) : 1u) >= cus / 2u && A.np > 128u && A.nk >= 512u) return launch_tiles<T, 256, 256, 2, 4, 2, kPT, kQT, true, kPT && kQT>(A, out, row_sums, ws, stream);
-    if ((uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u) >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u && A.nk > 2048u)) return launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, true>(A, out, row_sums, ws, stream);
-    return launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, true>(A, out, row_sums, ws, stream);
+    if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) * (kPT && kQT ? ceil_div(A.nk, 1024u) : 1u) >= cus / 2u && A.np > 128u && A.nk >= 512u)
+        return launch_tiles<T, 256, 256, 2, 4, 2, kPT, kQT, kDirect, kPT && kQT>(A, out, row_sums, ws, stream);
+    if (wider) return launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kDirect>(A, out, row_sums, ws, stream);
+    return launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kDirect>(A, out, row_sums, ws, stream);
 }
+
+// Whether a product is one of few tiles, and of how many 16 outputs a side: the
+// smallest tile of which the card takes all at once, two workgroups a CU; 0
+// where there are more, or so many k that workgroups should share them.
+constexpr uint32_t kFewMaxK = 4096u;
+bool few_operands(const Operands& A, bool pt, bool qt) { return A.nk <= kFewMaxK && !few_values(A, pt, qt); }
+uint64_t few_tiles(const Operands& A, uint32_t f) { return (uint64_t)ceil_div(A.np, 16u * f) * ceil_div(A.nq, 16u * f); }
 
 // rows beyond gridDim's range of 64-row tiles are taken in launches of this many.
 constexpr uint32_t kRowsPerLaunch = 65535u * 64u;
@@ -968,6 +1294,21 @@ template <typename T>
 NerfStatus forward(const NerfExtLinearDesc& d, const void* x, const void* w, const float* bias, const void* residual, void* y, void* pre, Workspace ws, hipStream_t stream) {
     const bool y32 = d.out_dtype == NERF_EXT_F32;
     const bool vec = d.out_features % 8u == 0u && d.y_stride % 8u == 0u && aligned(y, 16u) && aligned(pre, 16u) && (!residual || (d.residual_stride % 8u == 0u && aligned(residual, 16u)));
+    const Operands all{w, x, d.in_features, d.x_stride, d.out_features, d.rows, d.in_features, 0u};
+    if (few_operands(all, false, false)) {
+        const ForwardOut<T> out{bias, (const T*)residual, y, (T*)pre, d.residual_stride, d.y_stride, d.out_features, d.rows, d.activation, y32, vec};
+        const uint32_t most = 2u * device_cu_count();
+        auto launch         = [&](auto f) {
+            const dim3 grid(ceil_div(all.np, 16u * f()), ceil_div(all.nq, 16u * f()));
+            if (odd_rows(x, d.x_stride) || odd_rows(w, d.in_features)) k_few_forward<T, f(), true><<<grid, kFewWaves * 64u, 0, stream>>>(all, out);
+            else k_few_forward<T, f(), false><<<grid, kFewWaves * 64u, 0, stream>>>(all, out);
+            NERF_LAUNCH_CHECK("k_few_forward");
+            return NERF_STATUS_OK;
+        };
+        if (few_tiles(all, 1u) <= most) return launch(std::integral_constant<uint32_t, 1u>{});
+        if (few_tiles(all, 2u) <= most) return launch(std::integral_constant<uint32_t, 2u>{});
+        if (2u * few_tiles(all, 4u) <= most) return launch(std::integral_constant<uint32_t, 4u>{});
+    }
     for (uint64_t r0 = 0; r0 < d.rows; r0 += kRowsPerLaunch) {
         const uint32_t n = (uint32_t)std::min<uint64_t>(kRowsPerLaunch, d.rows - r0);
         const Operands A{w, (const T*)x + r0 * d.x_stride, d.in_features, d.x_stride, d.out_features, n, d.in_features, 0u};
@@ -980,8 +1321,27 @@ NerfStatus forward(const NerfExtLinearDesc& d, const void* x, const void* w, con
 
 template <typename T>
 NerfStatus backward(const NerfExtLinearDesc& d, const void* x, const void* w, const void* delta, const void* pre, const void* add, void* dx, void* dpre, float* dw, float* db, Workspace ws, hipStream_t stream) {
-    if (dx || dpre) {
-        const bool vec = d.in_features % 8u == 0u && (!(add || dx) || d.x_stride % 8u == 0u) && aligned(add, 16u) && aligned(dx, 16u) && aligned(pre, 16u) && aligned(dpre, 16u);
+    const bool vec = d.in_features % 8u == 0u && (!(add || dx) || d.x_stride % 8u == 0u) && aligned(add, 16u) && aligned(dx, 16u) && aligned(pre, 16u) && aligned(dpre, 16u);
+    const Operands all_x{w, delta, d.in_features, d.y_stride, d.in_features, d.rows, d.out_features, 0u}, all_w{x, delta, d.x_stride, d.y_stride, d.in_features, d.out_features, d.rows, 0u};
+    const SumOut w_out{dw, nullptr, 0u, db, d.in_features, d.out_features, d.in_features % 8u == 0u && aligned(dw, 16u)};
+    const bool to_x = (dx || dpre) && d.rows != 0u;
+    if ((!to_x || few_operands(all_x, true, false)) && (!dw || few_operands(all_w, true, true))) {
+        const InputGradientOut<T> x_out{(const T*)add, (T*)dx, (const T*)pre, (T*)dpre, d.x_stride, d.in_features, d.rows, d.activation, vec};
+        const uint32_t most = 2u * device_cu_count();
+        auto blocks         = [&](uint32_t f) { return (to_x ? few_tiles(all_x, f) : 0u) + (dw ? few_tiles(all_w, f) : 0u); };
+        auto launch         = [&](auto f) {
+            const uint32_t across = ceil_div(d.in_features, 16u * f());
+            const uint32_t x_blocks = to_x ? (uint32_t)few_tiles(all_x, f()) : 0u, grid = (uint32_t)blocks(f());
+            if (odd_rows(x, d.x_stride) || odd_rows(w, d.in_features) || odd_rows(delta, d.y_stride)) k_few_backward<T, f(), true><<<grid, kFewWaves * 64u, 0, stream>>>(all_x, x_out, across, x_blocks, all_w, w_out, across);
+            else k_few_backward<T, f(), false><<<grid, kFewWaves * 64u, 0, stream>>>(all_x, x_out, across, x_blocks, all_w, w_out, across);
+            NERF_LAUNCH_CHECK("k_few_backward");
+            return NERF_STATUS_OK;
+        };
+        if (blocks(1u) <= most) return launch(std::integral_constant<uint32_t, 1u>{});
+        if (blocks(2u) <= most) return launch(std::integral_constant<uint32_t, 2u>{});
+        if (blocks(4u) <= most) return launch(std::integral_constant<uint32_t, 4u>{});
+    }
+    if (to_x) {
         for (uint64_t r0 = 0; r0 < d.rows; r0 += kRowsPerLaunch) {
             const uint32_t n = (uint32_t)std::min<uint64_t>(kRowsPerLaunch, d.rows - r0);
             const Operands A{w, (const T*)delta + r0 * d.y_stride, d.in_features, d.y_stride, d.in_features, n, d.out_features, 0u};
@@ -990,11 +1350,7 @@ NerfStatus backward(const NerfExtLinearDesc& d, const void* x, const void* w, co
             NERF_HIP_TRY((launch_product<T, true, false>(A, out, nullptr, ws, stream)));
         }
     }
-    if (dw) {
-        const Operands A{x, delta, d.x_stride, d.y_stride, d.in_features, d.out_features, d.rows, 0u};
-        const SumOut out{dw, nullptr, 0u, db, d.in_features, d.out_features, d.in_features % 8u == 0u && aligned(dw, 16u)};
-        NERF_HIP_TRY((launch_product<T, true, true>(A, out, db, ws, stream)));
-    }
+    if (dw) NERF_HIP_TRY((launch_product<T, true, true>(all_w, w_out, db, ws, stream)));
     return NERF_STATUS_OK;
 }
 
