@@ -786,75 +786,95 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
     const uint32_t groups = kStreamWaves / p_waves, tiles = (A.nq + 15u) / 16u, stride = gridDim.x * groups;
     const uint32_t l = lane & 15u, g = lane >> 4;
     const uint32_t whole = A.nk / 32u;  // steps of 32 k that every row has in full
-    // kRagged, the step after them: `some` of the lane's 8 k are left.  They are fetched
-    // as 8 values that end with the row (or begin with the array, in its first
-    // rows), and moved down by `down` values when they are used.
+    // kRagged, the step after them: `some` of the lane's 8 k are left.  They are
+    // fetched as 8 values that end with the row (or begin with the array, in its
+    // first rows), and moved down by `down` values when they are used.
     const uint32_t left = A.nk % 32u, some = left > 8u * g ? min(8u, left - 8u * g) : 0u;
-    uint32_t down = 0u, place = 0u, place_last = 0u;  // place: see Eight::value
-    Eight<kWords> fq[kKS];
-#pragma unroll
-    for (uint32_t s = 0; s < kKS; ++s) fq[s] = Eight<kWords>{};
-    auto fetch_q = [&](uint32_t tile) {
-        const uint64_t first = (uint64_t)min(tile * 16u + l, A.nq - 1u) * A.ldq + 8u * g;
-        const T* at          = (const T*)A.q + first;
-        place                = value_number(at);
-#pragma unroll
-        for (uint32_t s = 0; s < kKS; ++s) {
-            if (s < whole) fq[s].fetch(at + 32u * s);
-            if (kRagged && s == whole) {
-                const uint64_t end = first + 32u * s + some, from = end > 8u ? end - 8u : 0ull;
-                down               = some ? (uint32_t)(first + 32u * s - from) : 0u;
-                const T* at_last   = (const T*)A.q + (some ? from : 0ull);
-                place_last         = value_number(at_last);
-                fq[s].fetch(at_last);
-            }
-        }
+    // What is on its way: the Q and the epilogue inputs of the kAhead next tiles of
+    // rows, as many as the registers hold beside P.  (With one, 100003 x 64 -> 256
+    // took 33 us from memory and 24 us from cache.)
+    constexpr uint32_t kAhead = kKS <= 2u ? 3u : kKS * kFP <= 16u && !(kKS == 8u && kWords) ? 2u : 1u;
+    // Where even one tile's epilogue inputs take more registers than there are
+    // beside this tile's, they are fetched in their place as these are used.
+    constexpr bool kLate = kKS * kFP == 32u && sizeof(typename Out::Aux) > 16u;
+    struct Coming {
+        Eight<kWords> q[kKS];
+        uint32_t down, place, place_last;  // place: see Eight::value
+        typename Out::Aux aux[kPasses];
     };
-    floatx4* strip = reinterpret_cast<floatx4*>(lds) + wave * (kSP * 4u);
+    Coming coming[kAhead];
     const uint32_t row = lane / kLanes, col = 8u * (lane % kLanes), p = p0 + wp + col;
     const uint32_t n = p < out.np ? min(8u, out.np - p) : 0u;
     auto inside = [&](uint32_t tile, uint32_t pass) { return tile < tiles && tile * 16u + (64u / kLanes) * pass + row < out.nq ? n : 0u; };
-    // The next rows' epilogue inputs: beside this rows', or where that takes more
-    // registers than there are, in their place as they are used.
-    constexpr bool kLate = kKS * kFP == 32u && sizeof(typename Out::Aux) > 16u;
-    typename Out::Aux aux[kPasses], next[kPasses];
-    uint32_t tile = __builtin_amdgcn_readfirstlane(blockIdx.x * groups + wave / p_waves);
-    if (tile >= tiles) return;
-    fetch_q(tile);
-#pragma unroll
-    for (uint32_t t = 0; t < kPasses; ++t) next[t] = out.load(tile * 16u, (64u / kLanes) * t + row, p, inside(tile, t));
-    for (; tile < tiles; tile += stride) {
-#pragma unroll
-        for (uint32_t t = 0; t < kPasses; ++t) aux[t] = next[t];
-        floatx4 acc[kFP];
-#pragma unroll
-        for (uint32_t i = 0; i < kFP; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto fetch_q = [&](Coming& c, uint32_t tile) {
+        const uint64_t first = (uint64_t)min(tile * 16u + l, A.nq - 1u) * A.ldq + 8u * g;
+        const T* at          = (const T*)A.q + first;
+        c.place              = value_number(at);
 #pragma unroll
         for (uint32_t s = 0; s < kKS; ++s) {
-            uint4 v = fq[s].value(place);
-            if (kRagged && s == whole) v = settled(fq[s].value(place_last), down, some);
-#pragma unroll
-            for (uint32_t i = 0; i < kFP; ++i) acc[i] = Vec<T>::mfma(fp[s][i], __builtin_bit_cast(x8, v), acc[i]);
+            if (s < whole) c.q[s].fetch(at + 32u * s);
+            if (kRagged && s == whole) {
+                const uint64_t end = first + 32u * s + some, from = end > 8u ? end - 8u : 0ull;
+                c.down             = some ? (uint32_t)(first + 32u * s - from) : 0u;
+                const T* at_last   = (const T*)A.q + (some ? from : 0ull);
+                c.place_last       = value_number(at_last);
+                c.q[s].fetch(at_last);
+            }
         }
-        if (tile + stride < tiles) {
-            fetch_q(tile + stride);
+    };
+    auto fetch_aux = [&](Coming& c, uint32_t tile, uint32_t t) { c.aux[t] = out.load(tile * 16u, (64u / kLanes) * t + row, p, inside(tile, t)); };
+    floatx4* strip = reinterpret_cast<floatx4*>(lds) + wave * (kSP * 4u);
+    const uint32_t first_tile = __builtin_amdgcn_readfirstlane(blockIdx.x * groups + wave / p_waves);
 #pragma unroll
-            for (uint32_t t = 0; t < kPasses; ++t)
-                if (!kLate) next[t] = out.load((tile + stride) * 16u, (64u / kLanes) * t + row, p, inside(tile + stride, t));
+    for (uint32_t d = 0; d < kAhead; ++d) {
+#pragma unroll
+        for (uint32_t s = 0; s < kKS; ++s) coming[d].q[s] = Eight<kWords>{};
+        if (first_tile + d * stride < tiles) {
+            fetch_q(coming[d], first_tile + d * stride);
+#pragma unroll
+            for (uint32_t t = 0; t < kPasses; ++t) fetch_aux(coming[d], first_tile + d * stride, t);
         }
+    }
+    for (uint32_t turn = first_tile; turn < tiles; turn += kAhead * stride) {
 #pragma unroll
-        for (uint32_t i = 0; i < kFP; ++i) strip[l * (kSP / 4u) + ((4u * i + g) ^ (l & 7u))] = acc[i];
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (uint32_t d = 0; d < kAhead; ++d) {
+            const uint32_t tile = turn + d * stride, later = tile + kAhead * stride;
+            Coming& c           = coming[d];
+            if (tile < tiles) {
+                floatx4 acc[kFP];
 #pragma unroll
-        for (uint32_t t = 0; t < kPasses; ++t) {
-            const uint32_t r = (64u / kLanes) * t + row;
-            floatx8 v;
-            v.lo = strip[r * (kSP / 4u) + ((col / 4u) ^ (r & 7u))];
-            v.hi = strip[r * (kSP / 4u) + ((col / 4u + 1u) ^ (r & 7u))];
-            out.put(tile * 16u, r, p, inside(tile, t), v, bias8<Out>(reinterpret_cast<const float*>(lds_bias), wp + col), aux[t]);
-            if (kLate) next[t] = out.load((tile + stride) * 16u, r, p, inside(tile + stride, t));
+                for (uint32_t i = 0; i < kFP; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (uint32_t s = 0; s < kKS; ++s) {
+                    uint4 v = c.q[s].value(c.place);
+                    if (kRagged && s == whole) v = settled(c.q[s].value(c.place_last), c.down, some);
+#pragma unroll
+                    for (uint32_t i = 0; i < kFP; ++i) acc[i] = Vec<T>::mfma(fp[s][i], __builtin_bit_cast(x8, v), acc[i]);
+                }
+                typename Out::Aux aux[kPasses];
+#pragma unroll
+                for (uint32_t t = 0; t < kPasses; ++t) aux[t] = c.aux[t];
+                if (later < tiles) {
+                    fetch_q(c, later);
+#pragma unroll
+                    for (uint32_t t = 0; t < kPasses; ++t)
+                        if (!kLate) fetch_aux(c, later, t);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kFP; ++i) strip[l * (kSP / 4u) + ((4u * i + g) ^ (l & 7u))] = acc[i];
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+                for (uint32_t t = 0; t < kPasses; ++t) {
+                    const uint32_t r = (64u / kLanes) * t + row;
+                    floatx8 v;
+                    v.lo = strip[r * (kSP / 4u) + ((col / 4u) ^ (r & 7u))];
+                    v.hi = strip[r * (kSP / 4u) + ((col / 4u + 1u) ^ (r & 7u))];
+                    out.put(tile * 16u, r, p, inside(tile, t), v, bias8<Out>(reinterpret_cast<const float*>(lds_bias), wp + col), aux[t]);
+                    if (kLate) fetch_aux(c, later, t);
+                }
+                asm volatile("" ::: "memory");
+            }
         }
-        asm volatile("" ::: "memory");
     }
 }
 
@@ -1087,13 +1107,14 @@ __global__ __launch_bounds__(256) void k_tiny(Operands A, Out out) {
     }
 }
 
-// Joins the parts of a sum that was split over k: 16 slices of a workgroup take
-// every 16th part each, in order, and the slices are added in theirs, so the
-// result is the same every time.  (With one thread an output the reads of 128
-// parts of 256 x 256 sums, one after another, took 73 us.)
-constexpr uint32_t kSlices = 16u, kJoined = 256u / kSlices;
-template <typename Out>
+// Joins the parts of a sum that was split over k: kSlices slices of a workgroup
+// take every kSlices-th part each, in order, and the slices are added in theirs,
+// so the result is the same every time.  (With one thread an output the reads of
+// 128 parts of 256 x 256 sums, one after another, took 73 us; with 16 slices for
+// two parts of 4096 x 2048 sums, 14 of them idle, 59 us where one takes 19 us.)
+template <uint32_t kSlices, typename Out>
 __global__ __launch_bounds__(256) void k_join(const float* first_part, const float* __restrict__ parts, uint64_t part, uint32_t count, const float* __restrict__ sums, float* __restrict__ row_sums, Out out) {
+    constexpr uint32_t kJoined = 256u / kSlices;
     __shared__ floatx4 slice_sum[2][kSlices][kJoined];
     const uint32_t eights = (out.np + 7u) / 8u, slice = threadIdx.x / kJoined, mine = threadIdx.x % kJoined;
     const uint64_t total = (uint64_t)eights * out.nq;
@@ -1101,6 +1122,9 @@ __global__ __launch_bounds__(256) void k_join(const float* first_part, const flo
     for (uint64_t base = (uint64_t)blockIdx.x * kJoined; base < total; base += (uint64_t)gridDim.x * kJoined) {
         const uint64_t at = base + mine;
         const uint32_t q = (uint32_t)(at / eights), p = 8u * (uint32_t)(at % eights), n = at < total ? min(8u, out.np - p) : 0u;
+        // The epilogues count rows from a uniform one: the workgroup's first.
+        const uint32_t q0 = (uint32_t)(base / eights);
+        const typename Out::Aux aux = out.load(q0, q - q0, p, slice == 0u ? n : 0u);
         floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (n) {
 #pragma unroll 8
@@ -1115,14 +1139,13 @@ __global__ __launch_bounds__(256) void k_join(const float* first_part, const flo
                 }
             }
         }
-        __syncthreads();
-        slice_sum[0][slice][mine] = v.lo;
-        slice_sum[1][slice][mine] = v.hi;
-        __syncthreads();
+        if constexpr (kSlices > 1u) {
+            __syncthreads();
+            slice_sum[0][slice][mine] = v.lo;
+            slice_sum[1][slice][mine] = v.hi;
+            __syncthreads();
+        }
         if (slice == 0u) {
-            // The epilogues count rows from a uniform one: the workgroup's first.
-            const uint32_t q0 = (uint32_t)(base / eights);
-            const typename Out::Aux aux = out.load(q0, q - q0, p, n);
 #pragma unroll
             for (uint32_t c = 1; c < kSlices; ++c) {
                 v.lo += slice_sum[0][c][mine];
@@ -1139,11 +1162,22 @@ __global__ __launch_bounds__(256) void k_join(const float* first_part, const flo
         }
     }
     if (row_sums) {
-        for (uint32_t q = blockIdx.x * 256u + threadIdx.x; q < out.nq; q += gridDim.x * 256u) {
+        float(*sum)[kJoined] = reinterpret_cast<float(*)[kJoined]>(slice_sum);
+        for (uint32_t base = blockIdx.x * kJoined; base < out.nq; base += gridDim.x * kJoined) {
+            const uint32_t q = base + mine;
             float s = 0.0f;
+            if (q < out.nq) {
 #pragma unroll 8
-            for (uint32_t c = 0; c < count; ++c) s += sums[(uint64_t)c * out.nq + q];
-            row_sums[q] = s;
+                for (uint32_t c = slice; c < count; c += kSlices) s += sums[(uint64_t)c * out.nq + q];
+            }
+            __syncthreads();
+            sum[slice][mine] = s;
+            __syncthreads();
+            if (slice == 0u && q < out.nq) {
+#pragma unroll
+                for (uint32_t c = 1; c < kSlices; ++c) s += sum[c][mine];
+                row_sums[q] = s;
+            }
         }
     }
 }
@@ -1205,7 +1239,10 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
             const uint64_t eights = (uint64_t)ceil_div(A.np, 8u) * A.nq;
-            k_join<Out><<<(uint32_t)std::min<uint64_t>(ceil_div(eights, kJoined), 4096u), 256, 0, stream>>>(so.out, rest, part, parts, sums, row_sums, out);
+            auto join = [&](auto slices) { k_join<slices(), Out><<<(uint32_t)std::min<uint64_t>(ceil_div(eights, 256u / slices()), 4096u), 256, 0, stream>>>(so.out, rest, part, parts, sums, row_sums, out); };
+            if (parts >= 16u) join(std::integral_constant<uint32_t, 16u>{});
+            else if (parts >= 4u) join(std::integral_constant<uint32_t, 4u>{});
+            else join(std::integral_constant<uint32_t, 1u>{});
             return hipGetLastError();
         }
     }

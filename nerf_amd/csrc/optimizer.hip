@@ -45,16 +45,16 @@ struct AdamList {
     uint32_t tensors, pieces, share;
 };
 
-// Workgroup b of a launch has pieces b * share and on, `share` of them, in their
-// order or (kBack) from the last: a pass after another over the same tensors
+// Worker w (a workgroup, or a wave of one) has pieces w * share and on, `share` of
+// them, in their order or (kBack) from the last: a pass after another over the same tensors
 // begins with what the one before read last, which the memory-side cache (256
 // MiB) still holds.  f(tensor, first element, elements).  Counts are 32-bit
 // words: of a select between 64-bit lengths (the piece's end or the tensor's)
 // the compiler kept the wrong condition here and let workgroups run past a
 // tensor's end.
 template <bool kBack, typename List, typename F>
-__device__ __forceinline__ void each_piece(const List& l, F&& f) {
-    const uint32_t begin = blockIdx.x * l.share, end = min(begin + l.share, l.pieces);
+__device__ __forceinline__ void each_piece(const List& l, uint32_t worker, F&& f) {
+    const uint32_t begin = worker * l.share, end = min(begin + l.share, l.pieces);
     if (begin >= end) return;
     // The tensor of the first piece to come: one less than those that start at
     // or before it, each lane asking for its own (a search by halves waited for
@@ -107,43 +107,60 @@ __device__ __forceinline__ void with_type(uint32_t dtype, F&& f) {
 }
 
 // Sum over the workgroup, in thread 0.
+template <uint32_t kCount>
 __device__ __forceinline__ double block_sum(double v) {
-    __shared__ double ws[kThreads / 64u];
+    __shared__ double ws[kCount / 64u];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) v += __shfl_down(v, d);
     if ((threadIdx.x & 63u) == 0u) ws[threadIdx.x >> 6] = v;
     __syncthreads();
     double s = 0.0;
-    for (uint32_t w = 0; w < kThreads / 64u; ++w) s += ws[w];
+    for (uint32_t w = 0; w < kCount / 64u; ++w) s += ws[w];
     return s;
 }
 
-// parts[b] = sum of the squares of workgroup b's pieces.
-__global__ __launch_bounds__(kThreads) void k_square_sums(NormList l, double* __restrict__ parts) {
+// The sum of the squares of a worker's pieces, the share of it that lane `lane`
+// of the worker's kLanes has.
+template <uint32_t kLanes>
+__device__ __forceinline__ double worker_squares(const NormList& l, uint32_t worker, uint32_t lane) {
     double s = 0.0;
-    each_piece<false>(l, [&](uint32_t t, uint64_t first, uint32_t n) {
+    each_piece<false>(l, worker, [&](uint32_t t, uint64_t first, uint32_t n) {
         with_type(l.dtype[t], [&](auto* tag) {
             using E       = std::remove_pointer_t<decltype(tag)>;
             const E* data = (const E*)l.data[t] + first;
-            constexpr uint32_t kN = 16u / sizeof(E), kTurns = kPiece / (kN * kThreads);
+            constexpr uint32_t kN = 16u / sizeof(E), kTurns = kPiece / (kN * kLanes);
             if (n == kPiece) {
                 typename Turn<E, kN>::Wide g[kTurns];
 #pragma unroll
-                for (uint32_t k = 0; k < kTurns; ++k) g[k] = Turn<E, kN>::load(data + kN * (k * kThreads + threadIdx.x));
+                for (uint32_t k = 0; k < kTurns; ++k) g[k] = Turn<E, kN>::load(data + kN * (k * kLanes + lane));
 #pragma unroll
                 for (uint32_t k = 0; k < kTurns; ++k)
 #pragma unroll
                     for (uint32_t r = 0; r < kN; ++r) s += (double)g[k][r] * (double)g[k][r];
             } else {
-                for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+                for (uint32_t i = lane; i < n; i += kLanes) {
                     const double g = (double)(float)data[i];
                     s += g * g;
                 }
             }
         });
     });
-    s = block_sum(s);
+    return s;
+}
+
+// parts[b] = sum of the squares of workgroup b's pieces.
+__global__ __launch_bounds__(kThreads) void k_square_sums(NormList l, double* __restrict__ parts) {
+    const double s = block_sum<kThreads>(worker_squares<kThreads>(l, blockIdx.x, threadIdx.x));
     if (threadIdx.x == 0u) parts[blockIdx.x] = s;
+}
+
+// A short list's norm in one launch: one workgroup, whose waves share the pieces.
+constexpr uint32_t kShortThreads = 1024u, kShortWaves = kShortThreads / 64u;
+constexpr uint32_t kShortPieces  = 4u * kShortWaves;
+__global__ __launch_bounds__(kShortThreads) void k_norm_short(NormList l, float* __restrict__ norm) {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const double s      = block_sum<kShortThreads>(worker_squares<64u>(l, wave, threadIdx.x & 63u));
+    if (threadIdx.x == 0u) *norm = (float)sqrt(s);
 }
 
 // sqrt of the sum of all parts, the same in every workgroup and thread.
@@ -151,7 +168,7 @@ __device__ __forceinline__ float norm_of(const double* __restrict__ parts, uint3
     __shared__ double total;
     double s = 0.0;
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) s += parts[i];
-    s = block_sum(s);
+    s = block_sum<kThreads>(s);
     if (threadIdx.x == 0u) total = s;
     __syncthreads();
     return (float)sqrt(total);
@@ -166,7 +183,7 @@ __global__ __launch_bounds__(kThreads) void k_clip(NormList l, const double* __r
     const float v      = norm_of(parts, n);
     const float factor = v > max_norm && isfinite(v) ? max_norm / v : 1.0f;
     if (blockIdx.x == 0u && threadIdx.x == 0u) *norm = v;
-    each_piece<true>(l, [&](uint32_t t, uint64_t first, uint32_t n) {
+    each_piece<true>(l, blockIdx.x, [&](uint32_t t, uint64_t first, uint32_t n) {
         with_type(l.dtype[t], [&](auto* tag) {
             using E       = std::remove_pointer_t<decltype(tag)>;
             const E* data = (const E*)l.data[t] + first;
@@ -195,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void k_adam_tensors(AdamList l, AdamRule 
     if (skipped && blockIdx.x == 0u && threadIdx.x == 0u) *skipped = skip ? 1u : 0u;
     if (skip) return;
     const float gs = (gn > r.clip && gn > 0.0f ? r.clip / gn : 1.0f) * (1.0f / r.loss_scale);
-    each_piece<true>(l, [&](uint32_t t, uint64_t first, uint32_t n) {
+    each_piece<true>(l, blockIdx.x, [&](uint32_t t, uint64_t first, uint32_t n) {
         float *param = l.param[t] + first, *ms = l.m[t] + first, *vs = l.v[t] + first;
         const float* grad = l.grad[t] + first;
         void* copy        = l.copy[t];
@@ -329,6 +346,18 @@ extern "C" {
 NERF_API NerfStatus nerf_ext_grad_norm(const NerfExtGradTensor* tensors, uint32_t count, float* norm, void* workspace, uint64_t workspace_bytes, void* stream) {
     const NerfStatus s = check_grads("nerf_ext_grad_norm", tensors, count, norm, workspace, workspace_bytes, false);
     if (s != NERF_STATUS_OK) return s;
+    // Up to 2^17 elements one workgroup takes 6 us, and two launches 9.
+    if (count <= kNormListed) {
+        uint64_t pieces = 0u;
+        for (uint32_t i = 0; i < count; ++i) pieces += (tensors[i].count + kPiece - 1u) / kPiece;
+        if (pieces > 0u && pieces <= kShortPieces) {
+            NERF_HIP_TRY((each_list<NormList, kNormListed>(tensors, count, kShortWaves, put_grad, [&](const NormList& l, uint32_t) {
+                k_norm_short<<<1, kShortThreads, 0, (hipStream_t)stream>>>(l, norm);
+                return hipGetLastError();
+            })));
+            return NERF_STATUS_OK;
+        }
+    }
     uint32_t n = 0u;
     NERF_HIP_TRY(square_sums(tensors, count, (double*)workspace, &n, (hipStream_t)stream));
     k_norm<<<1, kThreads, 0, (hipStream_t)stream>>>((const double*)workspace, n, norm);
