@@ -296,6 +296,7 @@ struct Operands {
     uint64_t ldp, ldq;  // elements between rows in memory
     uint32_t np, nq, nk;
     uint32_t k_split;   // k per part, a multiple of kBK
+    uint32_t tiles_p, tiles_q;
 };
 
 // A tile of kB rows x 64 k lies in LDS in 16-byte chunks of 8 values, the
@@ -524,6 +525,14 @@ __device__ __forceinline__ void arrived() {
     asm volatile("" ::: "memory");
 }
 
+// The card gives workgroups to its eight chips in turn, each with an L2 of its
+// own.  Tile number of workgroup b of n, so that a chip's workgroups have tiles in
+// a row: those share operands.
+__device__ __forceinline__ uint32_t chip_tile(uint32_t b, uint32_t n) {
+    const uint32_t chip = b % 8u, each = n / 8u, more = n % 8u;
+    return chip * each + min(chip, more) + b / 8u;
+}
+
 // kBP x kBQ outputs a workgroup, kWP x kWQ waves, kDepth tiles of 64 k at a time
 // in LDS or on their way there.  kMode: both operands go straight into LDS
 // (kDirect), or the tiles on their way wait in registers, fetched by chunks or as
@@ -542,8 +551,10 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     __shared__ floatx4 lds_bias[Out::kBias ? kBP / 4u : 1u];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t wp = (wave % kWP) * (kBP / kWP), wq = (wave / kWP) * (kBQ / kWQ);
-    const uint32_t p0 = blockIdx.x * kBP, q0 = blockIdx.y * kBQ;
-    const uint32_t k0 = blockIdx.z * A.k_split, k_end = min(A.nk, k0 + A.k_split);
+    const uint32_t tile = chip_tile(blockIdx.x, gridDim.x);
+    const uint32_t tile_p = tile % A.tiles_p, tile_q = tile / A.tiles_p % A.tiles_q, part = tile / A.tiles_p / A.tiles_q;
+    const uint32_t p0 = tile_p * kBP, q0 = tile_q * kBQ;
+    const uint32_t k0 = part * A.k_split, k_end = min(A.nk, k0 + A.k_split);
 
     // Sums of Q over k, for out.row_sums: a product with ones, the fragments of Q
     // shared out among the waves that hold the same.
@@ -563,7 +574,7 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
         for (uint32_t i = 0; i < kFP; ++i) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     bool take_sums = false;
-    if constexpr (kSums) take_sums = out.row_sums && blockIdx.x == 0u;
+    if constexpr (kSums) take_sums = out.row_sums && tile_p == 0u;
     typename Vec<T>::x8 ones;
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = (T)1.0f;
@@ -689,12 +700,12 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     }
 
     if constexpr (std::is_same_v<Out, SumOut>) {
-        if (blockIdx.z) out.out = out.parts + (blockIdx.z - 1u) * out.part;
+        if (part) out.out = out.parts + (part - 1u) * out.part;
         if (take_sums && lane < 16u) {  // every p of the product with ones holds the sum
 #pragma unroll
             for (uint32_t j = 0; j < kSumsQ; ++j) {
                 const uint32_t q = q0 + wq + 16u * (wave % kWP * kSumsQ + j) + lane;
-                if (q < out.nq) out.row_sums[(uint64_t)blockIdx.z * out.nq + q] = sums[j][0];
+                if (q < out.nq) out.row_sums[(uint64_t)part * out.nq + q] = sums[j][0];
             }
         }
     }
@@ -1210,13 +1221,15 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
     const uint64_t held = kSums ? (words + part) / (part + (row_sums ? A.nq : 0u)) : words / part;
     const uint64_t fill = (kBP == 256u ? 1u : 2u) * device_cu_count();
     uint64_t splits = kSplit ? fill / ((uint64_t)tp * tq) : 1u;
-    splits = std::min<uint64_t>({splits, ceil_div(A.nk, 4u * kBK), held, 65535u});
+    splits = std::min<uint64_t>({splits, ceil_div(A.nk, 4u * kBK), held});
     const bool split = splits > 1u;
     if (!split) splits = 1u;
     A.k_split = ceil_div(ceil_div(A.nk, kBK), splits) * kBK;
     if (A.k_split == 0u) A.k_split = kBK;
     const uint32_t parts = std::max(1u, ceil_div(A.nk, A.k_split));
-    const dim3 grid(tp, tq, parts);
+    A.tiles_p           = tp;
+    A.tiles_q           = tq;
+    const uint32_t grid = tp * tq * parts;
     constexpr uint32_t kThreads = kWP * kWQ * 64u;
     if constexpr (kSplit) {
         if (parts > 1u) {
@@ -1311,7 +1324,7 @@ hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hi
         if (wider) return odd ? launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
         return odd ? launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
     }
-    if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) * (kPT && kQT ? ceil_div(A.nk, 1024u) : 1u) >= cus / 2u && A.np > 128u && A.nk >= 512u)
+    if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) * (kPT && kQT ? ceil_div(A.nk, 1024u) : 1u) >= cus / 2u && A.np > 128u && A.nk >= 512u && (!(kPT && kQT) || A.np > 256u || A.nq > 256u))
         return launch_tiles<T, 256, 256, 2, 4, 2, kPT, kQT, kDirect, kPT && kQT>(A, out, row_sums, ws, stream);
     if (wider) return launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kDirect>(A, out, row_sums, ws, stream);
     return launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kDirect>(A, out, row_sums, ws, stream);
@@ -1331,7 +1344,7 @@ template <typename T>
 NerfStatus forward(const NerfExtLinearDesc& d, const void* x, const void* w, const float* bias, const void* residual, void* y, void* pre, Workspace ws, hipStream_t stream) {
     const bool y32 = d.out_dtype == NERF_EXT_F32;
     const bool vec = d.out_features % 8u == 0u && d.y_stride % 8u == 0u && aligned(y, 16u) && aligned(pre, 16u) && (!residual || (d.residual_stride % 8u == 0u && aligned(residual, 16u)));
-    const Operands all{w, x, d.in_features, d.x_stride, d.out_features, d.rows, d.in_features, 0u};
+    const Operands all{w, x, d.in_features, d.x_stride, d.out_features, d.rows, d.in_features, 0u, 0u, 0u};
     if (few_operands(all, false, false)) {
         const ForwardOut<T> out{bias, (const T*)residual, y, (T*)pre, d.residual_stride, d.y_stride, d.out_features, d.rows, d.activation, y32, vec};
         const uint32_t most = 2u * device_cu_count();
@@ -1348,7 +1361,7 @@ NerfStatus forward(const NerfExtLinearDesc& d, const void* x, const void* w, con
     }
     for (uint64_t r0 = 0; r0 < d.rows; r0 += kRowsPerLaunch) {
         const uint32_t n = (uint32_t)std::min<uint64_t>(kRowsPerLaunch, d.rows - r0);
-        const Operands A{w, (const T*)x + r0 * d.x_stride, d.in_features, d.x_stride, d.out_features, n, d.in_features, 0u};
+        const Operands A{w, (const T*)x + r0 * d.x_stride, d.in_features, d.x_stride, d.out_features, n, d.in_features, 0u, 0u, 0u};
         void* yo = y32 ? (void*)((float*)y + r0 * d.y_stride) : (void*)((T*)y + r0 * d.y_stride);
         const ForwardOut<T> out{bias, residual ? (const T*)residual + r0 * d.residual_stride : nullptr, yo, pre ? (T*)pre + r0 * d.out_features : nullptr, d.residual_stride, d.y_stride, d.out_features, n, d.activation, y32, vec};
         NERF_HIP_TRY((launch_product<T, false, false>(A, out, nullptr, ws, stream)));
@@ -1359,7 +1372,7 @@ NerfStatus forward(const NerfExtLinearDesc& d, const void* x, const void* w, con
 template <typename T>
 NerfStatus backward(const NerfExtLinearDesc& d, const void* x, const void* w, const void* delta, const void* pre, const void* add, void* dx, void* dpre, float* dw, float* db, Workspace ws, hipStream_t stream) {
     const bool vec = d.in_features % 8u == 0u && (!(add || dx) || d.x_stride % 8u == 0u) && aligned(add, 16u) && aligned(dx, 16u) && aligned(pre, 16u) && aligned(dpre, 16u);
-    const Operands all_x{w, delta, d.in_features, d.y_stride, d.in_features, d.rows, d.out_features, 0u}, all_w{x, delta, d.x_stride, d.y_stride, d.in_features, d.out_features, d.rows, 0u};
+    const Operands all_x{w, delta, d.in_features, d.y_stride, d.in_features, d.rows, d.out_features, 0u}, all_w{x, delta, d.x_stride, d.y_stride, d.in_features, d.out_features, d.rows, 0u, 0u, 0u};
     const SumOut w_out{dw, nullptr, 0u, db, d.in_features, d.out_features, d.in_features % 8u == 0u && aligned(dw, 16u)};
     const bool to_x = (dx || dpre) && d.rows != 0u;
     if ((!to_x || few_operands(all_x, true, false)) && (!dw || few_operands(all_w, true, true))) {
@@ -1381,7 +1394,7 @@ NerfStatus backward(const NerfExtLinearDesc& d, const void* x, const void* w, co
     if (to_x) {
         for (uint64_t r0 = 0; r0 < d.rows; r0 += kRowsPerLaunch) {
             const uint32_t n = (uint32_t)std::min<uint64_t>(kRowsPerLaunch, d.rows - r0);
-            const Operands A{w, (const T*)delta + r0 * d.y_stride, d.in_features, d.y_stride, d.in_features, n, d.out_features, 0u};
+            const Operands A{w, (const T*)delta + r0 * d.y_stride, d.in_features, d.y_stride, d.in_features, n, d.out_features, 0u, 0u, 0u};
             const InputGradientOut<T> out{add ? (const T*)add + r0 * d.x_stride : nullptr, dx ? (T*)dx + r0 * d.x_stride : nullptr, pre ? (const T*)pre + r0 * d.in_features : nullptr,
                                           dpre ? (T*)dpre + r0 * d.in_features : nullptr, d.x_stride, d.in_features, n, d.activation, vec};
             NERF_HIP_TRY((launch_product<T, true, false>(A, out, nullptr, ws, stream)));
