@@ -31,7 +31,7 @@ struct NormList {
     uint32_t first[kNormListed + 1u];  // pieces before the tensor's; all pieces behind the last
     uint16_t tail[kNormListed];        // elements of its last piece
     uint8_t dtype[kNormListed];
-    uint32_t tensors, pieces, share;
+    uint32_t tensors, pieces, workers;
 };
 struct AdamList {
     float* param[kAdamListed];
@@ -42,39 +42,36 @@ struct AdamList {
     uint32_t first[kAdamListed + 1u];
     uint16_t tail[kAdamListed];
     uint8_t dtype[kAdamListed];
-    uint32_t tensors, pieces, share;
+    uint32_t tensors, pieces, workers;
 };
 
-// Worker w (a workgroup, or a wave of one) has pieces w * share and on, `share` of
-// them, in their order or (kBack) from the last: a pass after another over the same tensors
-// begins with what the one before read last, which the memory-side cache (256
-// MiB) still holds.  f(tensor, first element, elements).  Counts are 32-bit
+// Worker w (a workgroup, or a wave of one) has every l.workers-th piece from w on
+// or (kBack) the same from the list's end: a pass after another over the same
+// tensors begins with what the one before read last, which the memory-side cache
+// (256 MiB) still holds.  f(tensor, first element, elements).  Counts are 32-bit
 // words: of a select between 64-bit lengths (the piece's end or the tensor's)
 // the compiler kept the wrong condition here and let workgroups run past a
 // tensor's end.
 template <bool kBack, typename List, typename F>
 __device__ __forceinline__ void each_piece(const List& l, uint32_t worker, F&& f) {
-    const uint32_t begin = worker * l.share, end = min(begin + l.share, l.pieces);
-    if (begin >= end) return;
+    if (worker >= l.pieces) return;
     // The tensor of the first piece to come: one less than those that start at
     // or before it, each lane asking for its own (a search by halves waited for
     // one load after another).
-    uint32_t piece = kBack ? end - 1u : begin, t = 0u;
+    uint32_t piece = kBack ? l.pieces - 1u - worker : worker, t = 0u;
     for (uint32_t base = 0; base < l.tensors; base += 64u) {
         const uint32_t i = base + (threadIdx.x & 63u);
         t += (uint32_t)__popcll(__ballot(i < l.tensors && l.first[i] <= piece));
     }
     t = __builtin_amdgcn_readfirstlane(t - 1u);
-    for (uint32_t left = end - begin; left > 0u; --left) {
-        const uint32_t first = l.first[t], next = l.first[t + 1u];
-        f(t, (uint64_t)(piece - first) * kPiece, piece + 1u == next ? l.tail[t] : kPiece);
+    for (uint32_t left = (l.pieces - 1u - worker) / l.workers + 1u; left > 0u; --left) {
         if (kBack) {
-            if (piece == first) --t;
-            --piece;
+            while (piece < l.first[t]) --t;
         } else {
-            ++piece;
-            if (piece == next) ++t;
+            while (piece >= l.first[t + 1u]) ++t;
         }
+        f(t, (uint64_t)(piece - l.first[t]) * kPiece, piece + 1u == l.first[t + 1u] ? l.tail[t] : kPiece);
+        piece = kBack ? piece - l.workers : piece + l.workers;
     }
 }
 
@@ -314,8 +311,8 @@ hipError_t each_list(const Tensor* tensors, uint32_t count, uint32_t most, Put&&
         }
         if (l.tensors == 0u) break;
         l.first[l.tensors] = l.pieces;
-        l.share            = (l.pieces + most - 1u) / most;
-        const hipError_t e = f(l, (l.pieces + l.share - 1u) / l.share);
+        l.workers          = std::min(l.pieces, most);
+        const hipError_t e = f(l, l.workers);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
