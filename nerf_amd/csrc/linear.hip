@@ -121,6 +121,27 @@ __device__ __forceinline__ void act_slopes(uint32_t act, floatx8& z) {
     }
 }
 
+// Eight values of which `some` are an operand's, fetched from `down` values
+// ahead of them: those moved to the front, zeros behind them.
+__device__ __forceinline__ uint4 settled(uint4 v, uint32_t down, uint32_t some) {
+    unsigned long long w[2];
+    __builtin_memcpy(w, &v, 16);
+    const uint32_t bits = 16u * (down & 3u);
+    if (down >= 4u) {
+        w[0] = w[1];
+        w[1] = 0ull;
+    }
+    if (bits) {
+        w[0] = w[0] >> bits | w[1] << (64u - bits);
+        w[1] >>= bits;
+    }
+    const unsigned long long ones = ~0ull;
+    w[0] &= some >= 4u ? ones : ~(ones << (16u * some));
+    w[1] &= some >= 8u ? ones : some > 4u ? ~(ones << (16u * (some - 4u))) : 0ull;
+    __builtin_memcpy(&v, w, 16);
+    return v;
+}
+
 // ------------------------------------------------------------- epilogues
 // What becomes of a finished sum.  Arrays are reached through buffer
 // descriptors that start at the workgroup's first row: offsets are 32 bits,
@@ -136,16 +157,18 @@ struct Rows {
     uint32_t ld;
     // Row `first` of an array with rows ld elements apart.
     __device__ __forceinline__ Rows(const void* data, uint64_t first, uint64_t ld_) : base((const E*)data + first * ld_), rsrc(__builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)0x7FFFFFFF, 0x00020000)), ld((uint32_t)ld_) {}
-    // Eight elements from (row, p), n of them inside; vec: all or none, aligned to
-    // 16 bytes.  Else eight go in one access at any alignment, fewer one by one.
     __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t p) const { return (row * ld + p) * (uint32_t)sizeof(E); }
-    __device__ __forceinline__ uintx4 load(uint32_t row, uint32_t p, uint32_t n, bool vec) const {
+    // Eight elements from (row, p), n of them inside; vec: all or none, aligned to
+    // 16 bytes.  Else (rows of at least eight) a lane with fewer fetches the eight
+    // that end with its row, and widen() moves them: every lane by the same load,
+    // since one that only some lanes take is waited for where they meet.
+    __device__ __forceinline__ uintx4 load(uint32_t row, uint32_t p, uint32_t n, bool vec, bool rows_of_eight) const {
         static_assert(sizeof(E) == 2);
         if (vec) return __builtin_bit_cast(uintx4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(n ? at(row, p) : kBeyond), 0, 0));
-        uintx4 o = {0u, 0u, 0u, 0u};
-        if (n == 8u) {
-            __builtin_memcpy(&o, base + row * ld + p, 16);
-        } else if (n) {
+        uintx4 o;
+        if (rows_of_eight) {
+            __builtin_memcpy(&o, base + (n ? row * ld + p + n - 8u : 0u), 16);
+        } else {
             short8_t v;
 #pragma unroll
             for (uint32_t r = 0; r < 8u; ++r) v[r] = (short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)(r < n ? at(row, p + r) : kBeyond), 0, 0);
@@ -186,8 +209,10 @@ struct Rows {
     }
 };
 
+// What Rows::load has fetched, as 32-bit values.
 template <typename T>
-__device__ __forceinline__ floatx8 widen(uintx4 v) {
+__device__ __forceinline__ floatx8 widen(uintx4 v, uint32_t n, bool vec, bool rows_of_eight) {
+    if (!vec && rows_of_eight) v = __builtin_bit_cast(uintx4, settled(__builtin_bit_cast(uint4, v), 8u - n, n));
     return __builtin_convertvector(__builtin_bit_cast(typename Vec<T>::x8, v), floatx8);
 }
 
@@ -230,13 +255,13 @@ struct ForwardOut {
     static constexpr bool kBias = true;
 
     __device__ __forceinline__ Aux load(uint32_t q0, uint32_t row, uint32_t p, uint32_t n) const {
-        return {residual ? Rows<T>(residual, q0, ldr).load(row, p, n, vec) : uintx4{0u, 0u, 0u, 0u}};
+        return {residual ? Rows<T>(residual, q0, ldr).load(row, p, n, vec, np >= 8u) : uintx4{0u, 0u, 0u, 0u}};
     }
     __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 z, const floatx8& b, const Aux& a) const {
         z += b;
         if (pre) Rows<T>(pre, q0, np).store(row, p, n, vec, z);
         act_values(act, z);
-        if (residual) z += widen<T>(a.residual);
+        if (residual) z += widen<T>(a.residual, n, vec, np >= 8u);
         if (y32) Rows<float>(y, q0, ldy).store(row, p, n, vec, z);
         else Rows<T>(y, q0, ldy).store(row, p, n, vec, z);
     }
@@ -258,15 +283,15 @@ struct InputGradientOut {
 
     __device__ __forceinline__ Aux load(uint32_t q0, uint32_t row, uint32_t p, uint32_t n) const {
         Aux a{};
-        if (add) a.add = Rows<T>(add, q0, ldx).load(row, p, n, vec);
-        if (dpre) a.pre = Rows<T>(pre, q0, np).load(row, p, n, vec);
+        if (add) a.add = Rows<T>(add, q0, ldx).load(row, p, n, vec, np >= 8u);
+        if (dpre) a.pre = Rows<T>(pre, q0, np).load(row, p, n, vec, np >= 8u);
         return a;
     }
     __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 g, const floatx8&, const Aux& a) const {
-        if (add) g += widen<T>(a.add);
+        if (add) g += widen<T>(a.add, n, vec, np >= 8u);
         if (dx) Rows<T>(dx, q0, ldx).store(row, p, n, vec, g);
         if (dpre) {
-            floatx8 s = widen<T>(a.pre);
+            floatx8 s = widen<T>(a.pre, n, vec, np >= 8u);
             act_slopes(act, s);
             Rows<T>(dpre, q0, np).store(row, p, n, vec, g * s);
         }
@@ -354,27 +379,6 @@ struct Eight {
 // Number of an address in values, for Eight::value.
 template <typename T>
 __device__ __forceinline__ uint32_t value_number(const T* p) { return (uint32_t)((uintptr_t)p >> 1); }
-
-// Eight values of which `some` are an operand's, fetched from `down` values
-// ahead of them: those moved to the front, zeros behind them.
-__device__ __forceinline__ uint4 settled(uint4 v, uint32_t down, uint32_t some) {
-    unsigned long long w[2];
-    __builtin_memcpy(w, &v, 16);
-    const uint32_t bits = 16u * (down & 3u);
-    if (down >= 4u) {
-        w[0] = w[1];
-        w[1] = 0ull;
-    }
-    if (bits) {
-        w[0] = w[0] >> bits | w[1] << (64u - bits);
-        w[1] >>= bits;
-    }
-    const unsigned long long ones = ~0ull;
-    w[0] &= some >= 4u ? ones : ~(ones << (16u * some));
-    w[1] &= some >= 8u ? ones : some > 4u ? ~(ones << (16u * (some - 4u))) : 0ull;
-    __builtin_memcpy(&v, w, 16);
-    return v;
-}
 
 // Where a lane finds eight values of an operand at its edges: from a place that
 // ends with the line (or begins with the array, which has eight values at
@@ -804,7 +808,7 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
     // What is on its way: the Q and the epilogue inputs of the kAhead next tiles of
     // rows, as many as the registers hold beside P.  (With one, 100003 x 64 -> 256
     // took 33 us from memory and 24 us from cache.)
-    constexpr uint32_t kAhead = kKS <= 2u ? 3u : kKS * kFP <= 16u && !(kKS == 8u && kWords) ? 2u : 1u;
+    constexpr uint32_t kAhead = kKS <= 2u ? 3u : kKS * kFP < 16u || (kKS * kFP == 16u && !kWords && sizeof(typename Out::Aux) <= 16u) ? 2u : 1u;
     // Where even one tile's epilogue inputs take more registers than there are
     // beside this tile's, they are fetched in their place as these are used.
     constexpr bool kLate = kKS * kFP == 32u && sizeof(typename Out::Aux) > 16u;
