@@ -550,7 +550,7 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
     // read of what is on its way into another.
     constexpr bool kAligned  = kMode == kDirect;
     constexpr uint32_t kTile = (kBP + kBQ) * 8u;
-    static_assert(kDepth == 2u || kDepth == 4u);
+    static_assert(!kAligned || kDepth == 2u || kDepth == 4u);
     __shared__ uint4 lds0[kTile], lds1[kAligned ? kTile : 1u], lds2[kAligned && kDepth == 4u ? kTile : 1u], lds3[kAligned && kDepth == 4u ? kTile : 1u];
     __shared__ floatx4 lds_bias[Out::kBias ? kBP / 4u : 1u];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
@@ -1325,7 +1325,7 @@ hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hi
     const bool wider    = wide >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u && A.nk > 2048u);
     if (!whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, kQT ? A.nq : A.nk)) {
         const bool odd = odd_rows(A.p, A.ldp) || odd_rows(A.q, A.ldq);
-        if (wider) return odd ? launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
+        if (wider) return odd ? launch_tiles<T, 128, 128, 2, 2, 3, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
         return odd ? launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
     }
     if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) * (kPT && kQT ? ceil_div(A.nk, 1024u) : 1u) >= cus / 2u && A.np > 128u && A.nk >= 512u && (!(kPT && kQT) || A.np > 256u || A.nq > 256u))

@@ -8,7 +8,7 @@ import pytest
 
 from conftest import announce
 from linear_cases import ACTS, CODES, backward, decode, encode, forward, within
-from nerf_amd import _lib as L
+from nerf_amd import _lib as L, ext
 from nerf_amd.device import DeviceArray, Stream, synchronize
 
 pytestmark = pytest.mark.gpu
@@ -199,6 +199,36 @@ def test_many_rows_with_strides():
     for strides, shift in (((272, 136, 144), 0), ((257, 131, 133), 1)):
         check_forward(17003, 256, 130, "f16", "f16", "silu", strides=strides, shift=shift)
         check_backward(17003, 256, 130, "f16", "silu", strides=strides[:2], shift=shift, dw=False, db=False)
+
+
+def test_more_rows_than_one_launch():
+    check_forward(65535 * 64 + 100, 9, 2, "f16", "f16", "relu")
+    check_backward(65535 * 64 + 100, 2, 9, "bf16", "relu")
+
+
+def test_offsets_beyond_32_bits():
+    """Rows 2^20 elements apart: offsets up to 2^36 bytes."""
+    n, i, o, stride = 16400, 64, 40, 1 << 20
+    v = _inputs(n, i, o, "f16", 9)
+    x, y = DeviceArray((n, stride), np.uint16), DeviceArray((n, stride // 4), np.float32)
+    bits = encode(v["x"], "f16")
+    for r in range(n):
+        ext.write_device(x.ptr + 2 * stride * r, bits[r])
+    w, b, d = Guarded(o, i, "f16", values=v["w"]), Guarded(1, o, "f32", values=v["bias"]), Guarded(n, o, "f16", values=v["delta"])
+    desc = L.NerfExtLinearDesc(n, i, o, CODES["f16"], CODES["f32"], ACTS["relu"], stride, stride // 4, 0, 0)
+    L.call("nerf_ext_linear_forward", C.byref(desc), x.ptr, w.ptr, b.ptr, None, y.ptr, None, None, 0, None)
+    synchronize()
+    got = np.stack([ext.read_device(y.ptr + stride * r, (o,), np.float32) for r in range(n)]).astype(np.float64)
+    want, _, bound, _ = forward(v["x"], v["w"], v["bias"], None, "relu", "f16", "f32")
+    within(got, want, bound, "y")
+    desc.y_stride = 0
+    dw, db = Guarded(o, i, "f32"), Guarded(1, o, "f32")
+    ws = DeviceArray((L.NERF_EXT_LINEAR_WORKSPACE,), np.uint8)
+    L.call("nerf_ext_linear_backward", C.byref(desc), x.ptr, None, d.ptr, None, None, None, None, dw.ptr, db.ptr, ws.ptr, ws.nbytes, None)
+    synchronize()
+    ref = backward(v["x"], v["w"], v["delta"], v["pre"], None, "relu", "f16")
+    within(dw.values(), *ref["dw"], "dw")
+    within(db.values()[0], *ref["db"], "db")
 
 
 def test_wide_layers():

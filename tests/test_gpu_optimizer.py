@@ -6,7 +6,7 @@ import pytest
 
 from conftest import announce
 from linear_cases import CODES, EPS, UNIT, decode, encode, within
-from nerf_amd import _lib as L
+from nerf_amd import _lib as L, ext
 from nerf_amd.device import DeviceArray, synchronize
 
 pytestmark = pytest.mark.gpu
@@ -114,6 +114,23 @@ def test_norm_that_is_not_finite_leaves_gradients(value):
     assert not np.isfinite(norm)
     for a, v in zip(out, values):
         assert np.array_equal(a, v, equal_nan=True)
+
+
+def test_more_elements_than_32_bits_count():
+    """2^32 + 4097 equal fp16 gradients, clipped in place."""
+    n = (1 << 32) + 4097
+    g = DeviceArray((n,), np.float16)
+    g.fill_bytes(0x3C)  # 0x3C3C = 1.05859375
+    value = float(np.uint16(0x3C3C).view(np.float16))
+    want = value * np.sqrt(float(n))
+    tensors = (L.NerfExtGradTensor * 1)(L.NerfExtGradTensor(g.ptr, g.ptr, n, CODES["f16"], 0))
+    norm, ws = DeviceArray((1,), np.float32), DeviceArray((L.NERF_EXT_NORM_WORKSPACE,), np.uint8)
+    L.call("nerf_ext_grad_clip", tensors, 1, float(np.float32(want / 4.0)), norm.ptr, ws.ptr, ws.nbytes, None)
+    synchronize()
+    assert abs(float(norm.numpy()[0]) - want) <= 2.0**-23 * want
+    for at in (0, (1 << 31) - 3, (1 << 32) - 5, n - 7):
+        got = ext.read_device(g.ptr + 2 * at, (7,), np.float16).astype(np.float64)
+        assert np.abs(got - value / 4.0).max() <= 2.0**-11 * value / 4.0 * 1.01, at
 
 
 def test_same_norm_every_time():

@@ -2,6 +2,8 @@
 decided on the host before any GPU work; and the 64-bit definitions that the
 GPU tests compare with, checked against finite differences."""
 import ctypes as C
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -101,6 +103,20 @@ def test_adam_arguments(lib):
         h = L.NerfHyperParams(1e-2, 0.9, 0.99, 1e-8, 1.0, 1e30, 128.0, 0)
         setattr(h, field, value)
         assert call(h=h) == BAD, (field, value)
+
+
+def test_structures_as_c_lays_them_out(tmp_path):
+    sizes = {"NerfExtLinearDesc": L.NerfExtLinearDesc, "NerfExtGradTensor": L.NerfExtGradTensor, "NerfExtAdamTensor": L.NerfExtAdamTensor}
+    lines = ["#include <stddef.h>", '#include "nerf_ext.h"']
+    for name, struct in sizes.items():
+        lines.append(f'_Static_assert(sizeof({name}) == {C.sizeof(struct)}, "{name}");')
+        lines += [f'_Static_assert(offsetof({name}, {field[0]}) == {getattr(struct, field[0]).offset}, "{name}.{field[0]}");' for field in struct._fields_]
+    for name in ("NERF_EXT_BF16", "NERF_EXT_ACT_NONE", "NERF_EXT_ACT_RELU", "NERF_EXT_ACT_SOFTPLUS", "NERF_EXT_ACT_SIGMOID", "NERF_EXT_ACT_SILU", "NERF_EXT_ACT_GELU", "NERF_EXT_LINEAR_WORKSPACE", "NERF_EXT_NORM_WORKSPACE"):
+        lines.append(f'_Static_assert({name} == {getattr(L, name)}, "{name}");')
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join(lines) + "\n")
+    include = Path(__file__).resolve().parent.parent / "include"
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", f"-I{include}", "-fsyntax-only", str(src)], check=True)
 
 
 @pytest.mark.parametrize("name", list(ACTS))
