@@ -1224,7 +1224,10 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
     const uint32_t tp = ceil_div(A.np, kBP), tq = ceil_div(A.nq, kBQ);
     // Split over k until every CU has its workgroups (two; one of the widest
     // tile, whose buffers take the LDS of a CU), with four tiles of k a part at
-    // least, as far as the workspace holds the parts.
+    // least, as far as the workspace holds the parts.  Outputs of 16 bits are split
+    // in four at least and from 1024 k on, where the parts' way through memory
+    // pays: 16 x 8192 -> 2048 12 us (whole 31), 1024 x 1024 -> 1024 14.5 in two
+    // parts and 8.6 whole, 512 x 1024 -> 1024 11.4 in four and 7.9 whole.
     // The first part of a plain sum is kept where the sum will be.
     const uint64_t part = (uint64_t)A.np * A.nq, words = ws.bytes / 4u;
     constexpr bool kSums = std::is_same_v<Out, SumOut>;
@@ -1232,8 +1235,7 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
     const uint64_t fill = (kBP == 256u ? 1u : 2u) * device_cu_count();
     uint64_t splits = kSplit ? fill / ((uint64_t)tp * tq) : 1u;
     splits = std::min<uint64_t>({splits, ceil_div(A.nk, 4u * kBK), held});
-    const bool split = splits > 1u;
-    if (!split) splits = 1u;
+    if (splits <= 1u || (!kSums && (splits < 4u || A.nk <= 1024u))) splits = 1u;
     A.k_split = ceil_div(ceil_div(A.nk, kBK), splits) * kBK;
     if (A.k_split == 0u) A.k_split = kBK;
     const uint32_t parts = std::max(1u, ceil_div(A.nk, A.k_split));
@@ -1282,9 +1284,8 @@ bool few_values(const Operands& A, bool pt, bool qt) {
 template <typename T, uint32_t kKS, bool kPT, typename Out>
 hipError_t launch_stream(const Operands& A, const Out& out, hipStream_t stream) {
     // p a wave holds: 64, whose 16-bit outputs are whole lines; 32 where there are
-    // no more, or where 64 and the work for cut rows take more registers than there
-    // are.
-    const bool ragged = A.nk % 32u != 0u, odd = odd_rows(A.q, A.ldq), narrow = A.np <= 32u || (kKS == 8u && (ragged || !out.vec || odd));
+    // no more.
+    const bool ragged = A.nk % 32u != 0u, odd = odd_rows(A.q, A.ldq), narrow = A.np <= 32u;
     const uint32_t wide = narrow ? 32u : 64u, most = 256u / wide;
     uint32_t p_waves = 1u;
     while (p_waves < most && wide * p_waves < A.np) p_waves *= 2u;
@@ -1293,56 +1294,89 @@ hipError_t launch_stream(const Operands& A, const Out& out, hipStream_t stream) 
     const dim3 grid(std::min(ceil_div(tiles, groups), std::max(1u, device_cu_count() / across)), across);
     constexpr uint32_t kThreads = kStreamWaves * 64u;
     auto launch = [&](auto p, auto cut, auto words) { k_stream<T, kKS, p(), kPT, cut(), words(), Out><<<grid, kThreads, 0, stream>>>(A, out, p_waves); };
-    const std::integral_constant<uint32_t, 2u> two{};
-    const std::integral_constant<uint32_t, 4u> four{};
-    const std::true_type yes{};
-    const std::false_type no{};
-    if (narrow) {
-        if (odd) launch(two, yes, yes);
-        else if (ragged) launch(two, yes, no);
-        else launch(two, no, no);
-    } else if constexpr (kKS < 8u) {
-        if (odd) launch(four, yes, yes);
-        else if (ragged) launch(four, yes, no);
-        else launch(four, no, no);
-    } else {
-        launch(four, no, no);
+    auto by_width = [&](auto cut, auto words) {
+        if (narrow) launch(std::integral_constant<uint32_t, 2u>{}, cut, words);
+        else launch(std::integral_constant<uint32_t, 4u>{}, cut, words);
+    };
+    if constexpr (kKS <= 2u) {
+        if (odd) {
+            by_width(std::true_type{}, std::true_type{});
+            return hipGetLastError();
+        }
+        if (ragged) {
+            by_width(std::true_type{}, std::false_type{});
+            return hipGetLastError();
+        }
     }
+    by_width(std::false_type{}, std::false_type{});
     return hipGetLastError();
+}
+
+// Whether the streamed kernel takes a product, by steps of 32 k (at most 8): with
+// so many rows that its start, a CU's weights, is small beside them, and beyond
+// two steps only where rows and outputs are whole; what cut ones need then takes
+// the registers of rows on their way.  Streamed against by tiles, in us: 262144
+// rows, 256 -> 256 with residual 116 / 130, and 65536 without 34 / 30; 128 -> 256,
+// 131072 rows 43 / 48 and 32768 rows 13 / 11; 64 -> 256, 65536 rows 17 / 19 and
+// 32768 rows 11.8 / 11.3; 32 -> 64, 131072 rows 11 / 17.  Cut: 262144 x 240 ->
+// 256 141 / 113, 100 -> 250 126 / 99, 256 -> 250 206 / 119; 65536 x 63 -> 255
+// 24 / 25.  Beyond 1024 p, 65536 x 256 -> 2048 211 / 192.  Input gradients move
+// more beside the product and come to it with fewer rows: 65536 x 256 -> 256
+// backward 69 / 79.
+bool streamed(const Operands& A, bool vec, bool gradient) {
+    const uint32_t steps = A.nk <= 32u ? 1u : A.nk <= 64u ? 2u : A.nk <= 128u ? 4u : 8u;
+    if (A.nk > 256u || A.np > 1024u || A.nq < 16384u * (gradient ? (steps + 1u) / 2u : steps)) return false;
+    return steps <= 2u || (A.nk % 32u == 0u && vec && !odd_rows(A.q, A.ldq));
 }
 
 template <typename T, bool kPT, bool kQT, typename Out>
 hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hipStream_t stream) {
-    const uint32_t cus = device_cu_count();
     if (few_values(A, kPT, kQT)) {
         const uint64_t threads = (uint64_t)ceil_div(A.np, 8u) * A.nq;
-        k_tiny<T, kPT, kQT, Out><<<(uint32_t)std::min<uint64_t>(ceil_div(threads, 256u), 8u * cus), 256, 0, stream>>>(A, out);
+        k_tiny<T, kPT, kQT, Out><<<(uint32_t)std::min<uint64_t>(ceil_div(threads, 256u), 8u * device_cu_count()), 256, 0, stream>>>(A, out);
         return hipGetLastError();
     }
     if constexpr (!kQT) {
-        if (A.nk <= 256u && A.np <= 1024u && A.nq >= 16384u) {
+        if (streamed(A, out.vec, kPT)) {
             if (A.nk <= 32u) return launch_stream<T, 1u, kPT>(A, out, stream);
             if (A.nk <= 64u) return launch_stream<T, 2u, kPT>(A, out, stream);
             if (A.nk <= 128u) return launch_stream<T, 4u, kPT>(A, out, stream);
             return launch_stream<T, 8u, kPT>(A, out, stream);
         }
     }
-    const uint64_t wide = (uint64_t)ceil_div(A.np, 128u) * ceil_div(A.nq, 128u);
-    const bool wider    = wide >= cus || (kPT && kQT && A.np > 64u && A.nq > 64u && A.nk > 2048u);
+    // The tile.  Larger ones read less, smaller ones occupy the card with fewer
+    // outputs.  In us, by tiles of 64 / 128 / 256:
+    //   16-bit outputs by their tiles' number: 128 from 7/8 of the CUs on, 256 from
+    //   as many as CUs.  2048 x 1024 -> 1024 13 / 19 / -, 3000 x 1200 -> 1200
+    //   26 / 23 / -, 8192 x 1024 -> 1024 37 / 24 / 37, 16384 x 1024 -> 1024
+    //   82 / 56 / 49, 16384 x 4096 -> 4096 - / - / 470.  Of less than 512 k the
+    //   largest have too few steps.
+    //   Gradients of weights, whose k is split until the card is full, by the work:
+    //   128 from 2^32 products on, 256 from 2^35.  65536 x 128 -> 128 (2^30)
+    //   16 / 21 / -, with dx 37 / 43 / -; 65536 x 256 -> 256 (2^32) with dx
+    //   76 / 69 / -, 32768 x 512 -> 512 (2^33) 36 / 38 / 46, 8192 x 1024 -> 1024 (2^33) 36 / 32 / 43, 262144 x 256 -> 256
+    //   (2^34) 97 / 77 / 96, 131072 x 512 -> 512 (2^35) 164 / 107 / 102,
+    //   16384 x 2048 -> 2048 (2^36) 324 / 165 / 153.
+    constexpr bool kLong = kPT && kQT;
+    const uint64_t cus  = device_cu_count(), work = (uint64_t)A.np * A.nq * A.nk;
+    auto tiles          = [&](uint32_t b) { return (uint64_t)ceil_div(A.np, b) * ceil_div(A.nq, b); };
+    const bool by_128   = A.np > 64u && A.nq > 64u && (kLong ? work >= 1ull << 32 : 8u * tiles(128u) >= 7u * cus);
     if (!whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, kQT ? A.nq : A.nk)) {
+        // Rows on their way as words, two tiles (86 us for 20011 x 1209 -> 487; with
+        // one 93); as chunks one (68 us for 20011 x 1210 -> 488, with two 75).
         const bool odd = odd_rows(A.p, A.ldp) || odd_rows(A.q, A.ldq);
-        if (wider) return odd ? launch_tiles<T, 128, 128, 2, 2, 3, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
+        if (by_128) return odd ? launch_tiles<T, 128, 128, 2, 2, 3, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
         return odd ? launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
     }
-    if ((uint64_t)ceil_div(A.np, 256u) * ceil_div(A.nq, 256u) * (kPT && kQT ? ceil_div(A.nk, 1024u) : 1u) >= cus / 2u && A.np > 128u && A.nk >= 512u && (!(kPT && kQT) || A.np > 256u || A.nq > 256u))
-        return launch_tiles<T, 256, 256, 2, 4, 2, kPT, kQT, kDirect, kPT && kQT>(A, out, row_sums, ws, stream);
-    if (wider) return launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kDirect>(A, out, row_sums, ws, stream);
+    if (A.np > 128u && A.nq > 128u && A.nk >= 512u && (kLong ? work >= 1ull << 35 : tiles(256u) >= cus))
+        return launch_tiles<T, 256, 256, 2, 4, 2, kPT, kQT, kDirect, kLong>(A, out, row_sums, ws, stream);
+    if (by_128) return launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kDirect>(A, out, row_sums, ws, stream);
     return launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kDirect>(A, out, row_sums, ws, stream);
 }
 
-// Whether a product is one of few tiles, and of how many 16 outputs a side: the
-// smallest tile of which the card takes all at once, two workgroups a CU; 0
-// where there are more, or so many k that workgroups should share them.
+// Products of few tiles are those of at most 4096 k (1 x 4096 -> 4096 9 us, by
+// larger tiles with k split over workgroups 13; 1 x 8192 -> 4096 17.5 against
+// 15.5) whose tiles the card takes at once.
 constexpr uint32_t kFewMaxK = 4096u;
 bool few_operands(const Operands& A, bool pt, bool qt) { return A.nk <= kFewMaxK && !few_values(A, pt, qt); }
 uint64_t few_tiles(const Operands& A, uint32_t f) { return (uint64_t)ceil_div(A.np, 16u * f) * ceil_div(A.nq, 16u * f); }
@@ -1357,17 +1391,20 @@ NerfStatus forward(const NerfExtLinearDesc& d, const void* x, const void* w, con
     const Operands all{w, x, d.in_features, d.x_stride, d.out_features, d.rows, d.in_features, 0u, 0u, 0u};
     if (few_operands(all, false, false)) {
         const ForwardOut<T> out{bias, (const T*)residual, y, (T*)pre, d.residual_stride, d.y_stride, d.out_features, d.rows, d.activation, y32, vec};
-        const uint32_t most = 2u * device_cu_count();
-        auto launch         = [&](auto f) {
+        // Tiles of 16 outputs a side up to two a CU; of 32 one (512 x 1024 -> 1024,
+        // two: 11 us, by tiles of 64 8) and with odd rows two (353 x 1115 -> 705 13.2
+        // us, by tiles of 64 14.7).
+        const uint32_t cus = device_cu_count();
+        const bool odd     = odd_rows(x, d.x_stride) || odd_rows(w, d.in_features);
+        auto launch        = [&](auto f) {
             const dim3 grid(ceil_div(all.np, 16u * f()), ceil_div(all.nq, 16u * f()));
-            if (odd_rows(x, d.x_stride) || odd_rows(w, d.in_features)) k_few_forward<T, f(), true><<<grid, kFewWaves * 64u, 0, stream>>>(all, out);
+            if (odd) k_few_forward<T, f(), true><<<grid, kFewWaves * 64u, 0, stream>>>(all, out);
             else k_few_forward<T, f(), false><<<grid, kFewWaves * 64u, 0, stream>>>(all, out);
             NERF_LAUNCH_CHECK("k_few_forward");
             return NERF_STATUS_OK;
         };
-        if (few_tiles(all, 1u) <= most) return launch(std::integral_constant<uint32_t, 1u>{});
-        if (few_tiles(all, 2u) <= most) return launch(std::integral_constant<uint32_t, 2u>{});
-        if (2u * few_tiles(all, 4u) <= most) return launch(std::integral_constant<uint32_t, 4u>{});
+        if (few_tiles(all, 1u) <= 2u * cus) return launch(std::integral_constant<uint32_t, 1u>{});
+        if (few_tiles(all, 2u) <= (odd ? 2u : 1u) * cus) return launch(std::integral_constant<uint32_t, 2u>{});
     }
     for (uint64_t r0 = 0; r0 < d.rows; r0 += kRowsPerLaunch) {
         const uint32_t n = (uint32_t)std::min<uint64_t>(kRowsPerLaunch, d.rows - r0);
@@ -1387,6 +1424,10 @@ NerfStatus backward(const NerfExtLinearDesc& d, const void* x, const void* w, co
     const bool to_x = (dx || dpre) && d.rows != 0u;
     if ((!to_x || few_operands(all_x, true, false)) && (!dw || few_operands(all_w, true, true))) {
         const InputGradientOut<T> x_out{(const T*)add, (T*)dx, (const T*)pre, (T*)dpre, d.x_stride, d.in_features, d.rows, d.activation, vec};
+        // The smallest tile of which the card takes all at once, two a CU; those of 64
+        // a side up to 2048 rows, which a workgroup of dW goes through (2048 x 256 ->
+        // 256 11 us and 15 in three launches, 1024 x 1024 -> 1024 18 and 21, but
+        // 4096 x 256 -> 256 23 and 17).
         const uint32_t most = 2u * device_cu_count();
         auto blocks         = [&](uint32_t f) { return (to_x ? few_tiles(all_x, f) : 0u) + (dw ? few_tiles(all_w, f) : 0u); };
         auto launch         = [&](auto f) {
@@ -1399,7 +1440,7 @@ NerfStatus backward(const NerfExtLinearDesc& d, const void* x, const void* w, co
         };
         if (blocks(1u) <= most) return launch(std::integral_constant<uint32_t, 1u>{});
         if (blocks(2u) <= most) return launch(std::integral_constant<uint32_t, 2u>{});
-        if (blocks(4u) <= most) return launch(std::integral_constant<uint32_t, 4u>{});
+        if (d.rows <= 2048u && blocks(4u) <= most) return launch(std::integral_constant<uint32_t, 4u>{});
     }
     if (to_x) {
         for (uint64_t r0 = 0; r0 < d.rows; r0 += kRowsPerLaunch) {

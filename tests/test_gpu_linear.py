@@ -201,6 +201,22 @@ def test_many_rows_with_strides():
         check_backward(17003, 256, 130, "f16", "silu", strides=strides[:2], shift=shift, dw=False, db=False)
 
 
+# So many rows that a CU keeps its weights for all 64, 128 and 256 k, and sums in
+# whole tiles beside them.
+@pytest.mark.parametrize("n,k,p", [(32800, 64, 40), (32771, 57, 24), (65541, 128, 72), (65536, 96, 32), (131077, 256, 136), (131072, 224, 24), (131073, 160, 300), (131075, 250, 24)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_very_many_rows(n, k, p, kind):
+    check_forward(n, k, p, kind, kind, "relu")
+    check_backward(n, p, k, kind, "relu", dw=False, db=False)
+
+
+# Around the sizes at which sums are split and tiles change.
+@pytest.mark.parametrize("n,i,o", [(16, 8192, 96), (70, 1088, 520), (500, 1100, 1032), (1500, 1048, 1160), (2050, 264, 256), (4096, 64, 1040), (4100, 1024, 1032)])
+def test_split_and_tile_choices(n, i, o):
+    check_forward(n, i, o, "f16", "f16", "silu")
+    check_backward(n, i, o, "f16", "silu")
+
+
 def test_more_rows_than_one_launch():
     check_forward(65535 * 64 + 100, 9, 2, "f16", "f16", "relu")
     check_backward(65535 * 64 + 100, 2, 9, "bf16", "relu")
