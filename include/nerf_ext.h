@@ -207,8 +207,8 @@ NERF_API NerfStatus nerf_ext_field_mlp(const uint16_t* density_params, const uin
  *
  * workspace: device memory aligned to 16 bytes that no other call uses at the
  * same time.  A linear layer's calls split a long sum over workgroups as far
- * as it holds the parts (NERF_EXT_LINEAR_WORKSPACE is enough for every split
- * they take) and need none to be right: NULL and 0 serve, slower.  Results
+ * as it holds the parts (NERF_EXT_LINEAR_WORKSPACE holds those of every layer
+ * measured here) and need none to be right: NULL and 0 serve, slower.  Results
  * are the same every time for the same arguments and workspace size. */
 enum { NERF_EXT_ACT_NONE = 0, NERF_EXT_ACT_RELU = 1, NERF_EXT_ACT_SOFTPLUS = 2, NERF_EXT_ACT_SIGMOID = 3, NERF_EXT_ACT_SILU = 4, NERF_EXT_ACT_GELU = 5 /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */ };
 enum { NERF_EXT_LINEAR_WORKSPACE = 64 << 20, NERF_EXT_NORM_WORKSPACE = 64 << 10 };
@@ -221,9 +221,9 @@ typedef struct NerfExtLinearDesc {
     uint32_t out_dtype;       /* of y: dtype or NERF_EXT_F32 */
     uint32_t activation;      /* NERF_EXT_ACT_*; forward: on this layer's output;
                                  backward: the one that made this layer's input */
-    uint32_t x_stride;        /* elements between rows of x, add and dx; 0: in_features */
-    uint32_t y_stride;        /* of y and delta; 0: out_features */
-    uint32_t residual_stride; /* of residual; 0: out_features */
+    uint32_t x_stride;        /* elements between rows of x, add and dx, at most 2^20; 0: in_features */
+    uint32_t y_stride;        /* of y and delta, at most 2^20; 0: out_features */
+    uint32_t residual_stride; /* of residual, at most 2^20; 0: out_features */
     uint32_t reserved;        /* 0 */
 } NerfExtLinearDesc;
 
