@@ -231,7 +231,8 @@ typedef struct NerfExtLinearDesc {
  * [out][in] (dense), bias fp32 [out] or NULL, residual [rows][out] of dtype or
  * NULL, y [rows][out] of out_dtype; pre (dense [rows][out] of dtype, or NULL)
  * gets z, which the backward pass of the next layer reads.  y may be residual
- * itself; no other two arrays may overlap.  Sums in 32 bits, one rounding of
+ * itself where both have one type and one row stride (otherwise that is
+ * refused); no other two arrays may overlap.  Sums in 32 bits, one rounding of
  * each output. */
 NERF_API NerfStatus nerf_ext_linear_forward(const NerfExtLinearDesc* desc, const void* x, const void* weight, const float* bias, const void* residual, void* y, void* pre, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Gradients of the layer from delta [rows][out] = d loss / d z:

@@ -1495,6 +1495,9 @@ NERF_API NerfStatus nerf_ext_linear_forward(const NerfExtLinearDesc* desc, const
     if (d.rows == 0u) return NERF_STATUS_OK;
     NERF_CHECK_ARG(x && weight && y, "nerf_ext_linear_forward: null x, weight or y");
     NERF_CHECK_ARG(aligned(x, 2u) && aligned(weight, 2u) && aligned(residual, 2u) && aligned(pre, 2u) && aligned(bias, 4u) && aligned(y, d.out_dtype == NERF_EXT_F32 ? 4u : 2u), "nerf_ext_linear_forward: an array is not aligned to its elements");
+    // A lane reads the residuals of the outputs that it writes, so y may take their
+    // place; laid out otherwise it would cover residuals that other lanes still need.
+    NERF_CHECK_ARG(y != residual || (d.out_dtype == d.dtype && (d.rows == 1u || d.y_stride == d.residual_stride)), "nerf_ext_linear_forward: y over residual must have its type and row stride");
     NERF_CHECK_ARG(aligned(workspace, 16u), "nerf_ext_linear_forward: workspace must be aligned to 16 bytes");
     const Workspace ws{(float*)workspace, workspace ? workspace_bytes : 0u};
     if (d.dtype == NERF_EXT_F16) return forward<half_t>(d, x, weight, bias, residual, y, pre, ws, (hipStream_t)stream);
