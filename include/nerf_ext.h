@@ -214,7 +214,7 @@ enum { NERF_EXT_ACT_NONE = 0, NERF_EXT_ACT_RELU = 1, NERF_EXT_ACT_SOFTPLUS = 2, 
 enum { NERF_EXT_LINEAR_WORKSPACE = 64 << 20, NERF_EXT_NORM_WORKSPACE = 64 << 10 };
 
 typedef struct NerfExtLinearDesc {
-    uint32_t rows;            /* at most 2^30; 0: gradients of weight and bias are 0 */
+    uint32_t rows;            /* at most 2^30; 0: gradients of weight and bias are 0, and nothing else is written */
     uint32_t in_features;     /* 1..65536 */
     uint32_t out_features;    /* 1..65536 */
     uint32_t dtype;           /* NERF_EXT_F16 or NERF_EXT_BF16: every 16-bit array */

@@ -1518,6 +1518,7 @@ NERF_API NerfStatus nerf_ext_linear_backward(const NerfExtLinearDesc* desc, cons
     NERF_CHECK_ARG(aligned(x, 2u) && aligned(weight, 2u) && aligned(delta, 2u) && aligned(pre, 2u) && aligned(add, 2u) && aligned(dx, 2u) && aligned(dpre, 2u) && aligned(dweight, 4u) && aligned(dbias, 4u),
                    "nerf_ext_linear_backward: an array is not aligned to its elements");
     NERF_CHECK_ARG(aligned(workspace, 16u), "nerf_ext_linear_backward: workspace must be aligned to 16 bytes");
+    if (d.rows == 0u && !dweight) return NERF_STATUS_OK;
     const Workspace ws{(float*)workspace, workspace ? workspace_bytes : 0u};
     if (d.dtype == NERF_EXT_F16) return backward<half_t>(d, x, weight, delta, pre, add, dx, dpre, dweight, dbias, ws, (hipStream_t)stream);
     return backward<bf16_t>(d, x, weight, delta, pre, add, dx, dpre, dweight, dbias, ws, (hipStream_t)stream);

@@ -23,3 +23,12 @@ def test_outputs_over_residuals_that_lie_otherwise(lib, change):
     status = L.status_of("nerf_ext_linear_forward", C.byref(_desc(**change)), A, A, None, A, A, None, None, 0, None)
     assert status == L.NERF_STATUS_INVALID_USAGE
     assert "nerf_ext_linear_forward" in L.last_error() and "residual" in L.last_error()
+
+
+@pytest.mark.parametrize("dx,dpre", [(A, None), (None, A), (A, A)])
+def test_no_rows_and_no_weight_gradient(lib, dx, dpre):
+    """Nothing to compute: nothing is launched, and arrays need not be there."""
+    for arrays in ((None, None, None, None, None), (A, A, A, A, A)):
+        x, w, delta, pre, add = arrays
+        status = L.status_of("nerf_ext_linear_backward", C.byref(_desc(rows=0)), x, w, delta, pre, add, dx, dpre, None, None, None, 0, None)
+        assert status == L.NERF_STATUS_OK, L.last_error()
