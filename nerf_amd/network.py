@@ -31,6 +31,17 @@ def linear_backward(desc: L.NerfExtLinearDesc, x: int | None, weight: int | None
     L.call("nerf_ext_linear_backward", C.byref(desc), x, weight, delta, pre, add, dx, dpre, dweight, dbias, workspace.ptr if workspace else None, workspace.nbytes if workspace else 0, stream.handle if stream else None)
 
 
+def _check_rows(array: DeviceArray, rows: int, width: int, what: str) -> None:
+    """Rows of `width` 16-bit values, `rows` of them at least: an array of rows of
+    any inner shape, or a flat one."""
+    if array.dtype not in (np.float16, np.uint16):
+        raise ValueError(f"{what} is {array.dtype}: it must be float16, or its bits as uint16")
+    size = int(np.prod(array.shape, dtype=np.int64))
+    fits = size >= rows * width if len(array.shape) == 1 else array.shape[0] >= rows and size == array.shape[0] * width
+    if not fits:
+        raise ValueError(f"{what} has shape {array.shape}: {rows} rows of {width} values are needed")
+
+
 class Network:
     """Layers widths[0] -> ... -> widths[-1]: hidden layers act(x W^T + b), plus
     x where a layer is as wide as its input, then a linear layer with fp32
@@ -90,8 +101,10 @@ class Network:
 
     def forward(self, x: DeviceArray, rows: int, stream: Stream | None = None) -> DeviceArray:
         """x: fp16 [rows][widths[0]].  Returns the fp32 outputs, the network's own
-        array; keeps what backward() needs (x is read again there)."""
+        array; keeps what backward() needs (x is read again there).  fp16 arrays may
+        be flat, hold more rows, or hold the numbers' bits as uint16."""
         self._check(rows)
+        _check_rows(x, rows, self.widths[0], "x")
         self._input = x
         for l in range(self.layers):
             last = l == self.layers - 1
@@ -106,6 +119,7 @@ class Network:
         """delta: fp16 [rows][widths[-1]], the loss' derivative in the outputs of the
         last forward() times the loss scale.  Fills the gradients."""
         self._check(rows)
+        _check_rows(delta, rows, self.widths[-1], "delta")
         g = delta  # the gradient in the layer's output, where a residual passes it on
         for l in reversed(range(self.layers)):
             i, o = self.widths[l], self.widths[l + 1]
