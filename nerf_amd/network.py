@@ -54,6 +54,7 @@ class Network:
             raise ValueError(f"unknown activation {activation!r}")
         self.widths, self.max_rows, self.steps_done = list(widths), int(max_rows), 0
         self.act = ACTIVATIONS[activation]
+        self._rows, self._input = None, None  # of the last forward pass
         self.layers = len(widths) - 1
         self.residual = [l < self.layers - 1 and widths[l] == widths[l + 1] for l in range(self.layers)]
         sizes, self._at, at = [], [], 0
@@ -105,7 +106,7 @@ class Network:
         be flat, hold more rows, or hold the numbers' bits as uint16."""
         self._check(rows)
         _check_rows(x, rows, self.widths[0], "x")
-        self._input = x
+        self._rows, self._input = None, x
         for l in range(self.layers):
             last = l == self.layers - 1
             i, o = self.widths[l], self.widths[l + 1]
@@ -113,12 +114,15 @@ class Network:
             src = (x if l == 0 else self._x[l]).ptr
             linear_forward(d, src, self.copies.ptr + 2 * self._at[2 * l], self.y.ptr if last else self._x[l + 1].ptr, bias=self.params.ptr + 4 * self._at[2 * l + 1], residual=src if self.residual[l] else None,
                            pre=None if last else self._z[l].ptr, workspace=self.workspace, stream=stream)
+        self._rows = rows
         return self.y
 
     def backward(self, delta: DeviceArray, rows: int, stream: Stream | None = None) -> None:
         """delta: fp16 [rows][widths[-1]], the loss' derivative in the outputs of the
-        last forward() times the loss scale.  Fills the gradients."""
-        self._check(rows)
+        last forward() times the loss scale; rows: that forward()'s.  Fills the
+        gradients."""
+        if rows != self._rows:
+            raise ValueError(f"{rows} rows: " + ("no forward pass" if self._rows is None else f"the last forward pass had {self._rows}"))
         _check_rows(delta, rows, self.widths[-1], "delta")
         g = delta  # the gradient in the layer's output, where a residual passes it on
         for l in reversed(range(self.layers)):

@@ -1,6 +1,6 @@
 """What Network refuses before it calls the library: arrays too small or of
-another type or width.  Device arrays and the library's calls are stand-ins
-here, so no GPU is needed."""
+another type or width, and a way back that no way forward leads to.  Device
+arrays and the library's calls are stand-ins here, so no GPU is needed."""
 import numpy as np
 import pytest
 
@@ -60,3 +60,35 @@ def test_arrays_that_fit(calls, x, delta):
     net.forward(HostArray(*x), 10)
     net.backward(HostArray(*delta), 10)
     assert calls == ["nerf_ext_linear_forward"] * 3 + ["nerf_ext_linear_backward"] * 3
+
+
+def test_backward_follows_its_forward(calls):
+    delta = HostArray((16, 3), np.float16)
+    net = _net()
+    with pytest.raises(ValueError):
+        net.backward(delta, 10)
+    net.forward(HostArray((16, 6), np.float16), 10)
+    for rows in (9, 11, 16, 0):
+        with pytest.raises(ValueError):
+            net.backward(delta, rows)
+    with pytest.raises(ValueError):
+        net.forward(HostArray((16, 6), np.float32), 12)  # refused: what the last forward kept stays
+    del calls[:]
+    net.backward(delta, 10)
+    net.backward(delta, 10)
+    assert calls == ["nerf_ext_linear_backward"] * 6
+
+
+def test_a_forward_that_failed_has_no_backward(calls, monkeypatch):
+    net, delta = _net(), HostArray((16, 3), np.float16)
+    net.forward(HostArray((16, 6), np.float16), 10)
+
+    def fails(name, *args):
+        raise network.L.NerfError(name, network.L.NERF_STATUS_INVALID_USAGE, "no")
+
+    with monkeypatch.context() as m:
+        m.setattr(network.L, "call", fails)
+        with pytest.raises(network.L.NerfError):
+            net.forward(HostArray((16, 6), np.float16), 10)
+    with pytest.raises(ValueError):
+        net.backward(delta, 10)
