@@ -80,8 +80,9 @@ __device__ __forceinline__ float act_slope(float z) {
     if constexpr (kAct == NERF_EXT_ACT_SIGMOID) return sigmoid_slope(z);
     if constexpr (kAct == NERF_EXT_ACT_SILU) return sigmoid(z) + z * sigmoid_slope(z);
     if constexpr (kAct == NERF_EXT_ACT_GELU) {
-        // The second term vanishes beyond |z| = 16: clamped, its factors stay finite.
-        const float c = fminf(fmaxf(z, -16.0f), 16.0f), t = 2.0f * kGeluA * c * (1.0f + kGeluB * c * c);
+        // The second term vanishes beyond |z| = 16: clamped, its factors stay finite,
+        // and a NaN stays one.
+        const float c = z < -16.0f ? -16.0f : z > 16.0f ? 16.0f : z, t = 2.0f * kGeluA * c * (1.0f + kGeluB * c * c);
         return sigmoid(t) + c * sigmoid_slope(t) * (2.0f * kGeluA) * (1.0f + 3.0f * kGeluB * c * c);
     }
     return 1.0f;
