@@ -78,7 +78,12 @@ __device__ __forceinline__ float act_slope(float z) {
     if constexpr (kAct == NERF_EXT_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
     if constexpr (kAct == NERF_EXT_ACT_SOFTPLUS) return sigmoid(z);
     if constexpr (kAct == NERF_EXT_ACT_SIGMOID) return sigmoid_slope(z);
-    if constexpr (kAct == NERF_EXT_ACT_SILU) return sigmoid(z) + z * sigmoid_slope(z);
+    if constexpr (kAct == NERF_EXT_ACT_SILU) {
+        // The second term vanishes beyond |z| = 110: clamped, it does so at an
+        // infinity too, as a finite z is stored beyond the range of 16 bits.
+        const float c = z < -128.0f ? -128.0f : z > 128.0f ? 128.0f : z;
+        return sigmoid(z) + c * sigmoid_slope(c);
+    }
     if constexpr (kAct == NERF_EXT_ACT_GELU) {
         // The second term vanishes beyond |z| = 16: clamped, its factors stay finite,
         // and a NaN stays one.

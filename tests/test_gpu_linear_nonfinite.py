@@ -9,7 +9,7 @@ from test_gpu_linear import run_backward, run_forward
 pytestmark = pytest.mark.gpu
 
 # act'(-inf), act'(+inf), act'(NaN).  The relu's is (z > 0), which a NaN is not.
-LIMITS = {"none": (1.0, 1.0, 1.0), "relu": (0.0, 1.0, 0.0), "softplus": (0.0, 1.0, np.nan), "sigmoid": (0.0, 0.0, np.nan), "gelu": (0.0, 1.0, np.nan)}
+LIMITS = {"none": (1.0, 1.0, 1.0), "relu": (0.0, 1.0, 0.0), "softplus": (0.0, 1.0, np.nan), "sigmoid": (0.0, 0.0, np.nan), "silu": (0.0, 1.0, np.nan), "gelu": (0.0, 1.0, np.nan)}
 
 
 def _values(pre):
@@ -31,7 +31,7 @@ def test_derivatives_of_infinities_and_nan(act, kind, rows):
     assert np.isfinite(got[pre == 0.25]).all()
 
 
-@pytest.mark.parametrize("act", ["gelu"])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_a_finite_layer_has_finite_gradients(act):
     """z = -90000 is finite in 32 bits and y is 0; its copy in fp16 is -inf."""
     v = _values(np.zeros((5, 8)))
