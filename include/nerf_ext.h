@@ -281,9 +281,9 @@ NERF_API NerfStatus nerf_ext_grad_clip(const NerfExtGradTensor* tensors, uint32_
 /* The trainer's update (backend-cuda.cu:1513-1554) on a caller's tensors: step
  * counts from 1, grad_norm (device) is nerf_ext_grad_norm's of the gradients as
  * they are (times loss_scale).  Nothing changes, and *skipped (device, or NULL)
- * is 1, where the norm / loss_scale is not finite or above
- * update_guard_grad_norm; gradients are scaled by grad_clip_norm / norm where
- * the norm is above it. */
+ * becomes 1, where the norm / loss_scale is not finite or above
+ * update_guard_grad_norm; otherwise *skipped becomes 0 (with empty lists too);
+ * gradients are scaled by grad_clip_norm / norm where the norm is above it. */
 NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_t count, const NerfHyperParams* hyper, uint32_t step, const float* grad_norm, uint32_t* skipped, void* stream);
 
 /* ------------------------------------------------------- context options */

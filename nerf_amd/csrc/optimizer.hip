@@ -434,6 +434,10 @@ NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_
             first = false;
             return hipGetLastError();
         })));
+    if (first && skipped) {  // nothing to update: the flag alone
+        k_adam_tensors<<<1, kThreads, 0, (hipStream_t)stream>>>(AdamList{}, r, grad_norm, skipped);
+        NERF_LAUNCH_CHECK("k_adam_tensors");
+    }
     return NERF_STATUS_OK;
 }
 
