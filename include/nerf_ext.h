@@ -230,10 +230,11 @@ typedef struct NerfExtLinearDesc {
 /* z = x weight^T + bias, y = act(z) + residual: x [rows][in], weight
  * [out][in] (dense), bias fp32 [out] or NULL, residual [rows][out] of dtype or
  * NULL, y [rows][out] of out_dtype; pre (dense [rows][out] of dtype, or NULL)
- * gets z, which the backward pass of the next layer reads.  y may be residual
- * itself where both have one type and one row stride (otherwise that is
- * refused); no other two arrays may overlap.  Sums in 32 bits, one rounding of
- * each output. */
+ * gets z, which the backward pass of the next layer reads.  Inputs may be
+ * one array (a layer with a residual around it: residual = x); an output
+ * overlaps no other array, except that y may be residual itself where both
+ * have one type and one row stride (y = residual is refused otherwise).  Sums
+ * in 32 bits, one rounding of each output. */
 NERF_API NerfStatus nerf_ext_linear_forward(const NerfExtLinearDesc* desc, const void* x, const void* weight, const float* bias, const void* residual, void* y, void* pre, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Gradients of the layer from delta [rows][out] = d loss / d z:
  *   g = delta weight + add     add [rows][in] or NULL: what reaches x on other ways,
@@ -246,7 +247,7 @@ NERF_API NerfStatus nerf_ext_linear_forward(const NerfExtLinearDesc* desc, const
  *   dweight = delta^T x        fp32 [out][in] or NULL, overwritten
  *   dbias = sum over rows of delta   fp32 [out] or NULL; with dweight only
  * The relu's derivative at 0 is 0.  dx may be add itself, dpre may be pre
- * itself; no other two arrays may overlap.  What an output does not need may be
+ * itself; an output overlaps no other array besides.  What an output does not need may be
  * NULL (weight, x, pre). */
 NERF_API NerfStatus nerf_ext_linear_backward(const NerfExtLinearDesc* desc, const void* x, const void* weight, const void* delta, const void* pre, const void* add, void* dx, void* dpre, float* dweight, float* dbias, void* workspace,
                                             uint64_t workspace_bytes, void* stream);
