@@ -279,12 +279,14 @@ NERF_API NerfStatus nerf_ext_grad_norm(const NerfExtGradTensor* tensors, uint32_
  * not finite (it is reported) leaves the values as they are.  A tensor's out
  * may be its grad; it may overlap no other tensor. */
 NERF_API NerfStatus nerf_ext_grad_clip(const NerfExtGradTensor* tensors, uint32_t count, float max_norm, float* norm, void* workspace, uint64_t workspace_bytes, void* stream);
-/* The trainer's update (backend-cuda.cu:1513-1554) on a caller's tensors: step
- * counts from 1, grad_norm (device) is nerf_ext_grad_norm's of the gradients as
+/* The trainer's update rule (backend-cuda.cu:1513-1554) on a caller's tensors;
+ * its coefficients are computed in 64 bits here, the trainer's in 32, so results
+ * agree to rounding and not bit for bit.  step counts from 1, grad_norm (device) is nerf_ext_grad_norm's of the gradients as
  * they are (times loss_scale).  Nothing changes, and *skipped (device, or NULL)
  * becomes 1, where the norm / loss_scale is not finite or above
- * update_guard_grad_norm; otherwise *skipped becomes 0 (with empty lists too);
- * gradients are scaled by grad_clip_norm / norm where the norm is above it. */
+ * update_guard_grad_norm; otherwise *skipped becomes 0 (with empty lists too).
+ * Gradients are divided by loss_scale, and scaled by grad_clip_norm over (norm /
+ * loss_scale) where that norm is above it. */
 NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_t count, const NerfHyperParams* hyper, uint32_t step, const float* grad_norm, uint32_t* skipped, void* stream);
 
 /* ------------------------------------------------------- context options */

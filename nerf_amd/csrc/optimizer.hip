@@ -406,7 +406,8 @@ NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_
         if (!aligned(t.param, 4u) || !aligned(t.grad, 4u) || !aligned(t.m, 4u) || !aligned(t.v, 4u) || !aligned(t.copy, 2u)) return refuse(fn, "a tensor is not aligned to its elements");
     }
     // The trainer's coefficients (backend-cuda.cu:1513-1536), those that do not
-    // depend on the norm computed here in 64 bits.
+    // depend on the norm computed here and in 64 bits (the trainer's kernel takes
+    // its powers in 32: the same rule, not the same bits).
     const double decay = (double)hyper->lr_decay_ksteps * 1000.0;
     AdamRule r;
     r.lr         = decay > 0.0 ? (float)(hyper->learning_rate * pow(0.1, step / decay)) : hyper->learning_rate;
