@@ -115,7 +115,8 @@ def test_workspaces(kind, parts):
 
 # Rows streamed past the weights: 1, 2, 4 and 8 steps of 32 k; whole, cut and odd
 # rows; one to four waves across, narrow outputs, more than 256 of them.
-STREAMED = [(16400, 32, 72), (16399, 24, 40), (16390, 31, 33), (16385, 1, 8), (32770, 64, 264), (32771, 57, 24), (32770, 58, 130), (65541, 128, 72), (65543, 96, 32), (65537, 128, 520), (131077, 256, 136), (131075, 224, 24), (131073, 160, 296)]
+STREAMED = [(16400, 32, 72), (16399, 24, 40), (16390, 31, 33), (16385, 1, 8), (32770, 64, 264), (32771, 57, 24), (32770, 58, 130), (65541, 128, 72), (65543, 96, 32), (65537, 128, 520), (131077, 256, 136), (131075, 224, 24), (131073, 160, 296),
+            (16400, 32, 24), (16399, 30, 32), (16390, 8, 5), (16400, 28, 100), (32770, 64, 32), (32772, 58, 24), (32771, 57, 72), (32769, 33, 256)]
 
 
 @pytest.mark.parametrize("kind", KINDS)
