@@ -1279,9 +1279,11 @@ hipError_t launch_tiles(Operands A, Out out, float* row_sums, Workspace ws, hipS
             if (e != hipSuccess) return e;
             const uint64_t eights = (uint64_t)ceil_div(A.np, 8u) * A.nq;
             auto join = [&](auto slices) { k_join<slices(), Out><<<(uint32_t)std::min<uint64_t>(ceil_div(eights, 256u / slices()), 4096u), 256, 0, stream>>>(so.out, rest, part, parts, sums, row_sums, out); };
+            // 16-bit outputs have four parts at least: four splits or more of at least
+            // 17 tiles of k make as many.
             if (parts >= 16u) join(std::integral_constant<uint32_t, 16u>{});
-            else if (parts >= 4u) join(std::integral_constant<uint32_t, 4u>{});
-            else join(std::integral_constant<uint32_t, 1u>{});
+            else if (!kSums || parts >= 4u) join(std::integral_constant<uint32_t, 4u>{});
+            else if constexpr (kSums) join(std::integral_constant<uint32_t, 1u>{});
             return hipGetLastError();
         }
     }
@@ -1371,6 +1373,8 @@ hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hi
     //   76 / 69 / -, 32768 x 512 -> 512 (2^33) 36 / 38 / 46, 8192 x 1024 -> 1024 (2^33) 36 / 32 / 43, 262144 x 256 -> 256
     //   (2^34) 97 / 77 / 96, 131072 x 512 -> 512 (2^35) 164 / 107 / 102,
     //   16384 x 2048 -> 2048 (2^36) 324 / 165 / 153.
+    // Of the larger tiles only those of weights' gradients (kLong) are split: 16-bit
+    // outputs get them where they are too many for a split in four.
     constexpr bool kLong = kPT && kQT;
     const uint64_t cus  = device_cu_count(), work = (uint64_t)A.np * A.nq * A.nk;
     auto tiles          = [&](uint32_t b) { return (uint64_t)ceil_div(A.np, b) * ceil_div(A.nq, b); };
@@ -1379,12 +1383,12 @@ hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hi
         // Rows on their way as words, two tiles (86 us for 20011 x 1209 -> 487; with
         // one 93); as chunks one (68 us for 20011 x 1210 -> 488, with two 75).
         const bool odd = odd_rows(A.p, A.ldp) || odd_rows(A.q, A.ldq);
-        if (by_128) return odd ? launch_tiles<T, 128, 128, 2, 2, 3, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
+        if (by_128) return odd ? launch_tiles<T, 128, 128, 2, 2, 3, kPT, kQT, kByWords, kLong>(A, out, row_sums, ws, stream) : launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kByChunks, kLong>(A, out, row_sums, ws, stream);
         return odd ? launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kByWords>(A, out, row_sums, ws, stream) : launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kByChunks>(A, out, row_sums, ws, stream);
     }
     if (A.np > 128u && A.nq > 128u && A.nk >= 512u && (kLong ? work >= 1ull << 35 : tiles(256u) >= cus))
         return launch_tiles<T, 256, 256, 2, 4, 2, kPT, kQT, kDirect, kLong>(A, out, row_sums, ws, stream);
-    if (by_128) return launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kDirect>(A, out, row_sums, ws, stream);
+    if (by_128) return launch_tiles<T, 128, 128, 2, 2, 2, kPT, kQT, kDirect, kLong>(A, out, row_sums, ws, stream);
     return launch_tiles<T, 64, 64, 2, 2, 4, kPT, kQT, kDirect>(A, out, row_sums, ws, stream);
 }
 
