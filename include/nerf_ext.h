@@ -246,9 +246,10 @@ NERF_API NerfStatus nerf_ext_linear_forward(const NerfExtLinearDesc* desc, const
  *                              gradient is made
  *   dweight = delta^T x        fp32 [out][in] or NULL, overwritten
  *   dbias = sum over rows of delta   fp32 [out] or NULL; with dweight only
- * The relu's derivative at 0 is 0.  dx may be add itself, dpre may be pre
- * itself; an output overlaps no other array besides.  What an output does not need may be
- * NULL (weight, x, pre). */
+ * The relu's derivative at 0 is 0; where pre is an infinity the derivatives are
+ * their limits.  dx may be add itself, dpre may be pre itself; an output
+ * overlaps no other array besides.  What an output does not need may be NULL
+ * (weight, x, pre). */
 NERF_API NerfStatus nerf_ext_linear_backward(const NerfExtLinearDesc* desc, const void* x, const void* weight, const void* delta, const void* pre, const void* add, void* dx, void* dpre, float* dweight, float* dbias, void* workspace,
                                             uint64_t workspace_bytes, void* stream);
 
@@ -281,12 +282,13 @@ NERF_API NerfStatus nerf_ext_grad_norm(const NerfExtGradTensor* tensors, uint32_
 NERF_API NerfStatus nerf_ext_grad_clip(const NerfExtGradTensor* tensors, uint32_t count, float max_norm, float* norm, void* workspace, uint64_t workspace_bytes, void* stream);
 /* The trainer's update rule (backend-cuda.cu:1513-1554) on a caller's tensors;
  * its coefficients are computed in 64 bits here, the trainer's in 32, so results
- * agree to rounding and not bit for bit.  step counts from 1, grad_norm (device) is nerf_ext_grad_norm's of the gradients as
- * they are (times loss_scale).  Nothing changes, and *skipped (device, or NULL)
- * becomes 1, where the norm / loss_scale is not finite or above
- * update_guard_grad_norm; otherwise *skipped becomes 0 (with empty lists too).
- * Gradients are divided by loss_scale, and scaled by grad_clip_norm over (norm /
- * loss_scale) where that norm is above it. */
+ * agree to rounding and not bit for bit.  step counts from 1, grad_norm (device)
+ * is nerf_ext_grad_norm's of the gradients as they are (times loss_scale).
+ * Nothing changes, and *skipped (device, or NULL) becomes 1, where the norm /
+ * loss_scale is not finite or above update_guard_grad_norm; otherwise *skipped
+ * becomes 0 (with empty lists too).  Gradients are divided by loss_scale, and
+ * scaled by grad_clip_norm over (norm / loss_scale) where that norm is above
+ * grad_clip_norm. */
 NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_t count, const NerfHyperParams* hyper, uint32_t step, const float* grad_norm, uint32_t* skipped, void* stream);
 
 /* ------------------------------------------------------- context options */

@@ -1394,7 +1394,7 @@ hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hi
 
 // Products of few tiles are those of at most 4096 k (1 x 4096 -> 4096 9 us, by
 // larger tiles with k split over workgroups 13; 1 x 8192 -> 4096 17.5 against
-// 15.5) whose tiles the card takes at once.
+// 15.5) with at most two tiles a CU.
 constexpr uint32_t kFewMaxK = 4096u;
 bool few_operands(const Operands& A, bool pt, bool qt) { return A.nk <= kFewMaxK && !few_values(A, pt, qt); }
 uint64_t few_tiles(const Operands& A, uint32_t f) { return (uint64_t)ceil_div(A.np, 16u * f) * ceil_div(A.nq, 16u * f); }
@@ -1442,10 +1442,11 @@ NerfStatus backward(const NerfExtLinearDesc& d, const void* x, const void* w, co
     const bool to_x = (dx || dpre) && d.rows != 0u;
     if ((!to_x || few_operands(all_x, true, false)) && (!dw || few_operands(all_w, true, true))) {
         const InputGradientOut<T> x_out{(const T*)add, (T*)dx, (const T*)pre, (T*)dpre, d.x_stride, d.in_features, d.rows, d.activation, vec};
-        // The smallest tile of which the card takes all at once, two a CU; those of 64
-        // a side up to 2048 rows, which a workgroup of dW goes through (2048 x 256 ->
-        // 256 11 us and 15 in three launches, 1024 x 1024 -> 1024 18 and 21, but
-        // 4096 x 256 -> 256 23 and 17).
+        // The smallest tile with at most two workgroups a CU.  Those of 16 and 32 a side
+        // run at once; those of 64, whose 130 KB of LDS leave a CU room for one, run in
+        // up to two turns, and are taken up to 2048 rows, which a workgroup of dW goes
+        // through (2048 x 256 -> 256 11 us and 15 in three launches, 1024 x 1024 -> 1024,
+        // 512 of them, 18 and 21, but 4096 x 256 -> 256 23 and 17).
         const uint32_t most = 2u * device_cu_count();
         auto blocks         = [&](uint32_t f) { return (to_x ? few_tiles(all_x, f) : 0u) + (dw ? few_tiles(all_w, f) : 0u); };
         auto launch         = [&](auto f) {
