@@ -291,6 +291,79 @@ NERF_API NerfStatus nerf_ext_grad_clip(const NerfExtGradTensor* tensors, uint32_
  * grad_clip_norm. */
 NERF_API NerfStatus nerf_ext_adam_step(const NerfExtAdamTensor* tensors, uint32_t count, const NerfHyperParams* hyper, uint32_t step, const float* grad_norm, uint32_t* skipped, void* stream);
 
+/* ------------------------- rows in groups: grouped layers and adapters */
+/* A host's networks for many regions, scenes or views at once, beside the linear
+ * layers above (no counterpart in the reference): rows are put in groups, every
+ * group has weights of its own (a grouped layer) or a low-rank adapter of its own
+ * beside weights that all share.  Arrays, workspaces, streams and graphs as for
+ * the linear layers. */
+enum { NERF_EXT_MAX_GROUPS = 4096, NERF_EXT_MAX_RANK = 256, NERF_EXT_GROUP_WORKSPACE = 16 << 20 };
+
+/* offsets [groups + 1]: offsets[g] = number of rows with ids[row] < g;
+ * order [rows]: the rows by their ids, those of one id in their own order, those
+ *   in no group (ids[row] >= groups) last: group g has order[offsets[g]] ..
+ *   order[offsets[g + 1] - 1];
+ * place [rows] or NULL: its inverse, place[order[i]] = i.
+ * rows: at most 2^30.  Up to 16384 rows no workspace is used;
+ * NERF_EXT_GROUP_WORKSPACE serves any number of rows and groups, less (or NULL
+ * and 0) is slower. */
+NERF_API NerfStatus nerf_ext_group_rows(const uint32_t* ids, uint32_t rows, uint32_t groups, uint32_t* offsets, uint32_t* order, uint32_t* place, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Positions 0 .. rows - 1 (NerfExtLinearDesc.rows of them) in the groups' order:
+ * group g has those from offsets[g] to offsets[g + 1].  Position i stands for row
+ * x_rows[i] of the arrays on the layer's input side (x, add, dx, pre of the
+ * backward pass, dpre), and for row y_rows[i] of those on its output side
+ * (y, residual, pre of the forward pass, delta); without an index for row i.
+ * offsets do not decrease; they are read as rows where they are beyond it, and
+ * positions before the first and from the last on are in no group.  An index may
+ * name a row twice where it is read; a row that is written is named once.
+ * Entries that are no row of the array (x_count, y_count) are read as rows of
+ * zeros, and nothing is written for them. */
+typedef struct NerfExtRowGroups {
+    const uint32_t* offsets; /* device, [groups + 1] */
+    const uint32_t* x_rows;  /* device, [rows], or NULL */
+    const uint32_t* y_rows;  /* device, [rows], or NULL */
+    uint32_t groups;         /* 1..4096 */
+    uint32_t x_count;        /* rows of the input side's arrays, with x_rows; 0: rows */
+    uint32_t y_count;        /* of the output side's, with y_rows; 0: rows */
+    uint32_t reserved;       /* 0 */
+} NerfExtRowGroups;
+
+/* nerf_ext_linear_forward with weights [groups][out][in] and bias fp32
+ * [groups][out] (or NULL).  Rows in no group keep what y and pre hold. */
+NERF_API NerfStatus nerf_ext_grouped_linear_forward(const NerfExtLinearDesc* desc, const NerfExtRowGroups* groups, const void* x, const void* weight, const float* bias, const void* residual, void* y, void* pre, void* workspace,
+                                                   uint64_t workspace_bytes, void* stream);
+/* nerf_ext_linear_backward with dweight [groups][out][in] and dbias [groups][out],
+ * sums over the group's rows (0 for a group without rows). */
+NERF_API NerfStatus nerf_ext_grouped_linear_backward(const NerfExtLinearDesc* desc, const NerfExtRowGroups* groups, const void* x, const void* weight, const void* delta, const void* pre, const void* add, void* dx, void* dpre, float* dweight,
+                                                    float* dbias, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* An adapter of every group: the layer's weights are W + scale up down. */
+typedef struct NerfExtAdapters {
+    const void* down;    /* [groups][rank][in] of dtype */
+    const void* up;      /* [groups][out][rank] of dtype */
+    const float* scales; /* fp32 [groups], or NULL: 1 */
+    uint32_t rank;       /* 1..256 */
+    uint32_t reserved;   /* 0 */
+} NerfExtAdapters;
+
+/* mid = down x, z = weight x + bias + scale up mid, y = act(z) + residual: weight
+ * [out][in] and bias [out] are shared, mid is fp32 [rows][rank] by position (for
+ * the backward pass).  Rows in no group have no adapter: z = weight x + bias, and
+ * mid keeps what it holds there. */
+NERF_API NerfStatus nerf_ext_adapter_linear_forward(const NerfExtLinearDesc* desc, const NerfExtRowGroups* groups, const NerfExtAdapters* adapters, const void* x, const void* weight, const float* bias, const void* residual, void* y, void* pre,
+                                                   float* mid, void* workspace, uint64_t workspace_bytes, void* stream);
+/* Gradients from delta, the shared weights held (theirs are
+ * nerf_ext_linear_backward's):
+ *   dmid = scale up^T delta      fp32 [rows][rank] by position; dx, dpre and ddown need it
+ *   g = delta weight + dmid down + add,  dx = g,  dpre = g act'(pre)
+ *   ddown = dmid^T x, dup = scale delta^T mid    fp32 [groups][rank][in] and
+ *                                [groups][out][rank], sums over the group's rows
+ * Outputs may be NULL, and what no output needs too.  Rows in no group: dmid keeps
+ * what it holds, g = delta weight + add. */
+NERF_API NerfStatus nerf_ext_adapter_linear_backward(const NerfExtLinearDesc* desc, const NerfExtRowGroups* groups, const NerfExtAdapters* adapters, const void* x, const void* weight, const void* delta, const float* mid, const void* pre,
+                                                    const void* add, void* dx, void* dpre, float* dmid, float* ddown, float* dup, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------- context options */
 /* Options of a nerf.h context (void* from nerf_create_context); nerf.h itself
  * cannot express them.

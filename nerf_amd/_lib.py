@@ -126,6 +126,7 @@ NERF_EXT_BF16 = 2
 NERF_EXT_ACT_NONE, NERF_EXT_ACT_RELU, NERF_EXT_ACT_SOFTPLUS, NERF_EXT_ACT_SIGMOID, NERF_EXT_ACT_SILU, NERF_EXT_ACT_GELU = range(6)
 NERF_EXT_LINEAR_WORKSPACE = 64 << 20
 NERF_EXT_NORM_WORKSPACE = 64 << 10
+NERF_EXT_MAX_GROUPS, NERF_EXT_MAX_RANK, NERF_EXT_GROUP_WORKSPACE = 4096, 256, 16 << 20
 NERF_EXT_MODEL_HASHGRID = 0
 NERF_EXT_MODEL_REFERENCE = 1
 NERF_EXT_SAMPLING_DEFAULT = 0
@@ -269,6 +270,14 @@ class NerfExtAdamTensor(C.Structure):
     _fields_ = [(k, C.c_void_p) for k in ("param", "grad", "m", "v", "copy")] + [("count", C.c_uint64), ("copy_dtype", C.c_uint32), ("reserved", C.c_uint32)]
 
 
+class NerfExtRowGroups(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("offsets", "x_rows", "y_rows")] + [(k, C.c_uint32) for k in ("groups", "x_count", "y_count", "reserved")]
+
+
+class NerfExtAdapters(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("down", "up", "scales")] + [("rank", C.c_uint32), ("reserved", C.c_uint32)]
+
+
 class NerfExtContextOptions(C.Structure):
     _fields_ = [("model_kind", C.c_uint32), ("inference_sampling", C.c_uint32)]
 
@@ -374,6 +383,12 @@ PROTOTYPES: dict[str, tuple] = {
     "nerf_ext_grad_norm": (_S, [C.POINTER(NerfExtGradTensor), _U32, _P, _P, _U64, _P]),
     "nerf_ext_grad_clip": (_S, [C.POINTER(NerfExtGradTensor), _U32, _F, _P, _P, _U64, _P]),
     "nerf_ext_adam_step": (_S, [C.POINTER(NerfExtAdamTensor), _U32, C.POINTER(NerfHyperParams), _U32, _P, _P, _P]),
+    # rows in groups
+    "nerf_ext_group_rows": (_S, [_P, _U32, _U32, _P, _P, _P, _P, _U64, _P]),
+    "nerf_ext_grouped_linear_forward": (_S, [C.POINTER(NerfExtLinearDesc), C.POINTER(NerfExtRowGroups), _P, _P, _P, _P, _P, _P, _P, _U64, _P]),
+    "nerf_ext_grouped_linear_backward": (_S, [C.POINTER(NerfExtLinearDesc), C.POINTER(NerfExtRowGroups), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P]),
+    "nerf_ext_adapter_linear_forward": (_S, [C.POINTER(NerfExtLinearDesc), C.POINTER(NerfExtRowGroups), C.POINTER(NerfExtAdapters), _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P]),
+    "nerf_ext_adapter_linear_backward": (_S, [C.POINTER(NerfExtLinearDesc), C.POINTER(NerfExtRowGroups), C.POINTER(NerfExtAdapters), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P]),
     # scene
     "nerf_ext_scene_gaussians": (_S, [C.POINTER(NerfExtSceneDesc), _P]),
     "nerf_ext_scene_density": (_S, [_P, _U32, _P, _U32, _P, _P]),

@@ -1,0 +1,476 @@
+// adapter.hip — linear layers with weights shared by all rows and a low-rank
+// adapter of every group of rows beside them (include/nerf_ext.h,
+// nerf_ext_adapter_linear_*).
+//
+//   forward:   m_i = A_g x_i,  z_i = W x_i + b + s_g B_g m_i,  y_i = act(z_i) + r_i
+//   backward:  n_i = s_g B_g^T d_i,  g_i = d_i W + n_i A_g + a_i,  dx = g,  dpre = g act'(pre),
+//              dA_g = sum_i n_i x_i^T,  dB_g = s_g sum_i d_i m_i^T
+//
+// m and n (rank values a row, 32 bits) are a grouped product of their own; the
+// shared product then goes over all rows in tiles of any groups, and each wave
+// adds its rows' low-rank part to its sums before they leave.  B_g m_i is summed
+// by the matrix instructions of the layer's type: each m is split into two values
+// of that type (three where fp32 outputs of bf16 values keep more), high and low
+// part, whose products are as if the rank were two or three times as large.  For
+// fp16 a row's m are first scaled by a power of two to less than 2 (8 at the end
+// of 32 bits' range), which keeps them and their low parts in its range.
+#include "grouped_device.hpp"
+
+using namespace nerf_hip;
+using namespace nerf_hip::grouped;
+
+namespace {
+
+// The low-rank part of a wave's sums: low [rows][rank] times wide, which is
+// [groups][np][rank] (kPT: [groups][rank][np]).
+template <typename T, bool kPT>
+struct LowRank {
+    static constexpr bool kOn = true;
+    using x8 = typename Vec<T>::x8;
+    const float* low;
+    const T* wide;
+    const float* scales;
+    Groups G;
+    uint32_t np, rank, pieces;
+    bool vec_low, vec_wide;  // rows of low / of wide in whole aligned chunks
+
+    // Eight of a row's values from r0, zeros beyond the rank.
+    __device__ __forceinline__ floatx8 low_eight(uint32_t position, uint32_t r0) const {
+        const float* at = low + (uint64_t)position * rank + r0;
+        floatx8 v;
+        if (vec_low) {
+            v.lo = reinterpret_cast<const floatx4*>(at)[0];
+            v.hi = reinterpret_cast<const floatx4*>(at)[1];
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) v[e] = r0 + e < rank ? at[e] : 0.0f;
+        }
+        return v;
+    }
+    __device__ __forceinline__ x8 wide_eight(uint32_t g, uint32_t p, uint32_t r0) const {
+        x8 v;
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) v[e] = (T)0.0f;
+        if (p < np) {
+            if constexpr (!kPT) {
+                const T* at = wide + ((uint64_t)g * np + p) * rank + r0;
+                if (vec_wide) return *reinterpret_cast<const x8*>(at);
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e)
+                    if (r0 + e < rank) v[e] = at[e];
+            } else {
+                const T* at = wide + ((uint64_t)g * rank + r0) * np + p;
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e)
+                    if (r0 + e < rank) v[e] = at[(uint64_t)e * np];
+            }
+        }
+        return v;
+    }
+    // Piece `piece` of eight values.
+    static __device__ __forceinline__ x8 piece_of(floatx8 v, uint32_t piece) {
+        x8 h = __builtin_convertvector(v, x8);
+        for (uint32_t i = 0; i < piece; ++i) {
+            const floatx8 back = __builtin_convertvector(h, floatx8);
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) v[e] = fabsf(back[e]) < __builtin_inff() ? v[e] - back[e] : 0.0f;  // nothing is left of an infinity or NaN
+            h = __builtin_convertvector(v, x8);
+        }
+        return h;
+    }
+
+    // acc[i][j]: 16 outputs from p0 + 16 i at 16 positions from q0 + 16 j, four
+    // consecutive outputs of position lane % 16 a lane.
+    template <uint32_t kFP, uint32_t kFQ>
+    __device__ __forceinline__ void add(floatx4 (&acc)[kFP][kFQ], uint32_t p0, uint32_t q0, uint32_t share, uint32_t shares) const {
+        const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, quarter = lane >> 4;
+        static_assert(16u * kFQ <= 64u);
+        // The group of position q0 + lane.
+        uint32_t mine = kNoRow;
+        if (lane < 16u * kFQ && q0 + lane < G.rows) {
+            uint32_t first = 0u, last = G.count;  // offsets[g] <= position for g < first, not for g >= last
+            while (first < last) {
+                const uint32_t middle = (first + last) / 2u;
+                if (G.offset(middle) <= q0 + lane) first = middle + 1u;
+                else last = middle;
+            }
+            if (first && q0 + lane < G.offset(first)) mine = first - 1u;
+        }
+        if (__ballot(mine != kNoRow) == 0ull) return;
+        const uint32_t chunks = (rank + 7u) / 8u, steps = (pieces * chunks + 3u) / 4u;
+        uint32_t group[kFQ];
+        float up[kFQ], down[kFQ];  // a power of two a row, and its inverse
+#pragma unroll
+        for (uint32_t j = 0; j < kFQ; ++j) {
+            group[j] = (uint32_t)__shfl((int)mine, (int)(16u * j + l));
+            up[j] = down[j] = 1.0f;
+            if constexpr (std::is_same_v<T, half_t>) {
+                float most = 0.0f;
+                if (group[j] != kNoRow) {
+                    for (uint32_t c = quarter; c < chunks; c += 4u) {
+                        const floatx8 v = low_eight(q0 + 16u * j + l, 8u * c);
+#pragma unroll
+                        for (uint32_t e = 0; e < 8u; ++e) most = fmaxf(most, fabsf(v[e]));
+                    }
+                }
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 1u), 252u);
+                if (most > 0.0f && most < __builtin_inff()) {
+                    up[j]   = __uint_as_float(exponent << 23);
+                    down[j] = __uint_as_float((254u - exponent) << 23);
+                }
+            }
+        }
+        for (uint32_t s = 0; s < steps; ++s) {
+            const uint32_t chunk = 4u * s + quarter, piece = chunk / chunks, r0 = 8u * (chunk - piece * chunks);
+            x8 fq[kFQ];
+#pragma unroll
+            for (uint32_t j = 0; j < kFQ; ++j) {
+                floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                if (group[j] != kNoRow && piece < pieces) v = low_eight(q0 + 16u * j + l, r0);
+                fq[j] = piece_of(v * down[j], piece < pieces ? piece : 0u);
+            }
+            // The groups of the wave's rows, one after another.
+            uint64_t left = __ballot(mine != kNoRow);
+            for (uint32_t turn = 0; left; ++turn) {
+                const uint32_t g = (uint32_t)__builtin_amdgcn_readlane((int)mine, __builtin_ctzll(left));
+                const uint64_t those = __ballot(mine == g);
+                left &= ~those;
+                if (turn % shares != share) continue;
+                const float scale = scales ? scales[g] : 1.0f;
+#pragma unroll
+                for (uint32_t i = 0; i < kFP; ++i) {
+                    x8 fp;
+#pragma unroll
+                    for (uint32_t e = 0; e < 8u; ++e) fp[e] = (T)0.0f;
+                    if (piece < pieces) fp = wide_eight(g, p0 + 16u * i + l, r0);
+#pragma unroll
+                    for (uint32_t j = 0; j < kFQ; ++j) {
+                        if (!(those >> (16u * j) & 0xFFFFull)) continue;
+                        const floatx4 part = Vec<T>::mfma(fp, fq[j], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+                        // Rows of other groups keep theirs, whatever this group's weights hold.
+                        const float factor = up[j] * scale;
+#pragma unroll
+                        for (uint32_t r = 0; r < 4u; ++r) acc[i][j][r] = group[j] == g ? acc[i][j][r] + factor * part[r] : acc[i][j][r];
+                    }
+                }
+            }
+        }
+    }
+};
+
+// The shared product in tiles, see product().
+template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, Mode kMode, bool kGather, typename Out>
+__global__ __launch_bounds__(kWP * kWQ * 64u) void k_adapter(GatheredOperands A, Out out, LowRank<T, kPT> more) {
+    __shared__ uint32_t rows[kBQ];
+    const uint32_t block = block_number(), tiles = A.tiles_p * A.tiles_q;
+    if (block >= tiles) return;
+    const uint32_t t = chip_tile(block, tiles), band = A.tiles_p > 4u ? 4u : 1u;
+    const uint32_t first = t / (band * A.tiles_p) * band, high = min(band, A.tiles_q - first), in_band = t - first * A.tiles_p;
+    const Place at{in_band / high * kBP, (first + in_band % high) * kBQ, 0u, A.nk, 0u, 0u};
+    find_rows<kBQ>(out, rows, at.q0, A.nq);
+    product<T, kBP, kBQ, kWP, kWQ, kDepth, kPT, false, kMode, kGather>(A, out, at, more);
+}
+
+// The same with few tiles: the waves share the groups.
+template <typename T, uint32_t kF, bool kPT, bool kWords, bool kGather, typename Out>
+__global__ __launch_bounds__(kFewWaves * 64u) void k_adapter_few(GatheredOperands A, Out out, LowRank<T, kPT> more) {
+    __shared__ floatx4 lds[few_lds(kF) / 16u];
+    __shared__ uint32_t rows[16u * kF];
+    const Place at{blockIdx.x % A.tiles_p * 16u * kF, blockIdx.x / A.tiles_p * 16u * kF, 0u, A.nk, 0u, 0u};
+    find_rows<16u * kF>(out, rows, at.q0, A.nq);
+    __syncthreads();
+    few_tile<T, kF, kPT, false, kWords, kGather>(A, out, at, reinterpret_cast<char*>(lds), nullptr, more);
+}
+
+// Operands of fewer than eight values in all: a thread an output of a position.
+template <typename T, bool kPT, typename Out>
+__global__ __launch_bounds__(64) void k_adapter_tiny(GatheredOperands A, Out out, LowRank<T, kPT> more) {
+    __shared__ uint32_t rows[1];
+    const Groups& G = more.G;
+    for (uint32_t position = blockIdx.x; position < A.nq; position += gridDim.x) {
+        Out mine = out;
+        __syncthreads();
+        find_rows<1u>(mine, rows, position, position + 1u);
+        __syncthreads();
+        const Part part     = part_at(G, 1u, position);
+        const bool member   = part.q0 < part.end;
+        const uint32_t g    = part.group, from = gathered_row(A.q_index, A.q_count, position, position + 1u);
+        const float scale   = member && more.scales ? more.scales[g] : 1.0f;
+        for (uint32_t p = 8u * threadIdx.x; p < A.np; p += 512u) {
+            const uint32_t n = min(8u, A.np - p);
+            const typename Out::Aux aux = mine.load(position, 0u, p, n);
+            floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, b = v;
+            for (uint32_t k = 0; k < A.nk; ++k) {
+                const float x = from == kNoRow ? 0.0f : (float)((const T*)A.q)[from * A.ldq + k];
+#pragma unroll
+                for (uint32_t r = 0; r < 8u; ++r)
+                    if (r < n) v[r] += x * (float)((const T*)A.p)[kPT ? k * A.ldp + p + r : (p + r) * A.ldp + k];
+            }
+            for (uint32_t k = 0; member && k < more.rank; ++k) {
+                const float m = scale * more.low[(uint64_t)position * more.rank + k];
+#pragma unroll
+                for (uint32_t r = 0; r < 8u; ++r)
+                    if (r < n) v[r] += m * (float)more.wide[kPT ? ((uint64_t)g * more.rank + k) * A.np + p + r : ((uint64_t)g * A.np + p + r) * more.rank + k];
+            }
+            if constexpr (Out::kBias) {
+                if (mine.bias) {
+#pragma unroll
+                    for (uint32_t r = 0; r < 8u; ++r)
+                        if (r < n) b[r] = mine.bias[p + r];
+                }
+            }
+            mine.put(position, 0u, p, n, v, b, aux);
+        }
+    }
+}
+
+// ------------------------------------------------------- gradients of adapters
+// out_g(w, r) = scale_g sum_i wide(i, w) low(i, r): wide 16-bit rows, as an index
+// names them, low 32-bit by position; kBW wide x kBR low values a workgroup, sums
+// over parts of `size` positions of a group.  The products are of 32-bit values,
+// so the matrix instruction is the 32-bit one, four positions at a time.  out is
+// [groups][nw][nr], or with `low_major` [groups][nr][nw].
+struct RankSums {
+    const void* wide;
+    const float* low;
+    const float* scales;
+    float *out, *parts;
+    const uint32_t* index;
+    uint64_t ld;
+    uint32_t count, nw, nr, tiles_w, tiles_r;
+    bool low_major;
+};
+constexpr uint32_t kBW = 128u;
+template <typename T, uint32_t kBR>
+__global__ __launch_bounds__(256) void k_rank_sums(RankSums A, Groups G, uint32_t size, uint32_t most) {
+    constexpr uint32_t kFR = kBR / 16u;
+    __shared__ uint4 lds_wide[kBW * 8u];
+    __shared__ float lds_low[kBK * kBR];
+    const uint32_t tiles = A.tiles_w * A.tiles_r, parts = min(most, part_count(G, size)), block = block_number();
+    if (block >= parts * tiles) return;
+    const uint32_t t = chip_tile(block, parts * tiles);
+    const Part part = part_of(G, size, t / tiles);
+    if (part.q0 >= part.end && part.number) return;
+    const uint32_t w0 = t % tiles % A.tiles_w * kBW, r0 = t % tiles / A.tiles_w * kBR;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, l = lane & 15u, quarter = lane >> 4;
+    const uint32_t end = min(part.end, part.q0 + size);
+    floatx4 acc[2][kFR];
+#pragma unroll
+    for (uint32_t i = 0; i < 2u; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < kFR; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    GatherStager<T, kBW, true, 256u> stage;
+    stage.begin(A.index, A.count, part.q0, end);
+    constexpr uint32_t kLow = kBK * kBR / 256u;
+    float held[kLow];
+    auto fetch = [&](uint32_t k) {
+        stage.fetch((const T*)A.wide, A.index, A.count, A.ld, A.nw, w0, k, end);
+#pragma unroll
+        for (uint32_t i = 0; i < kLow; ++i) {
+            const uint32_t e = i * 256u + threadIdx.x, line = k + e / kBR, r = r0 + e % kBR;
+            held[i] = line < end && r < A.nr ? A.low[(uint64_t)line * A.nr + r] : 0.0f;
+        }
+    };
+    const uint32_t base = fragment_base<kBW, true>(32u * wave);
+    if (part.q0 < end) fetch(part.q0);
+    for (uint32_t k = part.q0; k < end; k += kBK) {
+        stage.keep(lds_wide, (const T*)A.wide, A.ld, A.nw, w0, k, end);
+#pragma unroll
+        for (uint32_t i = 0; i < kLow; ++i) lds_low[i * 256u + threadIdx.x] = held[i];
+        __syncthreads();
+        if (k + kBK < end) fetch(k + kBK);
+#pragma unroll
+        for (uint32_t step = 0; step < 2u; ++step) {
+            floatx8 w[2];
+#pragma unroll
+            for (uint32_t i = 0; i < 2u; ++i) {
+                typename Vec<T>::x8 f = fragment<T, kBW, true>(lds_wide, base, i, step);
+                settle_here(f);
+                w[i] = __builtin_convertvector(f, floatx8);
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e)
+#pragma unroll
+                for (uint32_t j = 0; j < kFR; ++j) {
+                    const float m = lds_low[(32u * step + 8u * quarter + e) * kBR + 16u * j + l];
+#pragma unroll
+                    for (uint32_t i = 0; i < 2u; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i][e], m, acc[i][j], 0, 0, 0);
+                }
+        }
+        __syncthreads();
+    }
+    const uint64_t length = (uint64_t)A.nw * A.nr;
+    float* out = part.number ? A.parts + place_of(G, part, size) * length : A.out + part.group * length;
+    const float scale = A.scales ? A.scales[part.group] : 1.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 2u; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < kFR; ++j) {
+            const uint32_t r = r0 + 16u * j + l;
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) {
+                const uint32_t w = w0 + 32u * wave + 16u * i + 4u * quarter + e;
+                if (r < A.nr && w < A.nw) out[A.low_major ? (uint64_t)r * A.nw + w : (uint64_t)w * A.nr + r] = scale * acc[i][j][e];
+            }
+        }
+}
+
+// Wide arrays of fewer than eight values in all: one thread an output.
+template <typename T>
+__global__ __launch_bounds__(256) void k_rank_tiny_sums(RankSums A, Groups G) {
+    const uint64_t at = block_number() * 256ull + threadIdx.x, length = (uint64_t)A.nw * A.nr;
+    if (at >= G.count * length) return;
+    const uint32_t g = (uint32_t)(at / length), e = (uint32_t)(at % length), w = A.low_major ? e % A.nw : e / A.nr, r = A.low_major ? e / A.nw : e % A.nr;
+    float v = 0.0f;
+    for (uint32_t i = G.offset(g), end = G.offset(g + 1u); i < end; ++i) {
+        const uint32_t row = gathered_row(A.index, A.count, i, end);
+        v += (row == kNoRow ? 0.0f : (float)((const T*)A.wide)[row * A.ld + w]) * A.low[(uint64_t)i * A.nr + r];
+    }
+    A.out[at] = (A.scales ? A.scales[g] : 1.0f) * v;
+}
+
+// ------------------------------------------------------------------- host
+bool near(uint64_t count, uint64_t ld) { return count * ld * 2u < 1ull << 31; }
+
+template <typename T, bool kPT, typename Out>
+hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& more, hipStream_t stream) {
+    const uint64_t weights = (uint64_t)A.np * A.nk, values = (uint64_t)(A.q_count - 1u) * A.ldq + A.nk;
+    if (weights < 8u || values < 8u) {
+        k_adapter_tiny<T, kPT, Out><<<std::min(A.nq, 64u * device_cu_count()), 64, 0, stream>>>(A, out, more);
+        return hipGetLastError();
+    }
+    auto launch = [&](auto kernel, uint32_t bp, uint32_t bq, uint32_t threads) {
+        A.tiles_p = ceil_div(A.np, bp);
+        A.tiles_q = ceil_div(A.nq, bq);
+        kernel<<<grid_of((uint64_t)A.tiles_p * A.tiles_q), threads, 0, stream>>>(A, out, more);
+        return hipGetLastError();
+    };
+    const bool gather = A.q_index != nullptr;
+    const bool words  = !whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, A.nk) || (gather && !near(A.q_count, A.ldq));
+    if (words) return launch(k_adapter<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
+    return gather ? launch(k_adapter<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_adapter<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
+}
+
+template <typename T>
+hipError_t launch_rank_sums(RankSums A, const Groups& G, Workspace ws, hipStream_t stream) {
+    const uint64_t length = (uint64_t)A.nw * A.nr;
+    if (G.rows == 0u || (uint64_t)(A.count - 1u) * A.ld + A.nw < 8u) {
+        k_rank_tiny_sums<T><<<grid_of((G.count * length + 255u) / 256u), 256, 0, stream>>>(A, G);
+        return hipGetLastError();
+    }
+    auto launch = [&](auto kernel, uint32_t br) {
+        A.tiles_w = ceil_div(A.nw, kBW);
+        A.tiles_r = ceil_div(A.nr, br);
+        const uint64_t tiles = (uint64_t)A.tiles_w * A.tiles_r;
+        const uint32_t size  = part_size(G.rows, tiles, 4u * device_cu_count(), 4u * length, ws.bytes), most = G.rows / size + G.count;
+        A.parts              = ws.data;
+        kernel<<<grid_of(most * tiles), 256, 0, stream>>>(A, G, size, most);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || size >= G.rows) return e;
+        return launch_join(G, size, A.out, ws.data, length, nullptr, nullptr, 0u, stream);
+    };
+    if (A.nr <= 16u) return launch(k_rank_sums<T, 16>, 16u);
+    if (A.nr <= 32u) return launch(k_rank_sums<T, 32>, 32u);
+    return launch(k_rank_sums<T, 64>, 64u);
+}
+
+template <typename T, bool kPT>
+LowRank<T, kPT> low_rank(const float* low, const void* wide, const float* scales, const Groups& G, uint32_t np, uint32_t rank, uint32_t pieces) {
+    return {low, (const T*)wide, scales, G, np, rank, pieces, rank % 8u == 0u && aligned(low, 16u), rank % 8u == 0u && aligned(wide, 16u)};
+}
+
+template <typename T>
+NerfStatus forward(const NerfExtLinearDesc& d, const NerfExtRowGroups& r, const NerfExtAdapters& a, const void* x, const void* w, const float* bias, const void* residual, void* y, void* pre, float* mid, hipStream_t stream) {
+    const Groups G{r.offsets, r.groups, d.rows};
+    NERF_HIP_TRY((launch_ranks<T, false>(G, (const T*)x, d.x_stride, r.x_rows, r.x_count, (const T*)a.down, d.in_features, a.rank, nullptr, mid, stream)));
+    const bool vec = d.out_features % 8u == 0u && d.y_stride % 8u == 0u && aligned(y, 16u) && aligned(pre, 16u) && (!residual || (d.residual_stride % 8u == 0u && aligned(residual, 16u)));
+    const bool y32 = d.out_dtype == NERF_EXT_F32;
+    const GatheredOperands A{{w, x, d.in_features, d.x_stride, d.out_features, d.rows, d.in_features, 0u, 0u, 0u}, nullptr, r.x_rows, 0u, r.x_count};
+    const RowsForwardOut<T> out{bias, (const T*)residual, y, (T*)pre, d.residual_stride, d.y_stride, d.out_features, d.rows, d.activation, y32, vec, r.y_rows, r.y_count, nullptr};
+    NERF_HIP_TRY((launch_adapter<T, false>(A, out, low_rank<T, false>(mid, a.up, a.scales, G, d.out_features, a.rank, y32 && d.dtype == NERF_EXT_BF16 ? 3u : 2u), stream)));
+    return NERF_STATUS_OK;
+}
+
+template <typename T>
+NerfStatus backward(const NerfExtLinearDesc& d, const NerfExtRowGroups& r, const NerfExtAdapters& a, const void* x, const void* w, const void* delta, const float* mid, const void* pre, const void* add, void* dx, void* dpre, float* dmid,
+                    float* ddown, float* dup, Workspace ws, hipStream_t stream) {
+    const Groups G{r.offsets, r.groups, d.rows};
+    if (d.rows && dmid) NERF_HIP_TRY((launch_ranks<T, true>(G, (const T*)delta, d.y_stride, r.y_rows, r.y_count, (const T*)a.up, d.out_features, a.rank, a.scales, dmid, stream)));
+    if ((dx || dpre) && d.rows) {
+        const bool vec = d.in_features % 8u == 0u && (!(add || dx) || d.x_stride % 8u == 0u) && aligned(add, 16u) && aligned(dx, 16u) && aligned(pre, 16u) && aligned(dpre, 16u);
+        const GatheredOperands A{{w, delta, d.in_features, d.y_stride, d.in_features, d.rows, d.out_features, 0u, 0u, 0u}, nullptr, r.y_rows, 0u, r.y_count};
+        const RowsGradientOut<T> out{(const T*)add, (T*)dx, (const T*)pre, (T*)dpre, d.x_stride, d.in_features, d.rows, d.activation, vec, r.x_rows, r.x_count, nullptr};
+        NERF_HIP_TRY((launch_adapter<T, true>(A, out, low_rank<T, true>(dmid, a.down, nullptr, G, d.in_features, a.rank, 2u), stream)));
+    }
+    if (ddown) NERF_HIP_TRY((launch_rank_sums<T>(RankSums{x, dmid, nullptr, ddown, nullptr, r.x_rows, d.x_stride, r.x_count, d.in_features, a.rank, 0u, 0u, true}, G, ws, stream)));
+    if (dup) NERF_HIP_TRY((launch_rank_sums<T>(RankSums{delta, mid, a.scales, dup, nullptr, r.y_rows, d.y_stride, r.y_count, d.out_features, a.rank, 0u, 0u, false}, G, ws, stream)));
+    return NERF_STATUS_OK;
+}
+
+NerfStatus check_adapters(const NerfExtAdapters* adapters, NerfExtAdapters& a, const char* fn) {
+    auto refuse = [&](const char* why) {
+        set_error(std::string(fn) + ": " + why);
+        return NERF_STATUS_INVALID_USAGE;
+    };
+    if (!adapters) return refuse("null adapters");
+    a = *adapters;
+    if (a.rank == 0u || a.rank > (uint32_t)NERF_EXT_MAX_RANK) return refuse("rank must be 1..256");
+    if (a.reserved != 0u) return refuse("reserved of the adapters must be 0");
+    if (!aligned(a.down, 2u) || !aligned(a.up, 2u) || !aligned(a.scales, 4u)) return refuse("an adapter's array is not aligned to its elements");
+    return NERF_STATUS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+NERF_API NerfStatus nerf_ext_adapter_linear_forward(const NerfExtLinearDesc* desc, const NerfExtRowGroups* groups, const NerfExtAdapters* adapters, const void* x, const void* weight, const float* bias, const void* residual, void* y, void* pre,
+                                                   float* mid, void* workspace, uint64_t workspace_bytes, void* stream) {
+    NerfExtLinearDesc d;
+    NerfExtRowGroups r;
+    NerfExtAdapters a;
+    NerfStatus s = check_desc(desc, d, "nerf_ext_adapter_linear_forward");
+    if (s == NERF_STATUS_OK) s = check_groups(groups, d, r, "nerf_ext_adapter_linear_forward");
+    if (s == NERF_STATUS_OK) s = check_adapters(adapters, a, "nerf_ext_adapter_linear_forward");
+    if (s != NERF_STATUS_OK) return s;
+    (void)workspace_bytes;
+    if (d.rows == 0u) return NERF_STATUS_OK;
+    NERF_CHECK_ARG(x && weight && y && mid && a.down && a.up, "nerf_ext_adapter_linear_forward: null x, weight, y, mid, down or up");
+    NERF_CHECK_ARG(aligned(x, 2u) && aligned(weight, 2u) && aligned(residual, 2u) && aligned(pre, 2u) && aligned(bias, 4u) && aligned(mid, 4u) && aligned(y, d.out_dtype == NERF_EXT_F32 ? 4u : 2u),
+                   "nerf_ext_adapter_linear_forward: an array is not aligned to its elements");
+    NERF_CHECK_ARG(y != residual || (d.out_dtype == d.dtype && (r.y_count == 1u || d.y_stride == d.residual_stride)), "nerf_ext_adapter_linear_forward: y over residual must have its type and row stride");
+    NERF_CHECK_ARG(aligned(workspace, 16u), "nerf_ext_adapter_linear_forward: workspace must be aligned to 16 bytes");
+    if (d.dtype == NERF_EXT_F16) return forward<half_t>(d, r, a, x, weight, bias, residual, y, pre, mid, (hipStream_t)stream);
+    return forward<bf16_t>(d, r, a, x, weight, bias, residual, y, pre, mid, (hipStream_t)stream);
+}
+
+NERF_API NerfStatus nerf_ext_adapter_linear_backward(const NerfExtLinearDesc* desc, const NerfExtRowGroups* groups, const NerfExtAdapters* adapters, const void* x, const void* weight, const void* delta, const float* mid, const void* pre,
+                                                    const void* add, void* dx, void* dpre, float* dmid, float* ddown, float* dup, void* workspace, uint64_t workspace_bytes, void* stream) {
+    NerfExtLinearDesc d;
+    NerfExtRowGroups r;
+    NerfExtAdapters a;
+    NerfStatus s = check_desc(desc, d, "nerf_ext_adapter_linear_backward");
+    if (s == NERF_STATUS_OK) s = check_groups(groups, d, r, "nerf_ext_adapter_linear_backward");
+    if (s == NERF_STATUS_OK) s = check_adapters(adapters, a, "nerf_ext_adapter_linear_backward");
+    if (s != NERF_STATUS_OK) return s;
+    NERF_CHECK_ARG(dx || dpre || ddown || dup || dmid, "nerf_ext_adapter_linear_backward: no output");
+    const bool low = dx || dpre || ddown;  // what dmid is needed for
+    NERF_CHECK_ARG(d.rows == 0u || delta, "nerf_ext_adapter_linear_backward: null delta");
+    NERF_CHECK_ARG(d.rows == 0u || dmid || !low, "nerf_ext_adapter_linear_backward: dx, dpre and ddown need dmid");
+    NERF_CHECK_ARG(d.rows == 0u || a.up || !dmid, "nerf_ext_adapter_linear_backward: dmid needs up");
+    NERF_CHECK_ARG(d.rows == 0u || (weight && a.down) || !(dx || dpre), "nerf_ext_adapter_linear_backward: dx and dpre need weight and down");
+    NERF_CHECK_ARG(d.rows == 0u || pre || !dpre, "nerf_ext_adapter_linear_backward: dpre needs pre");
+    NERF_CHECK_ARG(d.rows == 0u || x || !ddown, "nerf_ext_adapter_linear_backward: ddown needs x");
+    NERF_CHECK_ARG(d.rows == 0u || mid || !dup, "nerf_ext_adapter_linear_backward: dup needs mid");
+    NERF_CHECK_ARG(aligned(x, 2u) && aligned(weight, 2u) && aligned(delta, 2u) && aligned(pre, 2u) && aligned(add, 2u) && aligned(dx, 2u) && aligned(dpre, 2u) && aligned(mid, 4u) && aligned(dmid, 4u) && aligned(ddown, 4u) && aligned(dup, 4u),
+                   "nerf_ext_adapter_linear_backward: an array is not aligned to its elements");
+    NERF_CHECK_ARG(aligned(workspace, 16u), "nerf_ext_adapter_linear_backward: workspace must be aligned to 16 bytes");
+    if (d.rows == 0u && !ddown && !dup) return NERF_STATUS_OK;
+    const Workspace ws{(float*)workspace, workspace ? workspace_bytes : 0u};
+    if (d.dtype == NERF_EXT_F16) return backward<half_t>(d, r, a, x, weight, delta, mid, pre, add, dx, dpre, dmid, ddown, dup, ws, (hipStream_t)stream);
+    return backward<bf16_t>(d, r, a, x, weight, delta, mid, pre, add, dx, dpre, dmid, ddown, dup, ws, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -31,6 +31,36 @@ def linear_backward(desc: L.NerfExtLinearDesc, x: int | None, weight: int | None
     L.call("nerf_ext_linear_backward", C.byref(desc), x, weight, delta, pre, add, dx, dpre, dweight, dbias, workspace.ptr if workspace else None, workspace.nbytes if workspace else 0, stream.handle if stream else None)
 
 
+def group_rows(ids: int, rows: int, groups: int, offsets: int, order: int, *, place: int | None = None, workspace: DeviceArray | None = None, stream: Stream | None = None) -> None:
+    """nerf_ext_group_rows on device addresses."""
+    L.call("nerf_ext_group_rows", ids, rows, groups, offsets, order, place, workspace.ptr if workspace else None, workspace.nbytes if workspace else 0, stream.handle if stream else None)
+
+
+def grouped_linear_forward(desc: L.NerfExtLinearDesc, groups: L.NerfExtRowGroups, x: int, weight: int, y: int, *, bias: int | None = None, residual: int | None = None, pre: int | None = None, workspace: DeviceArray | None = None,
+                           stream: Stream | None = None) -> None:
+    """nerf_ext_grouped_linear_forward on device addresses."""
+    L.call("nerf_ext_grouped_linear_forward", C.byref(desc), C.byref(groups), x, weight, bias, residual, y, pre, workspace.ptr if workspace else None, workspace.nbytes if workspace else 0, stream.handle if stream else None)
+
+
+def grouped_linear_backward(desc: L.NerfExtLinearDesc, groups: L.NerfExtRowGroups, x: int | None, weight: int | None, delta: int, *, pre: int | None = None, add: int | None = None, dx: int | None = None, dpre: int | None = None,
+                            dweight: int | None = None, dbias: int | None = None, workspace: DeviceArray | None = None, stream: Stream | None = None) -> None:
+    """nerf_ext_grouped_linear_backward on device addresses."""
+    L.call("nerf_ext_grouped_linear_backward", C.byref(desc), C.byref(groups), x, weight, delta, pre, add, dx, dpre, dweight, dbias, workspace.ptr if workspace else None, workspace.nbytes if workspace else 0, stream.handle if stream else None)
+
+
+def adapter_linear_forward(desc: L.NerfExtLinearDesc, groups: L.NerfExtRowGroups, adapters: L.NerfExtAdapters, x: int, weight: int, y: int, mid: int, *, bias: int | None = None, residual: int | None = None, pre: int | None = None,
+                           workspace: DeviceArray | None = None, stream: Stream | None = None) -> None:
+    """nerf_ext_adapter_linear_forward on device addresses."""
+    L.call("nerf_ext_adapter_linear_forward", C.byref(desc), C.byref(groups), C.byref(adapters), x, weight, bias, residual, y, pre, mid, workspace.ptr if workspace else None, workspace.nbytes if workspace else 0, stream.handle if stream else None)
+
+
+def adapter_linear_backward(desc: L.NerfExtLinearDesc, groups: L.NerfExtRowGroups, adapters: L.NerfExtAdapters, x: int | None, weight: int | None, delta: int, *, mid: int | None = None, pre: int | None = None, add: int | None = None,
+                            dx: int | None = None, dpre: int | None = None, dmid: int | None = None, ddown: int | None = None, dup: int | None = None, workspace: DeviceArray | None = None, stream: Stream | None = None) -> None:
+    """nerf_ext_adapter_linear_backward on device addresses."""
+    L.call("nerf_ext_adapter_linear_backward", C.byref(desc), C.byref(groups), C.byref(adapters), x, weight, delta, mid, pre, add, dx, dpre, dmid, ddown, dup, workspace.ptr if workspace else None, workspace.nbytes if workspace else 0,
+           stream.handle if stream else None)
+
+
 def _check_rows(array: DeviceArray, rows: int, width: int, what: str) -> None:
     """Rows of `width` 16-bit values, `rows` of them at least: an array of rows of
     any inner shape, or a flat one."""
