@@ -349,7 +349,22 @@ hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& mo
     };
     const bool gather = A.q_index != nullptr;
     const bool words  = !whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, A.nk) || (gather && !near(A.q_count, A.ldq));
-    if (words) return launch(k_adapter<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
+    const uint64_t cus = device_cu_count();
+    auto tiles         = [&](uint32_t b) { return (uint64_t)ceil_div(A.np, b) * ceil_div(A.nq, b); };
+    if (A.nk <= kFewMaxK) {
+        auto few = [&](auto f, bool as_words) {
+            if (as_words) return launch(k_adapter_few<T, f(), kPT, true, true, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
+            return launch(k_adapter_few<T, f(), kPT, false, true, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
+        };
+        const bool odd = odd_rows(A.p, A.ldp) || odd_rows(A.q, A.ldq);
+        if (tiles(16u) <= 2u * cus) return few(std::integral_constant<uint32_t, 1u>{}, odd);
+        if (tiles(32u) <= 2u * cus) return few(std::integral_constant<uint32_t, 2u>{}, odd);
+    }
+    const bool by_128 = A.np > 64u && A.nq > 64u && tiles(128u) >= cus;
+    if (words) return by_128 ? launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kByWords, true, Out>, 128u, 128u, 256u) : launch(k_adapter<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
+    if (A.np > 128u && A.nq > 128u && A.nk >= 512u && tiles(256u) >= cus)
+        return gather ? launch(k_adapter<T, 256, 256, 2, 4, 2, kPT, kDirect, true, Out>, 256u, 256u, 512u) : launch(k_adapter<T, 256, 256, 2, 4, 2, kPT, kDirect, false, Out>, 256u, 256u, 512u);
+    if (by_128) return gather ? launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kDirect, true, Out>, 128u, 128u, 256u) : launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kDirect, false, Out>, 128u, 128u, 256u);
     return gather ? launch(k_adapter<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_adapter<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
 }
 

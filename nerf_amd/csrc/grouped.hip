@@ -152,8 +152,30 @@ hipError_t launch_grouped(GatheredOperands A, Out out, const Groups& G, hipStrea
     };
     const bool gather = A.q_index != nullptr;
     const bool words  = !whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, A.nk) || (gather && !near(A.q_count, A.ldq));
-    if (words) return launch(k_grouped<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
-    return gather ? launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
+    const uint64_t cus = device_cu_count();
+    // Tiles that the rows make, group by group.
+    auto tiles = [&](uint32_t b) { return (uint64_t)ceil_div(A.np, b) * parts_of(G.rows, G.count, b).most; };
+    if (A.nk <= kFewMaxK) {
+        auto few = [&](auto f, bool as_words) {
+            if (as_words) return launch(k_grouped_few<T, f(), kPT, true, true, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
+            return launch(k_grouped_few<T, f(), kPT, false, true, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
+        };
+        const bool odd = odd_rows(A.p, A.ldp) || odd_rows(A.q, A.ldq) || ((uint64_t)A.np * A.nk) % 2u;
+        if (tiles(16u) <= 2u * cus) return few(std::integral_constant<uint32_t, 1u>{}, odd);
+        if (tiles(32u) <= 2u * cus) return few(std::integral_constant<uint32_t, 2u>{}, odd);
+    }
+    const uint32_t mean = G.rows / G.count;
+    if constexpr (!kHasRows<Out>) {
+        if (words) return launch(k_grouped<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
+        return gather ? launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
+    } else {
+        const bool by_128 = A.np > 64u && mean >= 128u && tiles(128u) >= cus;
+        if (words) return by_128 ? launch(k_grouped<T, 128, 128, 2, 2, 2, kPT, kByWords, true, Out>, 128u, 128u, 256u) : launch(k_grouped<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
+        if (A.np > 128u && mean >= 512u && A.nk >= 512u && tiles(256u) >= cus)
+            return gather ? launch(k_grouped<T, 256, 256, 2, 4, 2, kPT, kDirect, true, Out>, 256u, 256u, 512u) : launch(k_grouped<T, 256, 256, 2, 4, 2, kPT, kDirect, false, Out>, 256u, 256u, 512u);
+        if (by_128) return gather ? launch(k_grouped<T, 128, 128, 2, 2, 2, kPT, kDirect, true, Out>, 128u, 128u, 256u) : launch(k_grouped<T, 128, 128, 2, 2, 2, kPT, kDirect, false, Out>, 128u, 128u, 256u);
+        return gather ? launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
+    }
 }
 
 template <typename T>
@@ -179,7 +201,12 @@ hipError_t launch_sums(GatheredOperands A, const Groups& G, float* dw, float* db
     };
     const bool gather = A.p_index || A.q_index;
     const bool words  = !whole_chunks(A.p, A.ldp, A.np) || !whole_chunks(A.q, A.ldq, A.nq) || (gather && !(near(A.p_count, A.ldp) && near(A.q_count, A.ldq)));
-    if (words) return launch(k_grouped_sums<T, 64, 64, 2, 2, kByWords, true>, 64u, 64u, 256u);
+    const uint64_t work = length * G.rows;
+    const bool by_128   = A.np > 64u && A.nq > 64u && work >= 1ull << 32;
+    if (words) return by_128 ? launch(k_grouped_sums<T, 128, 128, 2, 2, kByWords, true>, 128u, 128u, 256u) : launch(k_grouped_sums<T, 64, 64, 2, 2, kByWords, true>, 64u, 64u, 256u);
+    if (A.np > 128u && A.nq > 128u && work >= 1ull << 35)
+        return gather ? launch(k_grouped_sums<T, 256, 256, 2, 4, kDirect, true>, 256u, 256u, 512u) : launch(k_grouped_sums<T, 256, 256, 2, 4, kDirect, false>, 256u, 256u, 512u);
+    if (by_128) return gather ? launch(k_grouped_sums<T, 128, 128, 2, 2, kDirect, true>, 128u, 128u, 256u) : launch(k_grouped_sums<T, 128, 128, 2, 2, kDirect, false>, 128u, 128u, 256u);
     return gather ? launch(k_grouped_sums<T, 64, 64, 2, 2, kDirect, true>, 64u, 64u, 256u) : launch(k_grouped_sums<T, 64, 64, 2, 2, kDirect, false>, 64u, 64u, 256u);
 }
 

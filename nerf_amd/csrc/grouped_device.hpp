@@ -147,7 +147,8 @@ __device__ __forceinline__ void store_eight(E* row, uint32_t p, uint32_t n, bool
 }
 
 // The epilogues get rows of a tile and look their place in the arrays up in LDS
-// (kNoRow: nothing is written).  of_group(): what belongs to the tile's group.
+// (kNoRow: nothing is written).  Threads without outputs (n = 0) may name rows
+// beyond the tile, which have no place.  of_group(): what belongs to the tile's group.
 template <typename T>
 struct RowsForwardOut {
     const float* bias;
@@ -170,12 +171,12 @@ struct RowsForwardOut {
     }
     __device__ __forceinline__ Aux load(uint32_t, uint32_t row, uint32_t p, uint32_t n) const {
         if (!residual) return {uintx4{0u, 0u, 0u, 0u}};
-        const uint32_t r = rows[row];
+        const uint32_t r = n ? rows[row] : kNoRow;
         return {load_eight<T>(residual + (r != kNoRow ? r : 0u) * ldr, p, r != kNoRow ? n : 0u, vec, np >= 8u)};
     }
     __device__ __forceinline__ void put(uint32_t, uint32_t row, uint32_t p, uint32_t n, floatx8 z, const floatx8& b, const Aux& a) const {
-        const uint32_t r = rows[row];
-        if (r == kNoRow || n == 0u) return;
+        const uint32_t r = n ? rows[row] : kNoRow;
+        if (r == kNoRow) return;
         z += b;
         if (pre) store_eight<T>(pre + (uint64_t)r * np, p, n, vec, z);
         act_values(act, z);
@@ -205,15 +206,15 @@ struct RowsGradientOut {
     __device__ __forceinline__ void of_group(uint32_t) {}
     __device__ __forceinline__ Aux load(uint32_t, uint32_t row, uint32_t p, uint32_t n) const {
         Aux a{};
-        const uint32_t r = rows[row], at = r != kNoRow ? r : 0u;
+        const uint32_t r = n ? rows[row] : kNoRow, at = r != kNoRow ? r : 0u;
         if (r == kNoRow) n = 0u;
         if (add) a.add = load_eight<T>(add + at * ldx, p, n, vec, np >= 8u);
         if (dpre) a.pre = load_eight<T>(pre + (uint64_t)at * np, p, n, vec, np >= 8u);
         return a;
     }
     __device__ __forceinline__ void put(uint32_t, uint32_t row, uint32_t p, uint32_t n, floatx8 g, const floatx8&, const Aux& a) const {
-        const uint32_t r = rows[row];
-        if (r == kNoRow || n == 0u) return;
+        const uint32_t r = n ? rows[row] : kNoRow;
+        if (r == kNoRow) return;
         if (add) g += widen<T>(a.add, n, vec, np >= 8u);
         if (dx) store_eight<T>(dx + r * ldx, p, n, vec, g);
         if (dpre) {

@@ -536,7 +536,6 @@ hipError_t launch_product(Operands A, Out out, float* row_sums, Workspace ws, hi
 // Products of few tiles are those of at most 4096 k (1 x 4096 -> 4096 9 us, by
 // larger tiles with k split over workgroups 13; 1 x 8192 -> 4096 17.5 against
 // 15.5) with at most two tiles a CU.
-constexpr uint32_t kFewMaxK = 4096u;
 bool few_operands(const Operands& A, bool pt, bool qt) { return A.nk <= kFewMaxK && !few_values(A, pt, qt); }
 uint64_t few_tiles(const Operands& A, uint32_t f) { return (uint64_t)ceil_div(A.np, 16u * f) * ceil_div(A.nq, 16u * f); }
 

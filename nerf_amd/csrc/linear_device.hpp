@@ -822,7 +822,7 @@ __device__ __forceinline__ void product(const Ops& A, Out out, const Place& at, 
 // tiles whose k were split over workgroups and a second one to join them took
 // 12 us for 7 x 1601 -> 999, this one 7; backward 37 x 788 -> 64 4 us, in three
 // launches 10.)
-constexpr uint32_t kFewWaves = 8u;
+constexpr uint32_t kFewWaves = 8u, kFewMaxK = 4096u;
 
 // 16 kF rows x 32 k of an operand, any alignment, on its way to one wave; the
 // edges as Stager has them.  Rows outside are other rows: their products are in
