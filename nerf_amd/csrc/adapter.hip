@@ -8,7 +8,8 @@
 //
 // m and n (rank values a row, 32 bits) are a grouped product of their own; the
 // shared product then goes over all rows in tiles of any groups, and each wave
-// adds its rows' low-rank part to its sums before they leave.  B_g m_i is summed
+// begins its sums with its rows' low-rank part, while the first tiles of the
+// shared operands are on their way.  B_g m_i is summed
 // by the matrix instructions of the layer's type: each m is split into two values
 // of that type (three where fp32 outputs of bf16 values keep more), high and low
 // part, whose products are as if the rank were two or three times as large.  For
@@ -34,37 +35,44 @@ struct LowRank {
     uint32_t np, rank, pieces;
     bool vec_low, vec_wide;  // rows of low / of wide in whole aligned chunks
 
-    // Eight of a row's values from r0, zeros beyond the rank.
+    // Eight of a row's values from r0, zeros beyond the rank.  Every load is made, from
+    // inside the arrays, and what does not count is dropped: a branch would have them
+    // wait for each other.
     __device__ __forceinline__ floatx8 low_eight(uint32_t position, uint32_t r0) const {
-        const float* at = low + (uint64_t)position * rank + r0;
+        const float* at = low + (uint64_t)min(position, G.rows - 1u) * rank;
+        const bool none = r0 >= rank;
         floatx8 v;
         if (vec_low) {
-            v.lo = reinterpret_cast<const floatx4*>(at)[0];
-            v.hi = reinterpret_cast<const floatx4*>(at)[1];
+            const floatx4* from = reinterpret_cast<const floatx4*>(at + (none ? 0u : r0));
+            v.lo = from[0];
+            v.hi = from[1];
         } else {
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) v[e] = r0 + e < rank ? at[e] : 0.0f;
+            for (uint32_t e = 0; e < 8u; ++e) v[e] = at[min(r0 + e, rank - 1u)];
         }
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) v[e] = r0 + e < rank ? v[e] : 0.0f;
         return v;
     }
+    // Eight of wide's values at p from r0, zeros outside.
     __device__ __forceinline__ x8 wide_eight(uint32_t g, uint32_t p, uint32_t r0) const {
+        const uint32_t column = min(p, np - 1u);
         x8 v;
-#pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) v[e] = (T)0.0f;
-        if (p < np) {
-            if constexpr (!kPT) {
-                const T* at = wide + ((uint64_t)g * np + p) * rank + r0;
-                if (vec_wide) return *reinterpret_cast<const x8*>(at);
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e)
-                    if (r0 + e < rank) v[e] = at[e];
+        if constexpr (!kPT) {
+            const T* at = wide + ((uint64_t)g * np + column) * rank;
+            if (vec_wide) {
+                v = *reinterpret_cast<const x8*>(at + (r0 < rank ? r0 : 0u));
             } else {
-                const T* at = wide + ((uint64_t)g * rank + r0) * np + p;
 #pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e)
-                    if (r0 + e < rank) v[e] = at[(uint64_t)e * np];
+                for (uint32_t e = 0; e < 8u; ++e) v[e] = at[min(r0 + e, rank - 1u)];
             }
+        } else {
+            const T* at = wide + (uint64_t)g * rank * np + column;
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) v[e] = at[(uint64_t)min(r0 + e, rank - 1u) * np];
         }
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) v[e] = p < np && r0 + e < rank ? v[e] : (T)0.0f;
         return v;
     }
     // Piece `piece` of eight values.
@@ -80,57 +88,64 @@ struct LowRank {
     }
 
     // acc[i][j]: 16 outputs from p0 + 16 i at 16 positions from q0 + 16 j, four
-    // consecutive outputs of position lane % 16 a lane.
+    // consecutive outputs of position lane % 16 a lane; zeros before.
     template <uint32_t kFP, uint32_t kFQ>
-    __device__ __forceinline__ void add(floatx4 (&acc)[kFP][kFQ], uint32_t p0, uint32_t q0, uint32_t share, uint32_t shares) const {
+    __device__ __forceinline__ void begin(floatx4 (&acc)[kFP][kFQ], uint32_t p0, uint32_t q0, uint32_t share, uint32_t shares) const {
         const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, quarter = lane >> 4;
         static_assert(16u * kFQ <= 64u);
-        // The group of position q0 + lane.
-        uint32_t mine = kNoRow;
-        if (lane < 16u * kFQ && q0 + lane < G.rows) {
-            uint32_t first = 0u, last = G.count;  // offsets[g] <= position for g < first, not for g >= last
-            while (first < last) {
-                const uint32_t middle = (first + last) / 2u;
-                if (G.offset(middle) <= q0 + lane) first = middle + 1u;
-                else last = middle;
-            }
-            if (first && q0 + lane < G.offset(first)) mine = first - 1u;
-        }
-        if (__ballot(mine != kNoRow) == 0ull) return;
         const uint32_t chunks = (rank + 7u) / 8u, steps = (pieces * chunks + 3u) / 4u;
-        uint32_t group[kFQ];
-        float up[kFQ], down[kFQ];  // a power of two a row, and its inverse
+        // The rows' values for the first step, whatever their groups.
+        floatx8 values[kFQ];
+        auto fetch = [&](uint32_t s) {
+            const uint32_t chunk = 4u * s + quarter, piece = chunk / chunks, r0 = 8u * (chunk - piece * chunks);
 #pragma unroll
-        for (uint32_t j = 0; j < kFQ; ++j) {
-            group[j] = (uint32_t)__shfl((int)mine, (int)(16u * j + l));
-            up[j] = down[j] = 1.0f;
-            if constexpr (std::is_same_v<T, half_t>) {
-                float most = 0.0f;
-                if (group[j] != kNoRow) {
-                    for (uint32_t c = quarter; c < chunks; c += 4u) {
-                        const floatx8 v = low_eight(q0 + 16u * j + l, 8u * c);
+            for (uint32_t j = 0; j < kFQ; ++j) values[j] = low_eight(q0 + 16u * j + l, piece < pieces ? r0 : rank);
+        };
+        // The widest tiles' sums leave few registers: values are fetched as they are used.
+        constexpr bool kTight = kFP * kFQ >= 32u;
+        if (!kTight) fetch(0u);
+        // The group of position q0 + lane: that of q0, and one more for every offset up
+        // to the position.  (before: offsets up to q0.)
+        const uint32_t before = count_at_most(G.count, q0, [&](uint32_t g) { return G.offset(g); });
+        uint32_t mine = before;
+        const uint32_t q_last = q0 + 16u * kFQ - 1u;
+        for (uint32_t first = before; first <= G.count; first += 64u) {
+            const uint32_t next = first + lane <= G.count ? G.offset(first + lane) : kNoRow;
+            const uint32_t some = (uint32_t)__popcll(__ballot(next <= q_last));
+            for (uint32_t c = 0; c < some; ++c) mine += (uint32_t)__builtin_amdgcn_readlane((int)next, (int)c) <= q0 + lane;
+            if (some < 64u) break;
+        }
+        mine = lane < 16u * kFQ && q0 + lane < G.rows && mine != 0u && mine <= G.count ? mine - 1u : kNoRow;
+        if (__ballot(mine != kNoRow) == 0ull) return;
+        // A power of two for the row of position q0 + lane, and its inverse.
+        float power = 1.0f, inverse = 1.0f;
+        if constexpr (std::is_same_v<T, half_t>) {
+            const float* at = low + (uint64_t)min(q0 + lane, G.rows - 1u) * rank;
+            float most = 0.0f;
+            if (vec_low) {
+                for (uint32_t r = 0; r < rank; r += 8u) {
+                    const floatx4 v = *reinterpret_cast<const floatx4*>(at + r), w = *reinterpret_cast<const floatx4*>(at + r + 4u);
 #pragma unroll
-                        for (uint32_t e = 0; e < 8u; ++e) most = fmaxf(most, fabsf(v[e]));
-                    }
+                    for (uint32_t e = 0; e < 4u; ++e) most = fmaxf(most, fmaxf(fabsf(v[e]), fabsf(w[e])));
                 }
-                most = fmaxf(most, __shfl_xor(most, 16));
-                most = fmaxf(most, __shfl_xor(most, 32));
-                const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 1u), 252u);
-                if (most > 0.0f && most < __builtin_inff()) {
-                    up[j]   = __uint_as_float(exponent << 23);
-                    down[j] = __uint_as_float((254u - exponent) << 23);
-                }
+            } else {
+#pragma unroll 4
+                for (uint32_t r = 0; r < rank; ++r) most = fmaxf(most, fabsf(at[r]));
+            }
+            const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 1u), 252u);
+            if (most > 0.0f && most < __builtin_inff()) {
+                power   = __uint_as_float(exponent << 23);
+                inverse = __uint_as_float((254u - exponent) << 23);
             }
         }
+        auto of_row = [&](float v, uint32_t j) { return std::is_same_v<T, half_t> ? __shfl(v, (int)(16u * j + l)) : 1.0f; };
         for (uint32_t s = 0; s < steps; ++s) {
             const uint32_t chunk = 4u * s + quarter, piece = chunk / chunks, r0 = 8u * (chunk - piece * chunks);
             x8 fq[kFQ];
+            if (kTight) fetch(s);
 #pragma unroll
-            for (uint32_t j = 0; j < kFQ; ++j) {
-                floatx8 v = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                if (group[j] != kNoRow && piece < pieces) v = low_eight(q0 + 16u * j + l, r0);
-                fq[j] = piece_of(v * down[j], piece < pieces ? piece : 0u);
-            }
+            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = piece_of(values[j] * of_row(inverse, j), piece < pieces ? piece : 0u);
+            if (!kTight && s + 1u < steps) fetch(s + 1u);
             // The groups of the wave's rows, one after another.
             uint64_t left = __ballot(mine != kNoRow);
             for (uint32_t turn = 0; left; ++turn) {
@@ -139,20 +154,24 @@ struct LowRank {
                 left &= ~those;
                 if (turn % shares != share) continue;
                 const float scale = scales ? scales[g] : 1.0f;
+                constexpr uint32_t kAtOnce = kTight ? 1u : kFP;
 #pragma unroll
-                for (uint32_t i = 0; i < kFP; ++i) {
-                    x8 fp;
+                for (uint32_t i0 = 0; i0 < kFP; i0 += kAtOnce) {
+                    x8 fp[kAtOnce];
 #pragma unroll
-                    for (uint32_t e = 0; e < 8u; ++e) fp[e] = (T)0.0f;
-                    if (piece < pieces) fp = wide_eight(g, p0 + 16u * i + l, r0);
+                    for (uint32_t i = 0; i < kAtOnce; ++i) fp[i] = wide_eight(g, p0 + 16u * (i0 + i) + l, piece < pieces ? r0 : rank);
 #pragma unroll
                     for (uint32_t j = 0; j < kFQ; ++j) {
                         if (!(those >> (16u * j) & 0xFFFFull)) continue;
-                        const floatx4 part = Vec<T>::mfma(fp, fq[j], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
-                        // Rows of other groups keep theirs, whatever this group's weights hold.
-                        const float factor = up[j] * scale;
+                        const float factor = of_row(power, j) * scale;
+                        const bool member  = those >> (16u * j + l) & 1ull;
 #pragma unroll
-                        for (uint32_t r = 0; r < 4u; ++r) acc[i][j][r] = group[j] == g ? acc[i][j][r] + factor * part[r] : acc[i][j][r];
+                        for (uint32_t i = 0; i < kAtOnce; ++i) {
+                            const floatx4 part = Vec<T>::mfma(fp[i], fq[j], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+                            // Rows of other groups keep theirs, whatever this group's weights hold.
+#pragma unroll
+                            for (uint32_t r = 0; r < 4u; ++r) acc[i0 + i][j][r] = member ? acc[i0 + i][j][r] + factor * part[r] : acc[i0 + i][j][r];
+                        }
                     }
                 }
             }
@@ -243,11 +262,39 @@ struct RankSums {
     bool low_major;
 };
 constexpr uint32_t kBW = 128u;
-template <typename T, uint32_t kBR>
+
+// Tile of 64 positions x kBR low values straight into LDS, for rows that are whole
+// multiples of 16 bytes; zeros outside.
+template <uint32_t kBR>
+struct LowLoader {
+    static constexpr uint32_t kLoads = kBK * kBR / 4u / 256u;
+    const float* base;
+    uint32_t step;
+
+    __device__ __forceinline__ void begin(const float* low, uint32_t nr, uint32_t r0, uint32_t k0) {
+        base = low + (uint64_t)k0 * nr + r0;
+        step = kBK * nr;
+    }
+    __device__ __forceinline__ void issue(float* lds, uint32_t nr, uint32_t r0, int left) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)0x7FFFFFFF, 0x00020000);
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            const uint32_t s = i * 256u + threadIdx.x, line = s / (kBR / 4u), r = s % (kBR / 4u) * 4u;
+            const uint32_t at = (int)line < left && r0 + r < nr ? (line * nr + r) * 4u : kBeyond;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + (i * 256u + wave * 64u) * 4u), 16, (int)at, 0, 0, 0);
+        }
+        base += step;
+    }
+};
+
+// kMode kDirect: both operands straight into LDS, the next tile's on their way;
+// else through registers, at any alignment.
+template <typename T, uint32_t kBR, Mode kMode, bool kGather>
 __global__ __launch_bounds__(256) void k_rank_sums(RankSums A, Groups G, uint32_t size, uint32_t most) {
     constexpr uint32_t kFR = kBR / 16u;
-    __shared__ uint4 lds_wide[kBW * 8u];
-    __shared__ float lds_low[kBK * kBR];
+    __shared__ uint4 wide0[kBW * 8u], wide1[kMode == kDirect ? kBW * 8u : 1u];
+    __shared__ float low0[kBK * kBR], low1[kMode == kDirect ? kBK * kBR : 1u];
     const uint32_t tiles = A.tiles_w * A.tiles_r, parts = min(most, part_count(G, size)), block = block_number();
     if (block >= parts * tiles) return;
     const uint32_t t = chip_tile(block, parts * tiles);
@@ -261,32 +308,14 @@ __global__ __launch_bounds__(256) void k_rank_sums(RankSums A, Groups G, uint32_
     for (uint32_t i = 0; i < 2u; ++i)
 #pragma unroll
         for (uint32_t j = 0; j < kFR; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    GatherStager<T, kBW, true, 256u> stage;
-    stage.begin(A.index, A.count, part.q0, end);
-    constexpr uint32_t kLow = kBK * kBR / 256u;
-    float held[kLow];
-    auto fetch = [&](uint32_t k) {
-        stage.fetch((const T*)A.wide, A.index, A.count, A.ld, A.nw, w0, k, end);
-#pragma unroll
-        for (uint32_t i = 0; i < kLow; ++i) {
-            const uint32_t e = i * 256u + threadIdx.x, line = k + e / kBR, r = r0 + e % kBR;
-            held[i] = line < end && r < A.nr ? A.low[(uint64_t)line * A.nr + r] : 0.0f;
-        }
-    };
     const uint32_t base = fragment_base<kBW, true>(32u * wave);
-    if (part.q0 < end) fetch(part.q0);
-    for (uint32_t k = part.q0; k < end; k += kBK) {
-        stage.keep(lds_wide, (const T*)A.wide, A.ld, A.nw, w0, k, end);
-#pragma unroll
-        for (uint32_t i = 0; i < kLow; ++i) lds_low[i * 256u + threadIdx.x] = held[i];
-        __syncthreads();
-        if (k + kBK < end) fetch(k + kBK);
+    auto multiply = [&](const uint4* wide, const float* low) {
 #pragma unroll
         for (uint32_t step = 0; step < 2u; ++step) {
             floatx8 w[2];
 #pragma unroll
             for (uint32_t i = 0; i < 2u; ++i) {
-                typename Vec<T>::x8 f = fragment<T, kBW, true>(lds_wide, base, i, step);
+                typename Vec<T>::x8 f = fragment<T, kBW, true>(wide, base, i, step);
                 settle_here(f);
                 w[i] = __builtin_convertvector(f, floatx8);
             }
@@ -294,12 +323,57 @@ __global__ __launch_bounds__(256) void k_rank_sums(RankSums A, Groups G, uint32_
             for (uint32_t e = 0; e < 8u; ++e)
 #pragma unroll
                 for (uint32_t j = 0; j < kFR; ++j) {
-                    const float m = lds_low[(32u * step + 8u * quarter + e) * kBR + 16u * j + l];
+                    const float m = low[(32u * step + 8u * quarter + e) * kBR + 16u * j + l];
 #pragma unroll
                     for (uint32_t i = 0; i < 2u; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i][e], m, acc[i][j], 0, 0, 0);
                 }
         }
-        __syncthreads();
+    };
+    if constexpr (kMode == kDirect) {
+        std::conditional_t<kGather, GatherLoader<T, kBW, true, 256u>, Loader<T, kBW, true, 256u>> load;
+        LowLoader<kBR> load_low;
+        if constexpr (kGather) load.begin((const T*)A.wide, A.index, A.count, A.ld, A.nw, w0, part.q0, end);
+        else load.begin((const T*)A.wide, A.ld, A.nw, w0, part.q0);
+        load_low.begin(A.low, A.nr, r0, part.q0);
+        auto issue = [&](uint4* wide, float* low, int left) {
+            load_low.issue(low, A.nr, r0, left);
+            if constexpr (kGather) load.issue(wide, left, A.index, A.count, A.ld, A.nw, w0);
+            else load.issue(wide, left);
+        };
+        constexpr int kStep = (int)kBK;
+        int left            = (int)(end - part.q0);
+        if (left > 0) issue(wide0, low0, left);
+        for (; left > 0; left -= 2 * kStep) {
+            arrived<0u>();
+            issue(wide1, low1, left - kStep);
+            multiply(wide0, low0);
+            arrived<0u>();
+            if (left > 2 * kStep) issue(wide0, low0, left - 2 * kStep);
+            multiply(wide1, low1);
+        }
+    } else {
+        GatherStager<T, kBW, true, 256u> stage;
+        stage.begin(A.index, A.count, part.q0, end);
+        constexpr uint32_t kLow = kBK * kBR / 256u;
+        float held[kLow];
+        auto fetch = [&](uint32_t k) {
+            stage.fetch((const T*)A.wide, A.index, A.count, A.ld, A.nw, w0, k, end);
+#pragma unroll
+            for (uint32_t i = 0; i < kLow; ++i) {
+                const uint32_t e = i * 256u + threadIdx.x, line = k + e / kBR, r = r0 + e % kBR;
+                held[i] = line < end && r < A.nr ? A.low[(uint64_t)line * A.nr + r] : 0.0f;
+            }
+        };
+        if (part.q0 < end) fetch(part.q0);
+        for (uint32_t k = part.q0; k < end; k += kBK) {
+            stage.keep(wide0, (const T*)A.wide, A.ld, A.nw, w0, k, end);
+#pragma unroll
+            for (uint32_t i = 0; i < kLow; ++i) low0[i * 256u + threadIdx.x] = held[i];
+            __syncthreads();
+            if (k + kBK < end) fetch(k + kBK);
+            multiply(wide0, low0);
+            __syncthreads();
+        }
     }
     const uint64_t length = (uint64_t)A.nw * A.nr;
     float* out = part.number ? A.parts + place_of(G, part, size) * length : A.out + part.group * length;
@@ -332,8 +406,6 @@ __global__ __launch_bounds__(256) void k_rank_tiny_sums(RankSums A, Groups G) {
 }
 
 // ------------------------------------------------------------------- host
-bool near(uint64_t count, uint64_t ld) { return count * ld * 2u < 1ull << 31; }
-
 template <typename T, bool kPT, typename Out>
 hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& more, hipStream_t stream) {
     const uint64_t weights = (uint64_t)A.np * A.nk, values = (uint64_t)(A.q_count - 1u) * A.ldq + A.nk;
@@ -386,9 +458,14 @@ hipError_t launch_rank_sums(RankSums A, const Groups& G, Workspace ws, hipStream
         if (e != hipSuccess || size >= G.rows) return e;
         return launch_join(G, size, A.out, ws.data, length, nullptr, nullptr, 0u, stream);
     };
-    if (A.nr <= 16u) return launch(k_rank_sums<T, 16>, 16u);
-    if (A.nr <= 32u) return launch(k_rank_sums<T, 32>, 32u);
-    return launch(k_rank_sums<T, 64>, 64u);
+    auto by_rank = [&](auto mode, auto gather) {
+        if (A.nr <= 16u) return launch(k_rank_sums<T, 16, mode(), gather()>, 16u);
+        if (A.nr <= 32u) return launch(k_rank_sums<T, 32, mode(), gather()>, 32u);
+        return launch(k_rank_sums<T, 64, mode(), gather()>, 64u);
+    };
+    using Direct = std::integral_constant<Mode, kDirect>;
+    if (!whole_chunks(A.wide, A.ld, A.nw) || A.nr % 4u != 0u || !aligned(A.low, 16u) || (A.index && !near(A.count, A.ld))) return by_rank(std::integral_constant<Mode, kByWords>{}, std::true_type{});
+    return A.index ? by_rank(Direct{}, std::true_type{}) : by_rank(Direct{}, std::false_type{});
 }
 
 template <typename T, bool kPT>

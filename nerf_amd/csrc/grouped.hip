@@ -133,10 +133,6 @@ __global__ __launch_bounds__(256) void k_grouped_join(Groups G, uint32_t size, f
 }
 
 // ------------------------------------------------------------------- host
-// Whether an operand whose lines an index names can go straight into LDS: by 32-bit
-// offsets from the array's start.
-bool near(uint64_t count, uint64_t ld) { return count * ld * 2u < 1ull << 31; }
-
 template <typename T, bool kPT, typename Out>
 hipError_t launch_grouped(GatheredOperands A, Out out, const Groups& G, hipStream_t stream) {
     const uint64_t weights = (uint64_t)G.count * A.np * A.nk, values = (uint64_t)(A.q_count - 1u) * A.ldq + A.nk;
@@ -166,6 +162,7 @@ hipError_t launch_grouped(GatheredOperands A, Out out, const Groups& G, hipStrea
     }
     const uint32_t mean = G.rows / G.count;
     if constexpr (!kHasRows<Out>) {
+        if (!words && A.np <= 32u) return gather ? launch(k_grouped<T, 32, 128, 1, 4, 2, kPT, kDirect, true, Out>, 32u, 128u, 256u) : launch(k_grouped<T, 32, 128, 1, 4, 2, kPT, kDirect, false, Out>, 32u, 128u, 256u);
         if (words) return launch(k_grouped<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
         return gather ? launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
     } else {

@@ -269,12 +269,12 @@ struct GatheredOperands : Operands {
     uint32_t p_count, q_count;
 };
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
-// Row of line `line` (of `lines`) of an operand, or kNoRow.
-__device__ __forceinline__ uint32_t gathered_row(const uint32_t* index, uint32_t count, uint32_t line, uint32_t lines) {
-    uint32_t row = line;
-    if (index) row = index[line < lines ? line : 0u];
-    return line < lines && row < count ? row : kNoRow;
-}
+// Row of line `line` (of `lines`) of an operand, or kNoRow, in two steps: what the
+// index says, and what it means, so that a row can be asked for ahead of its use.
+// (The index has an entry at least.)
+__device__ __forceinline__ uint32_t ask_row(const uint32_t* index, uint32_t line, uint32_t lines) { return index ? index[min(line, max(lines, 1u) - 1u)] : line; }
+__device__ __forceinline__ uint32_t judge_row(uint32_t row, uint32_t count, uint32_t line, uint32_t lines) { return line < lines && row < count ? row : kNoRow; }
+__device__ __forceinline__ uint32_t gathered_row(const uint32_t* index, uint32_t count, uint32_t line, uint32_t lines) { return judge_row(ask_row(index, line, lines), count, line, lines); }
 
 // Where a workgroup's tile lies: its first outputs, its k, and what P's rows and k
 // are counted from (a group's weights in the array of all groups').
@@ -294,6 +294,7 @@ struct Place {
 template <uint32_t kB, bool kT>
 __device__ __forceinline__ constexpr uint32_t chunk_key(uint32_t line) {
     if (!kT) return line & 7u;
+    if (kB == 32u) return ((line >> 2 ^ line >> 3) & 1u) << 1;
     if (kB >= 128u) return ((line & 3u) | ((line >> 3) & 1u) << 2) << 1;
     return (((line >> 1) & 1u) | ((line >> 3) & 1u) << 1) << 1;
 }
@@ -456,7 +457,10 @@ struct GatherStager {
     static __device__ __forceinline__ uint32_t chunk(uint32_t i) { return (i * kThreads + threadIdx.x) % kChunks; }
     __device__ __forceinline__ void begin(const uint32_t* index, uint32_t count, uint32_t first, uint32_t end) {
 #pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i) (kT ? next[i] : rows[i]) = gathered_row(index, count, first + line(i), end);
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            if constexpr (kT) next[i] = ask_row(index, first + line(i), end);
+            else rows[i] = gathered_row(index, count, first + line(i), end);
+        }
     }
     __device__ __forceinline__ Edge place(uint32_t i, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) const {
         return kT ? edge(ld, rows[i], kNoRow, row0 + 8u * chunk(i), n) : edge(ld, rows[i], kNoRow, k0 + 8u * chunk(i), k_end);
@@ -464,7 +468,7 @@ struct GatherStager {
     __device__ __forceinline__ void fetch(const T* __restrict__ src, const uint32_t* index, uint32_t count, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) {
         if constexpr (kT) {
 #pragma unroll
-            for (uint32_t i = 0; i < kLoads; ++i) rows[i] = next[i];
+            for (uint32_t i = 0; i < kLoads; ++i) rows[i] = judge_row(next[i], count, k0 + line(i), k_end);
         }
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) held[i].fetch(src + place(i, ld, n, row0, k0, k_end).at);
@@ -487,23 +491,24 @@ struct GatherLoader {
     static constexpr uint32_t kChunks = kT ? kB / 8u : 8u;
     static constexpr uint32_t kLoads  = kB * 8u / kThreads;
     const T* base;
-    uint32_t offset[kLoads];  // bytes, kBeyond for lines outside; kT: of the next tile
+    uint32_t offset[kLoads];  // bytes, kBeyond for lines outside; kT: what the index says of the next tile's
     uint32_t k, k_last;       // kT: the next tile's first k, and the end
 
     static __device__ __forceinline__ uint32_t line(uint32_t i) { return (i * kThreads + threadIdx.x) / kChunks; }
     static __device__ __forceinline__ uint32_t chunk(uint32_t i) { return ((i * kThreads + threadIdx.x) % kChunks) ^ chunk_key<kB, kT>(line(i)); }
-    __device__ __forceinline__ void next_rows(const uint32_t* index, uint32_t count, uint64_t ld, uint32_t n, uint32_t row0) {
-#pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i) {
-            const uint32_t row = gathered_row(index, count, (kT ? k : row0) + line(i), kT ? k_last : n);
-            offset[i]          = row != kNoRow && (!kT || row0 + 8u * chunk(i) < n) ? (row * (uint32_t)ld + 8u * chunk(i)) * 2u : kBeyond;
-        }
-    }
     __device__ __forceinline__ void begin(const T* src, const uint32_t* index, uint32_t count, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0, uint32_t k_end) {
         base   = src + (kT ? row0 : k0);
         k      = k0;
         k_last = k_end;
-        next_rows(index, count, ld, n, row0);
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            if constexpr (kT) {
+                offset[i] = ask_row(index, k + line(i), k_last);
+            } else {
+                const uint32_t row = gathered_row(index, count, row0 + line(i), n);
+                offset[i]          = row != kNoRow ? (row * (uint32_t)ld + 8u * chunk(i)) * 2u : kBeyond;
+            }
+        }
     }
     __device__ __forceinline__ void issue(uint4* lds, int left, const uint32_t* index, uint32_t count, uint64_t ld, uint32_t n, uint32_t row0) {
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)0x7FFFFFFF, 0x00020000);
@@ -511,12 +516,18 @@ struct GatherLoader {
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
             uint32_t at = offset[i];
-            if (!kT && left < (int)kBK && (int)(8u * chunk(i)) >= left) at = kBeyond;
+            if constexpr (kT) {
+                const uint32_t row = judge_row(offset[i], count, k + line(i), k_last);
+                at                 = row != kNoRow && row0 + 8u * chunk(i) < n ? (row * (uint32_t)ld + 8u * chunk(i)) * 2u : kBeyond;
+            } else if (left < (int)kBK && (int)(8u * chunk(i)) >= left) {
+                at = kBeyond;
+            }
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + i * kThreads + wave * 64u), 16, (int)at, 0, 0, 0);
         }
         if constexpr (kT) {
             k += kBK;
-            next_rows(index, count, ld, n, row0);
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) offset[i] = ask_row(index, k + line(i), k_last);
         } else {
             base += kBK;
         }
@@ -585,9 +596,9 @@ __device__ __forceinline__ uint32_t chip_tile(uint32_t b, uint32_t n) {
 // library's product alone reaches 1.24.  Four buffers of 32 k there, with the next
 // tile's first fragments read a barrier ahead, took 493.  Where they are narrow the
 // memory does: the weights' gradient of 262144 x 256 -> 256 69 us = 3.9 TB/s.
-// kGather: lines in another order (Ops = GatheredOperands).  more.add() adds what else
-// belongs to the sums before they leave (by several waves that add to the same
-// ones: each its share).
+// kGather: lines in another order (Ops = GatheredOperands).  more.begin() gives what the
+// sums begin with, while the first tiles are on their way (by several waves that
+// add to the same ones: each its share).
 enum Mode : uint32_t { kDirect, kByChunks, kByWords };
 struct NothingMore {
     static constexpr bool kOn = false;
@@ -691,6 +702,10 @@ __device__ __forceinline__ void product(const Ops& A, Out out, const Place& at, 
             if constexpr (kGather) load_q.issue(lds + kBP * 8u, left, A.q_index, A.q_count, A.ldq, A.nq, q0);
             else load_q.issue(lds + kBP * 8u, left);
         };
+        auto before = [&] {
+            keep_bias();
+            if constexpr (More::kOn) more.template begin<kFP, kFQ>(acc, p0 + wp, q0 + wq, 0u, 1u);
+        };
         constexpr int kStep = (int)kBK;
         int left            = (int)(k_end - k0);
         if constexpr (kDepth == 2u) {
@@ -699,7 +714,7 @@ __device__ __forceinline__ void product(const Ops& A, Out out, const Place& at, 
             // everyone's part of the tile has come, and everyone is done with the
             // other buffer.
             issue(lds0, left);
-            keep_bias();
+            before();
             for (; left > 0; left -= 2 * kStep) {
                 arrived<0u>();
                 issue(lds1, left - kStep);
@@ -713,7 +728,7 @@ __device__ __forceinline__ void product(const Ops& A, Out out, const Place& at, 
             issue(lds0, left);
             issue(lds1, left - kStep);
             issue(lds2, left - 2 * kStep);
-            keep_bias();
+            before();
             for (; left > 0; left -= 4 * kStep) {
                 arrived<2u * kLoads>();
                 issue(lds3, left - 3 * kStep);
@@ -747,6 +762,7 @@ __device__ __forceinline__ void product(const Ops& A, Out out, const Place& at, 
         for (uint32_t d = 0; d < kDepth - 1u; ++d)
             if (k0 + kBK * d < k_end) fetch(d, k0 + kBK * d);
         keep_bias();
+        if constexpr (More::kOn) more.template begin<kFP, kFQ>(acc, p0 + wp, q0 + wq, 0u, 1u);
         for (uint32_t k = k0; k < k_end; k += kBK * (kDepth - 1u)) {
 #pragma unroll
             for (uint32_t d = 0; d < kDepth - 1u; ++d) {
@@ -774,7 +790,6 @@ __device__ __forceinline__ void product(const Ops& A, Out out, const Place& at, 
         }
     }
 
-    if constexpr (More::kOn) more.template add<kFP, kFQ>(acc, p0 + wp, q0 + wq, 0u, 1u);
     // The wave's sums, 16 q x kSP p at a time, through LDS of its own into rows:
     // a lane then has eight consecutive p, and eight lanes one 128-byte line
     // (16-bit outputs).  Chunks of four p, their place xor-ed with the row.
@@ -953,6 +968,7 @@ __device__ __forceinline__ void few_tile(const Ops& A, const Out& out, const Pla
 #pragma unroll
     for (uint32_t d = 0; d < kDepth; ++d)
         if (32u * wave + kStride * d < A.nk) fetch(d, 32u * wave + kStride * d);
+    if constexpr (More::kOn) more.template begin<kF, kF>(acc, p0, q0, wave, kFewWaves);
     for (uint32_t k = 32u * wave; k < A.nk; k += kStride * kDepth) {
 #pragma unroll
         for (uint32_t d = 0; d < kDepth; ++d) {
@@ -974,7 +990,6 @@ __device__ __forceinline__ void few_tile(const Ops& A, const Out& out, const Pla
         }
     }
 
-    if constexpr (More::kOn) more.template add<kF, kF>(acc, p0, q0, wave, kFewWaves);
     __syncthreads();  // the waves' own pieces become those of the sums
     floatx4* strips = reinterpret_cast<floatx4*>(lds);
     constexpr uint32_t kStrip = 16u * kF * kSP / 4u;
