@@ -22,6 +22,19 @@ using namespace nerf_hip::grouped;
 
 namespace {
 
+// The power of two that scales values of at most `most` to less than 2 (8), and its
+// inverse.
+struct Power {
+    float value, inverse;
+};
+__device__ __forceinline__ Power power_of(float most) {
+    const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 1u), 252u);
+    if (most > 0.0f && most < __builtin_inff()) return {__uint_as_float(exponent << 23), __uint_as_float((254u - exponent) << 23)};
+    return {1.0f, 1.0f};
+}
+// What a rounding leaves of a value: nothing of an infinity or NaN.
+__device__ __forceinline__ float rest_of(float value, float rounded) { return fabsf(rounded) < __builtin_inff() ? value - rounded : 0.0f; }
+
 // The low-rank part of a wave's sums: low [rows][rank] times wide, which is
 // [groups][np][rank] (kPT: [groups][rank][np]).
 template <typename T, bool kPT>
@@ -81,7 +94,7 @@ struct LowRank {
         for (uint32_t i = 0; i < piece; ++i) {
             const floatx8 back = __builtin_convertvector(h, floatx8);
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) v[e] = fabsf(back[e]) < __builtin_inff() ? v[e] - back[e] : 0.0f;  // nothing is left of an infinity or NaN
+            for (uint32_t e = 0; e < 8u; ++e) v[e] = rest_of(v[e], back[e]);
             h = __builtin_convertvector(v, x8);
         }
         return h;
@@ -132,11 +145,9 @@ struct LowRank {
 #pragma unroll 4
                 for (uint32_t r = 0; r < rank; ++r) most = fmaxf(most, fabsf(at[r]));
             }
-            const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 1u), 252u);
-            if (most > 0.0f && most < __builtin_inff()) {
-                power   = __uint_as_float(exponent << 23);
-                inverse = __uint_as_float((254u - exponent) << 23);
-            }
+            const Power two = power_of(most);
+            power           = two.value;
+            inverse         = two.inverse;
         }
         auto of_row = [&](float v, uint32_t j) { return std::is_same_v<T, half_t> ? __shfl(v, (int)(16u * j + l)) : 1.0f; };
         for (uint32_t s = 0; s < steps; ++s) {
@@ -162,9 +173,10 @@ struct LowRank {
                     for (uint32_t i = 0; i < kAtOnce; ++i) fp[i] = wide_eight(g, p0 + 16u * (i0 + i) + l, piece < pieces ? r0 : rank);
 #pragma unroll
                     for (uint32_t j = 0; j < kFQ; ++j) {
-                        if (!(those >> (16u * j) & 0xFFFFull)) continue;
+                        const uint32_t rows = (uint32_t)(those >> (16u * j)) & 0xFFFFu;
+                        if (rows == 0u) continue;
                         const float factor = of_row(power, j) * scale;
-                        const bool member  = those >> (16u * j + l) & 1ull;
+                        const bool member  = rows >> l & 1u;
 #pragma unroll
                         for (uint32_t i = 0; i < kAtOnce; ++i) {
                             const floatx4 part = Vec<T>::mfma(fp[i], fq[j], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
@@ -201,6 +213,229 @@ __global__ __launch_bounds__(kFewWaves * 64u) void k_adapter_few(GatheredOperand
     find_rows<16u * kF>(out, rows, at.q0, A.nq);
     __syncthreads();
     few_tile<T, kF, kPT, false, kWords, kGather>(A, out, at, reinterpret_cast<char*>(lds), nullptr, more);
+}
+
+// Many rows, at most 32 kKS <= 256 k and 16 kRB <= 64 ranks, whole chunks: both
+// low-rank products and the shared one in one pass over the rows, with the shared
+// weights in registers (as k_stream in linear.hip) and the group's adapter in LDS.
+// A wave computes its rows' m, 16 ranks at a time, from the same registers as the
+// shared product (the waves of a row that hold other p do so again); lane 16 g + l
+// ends with ranks 4 g .. 4 g + 3 of row l, and their high and low parts are what it
+// has to hold for the next product, if that counts its k as (g, part, rank): no
+// value moves between lanes.  A workgroup has consecutive positions, group by group.
+constexpr uint32_t kStreamChunk = 1024u;  // positions whose rows are looked up at a time
+struct StreamRanks {
+    const void* shrink;  // down [groups][rank][nk]; kPT: up [groups][nk][rank]
+    float* low;          // m
+    const uint32_t* index;  // of the outputs
+    uint32_t count;
+};
+template <typename T, uint32_t kKS, uint32_t kRB, bool kPT, typename Out>
+__global__ __launch_bounds__(kStreamWaves * 64u) void k_adapter_stream(GatheredOperands A, Out out, LowRank<T, kPT> more, StreamRanks R, uint32_t p_waves) {
+    out.vec = true;
+    constexpr uint32_t kThreads = kStreamWaves * 64u, kFP = 4u, kSP = 16u * kFP, kBP = 256u, kLanes = kSP / 8u, kPasses = 16u * kLanes / 64u;
+    using x8 = typename Vec<T>::x8;
+    typedef T x4 __attribute__((ext_vector_type(4)));
+    __shared__ uint4 lds[kBP * 8u];
+    __shared__ floatx4 lds_bias[Out::kBias ? kBP / 4u : 1u];
+    __shared__ uint32_t x_rows[kStreamChunk], y_rows[kStreamChunk];
+    __shared__ x8 lds_shrink[kRB * kKS * 64u];
+    __shared__ x4 lds_grow[kRB * kBP * 4u];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, l = lane & 15u, quarter = lane >> 4;
+    const uint32_t wp = wave % p_waves * kSP, p0 = blockIdx.y * p_waves * kSP, waves_q = kStreamWaves / p_waves;
+    const Groups& G = more.G;
+
+    x8 fp[kKS][kFP];
+    {
+        const float bias = thread_bias<kBP>(out, p0);
+        Stager<T, kBP, kPT, kThreads, true> stager;
+        stager.fetch((const T*)A.p, A.ldp, A.np, p0, 0u, A.nk);
+        if (Out::kBias && threadIdx.x < kBP) reinterpret_cast<float*>(lds_bias)[threadIdx.x] = bias;
+        const uint32_t base = fragment_base<kBP, kPT>(wp & ~127u);
+#pragma unroll
+        for (uint32_t s = 0; s < kKS; s += 2u) {
+            stager.keep(lds, (const T*)A.p, A.ldp, A.np, p0, 32u * s, A.nk);
+            __syncthreads();
+            if (s + 2u < kKS) stager.fetch((const T*)A.p, A.ldp, A.np, p0, 32u * (s + 2u), A.nk);
+#pragma unroll
+            for (uint32_t i = 0; i < kFP; ++i)
+#pragma unroll
+                for (uint32_t h = 0; h < 2u; ++h)
+                    if (s + h < kKS) {
+                        fp[s + h][i] = fragment<T, kBP, kPT>(lds, base, (wp & 127u) / 16u + i, h);
+                        settle_here(fp[s + h][i]);
+                    }
+            __syncthreads();
+        }
+    }
+
+    const uint32_t row = lane / kLanes, col = 8u * (lane % kLanes), p = p0 + wp + col;
+    const uint32_t n = p < A.np ? min(8u, A.np - p) : 0u;
+    floatx4* strip = reinterpret_cast<floatx4*>(lds) + wave * (kSP * 4u);
+    constexpr bool kLate = sizeof(typename Out::Aux) > 16u;
+    const uint32_t each = (A.nq + 16u * gridDim.x - 1u) / (16u * gridDim.x) * 16u;
+    const uint64_t from = (uint64_t)chip_tile(blockIdx.x, gridDim.x) * each;
+    const uint32_t last = (uint32_t)min((uint64_t)A.nq, from + each);
+    const bool keeps_low = wp == 0u && blockIdx.y == 0u;
+    for (uint32_t pos = (uint32_t)min(from, (uint64_t)last), part_end; pos < last; pos = part_end) {
+        // The group of the next positions, or none, and where its part of them ends.
+        const uint32_t c = __builtin_amdgcn_readfirstlane(count_at_most(G.count, pos, [&](uint32_t g) { return G.offset(g); }));
+        const uint32_t group_end = c ? G.offset(c) : 0u, g = c ? c - 1u : 0u;
+        const bool member = pos < group_end;
+        const uint32_t limit = member ? group_end : c < G.count ? G.offset(c) : A.nq;
+        part_end = min(min(limit > pos ? limit : A.nq, last), pos + kStreamChunk);
+        const uint32_t end = part_end, tiles = (end - pos + 15u) / 16u;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < end - pos; i += kThreads) {
+            x_rows[i] = gathered_row(A.q_index, A.q_count, pos + i, end);
+            y_rows[i] = R.index ? gathered_row(R.index, R.count, pos + i, end) : i;
+        }
+        if (member) {
+            const T* shrink = (const T*)R.shrink;
+            for (uint32_t i = threadIdx.x; i < kRB * kKS * 64u; i += kThreads) {
+                const uint32_t r = i / (kKS * 64u) * 16u + i % 16u, k = i / 64u % kKS * 32u + i / 16u % 4u * 8u;
+                const bool inner = r < more.rank && k < A.nk;
+                x8 v;
+                if constexpr (!kPT) {
+                    v = *reinterpret_cast<const x8*>(shrink + (inner ? ((uint64_t)g * more.rank + r) * A.nk + k : 0ull));
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 8u; ++e) v[e] = shrink[inner ? ((uint64_t)g * A.nk + k + e) * more.rank + r : 0ull];
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e) v[e] = inner ? v[e] : (T)0.0f;
+                lds_shrink[i] = v;
+            }
+            for (uint32_t i = threadIdx.x; i < kRB * kBP * 4u; i += kThreads) {
+                const uint32_t r = i / (kBP * 4u) * 16u + i / 16u % 4u * 4u, at = p0 + i / 64u % (kBP / 16u) * 16u + i % 16u;
+                x4 v;
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) {
+                    const bool inner = at < A.np && r + e < more.rank;
+                    const T w = more.wide[!inner ? 0ull : kPT ? ((uint64_t)g * more.rank + r + e) * A.np + at : ((uint64_t)g * A.np + at) * more.rank + r + e];
+                    v[e] = inner ? w : (T)0.0f;
+                }
+                lds_grow[i] = v;
+            }
+        }
+        const float scale = member && more.scales ? more.scales[g] : 1.0f;
+        __syncthreads();
+
+        struct Coming {
+            uint4 q[kKS];
+            uint32_t none;
+            typename Out::Aux aux[kPasses];
+        } c0;
+        const uint32_t q0 = R.index ? 0u : pos;
+        auto row_of       = [&](uint32_t tile, uint32_t pass) {
+            const uint32_t r = tile * 16u + (64u / kLanes) * pass + row;
+            return r < end - pos ? y_rows[r] : kNoRow;
+        };
+        auto fetch_q = [&](uint32_t tile) {
+            const uint32_t r = x_rows[min(tile * 16u + l, end - pos - 1u)];
+            c0.none          = r == kNoRow;
+            const T* at      = (const T*)A.q + (uint64_t)(r == kNoRow ? 0u : r) * A.ldq + 8u * quarter;
+#pragma unroll
+            for (uint32_t s = 0; s < kKS; ++s)
+                if (32u * s < A.nk) c0.q[s] = *reinterpret_cast<const uint4*>(at + 32u * s);
+        };
+        auto fetch_aux = [&](uint32_t tile, uint32_t t) {
+            const uint32_t r = row_of(tile, t);
+            c0.aux[t]        = out.load(q0, r, p, r != kNoRow ? n : 0u);
+        };
+#pragma unroll
+        for (uint32_t s = 0; s < kKS; ++s) c0.q[s] = uint4{0u, 0u, 0u, 0u};
+        const uint32_t first_tile = __builtin_amdgcn_readfirstlane(wave / p_waves);
+        if (first_tile < tiles) {
+            fetch_q(first_tile);
+#pragma unroll
+            for (uint32_t t = 0; t < kPasses; ++t) fetch_aux(first_tile, t);
+        }
+        for (uint32_t tile = first_tile; tile < tiles; tile += waves_q) {
+            const uint32_t later = tile + waves_q;
+            if (c0.none) {
+#pragma unroll
+                for (uint32_t s = 0; s < kKS; ++s) c0.q[s] = uint4{0u, 0u, 0u, 0u};
+            }
+            floatx4 acc[kFP];
+#pragma unroll
+            for (uint32_t i = 0; i < kFP; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (member) {
+#pragma unroll
+                for (uint32_t rb = 0; rb < kRB; ++rb) {
+                    floatx4 m = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (uint32_t s = 0; s < kKS; ++s) m = Vec<T>::mfma(lds_shrink[(rb * kKS + s) * 64u + lane], __builtin_bit_cast(x8, c0.q[s]), m);
+                    if constexpr (kPT) m *= scale;
+                    const uint32_t position = pos + tile * 16u + l, r = 16u * rb + 4u * quarter;
+                    if (keeps_low && position < end) {
+                        float* to = R.low + (uint64_t)position * more.rank + r;
+                        if (more.vec_low) {
+                            if (r < more.rank) *reinterpret_cast<floatx4*>(to) = m;
+                        } else {
+#pragma unroll
+                            for (uint32_t e = 0; e < 4u; ++e)
+                                if (r + e < more.rank) to[e] = m[e];
+                        }
+                    }
+                    float factor = kPT ? 1.0f : scale;
+                    if constexpr (std::is_same_v<T, half_t>) {
+                        float most = fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3])));
+                        most = fmaxf(most, __shfl_xor(most, 16));
+                        most = fmaxf(most, __shfl_xor(most, 32));
+                        const Power power = power_of(most);
+                        m *= power.inverse;
+                        factor *= power.value;
+                    }
+                    const floatx8 both = {m[0], m[1], m[2], m[3], m[0], m[1], m[2], m[3]};
+                    const x8 high = __builtin_convertvector(both, x8);
+                    floatx8 rest;
+#pragma unroll
+                    for (uint32_t e = 0; e < 8u; ++e) rest[e] = e < 4u ? both[e] : rest_of(both[e], (float)high[e]);
+                    const x8 pieces = __builtin_convertvector(rest, x8);
+                    x8 third;
+                    if (more.pieces == 3u) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 8u; ++e) third[e] = e < 4u ? (T)0.0f : (T)rest_of(rest[e], (float)pieces[e]);
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < kFP; ++i) {
+                        const x4 w = lds_grow[(rb * (kBP / 16u) + wp / 16u + i) * 64u + lane];
+                        const x8 twice = __builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7);
+                        floatx4 part = Vec<T>::mfma(twice, pieces, floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+                        if (more.pieces == 3u) part = Vec<T>::mfma(twice, third, part);
+                        acc[i] += factor * part;
+                    }
+                }
+            }
+#pragma unroll
+            for (uint32_t s = 0; s < kKS; ++s)
+#pragma unroll
+                for (uint32_t i = 0; i < kFP; ++i) acc[i] = Vec<T>::mfma(fp[s][i], __builtin_bit_cast(x8, c0.q[s]), acc[i]);
+            typename Out::Aux aux[kPasses];
+#pragma unroll
+            for (uint32_t t = 0; t < kPasses; ++t) aux[t] = c0.aux[t];
+            if (later < tiles) {
+                fetch_q(later);
+#pragma unroll
+                for (uint32_t t = 0; t < kPasses; ++t)
+                    if (!kLate) fetch_aux(later, t);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kFP; ++i) strip[l * (kSP / 4u) + ((4u * i + quarter) ^ (l & 7u))] = acc[i];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (uint32_t t = 0; t < kPasses; ++t) {
+                const uint32_t r = (64u / kLanes) * t + row, to_row = row_of(tile, t);
+                floatx8 v;
+                v.lo = strip[r * (kSP / 4u) + ((col / 4u) ^ (r & 7u))];
+                v.hi = strip[r * (kSP / 4u) + ((col / 4u + 1u) ^ (r & 7u))];
+                out.put(q0, to_row, p, to_row != kNoRow ? n : 0u, v, bias8<Out>(reinterpret_cast<const float*>(lds_bias), wp + col), aux[t]);
+                if (kLate) fetch_aux(later, t);
+            }
+            asm volatile("" ::: "memory");
+        }
+    }
 }
 
 // Operands of fewer than eight values in all: a thread an output of a position.
@@ -295,9 +530,8 @@ __global__ __launch_bounds__(256) void k_rank_sums(RankSums A, Groups G, uint32_
     constexpr uint32_t kFR = kBR / 16u;
     __shared__ uint4 wide0[kBW * 8u], wide1[kMode == kDirect ? kBW * 8u : 1u];
     __shared__ float low0[kBK * kBR], low1[kMode == kDirect ? kBK * kBR : 1u];
-    const uint32_t tiles = A.tiles_w * A.tiles_r, parts = min(most, part_count(G, size)), block = block_number();
-    if (block >= parts * tiles) return;
-    const uint32_t t = chip_tile(block, parts * tiles);
+    const uint32_t tiles = A.tiles_w * A.tiles_r, t = dealt_tile(block_number(), most, tiles);
+    if (t >= most * tiles) return;
     const Part part = part_of(G, size, t / tiles);
     if (part.q0 >= part.end && part.number) return;
     const uint32_t w0 = t % tiles % A.tiles_w * kBW, r0 = t % tiles / A.tiles_w * kBR;
@@ -440,6 +674,37 @@ hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& mo
     return gather ? launch(k_adapter<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_adapter<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
 }
 
+// Whether k_adapter_stream takes a layer: with so many rows that its start is small
+// beside them.  Streamed against by tiles with the low-rank products before them, in
+// us, fp16, residual and pre, 16 groups: 262144 x 256 -> 256 rank 16 168 / 209, rank
+// 64 310 / 316, -> 512 280 / 353; 65536 x 256 -> 256 49 / 52, 128 -> 256 35 / 39;
+// 32768 x 256 -> 256 32 / 27.  Gradients: 262144 rows 268 / 339, rank 64 536 / 589,
+// 65536 rows 90 / 105, 32768 rows 60 / 60.
+template <typename T, bool kPT>
+bool streamed(const GatheredOperands& A, const LowRank<T, kPT>& more, const void* shrink, bool vec, const uint32_t* index, uint32_t count, uint64_t widest) {
+    return A.nk <= 256u && A.nk % 32u == 0u && A.np <= 512u && more.rank <= 64u && A.nq >= 65536u && vec && whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) && whole_chunks(A.q, A.ldq, A.nk) && aligned(shrink, 16u) && (!index || near(count, widest));
+}
+
+template <typename T, bool kPT, typename Out>
+hipError_t launch_stream(const GatheredOperands& A, const Out& out, const LowRank<T, kPT>& more, const StreamRanks& R, hipStream_t stream) {
+    uint32_t p_waves = 1u;
+    while (p_waves < 4u && 64u * p_waves < A.np) p_waves *= 2u;
+    const uint32_t across = ceil_div(A.np, 64u * p_waves);
+    const dim3 grid(std::max(1u, device_cu_count() / across), across);
+    auto launch = [&](auto steps, auto ranks) {
+        k_adapter_stream<T, steps(), ranks(), kPT, Out><<<grid, kStreamWaves * 64u, 0, stream>>>(A, out, more, R, p_waves);
+        return hipGetLastError();
+    };
+    auto by_rank = [&](auto steps) {
+        if (more.rank <= 16u) return launch(steps, std::integral_constant<uint32_t, 1u>{});
+        if (more.rank <= 32u) return launch(steps, std::integral_constant<uint32_t, 2u>{});
+        return launch(steps, std::integral_constant<uint32_t, 4u>{});
+    };
+    if (A.nk <= 64u) return by_rank(std::integral_constant<uint32_t, 2u>{});
+    if (A.nk <= 128u) return by_rank(std::integral_constant<uint32_t, 4u>{});
+    return by_rank(std::integral_constant<uint32_t, 8u>{});
+}
+
 template <typename T>
 hipError_t launch_rank_sums(RankSums A, const Groups& G, Workspace ws, hipStream_t stream) {
     const uint64_t length = (uint64_t)A.nw * A.nr;
@@ -451,9 +716,9 @@ hipError_t launch_rank_sums(RankSums A, const Groups& G, Workspace ws, hipStream
         A.tiles_w = ceil_div(A.nw, kBW);
         A.tiles_r = ceil_div(A.nr, br);
         const uint64_t tiles = (uint64_t)A.tiles_w * A.tiles_r;
-        const uint32_t size  = part_size(G.rows, tiles, 4u * device_cu_count(), 4u * length, ws.bytes), most = G.rows / size + G.count;
+        const uint32_t size  = part_size(G.rows, tiles, 2u * device_cu_count(), 4u * length, ws.bytes), most = G.rows / size + G.count;
         A.parts              = ws.data;
-        kernel<<<grid_of(most * tiles), 256, 0, stream>>>(A, G, size, most);
+        kernel<<<grid_of(dealt_blocks(most, (uint32_t)tiles)), 256, 0, stream>>>(A, G, size, most);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || size >= G.rows) return e;
         return launch_join(G, size, A.out, ws.data, length, nullptr, nullptr, 0u, stream);
@@ -476,12 +741,17 @@ LowRank<T, kPT> low_rank(const float* low, const void* wide, const float* scales
 template <typename T>
 NerfStatus forward(const NerfExtLinearDesc& d, const NerfExtRowGroups& r, const NerfExtAdapters& a, const void* x, const void* w, const float* bias, const void* residual, void* y, void* pre, float* mid, hipStream_t stream) {
     const Groups G{r.offsets, r.groups, d.rows};
-    NERF_HIP_TRY((launch_ranks<T, false>(G, (const T*)x, d.x_stride, r.x_rows, r.x_count, (const T*)a.down, d.in_features, a.rank, nullptr, mid, stream)));
     const bool vec = d.out_features % 8u == 0u && d.y_stride % 8u == 0u && aligned(y, 16u) && aligned(pre, 16u) && (!residual || (d.residual_stride % 8u == 0u && aligned(residual, 16u)));
     const bool y32 = d.out_dtype == NERF_EXT_F32;
     const GatheredOperands A{{w, x, d.in_features, d.x_stride, d.out_features, d.rows, d.in_features, 0u, 0u, 0u}, nullptr, r.x_rows, 0u, r.x_count};
     const RowsForwardOut<T> out{bias, (const T*)residual, y, (T*)pre, d.residual_stride, d.y_stride, d.out_features, d.rows, d.activation, y32, vec, r.y_rows, r.y_count, nullptr};
-    NERF_HIP_TRY((launch_adapter<T, false>(A, out, low_rank<T, false>(mid, a.up, a.scales, G, d.out_features, a.rank, y32 && d.dtype == NERF_EXT_BF16 ? 3u : 2u), stream)));
+    const LowRank<T, false> more = low_rank<T, false>(mid, a.up, a.scales, G, d.out_features, a.rank, y32 && d.dtype == NERF_EXT_BF16 ? 3u : 2u);
+    if (streamed(A, more, a.down, vec, r.y_rows, r.y_count, out.widest_row())) {
+        NERF_HIP_TRY((launch_stream<T, false>(A, out.near(), more, StreamRanks{a.down, mid, r.y_rows, r.y_count}, stream)));
+        return NERF_STATUS_OK;
+    }
+    NERF_HIP_TRY((launch_ranks<T, false>(G, (const T*)x, d.x_stride, r.x_rows, r.x_count, (const T*)a.down, d.in_features, a.rank, nullptr, mid, stream)));
+    NERF_HIP_TRY((launch_adapter<T, false>(A, out, more, stream)));
     return NERF_STATUS_OK;
 }
 
@@ -489,13 +759,23 @@ template <typename T>
 NerfStatus backward(const NerfExtLinearDesc& d, const NerfExtRowGroups& r, const NerfExtAdapters& a, const void* x, const void* w, const void* delta, const float* mid, const void* pre, const void* add, void* dx, void* dpre, float* dmid,
                     float* ddown, float* dup, Workspace ws, hipStream_t stream) {
     const Groups G{r.offsets, r.groups, d.rows};
-    if (d.rows && dmid) NERF_HIP_TRY((launch_ranks<T, true>(G, (const T*)delta, d.y_stride, r.y_rows, r.y_count, (const T*)a.up, d.out_features, a.rank, a.scales, dmid, stream)));
-    if ((dx || dpre) && d.rows) {
+    const bool to_x = (dx || dpre) && d.rows;
+    bool have_low   = !d.rows || !dmid;
+    if (to_x) {
         const bool vec = d.in_features % 8u == 0u && (!(add || dx) || d.x_stride % 8u == 0u) && aligned(add, 16u) && aligned(dx, 16u) && aligned(pre, 16u) && aligned(dpre, 16u);
         const GatheredOperands A{{w, delta, d.in_features, d.y_stride, d.in_features, d.rows, d.out_features, 0u, 0u, 0u}, nullptr, r.y_rows, 0u, r.y_count};
         const RowsGradientOut<T> out{(const T*)add, (T*)dx, (const T*)pre, (T*)dpre, d.x_stride, d.in_features, d.rows, d.activation, vec, r.x_rows, r.x_count, nullptr};
-        NERF_HIP_TRY((launch_adapter<T, true>(A, out, low_rank<T, true>(dmid, a.down, nullptr, G, d.in_features, a.rank, 2u), stream)));
+        LowRank<T, true> more = low_rank<T, true>(dmid, a.down, nullptr, G, d.in_features, a.rank, 2u);
+        if (streamed(A, more, a.up, vec, r.x_rows, r.x_count, out.widest_row())) {
+            more.scales = a.scales;
+            NERF_HIP_TRY((launch_stream<T, true>(A, out.near(), more, StreamRanks{a.up, dmid, r.x_rows, r.x_count}, stream)));
+        } else {
+            NERF_HIP_TRY((launch_ranks<T, true>(G, (const T*)delta, d.y_stride, r.y_rows, r.y_count, (const T*)a.up, d.out_features, a.rank, a.scales, dmid, stream)));
+            NERF_HIP_TRY((launch_adapter<T, true>(A, out, more, stream)));
+        }
+        have_low = true;
     }
+    if (!have_low) NERF_HIP_TRY((launch_ranks<T, true>(G, (const T*)delta, d.y_stride, r.y_rows, r.y_count, (const T*)a.up, d.out_features, a.rank, a.scales, dmid, stream)));
     if (ddown) NERF_HIP_TRY((launch_rank_sums<T>(RankSums{x, dmid, nullptr, ddown, nullptr, r.x_rows, d.x_stride, r.x_count, d.in_features, a.rank, 0u, 0u, true}, G, ws, stream)));
     if (dup) NERF_HIP_TRY((launch_rank_sums<T>(RankSums{delta, mid, a.scales, dup, nullptr, r.y_rows, d.y_stride, r.y_count, d.out_features, a.rank, 0u, 0u, false}, G, ws, stream)));
     return NERF_STATUS_OK;

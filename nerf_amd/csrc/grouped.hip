@@ -82,9 +82,8 @@ __global__ __launch_bounds__(64) void k_grouped_tiny(GatheredOperands A, Out out
 // dW_g, and db_g with it: sums over parts of `size` rows of a group.
 template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, Mode kMode, bool kGather>
 __global__ __launch_bounds__(kWP * kWQ * 64u) void k_grouped_sums(GatheredOperands A, SumOut out, Groups G, uint32_t size, uint32_t most, float* sum_parts) {
-    const uint32_t tiles = A.tiles_p * A.tiles_q, parts = min(most, part_count(G, size)), block = block_number();
-    if (block >= parts * tiles) return;
-    const uint32_t t = chip_tile(block, parts * tiles);
+    const uint32_t tiles = A.tiles_p * A.tiles_q, t = dealt_tile(block_number(), most, tiles);
+    if (t >= most * tiles) return;
     const Part part = part_of(G, size, t / tiles);
     if (part.q0 >= part.end && part.number) return;
     const uint64_t length = (uint64_t)A.np * A.nq;
@@ -188,10 +187,10 @@ hipError_t launch_sums(GatheredOperands A, const Groups& G, float* dw, float* db
         A.tiles_p = ceil_div(A.np, bp);
         A.tiles_q = ceil_div(A.nq, bq);
         const uint64_t tiles = (uint64_t)A.tiles_p * A.tiles_q;
-        const uint32_t size  = part_size(G.rows, tiles, 4u * device_cu_count(), bytes, ws.bytes), most = G.rows / size + G.count;
+        const uint32_t size  = part_size(G.rows, tiles, device_cu_count(), bytes, ws.bytes), most = G.rows / size + G.count;
         out.parts            = ws.data;
         float* sum_parts     = ws.data + (G.rows / size) * length;
-        kernel<<<grid_of(most * tiles), threads, 0, stream>>>(A, out, G, size, most, sum_parts);
+        kernel<<<grid_of(dealt_blocks(most, (uint32_t)tiles)), threads, 0, stream>>>(A, out, G, size, most, sum_parts);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || size >= G.rows) return e;
         return launch_join(G, size, dw, ws.data, length, db, sum_parts, db ? A.nq : 0u, stream);
@@ -247,6 +246,7 @@ NerfStatus nerf_hip::grouped::check_groups(const NerfExtRowGroups* groups, const
     if (out.x_count == 0u) out.x_count = d.rows;
     if (out.y_count == 0u) out.y_count = d.rows;
     if (out.x_count > kMaxRows || out.y_count > kMaxRows) return refuse("more than 2^30 rows");
+    if (((uint64_t)d.rows / 64u + out.groups) * ceil_div(std::max(d.in_features, d.out_features), 64u) >= 1ull << 31) return refuse("more than 2^31 tiles of 64 x 64 outputs");
     if ((!out.x_rows && out.x_count != d.rows) || (!out.y_rows && out.y_count != d.rows)) return refuse("x_count and y_count come with x_rows and y_rows");
     return NERF_STATUS_OK;
 }

@@ -48,10 +48,12 @@ struct Part {
     uint32_t group, q0, end, number;  // number: of the part within its group
 };
 
-// Part number `s` of the parts of `size` positions each.
+// Part number `s` of the parts of `size` positions each.  Every group has a first part
+// (number 0), also one without positions; numbers before the first group's, where
+// offsets[0] > 0, are of no group's first part.
 __device__ __forceinline__ Part part_of(const Groups& G, uint32_t size, uint32_t s) {
     const uint32_t c = count_at_most(G.count, s, [&](uint32_t g) { return G.offset(g) / size + g; });
-    if (c == 0u) return {0u, 0u, 0u, 0u};
+    if (c == 0u) return {0u, 0u, 0u, 1u};
     const uint32_t g = __builtin_amdgcn_readfirstlane(c - 1u), begin = G.offset(g), end = G.offset(g + 1u), number = s - (begin / size + g);
     const uint64_t q0 = begin + (uint64_t)number * size;
     return {g, q0 < end ? (uint32_t)q0 : end, end, number};
@@ -166,6 +168,9 @@ struct RowsForwardOut {
     };
     static constexpr bool kBias = true;
 
+    // The same for rows within 32-bit offsets, and how many 16-bit values a row has.
+    ForwardOut<T> near() const { return {bias, residual, y, pre, ldr, ldy, np, nq, act, y32, vec}; }
+    uint64_t widest_row() const { return std::max({(y32 ? 2u : 1u) * ldy, residual ? ldr : 0u, (uint64_t)np}); }
     __device__ __forceinline__ void of_group(uint32_t g) {
         if (bias) bias += (uint64_t)g * np;
     }
@@ -203,6 +208,8 @@ struct RowsGradientOut {
     };
     static constexpr bool kBias = false;
 
+    InputGradientOut<T> near() const { return {add, dx, pre, dpre, ldx, np, nq, act, vec}; }
+    uint64_t widest_row() const { return std::max(ldx, (uint64_t)np); }
     __device__ __forceinline__ void of_group(uint32_t) {}
     __device__ __forceinline__ Aux load(uint32_t, uint32_t row, uint32_t p, uint32_t n) const {
         Aux a{};
@@ -236,7 +243,7 @@ struct PositionOut {
     static constexpr bool kBias = false;
     __device__ __forceinline__ void of_group(uint32_t g) { scale = scales ? scales[g] : 1.0f; }
     __device__ __forceinline__ Aux load(uint32_t, uint32_t, uint32_t, uint32_t) const { return {}; }
-    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, const floatx8& v, const floatx8&, const Aux&) const { store_eight<float>(out + (uint64_t)(q0 + row) * np, p, n, vec, v * scale); }
+    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, const floatx8& v, const floatx8&, const Aux&) const { Rows<float>(out, q0, np).store(row, p, n, vec, v * scale); }
 };
 
 template <typename Out>
@@ -251,6 +258,26 @@ __device__ __forceinline__ void find_rows(Out& out, uint32_t* lds, uint32_t q0, 
 }
 
 // -------------------------------------------------------------------- sums
+// Parts are of uneven length, so their tiles are dealt to the eight chips in turn, a
+// few at a time that share operands: a whole part's (32 at most) where there are
+// many parts, else an eighth, so that no chip has the longest group to itself.
+// (16384 x 2048 -> 4096 in 8 groups of up to 6200 rows, sums alone: 770 us with a
+// chip's tiles in a row, 320 dealt by eighths; 262144 x 256 -> 256 in 64 groups
+// 97 us by single tiles, 87 by parts.)  A workgroup beyond the last tile gets a
+// number beyond it.
+inline __host__ __device__ uint32_t dealt_at_once(uint32_t parts, uint32_t tiles) {
+    const uint32_t u = parts >= 64u ? tiles : tiles / 8u;
+    return u < 1u ? 1u : u > 32u ? 32u : u;
+}
+__device__ __forceinline__ uint32_t dealt_tile(uint32_t b, uint32_t parts, uint32_t tiles) {
+    const uint32_t u = dealt_at_once(parts, tiles), j = b / 8u;
+    return (j / u * 8u + b % 8u) * u + j % u;
+}
+inline uint64_t dealt_blocks(uint32_t parts, uint32_t tiles) {
+    const uint64_t turn = 8u * dealt_at_once(parts, tiles);
+    return ((uint64_t)parts * tiles + turn - 1u) / turn * turn;
+}
+
 // Sums over a group's rows are made of parts of `size` positions: the first part
 // is in the output, part t > 0 of group g in place offsets[g] / size + t - 1 of
 // the others (no two parts share one, and there are rows / size of them at most,
@@ -275,7 +302,7 @@ hipError_t launch_join(const Groups& G, uint32_t size, float* out, const float* 
 inline uint32_t part_size(uint32_t rows, uint64_t tiles, uint64_t fill, uint64_t bytes_a_part, uint64_t workspace_bytes) {
     const uint64_t wanted = std::max<uint64_t>(1u, fill / std::max<uint64_t>(1u, tiles)), held = workspace_bytes / bytes_a_part;
     uint64_t size = std::max<uint64_t>(256u, (rows + wanted - 1u) / wanted);
-    if (rows / size > held) size = held ? rows / held + 1u : (uint64_t)rows + 1u;
+    if (rows / size > held) size = rows / (held + 1u) + 1u;  // rows / size <= held
     return (uint32_t)std::min<uint64_t>((size + kBK - 1u) / kBK * kBK, 1u << 31);
 }
 

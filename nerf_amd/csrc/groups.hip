@@ -117,7 +117,7 @@ __device__ __forceinline__ void place_rows(const uint32_t* __restrict__ ids, uin
             }
             if (id[i] != ~0u) {
                 const uint32_t shift = 16u * (id[i] & 1u), before = mine[id[i] / 2u] >> shift & 0xFFFFu;
-                const uint32_t rank = (uint32_t)__popcll(same & ((1ull << lane) - 1ull)), all = (uint32_t)__popcll(same);
+                const uint32_t rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0u)), all = (uint32_t)__popcll(same);
                 const uint32_t at = S.start[id[i]] + before + rank, row = (uint32_t)base + (wave * kEach + i) * 64u + lane;
                 order[at] = row;
                 if (place) place[row] = at;

@@ -21,68 +21,6 @@ using namespace nerf_hip::linear;
 
 namespace {
 
-
-// Each epilogue gets eight consecutive p of one row q0 + row at a time, n of
-// them inside the output (0 for a row outside), with their biases, and first
-// loads what else it needs, so that a caller can have that under way early.
-template <typename T>
-struct ForwardOut {
-    const float* bias;
-    const T* residual;
-    void* y;
-    T* pre;
-    uint64_t ldr, ldy;
-    uint32_t np, nq, act;
-    bool y32, vec;
-    struct Aux {
-        uintx4 residual;
-    };
-    static constexpr bool kBias = true;
-
-    __device__ __forceinline__ Aux load(uint32_t q0, uint32_t row, uint32_t p, uint32_t n) const {
-        return {residual ? Rows<T>(residual, q0, ldr).load(row, p, n, vec, np >= 8u) : uintx4{0u, 0u, 0u, 0u}};
-    }
-    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 z, const floatx8& b, const Aux& a) const {
-        z += b;
-        if (pre) Rows<T>(pre, q0, np).store(row, p, n, vec, z);
-        act_values(act, z);
-        if (residual) z += widen<T>(a.residual, n, vec, np >= 8u);
-        if (y32) Rows<float>(y, q0, ldy).store(row, p, n, vec, z);
-        else Rows<T>(y, q0, ldy).store(row, p, n, vec, z);
-    }
-};
-
-template <typename T>
-struct InputGradientOut {
-    const T* add;
-    T* dx;
-    const T* pre;
-    T* dpre;
-    uint64_t ldx;
-    uint32_t np, nq, act;
-    bool vec;
-    struct Aux {
-        uintx4 add, pre;
-    };
-    static constexpr bool kBias = false;
-
-    __device__ __forceinline__ Aux load(uint32_t q0, uint32_t row, uint32_t p, uint32_t n) const {
-        Aux a{};
-        if (add) a.add = Rows<T>(add, q0, ldx).load(row, p, n, vec, np >= 8u);
-        if (dpre) a.pre = Rows<T>(pre, q0, np).load(row, p, n, vec, np >= 8u);
-        return a;
-    }
-    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 g, const floatx8&, const Aux& a) const {
-        if (add) g += widen<T>(a.add, n, vec, np >= 8u);
-        if (dx) Rows<T>(dx, q0, ldx).store(row, p, n, vec, g);
-        if (dpre) {
-            floatx8 s = widen<T>(a.pre, n, vec, np >= 8u);
-            act_slopes(act, s);
-            Rows<T>(dpre, q0, np).store(row, p, n, vec, g * s);
-        }
-    }
-};
-
 // ----------------------------------------------------------------- product
 template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, bool kQT, Mode kMode, typename Out>
 __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out) {
@@ -112,7 +50,6 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_product(Operands A, Out out
 // workgroup that hold other p read the same Q at about the same time, from the
 // CU's cache.  262144 x 256 -> 256 with residual and pre takes 109 us = 4.9 TB/s, a
 // copy's rate (by tiles 130); its input gradient 129.
-constexpr uint32_t kStreamWaves = 8u;
 template <typename T, uint32_t kKS, uint32_t kFP, bool kPT, bool kRagged, bool kWords, typename Out>
 __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out out, uint32_t p_waves) {
     // Where P takes half of the registers, the outputs' edges have to do without any.

@@ -117,24 +117,24 @@ __device__ __forceinline__ void act_slopes(uint32_t act, floatx8& z) {
 }
 
 // Eight values of which `some` are an operand's, fetched from `down` values
-// ahead of them: those moved to the front, zeros behind them.
+// ahead of them: those moved to the front, zeros behind them.  By 32-bit words: a
+// 64-bit shift whose amount was in the last register of a wave's allocation has
+// given wrong bits here now and then (tests/test_code_objects.py).
 __device__ __forceinline__ uint4 settled(uint4 v, uint32_t down, uint32_t some) {
-    unsigned long long w[2];
-    __builtin_memcpy(w, &v, 16);
-    const uint32_t bits = 16u * (down & 3u);
-    if (down >= 4u) {
-        w[0] = w[1];
-        w[1] = 0ull;
-    }
-    if (bits) {
-        w[0] = w[0] >> bits | w[1] << (64u - bits);
-        w[1] >>= bits;
-    }
-    const unsigned long long ones = ~0ull;
-    w[0] &= some >= 4u ? ones : ~(ones << (16u * some));
-    w[1] &= some >= 8u ? ones : some > 4u ? ~(ones << (16u * (some - 4u))) : 0ull;
-    __builtin_memcpy(&v, w, 16);
-    return v;
+    const uint32_t bits = 16u * (down & 1u);
+    uint32_t w[4] = {__builtin_amdgcn_alignbit(v.y, v.x, bits), __builtin_amdgcn_alignbit(v.z, v.y, bits), __builtin_amdgcn_alignbit(v.w, v.z, bits), v.w >> bits};
+    const bool one = down & 2u, two = down & 4u;
+    w[0] = one ? w[1] : w[0];
+    w[1] = one ? w[2] : w[1];
+    w[2] = one ? w[3] : w[2];
+    w[3] = one ? 0u : w[3];
+    w[0] = two ? w[2] : w[0];
+    w[1] = two ? w[3] : w[1];
+    w[2] = two ? 0u : w[2];
+    w[3] = two ? 0u : w[3];
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) w[i] &= some > 2u * i + 1u ? ~0u : some > 2u * i ? 0xFFFFu : 0u;
+    return uint4{w[0], w[1], w[2], w[3]};
 }
 
 // ------------------------------------------------------------- epilogues
@@ -235,6 +235,67 @@ __device__ __forceinline__ floatx8 bias8(const float* lds, uint32_t at) {
 // Each epilogue gets eight consecutive p of one row q0 + row at a time, n of
 // them inside the output (0 for a row outside), with their biases, and first
 
+// Each epilogue gets eight consecutive p of one row q0 + row at a time, n of
+// them inside the output (0 for a row outside), with their biases, and first
+// loads what else it needs, so that a caller can have that under way early.
+template <typename T>
+struct ForwardOut {
+    const float* bias;
+    const T* residual;
+    void* y;
+    T* pre;
+    uint64_t ldr, ldy;
+    uint32_t np, nq, act;
+    bool y32, vec;
+    struct Aux {
+        uintx4 residual;
+    };
+    static constexpr bool kBias = true;
+
+    __device__ __forceinline__ Aux load(uint32_t q0, uint32_t row, uint32_t p, uint32_t n) const {
+        return {residual ? Rows<T>(residual, q0, ldr).load(row, p, n, vec, np >= 8u) : uintx4{0u, 0u, 0u, 0u}};
+    }
+    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 z, const floatx8& b, const Aux& a) const {
+        z += b;
+        if (pre) Rows<T>(pre, q0, np).store(row, p, n, vec, z);
+        act_values(act, z);
+        if (residual) z += widen<T>(a.residual, n, vec, np >= 8u);
+        if (y32) Rows<float>(y, q0, ldy).store(row, p, n, vec, z);
+        else Rows<T>(y, q0, ldy).store(row, p, n, vec, z);
+    }
+};
+
+template <typename T>
+struct InputGradientOut {
+    const T* add;
+    T* dx;
+    const T* pre;
+    T* dpre;
+    uint64_t ldx;
+    uint32_t np, nq, act;
+    bool vec;
+    struct Aux {
+        uintx4 add, pre;
+    };
+    static constexpr bool kBias = false;
+
+    __device__ __forceinline__ Aux load(uint32_t q0, uint32_t row, uint32_t p, uint32_t n) const {
+        Aux a{};
+        if (add) a.add = Rows<T>(add, q0, ldx).load(row, p, n, vec, np >= 8u);
+        if (dpre) a.pre = Rows<T>(pre, q0, np).load(row, p, n, vec, np >= 8u);
+        return a;
+    }
+    __device__ __forceinline__ void put(uint32_t q0, uint32_t row, uint32_t p, uint32_t n, floatx8 g, const floatx8&, const Aux& a) const {
+        if (add) g += widen<T>(a.add, n, vec, np >= 8u);
+        if (dx) Rows<T>(dx, q0, ldx).store(row, p, n, vec, g);
+        if (dpre) {
+            floatx8 s = widen<T>(a.pre, n, vec, np >= 8u);
+            act_slopes(act, s);
+            Rows<T>(dpre, q0, np).store(row, p, n, vec, g * s);
+        }
+    }
+};
+
 // Plain sums in 32 bits: dW, or one part of a sum that was split over k.
 struct SumOut {
     float* out;       // the first part, or all of it
@@ -251,6 +312,7 @@ struct SumOut {
 
 // ----------------------------------------------------------------- product
 constexpr uint32_t kBK = 64u;  // k per tile: two matrix instructions' worth
+constexpr uint32_t kStreamWaves = 8u;  // of the kernels that stream rows past weights in registers
 
 struct Operands {
     const void* p;
@@ -294,7 +356,7 @@ struct Place {
 template <uint32_t kB, bool kT>
 __device__ __forceinline__ constexpr uint32_t chunk_key(uint32_t line) {
     if (!kT) return line & 7u;
-    if (kB == 32u) return ((line >> 2 ^ line >> 3) & 1u) << 1;
+    if (kB == 32u) return ((line >> 1 ^ line >> 3) & 1u) << 1;  // as all of them, the same for k 4 on
     if (kB >= 128u) return ((line & 3u) | ((line >> 3) & 1u) << 2) << 1;
     return (((line >> 1) & 1u) | ((line >> 3) & 1u) << 1) << 1;
 }

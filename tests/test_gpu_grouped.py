@@ -160,3 +160,38 @@ def test_random_values(workspace, name, kind, y_kind, rank):
     want, got = G.backward(c, name, mid=mid), run_backward(c, name, workspace, mid=mid)
     for k in got:
         within(got[k], *want[k], k)
+
+
+# Enough rows for the kernels that stream them, and for tiles of every size.
+LARGE = [(40001, 7, 256, 256), (70000, 300, 32, 64), (33000, 5, 128, 264), (33001, 3, 63, 64), (40000, 9, 64, 31), (36000, 11, 96, 32), (33000, 2, 256, 520), (20000, 3, 520, 264), (9000, 2, 1032, 1024), (5000, 20, 600, 300)]
+
+
+@pytest.mark.parametrize("n,groups,i,o", LARGE)
+@pytest.mark.parametrize("kind,index", [("f16", 1), ("bf16", 0)])
+def test_grouped_many_rows(workspace, n, groups, i, o, kind, index):
+    announce(f"grouped {n} x {i} -> {o}, {groups} groups, {kind}, {INDEXES[index]}")
+    c = G.Case(n, groups, i, o, kind, seed=n, whole=True, **INDEXES[index])
+    forward_equal(c, "relu", "f32" if kind == "bf16" else kind, workspace)
+    backward_equal(c, "relu", workspace)
+
+
+@pytest.mark.parametrize("n,groups,i,o,rank", [(66001, 7, 256, 256, 16), (66000, 300, 64, 64, 12), (65536, 5, 128, 264, 20), (66000, 3, 96, 72, 64), (66000, 4, 256, 512, 9), (33000, 2, 63, 64, 16), (20000, 3, 520, 264, 48), (9000, 2, 1032, 1024, 128), (5000, 20, 600, 300, 7)])
+@pytest.mark.parametrize("kind,index", [("f16", 1), ("bf16", 0)])
+def test_adapter_many_rows(workspace, n, groups, i, o, rank, kind, index):
+    announce(f"adapter {n} x {i} -> {o}, {groups} groups, rank {rank}, {kind}, {INDEXES[index]}")
+    c = G.Case(n, groups, i, o, kind, seed=n, rank=rank, whole=True, **INDEXES[index])
+    forward_equal(c, "relu", "f32" if kind == "bf16" else kind, workspace)
+    backward_equal(c, "relu", workspace)
+
+
+@pytest.mark.parametrize("kind,y_kind", [("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f32")])
+def test_adapter_many_random_rows(workspace, kind, y_kind):
+    announce(f"adapter, many random rows, {kind} -> {y_kind}")
+    c = G.Case(65600, 6, 128, 96, kind, seed=6, rank=16)
+    want, got = G.forward(c, "silu", y_kind), run_forward(c, "silu", y_kind, workspace)
+    for k in got:
+        within(got[k], *want[k], k)
+    mid = want["mid"][0].astype(np.float32).astype(np.float64)
+    want, got = G.backward(c, "silu", mid=mid), run_backward(c, "silu", workspace, mid=mid)
+    for k in got:
+        within(got[k], *want[k], k)
