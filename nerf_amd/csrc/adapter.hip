@@ -100,93 +100,197 @@ struct LowRank {
         return h;
     }
 
+    // The group of position q0 + lane, of `count` positions: that of q0, and one more
+    // for every offset up to the position.
+    // asked: ask_offset()'s, the lane's offset where there are as many lanes.
+    __device__ __forceinline__ uint32_t ask_offset() const {
+        const uint32_t lane = threadIdx.x & 63u;
+        return G.count < 64u && lane <= G.count ? G.offset(lane) : kNoRow;
+    }
+    __device__ __forceinline__ uint32_t group_of_lane(uint32_t asked, uint32_t q0, uint32_t count) const {
+        const uint32_t lane = threadIdx.x & 63u, q_last = q0 + count - 1u;
+        uint32_t mine;
+        if (G.count < 64u) {
+            const uint32_t offset = asked;
+            const uint32_t before = (uint32_t)__popcll(__ballot(lane < G.count && offset <= q0)), end = (uint32_t)__popcll(__ballot(offset <= q_last));
+            mine = before;
+            for (uint32_t c = before; c < end; ++c) mine += (uint32_t)__builtin_amdgcn_readlane((int)offset, (int)c) <= q0 + lane;
+        } else {
+            const uint32_t before = count_at_most(G.count, q0, [&](uint32_t g) { return G.offset(g); });
+            mine = before;
+            for (uint32_t first = before; first <= G.count; first += 64u) {
+                const uint32_t offset = first + lane <= G.count ? G.offset(first + lane) : kNoRow;
+                const uint32_t some = (uint32_t)__popcll(__ballot(offset <= q_last));
+                for (uint32_t c = 0; c < some; ++c) mine += (uint32_t)__builtin_amdgcn_readlane((int)offset, (int)c) <= q0 + lane;
+                if (some < 64u) break;
+            }
+        }
+        return lane < count && q0 + lane < G.rows && mine != 0u && mine <= G.count ? mine - 1u : kNoRow;
+    }
+
+    // Values of kFQ rows a lane for step `s` of 32 k, k counted as (piece, rank): a
+    // quarter of the wave has eight of one piece.
+    struct Step {
+        uint32_t piece, r0;
+    };
+    __device__ __forceinline__ Step step_of(uint32_t s) const {
+        const uint32_t chunks = (rank + 7u) / 8u, chunk = 4u * s + ((threadIdx.x & 63u) >> 4), piece = chunk / chunks;
+        return {piece < pieces ? piece : 0u, piece < pieces ? 8u * (chunk - piece * chunks) : rank};
+    }
+    __device__ __forceinline__ uint32_t steps() const { return (pieces * ((rank + 7u) / 8u) + 3u) / 4u; }
+    template <uint32_t kFQ>
+    __device__ __forceinline__ void fetch(floatx8 (&values)[kFQ], uint32_t q0, uint32_t s) const {
+#pragma unroll
+        for (uint32_t j = 0; j < kFQ; ++j) values[j] = low_eight(q0 + 16u * j + (threadIdx.x & 15u), step_of(s).r0);
+    }
+    // The power of two of the row of position q0 + lane.
+    __device__ __forceinline__ Power power_of_lane(uint32_t q0) const {
+        if constexpr (!std::is_same_v<T, half_t>) return {1.0f, 1.0f};
+        const float* at = low + (uint64_t)min(q0 + (threadIdx.x & 63u), G.rows - 1u) * rank;
+        float most = 0.0f;
+        if (vec_low) {
+            for (uint32_t r = 0; r < rank; r += 8u) {
+                const floatx4 v = *reinterpret_cast<const floatx4*>(at + r), w = *reinterpret_cast<const floatx4*>(at + r + 4u);
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) most = fmaxf(most, fmaxf(fabsf(v[e]), fabsf(w[e])));
+            }
+        } else {
+#pragma unroll 4
+            for (uint32_t r = 0; r < rank; ++r) most = fmaxf(most, fabsf(at[r]));
+        }
+        return power_of(most);
+    }
+    // What position 16 j + lane % 16 has of a value that lane 16 j + lane % 16 holds.
+    static __device__ __forceinline__ float of_row(float v, uint32_t j) { return std::is_same_v<T, half_t> ? __shfl(v, (int)(16u * j + (threadIdx.x & 15u))) : 1.0f; }
+    // acc[i][j] of group g's rows += factor times the product of one step.  Rows of
+    // other groups keep theirs, whatever this group's weights hold.
+    template <uint32_t kN, uint32_t kFP, uint32_t kFQ>
+    __device__ __forceinline__ void add_group(floatx4 (&acc)[kFP][kFQ], uint32_t i0, const x8 (&fp)[kN], const x8 (&fq)[kFQ], uint64_t those, float power, float scale) const {
+#pragma unroll
+        for (uint32_t j = 0; j < kFQ; ++j) {
+            const uint32_t rows = (uint32_t)(those >> (16u * j)) & 0xFFFFu;
+            if (rows == 0u) continue;
+            const float factor = of_row(power, j) * scale;
+            const bool member  = rows >> (threadIdx.x & 15u) & 1u;
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) {
+                const floatx4 part = Vec<T>::mfma(fp[i], fq[j], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                for (uint32_t r = 0; r < 4u; ++r) acc[i0 + i][j][r] = member ? acc[i0 + i][j][r] + factor * part[r] : acc[i0 + i][j][r];
+            }
+        }
+    }
+
     // acc[i][j]: 16 outputs from p0 + 16 i at 16 positions from q0 + 16 j, four
     // consecutive outputs of position lane % 16 a lane; zeros before.
     template <uint32_t kFP, uint32_t kFQ>
-    __device__ __forceinline__ void begin(floatx4 (&acc)[kFP][kFQ], uint32_t p0, uint32_t q0, uint32_t share, uint32_t shares) const {
-        const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, quarter = lane >> 4;
+    __device__ __forceinline__ void begin(floatx4 (&acc)[kFP][kFQ], uint32_t p0, uint32_t q0) const {
         static_assert(16u * kFQ <= 64u);
-        const uint32_t chunks = (rank + 7u) / 8u, steps = (pieces * chunks + 3u) / 4u;
-        // The rows' values for the first step, whatever their groups.
-        floatx8 values[kFQ];
-        auto fetch = [&](uint32_t s) {
-            const uint32_t chunk = 4u * s + quarter, piece = chunk / chunks, r0 = 8u * (chunk - piece * chunks);
-#pragma unroll
-            for (uint32_t j = 0; j < kFQ; ++j) values[j] = low_eight(q0 + 16u * j + l, piece < pieces ? r0 : rank);
-        };
         // The widest tiles' sums leave few registers: values are fetched as they are used.
         constexpr bool kTight = kFP * kFQ >= 32u;
-        if (!kTight) fetch(0u);
-        // The group of position q0 + lane: that of q0, and one more for every offset up
-        // to the position.  (before: offsets up to q0.)
-        const uint32_t before = count_at_most(G.count, q0, [&](uint32_t g) { return G.offset(g); });
-        uint32_t mine = before;
-        const uint32_t q_last = q0 + 16u * kFQ - 1u;
-        for (uint32_t first = before; first <= G.count; first += 64u) {
-            const uint32_t next = first + lane <= G.count ? G.offset(first + lane) : kNoRow;
-            const uint32_t some = (uint32_t)__popcll(__ballot(next <= q_last));
-            for (uint32_t c = 0; c < some; ++c) mine += (uint32_t)__builtin_amdgcn_readlane((int)next, (int)c) <= q0 + lane;
-            if (some < 64u) break;
-        }
-        mine = lane < 16u * kFQ && q0 + lane < G.rows && mine != 0u && mine <= G.count ? mine - 1u : kNoRow;
+        floatx8 values[kFQ];
+        if (!kTight) fetch(values, q0, 0u);
+        const uint32_t mine = group_of_lane(ask_offset(), q0, 16u * kFQ);
         if (__ballot(mine != kNoRow) == 0ull) return;
-        // A power of two for the row of position q0 + lane, and its inverse.
-        float power = 1.0f, inverse = 1.0f;
-        if constexpr (std::is_same_v<T, half_t>) {
-            const float* at = low + (uint64_t)min(q0 + lane, G.rows - 1u) * rank;
-            float most = 0.0f;
-            if (vec_low) {
-                for (uint32_t r = 0; r < rank; r += 8u) {
-                    const floatx4 v = *reinterpret_cast<const floatx4*>(at + r), w = *reinterpret_cast<const floatx4*>(at + r + 4u);
-#pragma unroll
-                    for (uint32_t e = 0; e < 4u; ++e) most = fmaxf(most, fmaxf(fabsf(v[e]), fabsf(w[e])));
-                }
-            } else {
-#pragma unroll 4
-                for (uint32_t r = 0; r < rank; ++r) most = fmaxf(most, fabsf(at[r]));
-            }
-            const Power two = power_of(most);
-            power           = two.value;
-            inverse         = two.inverse;
-        }
-        auto of_row = [&](float v, uint32_t j) { return std::is_same_v<T, half_t> ? __shfl(v, (int)(16u * j + l)) : 1.0f; };
-        for (uint32_t s = 0; s < steps; ++s) {
-            const uint32_t chunk = 4u * s + quarter, piece = chunk / chunks, r0 = 8u * (chunk - piece * chunks);
+        const Power power = power_of_lane(q0);
+        for (uint32_t s = 0; s < steps(); ++s) {
+            const Step step = step_of(s);
             x8 fq[kFQ];
-            if (kTight) fetch(s);
+            if (kTight) fetch(values, q0, s);
 #pragma unroll
-            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = piece_of(values[j] * of_row(inverse, j), piece < pieces ? piece : 0u);
-            if (!kTight && s + 1u < steps) fetch(s + 1u);
+            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = piece_of(values[j] * of_row(power.inverse, j), step.piece);
+            if (!kTight && s + 1u < steps()) fetch(values, q0, s + 1u);
             // The groups of the wave's rows, one after another.
-            uint64_t left = __ballot(mine != kNoRow);
-            for (uint32_t turn = 0; left; ++turn) {
+            for (uint64_t left = __ballot(mine != kNoRow); left;) {
                 const uint32_t g = (uint32_t)__builtin_amdgcn_readlane((int)mine, __builtin_ctzll(left));
                 const uint64_t those = __ballot(mine == g);
                 left &= ~those;
-                if (turn % shares != share) continue;
                 const float scale = scales ? scales[g] : 1.0f;
                 constexpr uint32_t kAtOnce = kTight ? 1u : kFP;
 #pragma unroll
                 for (uint32_t i0 = 0; i0 < kFP; i0 += kAtOnce) {
                     x8 fp[kAtOnce];
 #pragma unroll
-                    for (uint32_t i = 0; i < kAtOnce; ++i) fp[i] = wide_eight(g, p0 + 16u * (i0 + i) + l, piece < pieces ? r0 : rank);
-#pragma unroll
-                    for (uint32_t j = 0; j < kFQ; ++j) {
-                        const uint32_t rows = (uint32_t)(those >> (16u * j)) & 0xFFFFu;
-                        if (rows == 0u) continue;
-                        const float factor = of_row(power, j) * scale;
-                        const bool member  = rows >> l & 1u;
-#pragma unroll
-                        for (uint32_t i = 0; i < kAtOnce; ++i) {
-                            const floatx4 part = Vec<T>::mfma(fp[i], fq[j], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
-                            // Rows of other groups keep theirs, whatever this group's weights hold.
-#pragma unroll
-                            for (uint32_t r = 0; r < 4u; ++r) acc[i0 + i][j][r] = member ? acc[i0 + i][j][r] + factor * part[r] : acc[i0 + i][j][r];
-                        }
-                    }
+                    for (uint32_t i = 0; i < kAtOnce; ++i) fp[i] = wide_eight(g, p0 + 16u * (i0 + i) + (threadIdx.x & 15u), step.r0);
+                    add_group(acc, i0, fp, fq, those, power.value, scale);
                 }
             }
+        }
+    }
+
+    // The same by several waves that add to the same sums, each its share of the
+    // groups, in two parts: what is asked for first (the first step of the wave's
+    // first groups) and what is added last.
+    static constexpr uint32_t kAsked = 4u;
+    template <uint32_t kFP, uint32_t kFQ>
+    struct Asked {
+        uint32_t offset, mine;
+        floatx8 values[kFQ];
+        Power power;
+        x8 fp[kAsked][kFP];
+        float scale[kAsked];
+    };
+    // The wave's groups: turn(number among them, group, its rows).
+    template <typename Turn>
+    __device__ __forceinline__ void for_groups(uint32_t mine, uint32_t share, uint32_t shares, Turn turn) const {
+        uint32_t number = 0u, of_wave = 0u;
+        for (uint64_t left = __ballot(mine != kNoRow); left; ++number) {
+            const uint32_t g = (uint32_t)__builtin_amdgcn_readlane((int)mine, __builtin_ctzll(left));
+            const uint64_t those = __ballot(mine == g);
+            left &= ~those;
+            if (number % shares == share) turn(of_wave++, g, those);
+        }
+    }
+    template <uint32_t kFP, uint32_t kFQ>
+    __device__ __forceinline__ Asked<kFP, kFQ> ask(uint32_t q0) const {
+        Asked<kFP, kFQ> a;
+        a.offset = ask_offset();
+        fetch(a.values, q0, 0u);
+        a.power = power_of_lane(q0);
+        return a;
+    }
+    template <uint32_t kFP, uint32_t kFQ>
+    __device__ __forceinline__ void ask_more(Asked<kFP, kFQ>& a, uint32_t p0, uint32_t q0, uint32_t share, uint32_t shares) const {
+        a.mine = group_of_lane(a.offset, q0, 16u * kFQ);
+        const Step step = step_of(0u);
+        for_groups(a.mine, share, shares, [&](uint32_t n, uint32_t g, uint64_t) {
+#pragma unroll
+            for (uint32_t t = 0; t < kAsked; ++t)
+                if (n == t) {
+                    a.scale[t] = scales ? scales[g] : 1.0f;
+#pragma unroll
+                    for (uint32_t i = 0; i < kFP; ++i) a.fp[t][i] = wide_eight(g, p0 + 16u * i + (threadIdx.x & 15u), step.r0);
+                }
+        });
+    }
+    template <uint32_t kFP, uint32_t kFQ>
+    __device__ __forceinline__ void add(floatx4 (&acc)[kFP][kFQ], const Asked<kFP, kFQ>& a, uint32_t p0, uint32_t q0, uint32_t share, uint32_t shares) const {
+        if (__ballot(a.mine != kNoRow) == 0ull) return;
+        for (uint32_t s = 0; s < steps(); ++s) {
+            const Step step = step_of(s);
+            floatx8 values[kFQ];
+            x8 fq[kFQ];
+            if (s) fetch(values, q0, s);
+#pragma unroll
+            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = piece_of((s ? values[j] : a.values[j]) * of_row(a.power.inverse, j), step.piece);
+            for_groups(a.mine, share, shares, [&](uint32_t n, uint32_t g, uint64_t those) {
+                x8 fp[kFP];
+                float scale;
+                if (s == 0u && n < kAsked) {
+#pragma unroll
+                    for (uint32_t t = 0; t < kAsked; ++t)
+                        if (n == t) {
+                            scale = a.scale[t];
+#pragma unroll
+                            for (uint32_t i = 0; i < kFP; ++i) fp[i] = a.fp[t][i];
+                        }
+                } else {
+                    scale = scales ? scales[g] : 1.0f;
+#pragma unroll
+                    for (uint32_t i = 0; i < kFP; ++i) fp[i] = wide_eight(g, p0 + 16u * i + (threadIdx.x & 15u), step.r0);
+                }
+                add_group(acc, 0u, fp, fq, those, a.power.value, scale);
+            });
         }
     }
 };
@@ -205,14 +309,12 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_adapter(GatheredOperands A,
 }
 
 // The same with few tiles: the waves share the groups.
-template <typename T, uint32_t kF, bool kPT, bool kWords, bool kGather, typename Out>
+template <typename T, uint32_t kFP, uint32_t kFQ, bool kPT, bool kWhole, typename Out>
 __global__ __launch_bounds__(kFewWaves * 64u) void k_adapter_few(GatheredOperands A, Out out, LowRank<T, kPT> more) {
-    __shared__ floatx4 lds[few_lds(kF) / 16u];
-    __shared__ uint32_t rows[16u * kF];
-    const Place at{blockIdx.x % A.tiles_p * 16u * kF, blockIdx.x / A.tiles_p * 16u * kF, 0u, A.nk, 0u, 0u};
-    find_rows<16u * kF>(out, rows, at.q0, A.nq);
-    __syncthreads();
-    few_tile<T, kF, kPT, false, kWords, kGather>(A, out, at, reinterpret_cast<char*>(lds), nullptr, more);
+    __shared__ floatx4 lds[few_lds(kFP, kFQ) / 16u];
+    __shared__ uint32_t rows[16u * kFQ];
+    const Place at{blockIdx.x % A.tiles_p * 16u * kFP, blockIdx.x / A.tiles_p * 16u * kFQ, 0u, A.nk, 0u, 0u};
+    few_tile<T, kFP, kFQ, kPT, false, !kWhole, true, kWhole>(A, out, at, reinterpret_cast<char*>(lds), nullptr, rows, more);
 }
 
 // Many rows, at most 32 kKS <= 256 k and 16 kRB <= 64 ranks, whole chunks: both
@@ -656,15 +758,19 @@ hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& mo
     const bool gather = A.q_index != nullptr;
     const bool words  = !whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, A.nk) || (gather && !near(A.q_count, A.ldq));
     const uint64_t cus = device_cu_count();
-    auto tiles         = [&](uint32_t b) { return (uint64_t)ceil_div(A.np, b) * ceil_div(A.nq, b); };
+    auto tiles_of      = [&](uint32_t p, uint32_t q) { return (uint64_t)ceil_div(A.np, p) * ceil_div(A.nq, q); };
+    auto tiles         = [&](uint32_t b) { return tiles_of(b, b); };
     if (A.nk <= kFewMaxK) {
-        auto few = [&](auto f, bool as_words) {
-            if (as_words) return launch(k_adapter_few<T, f(), kPT, true, true, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
-            return launch(k_adapter_few<T, f(), kPT, false, true, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
+        auto few = [&](auto fp, auto fq) {
+            const bool whole = A.nk % 32u == 0u && (!kPT || A.np % (16u * fp()) == 0u) && !odd_rows(A.p, A.ldp) && !odd_rows(A.q, A.ldq);
+            if (whole) return launch(k_adapter_few<T, fp(), fq(), kPT, true, Out>, 16u * fp(), 16u * fq(), kFewWaves * 64u);
+            return launch(k_adapter_few<T, fp(), fq(), kPT, false, Out>, 16u * fp(), 16u * fq(), kFewWaves * 64u);
         };
-        const bool odd = odd_rows(A.p, A.ldp) || odd_rows(A.q, A.ldq);
-        if (tiles(16u) <= 2u * cus) return few(std::integral_constant<uint32_t, 1u>{}, odd);
-        if (tiles(32u) <= 2u * cus) return few(std::integral_constant<uint32_t, 2u>{}, odd);
+        using One = std::integral_constant<uint32_t, 1u>;
+        using Two = std::integral_constant<uint32_t, 2u>;
+        if (tiles(16u) <= cus) return few(One{}, One{});
+        if (tiles_of(16u, 32u) <= cus) return few(One{}, Two{});
+        if (tiles(32u) <= 2u * cus) return few(Two{}, Two{});
     }
     const bool by_128 = A.np > 64u && A.nq > 64u && tiles(128u) >= cus;
     if (words) return by_128 ? launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kByWords, true, Out>, 128u, 128u, 256u) : launch(k_adapter<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);

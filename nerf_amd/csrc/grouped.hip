@@ -28,19 +28,17 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_grouped(GatheredOperands A,
     product<T, kBP, kBQ, kWP, kWQ, kDepth, kPT, false, kMode, kGather>(A, out, Place{tile.tile_p * kBP, part.q0, 0u, A.nk, kPT ? 0u : part.group * A.np, kPT ? part.group * A.nk : 0u});
 }
 
-// The same with few tiles.
-template <typename T, uint32_t kF, bool kPT, bool kWords, bool kGather, typename Out>
+// The same with few tiles; kWhole: whole steps and rows that start at even values.
+template <typename T, uint32_t kF, bool kPT, bool kWhole, typename Out>
 __global__ __launch_bounds__(kFewWaves * 64u) void k_grouped_few(GatheredOperands A, Out out, Groups G, Parts parts) {
-    __shared__ floatx4 lds[few_lds(kF) / 16u];
+    __shared__ floatx4 lds[few_lds(kF, kF) / 16u];
     __shared__ uint32_t rows[kHasRows<Out> ? 16u * kF : 1u];
     const GroupTile tile = group_tile(G, 16u * kF, A.tiles_p, parts.by_position, parts.most);
     const Part& part = tile.part;
     if (part.q0 >= part.end) return;
-    find_rows<16u * kF>(out, rows, part.q0, part.end);
-    __syncthreads();
     out.of_group(part.group);
     out.nq = A.nq = part.end;
-    few_tile<T, kF, kPT, false, kWords, kGather>(A, out, Place{tile.tile_p * 16u * kF, part.q0, 0u, A.nk, kPT ? 0u : part.group * A.np, kPT ? part.group * A.nk : 0u}, reinterpret_cast<char*>(lds), nullptr);
+    few_tile<T, kF, kF, kPT, false, !kWhole, true, kWhole>(A, out, Place{tile.tile_p * 16u * kF, part.q0, 0u, A.nk, kPT ? 0u : part.group * A.np, kPT ? part.group * A.nk : 0u}, reinterpret_cast<char*>(lds), nullptr, rows);
 }
 
 // Weights or rows of fewer than eight values in all: a thread computes eight
@@ -151,13 +149,13 @@ hipError_t launch_grouped(GatheredOperands A, Out out, const Groups& G, hipStrea
     // Tiles that the rows make, group by group.
     auto tiles = [&](uint32_t b) { return (uint64_t)ceil_div(A.np, b) * parts_of(G.rows, G.count, b).most; };
     if (A.nk <= kFewMaxK) {
-        auto few = [&](auto f, bool as_words) {
-            if (as_words) return launch(k_grouped_few<T, f(), kPT, true, true, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
-            return launch(k_grouped_few<T, f(), kPT, false, true, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
+        auto few = [&](auto f) {
+            const bool whole = A.nk % 32u == 0u && (!kPT || A.np % (16u * f()) == 0u) && !odd_rows(A.p, A.ldp) && !odd_rows(A.q, A.ldq) && ((uint64_t)A.np * A.nk) % 2u == 0u;
+            if (whole) return launch(k_grouped_few<T, f(), kPT, true, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
+            return launch(k_grouped_few<T, f(), kPT, false, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
         };
-        const bool odd = odd_rows(A.p, A.ldp) || odd_rows(A.q, A.ldq) || ((uint64_t)A.np * A.nk) % 2u;
-        if (tiles(16u) <= 2u * cus) return few(std::integral_constant<uint32_t, 1u>{}, odd);
-        if (tiles(32u) <= 2u * cus) return few(std::integral_constant<uint32_t, 2u>{}, odd);
+        if (tiles(16u) <= 2u * cus) return few(std::integral_constant<uint32_t, 1u>{});
+        if (tiles(32u) <= 2u * cus) return few(std::integral_constant<uint32_t, 2u>{});
     }
     const uint32_t mean = G.rows / G.count;
     if constexpr (!kHasRows<Out>) {

@@ -185,21 +185,21 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
 
 template <typename T, uint32_t kF, bool kWords>
 __global__ __launch_bounds__(kFewWaves * 64u) void k_few_forward(Operands A, ForwardOut<T> out) {
-    __shared__ floatx4 lds[few_lds(kF) / 16u];
-    few_tile<T, kF, false, false, kWords>(A, out, Place{blockIdx.x * 16u * kF, blockIdx.y * 16u * kF, 0u, A.nk, 0u, 0u}, reinterpret_cast<char*>(lds), nullptr);
+    __shared__ floatx4 lds[few_lds(kF, kF) / 16u];
+    few_tile<T, kF, kF, false, false, kWords>(A, out, Place{blockIdx.x * 16u * kF, blockIdx.y * 16u * kF, 0u, A.nk, 0u, 0u}, reinterpret_cast<char*>(lds), nullptr);
 }
 
 // Both gradients in one launch: first the tiles of dx, x_tiles across and
 // x_blocks in all, then those of dW.
 template <typename T, uint32_t kF, bool kWords>
 __global__ __launch_bounds__(kFewWaves * 64u) void k_few_backward(Operands X, InputGradientOut<T> x_out, uint32_t x_tiles, uint32_t x_blocks, Operands W, SumOut w_out, uint32_t w_tiles) {
-    __shared__ floatx4 lds[few_lds(kF) / 16u];
+    __shared__ floatx4 lds[few_lds(kF, kF) / 16u];
     __shared__ float lds_sums[kFewWaves * 16u * kF];
     if (blockIdx.x < x_blocks) {
-        few_tile<T, kF, true, false, kWords>(X, x_out, Place{blockIdx.x % x_tiles * 16u * kF, blockIdx.x / x_tiles * 16u * kF, 0u, X.nk, 0u, 0u}, reinterpret_cast<char*>(lds), nullptr);
+        few_tile<T, kF, kF, true, false, kWords>(X, x_out, Place{blockIdx.x % x_tiles * 16u * kF, blockIdx.x / x_tiles * 16u * kF, 0u, X.nk, 0u, 0u}, reinterpret_cast<char*>(lds), nullptr);
     } else {
         const uint32_t b = blockIdx.x - x_blocks;
-        few_tile<T, kF, true, true, kWords>(W, w_out, Place{b % w_tiles * 16u * kF, b / w_tiles * 16u * kF, 0u, W.nk, 0u, 0u}, reinterpret_cast<char*>(lds), lds_sums);
+        few_tile<T, kF, kF, true, true, kWords>(W, w_out, Place{b % w_tiles * 16u * kF, b / w_tiles * 16u * kF, 0u, W.nk, 0u, 0u}, reinterpret_cast<char*>(lds), lds_sums);
     }
 }
 

@@ -659,11 +659,15 @@ __device__ __forceinline__ uint32_t chip_tile(uint32_t b, uint32_t n) {
 // tile's first fragments read a barrier ahead, took 493.  Where they are narrow the
 // memory does: the weights' gradient of 262144 x 256 -> 256 69 us = 3.9 TB/s.
 // kGather: lines in another order (Ops = GatheredOperands).  more.begin() gives what the
-// sums begin with, while the first tiles are on their way (by several waves that
-// add to the same ones: each its share).
+// sums begin with, while the first tiles are on their way.
 enum Mode : uint32_t { kDirect, kByChunks, kByWords };
 struct NothingMore {
     static constexpr bool kOn = false;
+    template <uint32_t kFP, uint32_t kFQ>
+    __device__ __forceinline__ uint32_t ask(uint32_t) const { return 0u; }
+    __device__ __forceinline__ void ask_more(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) const {}
+    template <uint32_t kFP, uint32_t kFQ>
+    __device__ __forceinline__ void add(floatx4 (&)[kFP][kFQ], uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) const {}
 };
 template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, bool kQT, Mode kMode, bool kGather = false, typename Ops, typename Out, typename More = NothingMore>
 __device__ __forceinline__ void product(const Ops& A, Out out, const Place& at, const More& more = {}) {
@@ -766,7 +770,7 @@ __device__ __forceinline__ void product(const Ops& A, Out out, const Place& at, 
         };
         auto before = [&] {
             keep_bias();
-            if constexpr (More::kOn) more.template begin<kFP, kFQ>(acc, p0 + wp, q0 + wq, 0u, 1u);
+            if constexpr (More::kOn) more.template begin<kFP, kFQ>(acc, p0 + wp, q0 + wq);
         };
         constexpr int kStep = (int)kBK;
         int left            = (int)(k_end - k0);
@@ -824,7 +828,7 @@ __device__ __forceinline__ void product(const Ops& A, Out out, const Place& at, 
         for (uint32_t d = 0; d < kDepth - 1u; ++d)
             if (k0 + kBK * d < k_end) fetch(d, k0 + kBK * d);
         keep_bias();
-        if constexpr (More::kOn) more.template begin<kFP, kFQ>(acc, p0 + wp, q0 + wq, 0u, 1u);
+        if constexpr (More::kOn) more.template begin<kFP, kFQ>(acc, p0 + wp, q0 + wq);
         for (uint32_t k = k0; k < k_end; k += kBK * (kDepth - 1u)) {
 #pragma unroll
             for (uint32_t d = 0; d < kDepth - 1u; ++d) {
@@ -892,7 +896,7 @@ __device__ __forceinline__ void product(const Ops& A, Out out, const Place& at, 
 // --------------------------------------------------------------- few tiles
 // Products of too few outputs to occupy the card by tiles: what counts is the
 // time of one workgroup and the number of launches.  A workgroup has a tile of
-// 16 kF x 16 kF outputs, its eight waves every eighth 32 k each; a wave fetches
+// 16 kFP x 16 kFQ outputs, its eight waves every eighth 32 k each; a wave fetches
 // its operands from memory itself, several steps at a time and without waiting
 // for the others, and the eight sums are added in LDS in their order.  (A
 // launch costs the host 3.5 us, about what such a kernel takes; one with 64 x 64
@@ -904,8 +908,11 @@ constexpr uint32_t kFewWaves = 8u, kFewMaxK = 4096u;
 // 16 kF rows x 32 k of an operand, any alignment, on its way to one wave; the
 // edges as Stager has them.  Rows outside are other rows: their products are in
 // outputs that nothing reads.
-// kGather: rows in another order, as begin() finds them.
-template <typename T, uint32_t kF, bool kT, bool kWords, bool kGather = false>
+// kGather: rows in another order, the lane's in `rows`.  kWhole: no edges (whole steps
+// of k, and of rows where those are contiguous), and none of their code, which a
+// kernel that runs through its own once waits for: 32 rows of 32 adapters, 4096 ->
+// 4096, 21 us with it.
+template <typename T, uint32_t kF, bool kT, bool kWords, bool kGather = false, bool kWhole = false>
 struct FewOperand {
     static_assert(!kGather || !kT);
     using x8 = typename Vec<T>::x8;
@@ -913,12 +920,9 @@ struct FewOperand {
     Eight<kWords> held[kF];
     uint32_t rows[kGather ? kF : 1u];
 
-    __device__ __forceinline__ void begin(const uint32_t* index, uint32_t count, uint32_t n, uint32_t row0) {
-#pragma unroll
-        for (uint32_t i = 0; i < kF; ++i) rows[i] = gathered_row(index, count, row0 + 16u * i + (threadIdx.x & 15u), n);
-    }
-    static __device__ __forceinline__ uint64_t own(uint32_t i, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0) {
+    __device__ __forceinline__ uint64_t own(uint32_t i, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0) const {
         const uint32_t lane = threadIdx.x & 63u;
+        if constexpr (kGather) return (uint64_t)(rows[i] == kNoRow ? 0u : rows[i]) * ld + k0 + 8u * (lane >> 4);
         if (kT) return (uint64_t)(k0 + (i * 64u + lane) / kChunks) * ld + row0 + 8u * ((i * 64u + lane) % kChunks);
         return (uint64_t)min(row0 + 16u * i + (lane & 15u), n - 1u) * ld + k0 + 8u * (lane >> 4);
     }
@@ -928,7 +932,7 @@ struct FewOperand {
         if (kT) return edge(ld, k0 + (i * 64u + lane) / kChunks, nk, row0 + 8u * ((i * 64u + lane) % kChunks), n);
         return edge(ld, min(row0 + 16u * i + (lane & 15u), n - 1u), n, k0 + 8u * (lane >> 4), nk);
     }
-    static __device__ __forceinline__ bool inner(uint32_t n, uint32_t nk, uint32_t row0, uint32_t k0) { return !kGather && k0 + 32u <= nk && (!kT || row0 + 16u * kF <= n); }
+    static __device__ __forceinline__ bool inner(uint32_t n, uint32_t nk, uint32_t row0, uint32_t k0) { return kWhole || (k0 + 32u <= nk && (!kT || row0 + 16u * kF <= n)); }
 
     __device__ __forceinline__ void fetch(uint32_t nk, const T* __restrict__ src, uint64_t ld, uint32_t n, uint32_t row0, uint32_t k0) {
         uint64_t at[kF];
@@ -947,7 +951,10 @@ struct FewOperand {
         uint4 v[kF];
         if (inner(n, nk, row0, k0)) {
 #pragma unroll
-            for (uint32_t i = 0; i < kF; ++i) v[i] = held[i].value(first + (uint32_t)own(i, ld, n, row0, k0));
+            for (uint32_t i = 0; i < kF; ++i) {
+                v[i] = held[i].value(first + (uint32_t)own(i, ld, n, row0, k0));
+                if (kGather && rows[i] == kNoRow) v[i] = uint4{0u, 0u, 0u, 0u};
+            }
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < kF; ++i) {
@@ -981,14 +988,14 @@ struct FewOperand {
     }
 };
 
-constexpr uint32_t few_lds(uint32_t f) { return kFewWaves * std::max(16u * f * 16u * f * 4u, 2048u * f); }
+constexpr uint32_t few_lds(uint32_t fp, uint32_t fq) { return kFewWaves * std::max(16u * fp * 16u * fq * 4u, 1024u * (fp + fq)); }
 
-template <typename T, uint32_t kF, bool kPT, bool kQT, bool kWords, bool kGather = false, typename Ops, typename Out, typename More = NothingMore>
-__device__ __forceinline__ void few_tile(const Ops& A, const Out& out, const Place& at, char* lds, float* lds_sums, const More& more = {}) {
+template <typename T, uint32_t kFP, uint32_t kFQ, bool kPT, bool kQT, bool kWords, bool kGather = false, bool kWhole = false, typename Ops, typename Out, typename More = NothingMore>
+__device__ __forceinline__ void few_tile(const Ops& A, Out out, const Place& at, char* lds, float* lds_sums, uint32_t* lds_rows = nullptr, const More& more = {}) {
     const uint32_t p0 = at.p0, q0 = at.q0;
     constexpr bool kSums = std::is_same_v<Out, SumOut>;
-    constexpr uint32_t kDepth = kF == 1u ? 8u : kF == 2u ? 3u : 2u;  // steps on their way
-    constexpr uint32_t kSP = 16u * kF, kEights = 16u * kF * kSP / 8u;
+    constexpr uint32_t kDepth = kFP * kFQ <= 2u ? 8u : kFP * kFQ == 4u ? 3u : 2u;  // steps on their way
+    constexpr uint32_t kSP = 16u * kFP, kEights = 16u * kFQ * kSP / 8u;
     using x8 = typename Vec<T>::x8;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
 
@@ -996,71 +1003,94 @@ __device__ __forceinline__ void few_tile(const Ops& A, const Out& out, const Pla
     const uint32_t row = threadIdx.x / (kSP / 8u), col = 8u * (threadIdx.x % (kSP / 8u)), p = p0 + col;
     const uint32_t n = threadIdx.x < kEights && q0 + row < out.nq && p < out.np ? min(8u, out.np - p) : 0u;
     floatx8 bias = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (Out::kBias) {
-        if (out.bias) {
+    typename Out::Aux aux;
+    auto ask_outputs = [&] {
+        if constexpr (Out::kBias) {
+            if (out.bias) {
 #pragma unroll
-            for (uint32_t r = 0; r < 8u; ++r) bias[r] = r < n ? out.bias[p + r] : 0.0f;
+                for (uint32_t r = 0; r < 8u; ++r) bias[r] = r < n ? out.bias[p + r] : 0.0f;
+            }
         }
-    }
-    const typename Out::Aux aux = out.load(q0, row, p, n);
+        aux = out.load(q0, row, p, n);
+    };
+    if constexpr (!kGather) ask_outputs();
 
-    floatx4 acc[kF][kF], sums[kF];
+    floatx4 acc[kFP][kFQ], sums[kFQ];
 #pragma unroll
-    for (uint32_t j = 0; j < kF; ++j) {
+    for (uint32_t j = 0; j < kFQ; ++j) {
         sums[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (uint32_t i = 0; i < kF; ++i) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t i = 0; i < kFP; ++i) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const bool take_sums = kSums && p0 == 0u;
     x8 ones;
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = (T)1.0f;
-    FewOperand<T, kF, kPT, kWords> op[kDepth];
-    FewOperand<T, kF, kQT, kWords, kGather> oq[kDepth];
-    if constexpr (kGather) {
-#pragma unroll
-        for (uint32_t d = 0; d < kDepth; ++d) oq[d].begin(A.q_index, A.q_count, A.nq, q0);
-    }
-    char* mine = lds + wave * 2048u * kF;
+    FewOperand<T, kFP, kPT, kWords, false, kWhole> op[kDepth];
+    FewOperand<T, kFQ, kQT, kWords, kGather, kWhole> oq[kDepth];
+    char* mine = lds + wave * 1024u * (kFP + kFQ);
     auto fetch = [&](uint32_t d, uint32_t k) {
         op[d].fetch(A.nk + at.p_k, (const T*)A.p, A.ldp, at.p_line + A.np, at.p_line + p0, k + at.p_k);
         oq[d].fetch(A.nk, (const T*)A.q, A.ldq, A.nq, q0, k);
     };
     constexpr uint32_t kStride = 32u * kFewWaves;
+    auto ask_steps = [&](auto one) {
 #pragma unroll
-    for (uint32_t d = 0; d < kDepth; ++d)
-        if (32u * wave + kStride * d < A.nk) fetch(d, 32u * wave + kStride * d);
-    if constexpr (More::kOn) more.template begin<kF, kF>(acc, p0, q0, wave, kFewWaves);
+        for (uint32_t d = 0; d < kDepth; ++d)
+            if (32u * wave + kStride * d < A.nk) one(d, 32u * wave + kStride * d);
+    };
+    // Loads come back in their order, so what addresses are made of is asked for
+    // first, then what needs no address from memory, and then the rest; what else
+    // belongs to the sums is added last.
+    auto asked = more.template ask<kFP, kFQ>(q0);
+    if constexpr (kGather) {
+        uint32_t rows[kFQ];
+#pragma unroll
+        for (uint32_t j = 0; j < kFQ; ++j) rows[j] = ask_row(A.q_index, q0 + 16u * j + (lane & 15u), A.nq);
+        ask_steps([&](uint32_t d, uint32_t k) { op[d].fetch(A.nk + at.p_k, (const T*)A.p, A.ldp, at.p_line + A.np, at.p_line + p0, k + at.p_k); });
+#pragma unroll
+        for (uint32_t j = 0; j < kFQ; ++j)
+#pragma unroll
+            for (uint32_t d = 0; d < kDepth; ++d) oq[d].rows[j] = judge_row(rows[j], A.q_count, q0 + 16u * j + (lane & 15u), A.nq);
+        ask_steps([&](uint32_t d, uint32_t k) { oq[d].fetch(A.nk, (const T*)A.q, A.ldq, A.nq, q0, k); });
+        more.ask_more(asked, p0, q0, wave, kFewWaves);
+        find_rows<16u * kFQ>(out, lds_rows, q0, out.nq);
+        __syncthreads();
+        ask_outputs();
+    } else {
+        ask_steps(fetch);
+    }
     for (uint32_t k = 32u * wave; k < A.nk; k += kStride * kDepth) {
 #pragma unroll
         for (uint32_t d = 0; d < kDepth; ++d) {
             const uint32_t kd = k + kStride * d;
             if (kd < A.nk) {
-                x8 fp[kF], fq[kF];
+                x8 fp[kFP], fq[kFQ];
                 op[d].take(A.nk + at.p_k, (const T*)A.p, A.ldp, at.p_line + A.np, at.p_line + p0, kd + at.p_k, mine, fp);
-                oq[d].take(A.nk, (const T*)A.q, A.ldq, A.nq, q0, kd, mine + 1024u * kF, fq);
+                oq[d].take(A.nk, (const T*)A.q, A.ldq, A.nq, q0, kd, mine + 1024u * kFP, fq);
                 if (kd + kStride * kDepth < A.nk) fetch(d, kd + kStride * kDepth);
 #pragma unroll
-                for (uint32_t i = 0; i < kF; ++i)
+                for (uint32_t i = 0; i < kFP; ++i)
 #pragma unroll
-                    for (uint32_t j = 0; j < kF; ++j) acc[i][j] = Vec<T>::mfma(fp[i], fq[j], acc[i][j]);
+                    for (uint32_t j = 0; j < kFQ; ++j) acc[i][j] = Vec<T>::mfma(fp[i], fq[j], acc[i][j]);
                 if (take_sums) {
 #pragma unroll
-                    for (uint32_t j = 0; j < kF; ++j) sums[j] = Vec<T>::mfma(ones, fq[j], sums[j]);
+                    for (uint32_t j = 0; j < kFQ; ++j) sums[j] = Vec<T>::mfma(ones, fq[j], sums[j]);
                 }
             }
         }
     }
 
+    more.add(acc, asked, p0, q0, wave, kFewWaves);
     __syncthreads();  // the waves' own pieces become those of the sums
     floatx4* strips = reinterpret_cast<floatx4*>(lds);
-    constexpr uint32_t kStrip = 16u * kF * kSP / 4u;
+    constexpr uint32_t kStrip = 16u * kFQ * kSP / 4u;
 #pragma unroll
-    for (uint32_t j = 0; j < kF; ++j) {
+    for (uint32_t j = 0; j < kFQ; ++j) {
         const uint32_t r = 16u * j + (lane & 15u);
 #pragma unroll
-        for (uint32_t i = 0; i < kF; ++i) strips[wave * kStrip + r * (kSP / 4u) + ((4u * i + (lane >> 4)) ^ (r & 3u))] = acc[i][j];
-        if (take_sums && lane < 16u) lds_sums[wave * 16u * kF + r] = sums[j][0];
+        for (uint32_t i = 0; i < kFP; ++i) strips[wave * kStrip + r * (kSP / 4u) + ((4u * i + (lane >> 4)) ^ (r & 3u))] = acc[i][j];
+        if (take_sums && lane < 16u) lds_sums[wave * 16u * kFQ + r] = sums[j][0];
     }
     __syncthreads();
     if (threadIdx.x < kEights) {
@@ -1073,10 +1103,10 @@ __device__ __forceinline__ void few_tile(const Ops& A, const Out& out, const Pla
         out.put(q0, row, p, n, v, bias, aux);
     }
     if constexpr (kSums) {
-        if (take_sums && out.row_sums && threadIdx.x < 16u * kF && q0 + threadIdx.x < out.nq) {
+        if (take_sums && out.row_sums && threadIdx.x < 16u * kFQ && q0 + threadIdx.x < out.nq) {
             float v = 0.0f;
 #pragma unroll
-            for (uint32_t w = 0; w < kFewWaves; ++w) v += lds_sums[w * 16u * kF + threadIdx.x];
+            for (uint32_t w = 0; w < kFewWaves; ++w) v += lds_sums[w * 16u * kFQ + threadIdx.x];
             out.row_sums[q0 + threadIdx.x] = v;
         }
     }
