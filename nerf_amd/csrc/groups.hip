@@ -16,7 +16,8 @@ using namespace nerf_hip;
 
 namespace {
 
-constexpr uint32_t kThreads = 1024u, kWaves = kThreads / 64u, kEach = 4u, kTurn = kThreads * kEach;  // rows a turn
+constexpr uint32_t kThreads = 1024u, kWaves = kThreads / 64u;
+constexpr uint32_t kEach = 4u, kTurn = kThreads * kEach;  // rows a turn; where one workgroup does all, twice as many
 constexpr uint32_t kOneRows = 16384u;
 
 // Counters of a workgroup: where the next row of an id goes, and how many of a
@@ -59,10 +60,11 @@ __device__ __forceinline__ void sums_before(uint32_t bins, uint32_t* lds_waves, 
 }
 
 // Rows [row0, row_end): their ids, counted into `counts` (LDS, cleared here).
+template <uint32_t kEach>
 __device__ __forceinline__ void count_rows(const uint32_t* __restrict__ ids, uint32_t row0, uint32_t row_end, uint32_t groups, uint32_t* counts) {
     for (uint32_t b = threadIdx.x; b <= groups; b += kThreads) counts[b] = 0u;
     __syncthreads();
-    for (uint64_t base = row0; base < row_end; base += kTurn) {
+    for (uint64_t base = row0; base < row_end; base += kThreads * kEach) {
         uint32_t id[kEach];
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
@@ -77,10 +79,11 @@ __device__ __forceinline__ void count_rows(const uint32_t* __restrict__ ids, uin
 }
 
 // Places of rows [row0, row_end), S.start holding the chunk's first of every id.
-template <uint32_t kBins>
+template <uint32_t kBins, uint32_t kEach>
 __device__ __forceinline__ void place_rows(const uint32_t* __restrict__ ids, uint32_t row0, uint32_t row_end, uint32_t groups, uint32_t* __restrict__ order, uint32_t* __restrict__ place, Counters<kBins>& S) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, words = (groups + 2u) / 2u;
     const uint32_t bits = 32u - (uint32_t)__builtin_clz(groups);  // of ids 0 .. groups
+    constexpr uint32_t kTurn = kThreads * kEach;
     for (uint64_t base = row0; base < row_end; base += kTurn) {
         // A wave has consecutive rows, so that waves and turns are in the rows' order.
         uint32_t id[kEach];
@@ -139,13 +142,13 @@ __global__ __launch_bounds__(kThreads) void k_group_one(const uint32_t* __restri
     __shared__ uint32_t waves[kWaves];
     uint32_t* counts = &S.turn[0][0];
     static_assert((kWaves + 1u) * Counters<kBins>::kWords >= kBins);
-    count_rows(ids, 0u, rows, groups, counts);
+    count_rows<2u * kEach>(ids, 0u, rows, groups, counts);
     sums_before<kThreads>(groups + 1u, waves, [&](uint32_t b) { return counts[b]; }, [&](uint32_t b, uint32_t sum) {
         S.start[b] = sum;
         offsets[b] = sum;
     });
     __syncthreads();
-    place_rows(ids, 0u, rows, groups, order, place, S);
+    place_rows<kBins, 2u * kEach>(ids, 0u, rows, groups, order, place, S);
 }
 
 // What the passes of more rows leave for each other.
@@ -159,7 +162,7 @@ template <uint32_t kBins>
 __global__ __launch_bounds__(kThreads) void k_group_count(const uint32_t* __restrict__ ids, Passes P) {
     __shared__ uint32_t counts[kBins];
     const uint32_t row0 = blockIdx.x * P.chunk;
-    count_rows(ids, row0, min(P.rows, row0 + P.chunk), P.groups, counts);
+    count_rows<kEach>(ids, row0, min(P.rows, row0 + P.chunk), P.groups, counts);
     for (uint32_t b = threadIdx.x; b <= P.groups; b += kThreads) P.counts[(uint64_t)blockIdx.x * (P.groups + 1u) + b] = counts[b];
 }
 
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void k_group_place(const uint32_t* __rest
         if (blockIdx.x == 0u) offsets[b] = sum;
     });
     __syncthreads();
-    place_rows(ids, row0, min(P.rows, row0 + P.chunk), P.groups, order, place, S);
+    place_rows<kBins, kEach>(ids, row0, min(P.rows, row0 + P.chunk), P.groups, order, place, S);
 }
 
 template <uint32_t kBins>
