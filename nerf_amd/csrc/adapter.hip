@@ -206,7 +206,7 @@ struct LowRank {
                 const uint64_t those = __ballot(mine == g);
                 left &= ~those;
                 const float scale = scales ? scales[g] : 1.0f;
-                constexpr uint32_t kAtOnce = kTight ? 1u : kFP;
+                constexpr uint32_t kAtOnce = kTight ? 4u : kFP;
 #pragma unroll
                 for (uint32_t i0 = 0; i0 < kFP; i0 += kAtOnce) {
                     x8 fp[kAtOnce];
