@@ -760,6 +760,10 @@ hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& mo
     const uint64_t cus = device_cu_count();
     auto tiles_of      = [&](uint32_t p, uint32_t q) { return (uint64_t)ceil_div(A.np, p) * ceil_div(A.nq, q); };
     auto tiles         = [&](uint32_t b) { return tiles_of(b, b); };
+    // us of a forward call, few of 16 x 16 / of 16 x 32 / of 32 x 32 / tiles of 64, bf16,
+    // rank 16, 4096 -> 4096: 16 rows 24 / 25 / 28 / 33; 32 rows 35 / 30 / 32 / 38; 64 rows 56 /
+    // 45 / 32 / 36; 128 rows 95 / 76 / 50 / 35; 1024 -> 1024: 64 rows 12 / 13 / 14 / 17, 128
+    // rows 16 / 13 / 14 / 15, 512 rows 43 / 33 / 23 / 15.
     if (A.nk <= kFewMaxK) {
         auto few = [&](auto fp, auto fq) {
             const bool whole = A.nk % 32u == 0u && (!kPT || A.np % (16u * fp()) == 0u) && !odd_rows(A.p, A.ldp) && !odd_rows(A.q, A.ldq);
@@ -770,11 +774,18 @@ hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& mo
         using Two = std::integral_constant<uint32_t, 2u>;
         if (tiles(16u) <= cus) return few(One{}, One{});
         if (tiles_of(16u, 32u) <= cus) return few(One{}, Two{});
-        if (tiles(32u) <= 2u * cus) return few(Two{}, Two{});
+        if (tiles(32u) <= cus) return few(Two{}, Two{});
     }
+    // us, tiles of 64 / of 128: 2048 -> 2048, 2048 rows (1024, 256 tiles) 44 / 39, 8192 rows
+    // 150 / 97; 256 -> 256, 16384 rows (1024, 256) 20.7 / 20.2.
     const bool by_128 = A.np > 64u && A.nq > 64u && tiles(128u) >= cus;
     if (words) return by_128 ? launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kByWords, true, Out>, 128u, 128u, 256u) : launch(k_adapter<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
-    if (A.np > 128u && A.nq > 128u && A.nk >= 512u && tiles(256u) >= cus)
+    // A tile of 256 takes a CU nearly as long as four of 128, so it needs full rounds: us of
+    // a call, 128 / 256, 2048 -> 2048 rank 16, 4096 rows (1 round for 2) 55 / 83, 8192 (1 for
+    // 4) 97 / 94; gradients of 4096 -> 2048, rank 64, 6144 rows (2 for 6) 294 / 323, 8192 (2 for
+    // 8) 374 / 357, 10240 (3 for 10) 445 / 467, 12288 rank 16 (3 for 12) 382 / 352; 512 -> 512,
+    // 65536 rows (2 for 8) 85 / 89.
+    if (A.np > 128u && A.nq > 128u && A.nk >= 1024u && 15u * ((tiles(256u) + cus - 1u) / cus) * cus <= 4u * tiles(128u))
         return gather ? launch(k_adapter<T, 256, 256, 2, 4, 2, kPT, kDirect, true, Out>, 256u, 256u, 512u) : launch(k_adapter<T, 256, 256, 2, 4, 2, kPT, kDirect, false, Out>, 256u, 256u, 512u);
     if (by_128) return gather ? launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kDirect, true, Out>, 128u, 128u, 256u) : launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kDirect, false, Out>, 128u, 128u, 256u);
     return gather ? launch(k_adapter<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_adapter<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
@@ -818,6 +829,7 @@ hipError_t launch_rank_sums(RankSums A, const Groups& G, Workspace ws, hipStream
         k_rank_tiny_sums<T><<<grid_of((G.count * length + 255u) / 256u), 256, 0, stream>>>(A, G);
         return hipGetLastError();
     }
+    // Parts enough for two workgroups a CU; one, four or eight: within 2 %.
     auto launch = [&](auto kernel, uint32_t br) {
         A.tiles_w = ceil_div(A.nw, kBW);
         A.tiles_r = ceil_div(A.nr, br);

@@ -146,26 +146,41 @@ hipError_t launch_grouped(GatheredOperands A, Out out, const Groups& G, hipStrea
     const bool gather = A.q_index != nullptr;
     const bool words  = !whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) || !whole_chunks(A.q, A.ldq, A.nk) || (gather && !near(A.q_count, A.ldq));
     const uint64_t cus = device_cu_count();
-    // Tiles that the rows make, group by group.
-    auto tiles = [&](uint32_t b) { return (uint64_t)ceil_div(A.np, b) * parts_of(G.rows, G.count, b).most; };
+    // Tiles that the rows can make, group by group, and about how many they do.
+    auto tiles   = [&](uint32_t b) { return (uint64_t)ceil_div(A.np, b) * parts_of(G.rows, G.count, b).most; };
+    auto on_mean = [&](uint32_t b) { return (uint64_t)ceil_div(A.np, b) * (G.rows / b + G.count / 2u); };
+    // Fewer tiles than CUs: the k of a tile over a workgroup's waves.  us, few of 16 / of
+    // 32 / tiles of 64, fp16, 4096 -> 1024: 32 rows 1 group (192, 64 tiles) 11 / 18 / 18;
+    // 32 rows 4 groups (384, 160) 18 / 16.5 / 18.6; 64 rows 8 groups (768, 320) 26 / 30 /
+    // 19.  1024 -> 1024: 1 row 5.5 / 6.5 / 7.5; 32 rows 4 groups 7.6 / 7.1 / 7.8; 256 rows 8
+    // groups 18 / 12 / 8.7.
     if (A.nk <= kFewMaxK) {
         auto few = [&](auto f) {
             const bool whole = A.nk % 32u == 0u && (!kPT || A.np % (16u * f()) == 0u) && !odd_rows(A.p, A.ldp) && !odd_rows(A.q, A.ldq) && ((uint64_t)A.np * A.nk) % 2u == 0u;
             if (whole) return launch(k_grouped_few<T, f(), kPT, true, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
             return launch(k_grouped_few<T, f(), kPT, false, Out>, 16u * f(), 16u * f(), kFewWaves * 64u);
         };
-        if (tiles(16u) <= 2u * cus) return few(std::integral_constant<uint32_t, 1u>{});
-        if (tiles(32u) <= 2u * cus) return few(std::integral_constant<uint32_t, 2u>{});
+        if (tiles(16u) <= cus) return few(std::integral_constant<uint32_t, 1u>{});
+        if (tiles(32u) <= cus) return few(std::integral_constant<uint32_t, 2u>{});
     }
     const uint32_t mean = G.rows / G.count;
     if constexpr (!kHasRows<Out>) {
-        if (!words && A.np <= 32u) return gather ? launch(k_grouped<T, 32, 128, 1, 4, 2, kPT, kDirect, true, Out>, 32u, 128u, 256u) : launch(k_grouped<T, 32, 128, 1, 4, 2, kPT, kDirect, false, Out>, 32u, 128u, 256u);
         if (words) return launch(k_grouped<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
         return gather ? launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
     } else {
+        // us, tiles of 64 / of 128, fp16 256 -> 256: 4096 rows in 64 groups 7.3 / 10.5, 8192
+        // 11.9 / 12.0, 16384 17 / 14, 131072 in 16 108 / 69; bf16 2048 -> 2048: 2048 rows in
+        // 8 groups 44 / 36.
         const bool by_128 = A.np > 64u && mean >= 128u && tiles(128u) >= cus;
         if (words) return by_128 ? launch(k_grouped<T, 128, 128, 2, 2, 2, kPT, kByWords, true, Out>, 128u, 128u, 256u) : launch(k_grouped<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
-        if (A.np > 128u && mean >= 512u && A.nk >= 512u && tiles(256u) >= cus)
+        // A CU has one tile of 256 at a time, as long as 2.75 of 128 take it, and the last
+        // round of them is seldom full.  us, 128 / 256, bf16: 4096 -> 4096, 16384 rows in 8
+        // groups (5 rounds for 16.5) 626 / 584, 8192 rows (3 for 8.5) 364 / 327; 2048 -> 2048,
+        // 16384 rows in 16 (3 for 8.5) 197 / 194, 8192 rows in 8 (2 for 4.25) 97 / 126, in 64
+        // groups 188 / 200; 65536 rows in 16, -> 1024 (5 for 16.5) 1024 224 / 211, 512 151 /
+        // 148, 256 113 / 116.
+        const uint64_t rounds = (on_mean(256u) + cus - 1u) / cus;
+        if (A.np > 128u && mean >= 256u && A.nk >= 512u && 11u * rounds * cus <= 4u * on_mean(128u))
             return gather ? launch(k_grouped<T, 256, 256, 2, 4, 2, kPT, kDirect, true, Out>, 256u, 256u, 512u) : launch(k_grouped<T, 256, 256, 2, 4, 2, kPT, kDirect, false, Out>, 256u, 256u, 512u);
         if (by_128) return gather ? launch(k_grouped<T, 128, 128, 2, 2, 2, kPT, kDirect, true, Out>, 128u, 128u, 256u) : launch(k_grouped<T, 128, 128, 2, 2, 2, kPT, kDirect, false, Out>, 128u, 128u, 256u);
         return gather ? launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
@@ -195,10 +210,16 @@ hipError_t launch_sums(GatheredOperands A, const Groups& G, float* dw, float* db
     };
     const bool gather = A.p_index || A.q_index;
     const bool words  = !whole_chunks(A.p, A.ldp, A.np) || !whole_chunks(A.q, A.ldq, A.nq) || (gather && !(near(A.p_count, A.ldp) && near(A.q_count, A.ldq)));
+    // us of a backward pass, sums by tiles of 64 / of 128, fp16: 16384 rows in 16 groups,
+    // 256 x 256 (2^30) 30 / 35, 512 x 512 (2^32) 66 / 61; 65536 rows, 256 x 256 (2^32) 82 / 72;
+    // 128 / 256: 2048 x 2048, 16384 rows in 8 (2^36) 381 / 409, bf16 4096 x 2048 (2^37) 725 /
+    // 688, in 32 groups 965 / 913, 4096 x 4096 (2^38) 1390 / 1239.  Parts enough for one
+    // workgroup a CU, for half, one, two and four: 262144 rows in 64 groups 279, 224, 234, 234;
+    // 16384 rows in 8 groups, 1024 x 1024, 180, 168, 172, 187.
     const uint64_t work = length * G.rows;
     const bool by_128   = A.np > 64u && A.nq > 64u && work >= 1ull << 32;
     if (words) return by_128 ? launch(k_grouped_sums<T, 128, 128, 2, 2, kByWords, true>, 128u, 128u, 256u) : launch(k_grouped_sums<T, 64, 64, 2, 2, kByWords, true>, 64u, 64u, 256u);
-    if (A.np > 128u && A.nq > 128u && work >= 1ull << 35)
+    if (A.np > 128u && A.nq > 128u && work >= 1ull << 37)
         return gather ? launch(k_grouped_sums<T, 256, 256, 2, 4, kDirect, true>, 256u, 256u, 512u) : launch(k_grouped_sums<T, 256, 256, 2, 4, kDirect, false>, 256u, 256u, 512u);
     if (by_128) return gather ? launch(k_grouped_sums<T, 128, 128, 2, 2, kDirect, true>, 128u, 128u, 256u) : launch(k_grouped_sums<T, 128, 128, 2, 2, kDirect, false>, 128u, 128u, 256u);
     return gather ? launch(k_grouped_sums<T, 64, 64, 2, 2, kDirect, true>, 64u, 64u, 256u) : launch(k_grouped_sums<T, 64, 64, 2, 2, kDirect, false>, 64u, 64u, 256u);

@@ -8,7 +8,7 @@
 // One pass counts every chunk's rows by id, one adds the counts up (over the
 // chunks, then over the groups), and one finds every row's place: the counts of
 // ids before its own, of its own in the chunks before, in the waves before and
-// in the lanes before.  No atomic's order decides a place.  Up to 16384 rows one
+// in the lanes before.  No atomic's order decides a place.  Up to 8192 rows one
 // workgroup does all of it in one launch.
 #include "common.hpp"
 
@@ -18,14 +18,16 @@ namespace {
 
 constexpr uint32_t kThreads = 1024u, kWaves = kThreads / 64u;
 constexpr uint32_t kEach = 4u, kTurn = kThreads * kEach;  // rows a turn; where one workgroup does all, twice as many
-constexpr uint32_t kOneRows = 16384u;
+// One workgroup / three launches, us: 4096 rows in 64 groups 8.4 / 11.5, 8192 10.9 /
+// 11.9, 16384 18.8 / 12.2; in 4000 groups 16 / 20, 18 / 20, 33 / 20.
+constexpr uint32_t kOneRows = 8192u;
 
 // Counters of a workgroup: where the next row of an id goes, and how many of a
 // turn's rows the waves before have (two 16-bit counters a word; the last line
-// has all waves').
-template <uint32_t kBins>
+// has all waves').  Sized for the most groups: smaller ones for fewer groups made no
+// difference (1048576 rows in 64 groups 16.0 us, in 512 19.7).
+constexpr uint32_t kBins = NERF_EXT_MAX_GROUPS + 1u, kWords = (kBins + 1u) / 2u;
 struct Counters {
-    static constexpr uint32_t kWords = (kBins + 1u) / 2u;
     uint32_t start[kBins];
     uint32_t turn[kWaves + 1u][kWords];
 };
@@ -79,8 +81,8 @@ __device__ __forceinline__ void count_rows(const uint32_t* __restrict__ ids, uin
 }
 
 // Places of rows [row0, row_end), S.start holding the chunk's first of every id.
-template <uint32_t kBins, uint32_t kEach>
-__device__ __forceinline__ void place_rows(const uint32_t* __restrict__ ids, uint32_t row0, uint32_t row_end, uint32_t groups, uint32_t* __restrict__ order, uint32_t* __restrict__ place, Counters<kBins>& S) {
+template <uint32_t kEach>
+__device__ __forceinline__ void place_rows(const uint32_t* __restrict__ ids, uint32_t row0, uint32_t row_end, uint32_t groups, uint32_t* __restrict__ order, uint32_t* __restrict__ place, Counters& S) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, words = (groups + 2u) / 2u;
     const uint32_t bits = 32u - (uint32_t)__builtin_clz(groups);  // of ids 0 .. groups
     constexpr uint32_t kTurn = kThreads * kEach;
@@ -136,19 +138,18 @@ __device__ __forceinline__ void place_rows(const uint32_t* __restrict__ ids, uin
     }
 }
 
-template <uint32_t kBins>
 __global__ __launch_bounds__(kThreads) void k_group_one(const uint32_t* __restrict__ ids, uint32_t rows, uint32_t groups, uint32_t* __restrict__ offsets, uint32_t* __restrict__ order, uint32_t* __restrict__ place) {
-    __shared__ Counters<kBins> S;
+    __shared__ Counters S;
     __shared__ uint32_t waves[kWaves];
     uint32_t* counts = &S.turn[0][0];
-    static_assert((kWaves + 1u) * Counters<kBins>::kWords >= kBins);
+    static_assert((kWaves + 1u) * kWords >= kBins);
     count_rows<2u * kEach>(ids, 0u, rows, groups, counts);
     sums_before<kThreads>(groups + 1u, waves, [&](uint32_t b) { return counts[b]; }, [&](uint32_t b, uint32_t sum) {
         S.start[b] = sum;
         offsets[b] = sum;
     });
     __syncthreads();
-    place_rows<kBins, 2u * kEach>(ids, 0u, rows, groups, order, place, S);
+    place_rows<2u * kEach>(ids, 0u, rows, groups, order, place, S);
 }
 
 // What the passes of more rows leave for each other.
@@ -158,7 +159,6 @@ struct Passes {
     uint32_t rows, groups, chunks, chunk;
 };
 
-template <uint32_t kBins>
 __global__ __launch_bounds__(kThreads) void k_group_count(const uint32_t* __restrict__ ids, Passes P) {
     __shared__ uint32_t counts[kBins];
     const uint32_t row0 = blockIdx.x * P.chunk;
@@ -194,9 +194,8 @@ __global__ __launch_bounds__(kIds * kSlices) void k_group_scan(Passes P) {
 // Every workgroup adds the totals up for itself (a launch of its own, or a wait for
 // the last workgroup of the pass before, takes longer: 1048576 rows, 4096 groups
 // 68 us with the latter).
-template <uint32_t kBins>
 __global__ __launch_bounds__(kThreads) void k_group_place(const uint32_t* __restrict__ ids, Passes P, uint32_t* __restrict__ offsets, uint32_t* __restrict__ order, uint32_t* __restrict__ place) {
-    __shared__ Counters<kBins> S;
+    __shared__ Counters S;
     __shared__ uint32_t waves[kWaves];
     const uint32_t row0 = blockIdx.x * P.chunk;
     uint32_t* totals    = &S.turn[0][0];
@@ -210,26 +209,25 @@ __global__ __launch_bounds__(kThreads) void k_group_place(const uint32_t* __rest
         if (blockIdx.x == 0u) offsets[b] = sum;
     });
     __syncthreads();
-    place_rows<kBins, kEach>(ids, row0, min(P.rows, row0 + P.chunk), P.groups, order, place, S);
+    place_rows<kEach>(ids, row0, min(P.rows, row0 + P.chunk), P.groups, order, place, S);
 }
 
-template <uint32_t kBins>
 NerfStatus group_rows(const uint32_t* ids, uint32_t rows, uint32_t groups, uint32_t* offsets, uint32_t* order, uint32_t* place, uint32_t* workspace, uint64_t words, hipStream_t stream) {
     // Chunks: two a CU at most, as many as the workspace holds.
     const uint64_t bins = groups + 1u, held = words > bins ? (words - bins) / bins : 0u;
     const uint64_t chunks = std::min<uint64_t>({held, 2u * device_cu_count(), (rows + kTurn - 1u) / kTurn});
     if (rows <= kOneRows || chunks <= 1u) {
-        k_group_one<kBins><<<1, kThreads, 0, stream>>>(ids, rows, groups, offsets, order, place);
+        k_group_one<<<1, kThreads, 0, stream>>>(ids, rows, groups, offsets, order, place);
         NERF_LAUNCH_CHECK("k_group_one");
         return NERF_STATUS_OK;
     }
     const uint32_t chunk = (uint32_t)((rows + chunks * kTurn - 1u) / (chunks * kTurn)) * kTurn;
     const Passes P{workspace, workspace + bins, rows, groups, (rows + chunk - 1u) / chunk, chunk};
-    k_group_count<kBins><<<P.chunks, kThreads, 0, stream>>>(ids, P);
+    k_group_count<<<P.chunks, kThreads, 0, stream>>>(ids, P);
     NERF_LAUNCH_CHECK("k_group_count");
     k_group_scan<<<groups / kIds + 1u, kIds * kSlices, 0, stream>>>(P);
     NERF_LAUNCH_CHECK("k_group_scan");
-    k_group_place<kBins><<<P.chunks, kThreads, 0, stream>>>(ids, P, offsets, order, place);
+    k_group_place<<<P.chunks, kThreads, 0, stream>>>(ids, P, offsets, order, place);
     NERF_LAUNCH_CHECK("k_group_place");
     return NERF_STATUS_OK;
 }
@@ -246,9 +244,7 @@ NERF_API NerfStatus nerf_ext_group_rows(const uint32_t* ids, uint32_t rows, uint
     NERF_CHECK_ARG(aligned(ids, 4u) && aligned(offsets, 4u) && aligned(order, 4u) && aligned(place, 4u), "nerf_ext_group_rows: an array is not aligned to its elements");
     NERF_CHECK_ARG(aligned(workspace, 16u), "nerf_ext_group_rows: workspace must be aligned to 16 bytes");
     const uint64_t words = workspace ? workspace_bytes / 4u : 0u;
-    if (groups < 128u) return group_rows<128u>(ids, rows, groups, offsets, order, place, (uint32_t*)workspace, words, (hipStream_t)stream);
-    if (groups < 1024u) return group_rows<1024u>(ids, rows, groups, offsets, order, place, (uint32_t*)workspace, words, (hipStream_t)stream);
-    return group_rows<NERF_EXT_MAX_GROUPS + 1u>(ids, rows, groups, offsets, order, place, (uint32_t*)workspace, words, (hipStream_t)stream);
+    return group_rows(ids, rows, groups, offsets, order, place, (uint32_t*)workspace, words, (hipStream_t)stream);
 }
 
 }  // extern "C"
