@@ -304,7 +304,7 @@ enum { NERF_EXT_MAX_GROUPS = 4096, NERF_EXT_MAX_RANK = 256, NERF_EXT_GROUP_WORKS
  *   in no group (ids[row] >= groups) last: group g has order[offsets[g]] ..
  *   order[offsets[g + 1] - 1];
  * place [rows] or NULL: its inverse, place[order[i]] = i.
- * rows: at most 2^30.  Up to 16384 rows no workspace is used;
+ * rows: at most 2^30.  Up to 8192 rows no workspace is used;
  * NERF_EXT_GROUP_WORKSPACE serves any number of rows and groups, less (or NULL
  * and 0) is slower. */
 NERF_API NerfStatus nerf_ext_group_rows(const uint32_t* ids, uint32_t rows, uint32_t groups, uint32_t* offsets, uint32_t* order, uint32_t* place, void* workspace, uint64_t workspace_bytes, void* stream);

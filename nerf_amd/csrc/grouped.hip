@@ -15,7 +15,14 @@ using namespace nerf_hip::grouped;
 
 namespace {
 
-// Output tiles of kBP x kBQ, see product().
+// Output tiles of kBP x kBQ, see product().  A tile's rows are looked up once, into
+// LDS; rows of an operand are asked for a tile of k ahead, since each is two loads
+// that wait for each other.  With 256 -> 256 fp16, residual and pre, 262144 rows in 64
+// groups, memory bounds it: 130 us, 4.1 TB/s (weights of a group are in L2 for its
+// rows, so a kernel that streams the rows past them in registers was 3 % faster
+// here and slower with many groups; it is not built).  With 4096 -> 4096 bf16 the
+// matrix instructions do: 16384 rows in 8 groups 550-565 us, 1.0 PFLOP/s, of which a
+// sixth is the last round of tiles, not full, and tiles half beyond a group's end.
 template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, Mode kMode, bool kGather, typename Out>
 __global__ __launch_bounds__(kWP * kWQ * 64u) void k_grouped(GatheredOperands A, Out out, Groups G, Parts parts) {
     __shared__ uint32_t rows[kHasRows<Out> ? kBQ : 1u];
@@ -28,7 +35,9 @@ __global__ __launch_bounds__(kWP * kWQ * 64u) void k_grouped(GatheredOperands A,
     product<T, kBP, kBQ, kWP, kWQ, kDepth, kPT, false, kMode, kGather>(A, out, Place{tile.tile_p * kBP, part.q0, 0u, A.nk, kPT ? 0u : part.group * A.np, kPT ? part.group * A.nk : 0u});
 }
 
-// The same with few tiles; kWhole: whole steps and rows that start at even values.
+// The same with few tiles, each one's k over a workgroup's waves, which bounds a call
+// by one pass of loads (8 rows in as many of 64 groups, 256 -> 256: 4.2-5.0 us, the
+// launch being 4).  kWhole: whole steps and rows that start at even values.
 template <typename T, uint32_t kF, bool kPT, bool kWhole, typename Out>
 __global__ __launch_bounds__(kFewWaves * 64u) void k_grouped_few(GatheredOperands A, Out out, Groups G, Parts parts) {
     __shared__ floatx4 lds[few_lds(kF, kF) / 16u];
@@ -77,7 +86,12 @@ __global__ __launch_bounds__(64) void k_grouped_tiny(GatheredOperands A, Out out
     }
 }
 
-// dW_g, and db_g with it: sums over parts of `size` rows of a group.
+// dW_g, and db_g with it: sums over parts of `size` rows of a group, both operands by
+// the transposing read.  Every product is of two rows' values that are read again
+// for each tile across, so it is bound by memory where a layer is narrow (262144
+// rows in 64 groups, 256 x 256: 88 us, 3.1 TB/s, and 9 for the join) and by the matrix
+// instructions where it is wide (16384 rows in 8 groups, 2048 x 4096: 326 us, 0.84
+// PFLOP/s: the groups' uneven rows leave CUs without work at the end).
 template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, Mode kMode, bool kGather>
 __global__ __launch_bounds__(kWP * kWQ * 64u) void k_grouped_sums(GatheredOperands A, SumOut out, Groups G, uint32_t size, uint32_t most, float* sum_parts) {
     const uint32_t tiles = A.tiles_p * A.tiles_q, t = dealt_tile(block_number(), most, tiles);
@@ -113,6 +127,7 @@ __global__ __launch_bounds__(256) void k_grouped_tiny_sums(GatheredOperands A, S
     if (out.row_sums && p == 0u) out.row_sums[(uint64_t)g * A.nq + q] = s;
 }
 
+// The parts of a group added to its first, in their order.
 __global__ __launch_bounds__(256) void k_grouped_join(Groups G, uint32_t size, float* out, const float* parts, uint64_t length, float* sums, const float* sum_parts, uint32_t sums_length, uint32_t blocks) {
     const uint32_t g = blockIdx.x / blocks, begin = G.offset(g), end = G.offset(g + 1u);
     if (end <= begin || end - begin <= size) return;

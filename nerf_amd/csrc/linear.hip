@@ -14,6 +14,7 @@
 // contiguous is read from LDS through the transposing read
 // (ds_read_b64_tr_b16), four k of one p a lane, so no operand is transposed in
 // memory.  Products are of 16-bit values, exact in 32 bits, and summed in 32
+// bits.  The tiles themselves are in linear_device.hpp.
 #include "linear_device.hpp"
 
 using namespace nerf_hip;
