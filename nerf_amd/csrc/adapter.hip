@@ -593,14 +593,17 @@ __global__ __launch_bounds__(64) void k_adapter_tiny(GatheredOperands A, Out out
 // ------------------------------------------------------- gradients of adapters
 // out_g(w, r) = scale_g sum_i wide(i, w) low(i, r): wide 16-bit rows, as an index
 // names them, low 32-bit by position; kBW wide x kBR low values a workgroup, sums
-// over parts of `size` positions of a group.  The products are of 32-bit values,
-// so the matrix instruction is the 32-bit one, four positions at a time, which is
-// at 39 % of its peak there: 8192 rows in 8 groups, rank 64, 4096 values 70 us and
-// 2048 values 42 (0.06 PFLOP/s; memory alone would take 13).  Sums of 16-bit pieces of
-// low would take a fifth of those instructions, but fp16's pieces need scales
-// that a sum over rows cannot take out again; not built.  262144 rows, rank 16, 256
-// values: 45 us, 3.3 TB/s.  out is
-// [groups][nw][nr], or with `low_major` [groups][nr][nw].
+// over parts of `size` positions of a group.  out is [groups][nw][nr], or with
+// `low_major` [groups][nr][nw].
+// For bf16 each low value is split into three of that type (24 bits; below 2^-110
+// their last ones are lost), whose products take three sixteenths of the
+// 32-bit instruction's time.  fp16 values would need a scale a row for that, which a
+// sum over rows cannot take out again: the 32-bit instruction, four positions at a
+// time.  8192 rows in 8 groups, rank 64, 4096 values: 45 us in bf16 (by the 32-bit
+// instruction, each wave with all of r, 72; split so, 63; one wave for 16 of r, as it
+// is now, reads and splits a value once), 2048 values 28.  What is left is the waits for
+// gathered rows, two loads after each other, in parts of a few tiles; memory
+// alone would take 13.  262144 rows, rank 16, 256 values, fp16: 45 us, 3.3 TB/s.
 struct RankSums {
     const void* wide;
     const float* low;
@@ -642,7 +645,9 @@ struct LowLoader {
 // else through registers, at any alignment.
 template <typename T, uint32_t kBR, Mode kMode, bool kGather>
 __global__ __launch_bounds__(256) void k_rank_sums(RankSums A, Groups G, uint32_t size, uint32_t most) {
-    constexpr uint32_t kFR = kBR / 16u;
+    // Waves side by side in r first, so that a low value is read and split by as few as
+    // can be.
+    constexpr uint32_t kWR = kBR / 16u, kFW = 2u * kWR;
     __shared__ uint4 wide0[kBW * 8u], wide1[kMode == kDirect ? kBW * 8u : 1u];
     __shared__ float low0[kBK * kBR], low1[kMode == kDirect ? kBK * kBR : 1u];
     const uint32_t tiles = A.tiles_w * A.tiles_r, t = dealt_tile(block_number(), most, tiles);
@@ -652,30 +657,41 @@ __global__ __launch_bounds__(256) void k_rank_sums(RankSums A, Groups G, uint32_
     const uint32_t w0 = t % tiles % A.tiles_w * kBW, r0 = t % tiles / A.tiles_w * kBR;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, l = lane & 15u, quarter = lane >> 4;
     const uint32_t end = min(part.end, part.q0 + size);
-    floatx4 acc[2][kFR];
+    const uint32_t wave_w = wave / kWR * 16u * kFW, wave_r = wave % kWR * 16u;
+    floatx4 acc[kFW];
 #pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i)
-#pragma unroll
-        for (uint32_t j = 0; j < kFR; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    const uint32_t base = fragment_base<kBW, true>(32u * wave);
+    for (uint32_t i = 0; i < kFW; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t base = fragment_base<kBW, true>(wave_w);
     auto multiply = [&](const uint4* wide, const float* low) {
 #pragma unroll
         for (uint32_t step = 0; step < 2u; ++step) {
-            floatx8 w[2];
+            typename Vec<T>::x8 w[kFW];
 #pragma unroll
-            for (uint32_t i = 0; i < 2u; ++i) {
-                typename Vec<T>::x8 f = fragment<T, kBW, true>(wide, base, i, step);
-                settle_here(f);
-                w[i] = __builtin_convertvector(f, floatx8);
+            for (uint32_t i = 0; i < kFW; ++i) {
+                w[i] = fragment<T, kBW, true>(wide, base, i, step);
+                settle_here(w[i]);
             }
+            floatx8 m;
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e)
+            for (uint32_t e = 0; e < 8u; ++e) m[e] = low[(32u * step + 8u * quarter + e) * kBR + wave_r + l];
+            if constexpr (std::is_same_v<T, bf16_t>) {
 #pragma unroll
-                for (uint32_t j = 0; j < kFR; ++j) {
-                    const float m = low[(32u * step + 8u * quarter + e) * kBR + 16u * j + l];
+                for (uint32_t piece = 0; piece < 3u; ++piece) {
+                    const typename Vec<T>::x8 h = __builtin_convertvector(m, typename Vec<T>::x8);
 #pragma unroll
-                    for (uint32_t i = 0; i < 2u; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i][e], m, acc[i][j], 0, 0, 0);
+                    for (uint32_t i = 0; i < kFW; ++i) acc[i] = Vec<T>::mfma(w[i], h, acc[i]);
+                    const floatx8 back = __builtin_convertvector(h, floatx8);
+#pragma unroll
+                    for (uint32_t e = 0; e < 8u; ++e) m[e] = rest_of(m[e], back[e]);
                 }
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < kFW; ++i) {
+                    const floatx8 v = __builtin_convertvector(w[i], floatx8);
+#pragma unroll
+                    for (uint32_t e = 0; e < 8u; ++e) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], m[e], acc[i], 0, 0, 0);
+                }
+            }
         }
     };
     if constexpr (kMode == kDirect) {
@@ -727,16 +743,13 @@ __global__ __launch_bounds__(256) void k_rank_sums(RankSums A, Groups G, uint32_
     const uint64_t length = (uint64_t)A.nw * A.nr;
     float* out = part.number ? A.parts + place_of(G, part, size) * length : A.out + part.group * length;
     const float scale = A.scales ? A.scales[part.group] : 1.0f;
+    const uint32_t r = r0 + wave_r + l;
 #pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i)
+    for (uint32_t i = 0; i < kFW; ++i)
 #pragma unroll
-        for (uint32_t j = 0; j < kFR; ++j) {
-            const uint32_t r = r0 + 16u * j + l;
-#pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) {
-                const uint32_t w = w0 + 32u * wave + 16u * i + 4u * quarter + e;
-                if (r < A.nr && w < A.nw) out[A.low_major ? (uint64_t)r * A.nw + w : (uint64_t)w * A.nr + r] = scale * acc[i][j][e];
-            }
+        for (uint32_t e = 0; e < 4u; ++e) {
+            const uint32_t w = w0 + wave_w + 16u * i + 4u * quarter + e;
+            if (r < A.nr && w < A.nw) out[A.low_major ? (uint64_t)r * A.nw + w : (uint64_t)w * A.nr + r] = scale * acc[i][e];
         }
 }
 
