@@ -164,8 +164,8 @@ struct LowRank {
     static __device__ __forceinline__ float of_row(float v, uint32_t j) { return std::is_same_v<T, half_t> ? __shfl(v, (int)(16u * j + (threadIdx.x & 15u))) : 1.0f; }
     // acc[i][j] of group g's rows += factor times the product of one step.  Rows of
     // other groups keep theirs, whatever this group's weights hold.
-    template <uint32_t kN, uint32_t kFP, uint32_t kFQ>
-    __device__ __forceinline__ void add_group(floatx4 (&acc)[kFP][kFQ], uint32_t i0, const x8 (&fp)[kN], const x8 (&fq)[kFQ], uint64_t those, float power, float scale) const {
+    template <uint32_t kFP, uint32_t kFQ>
+    __device__ __forceinline__ void add_group(floatx4 (&acc)[kFP][kFQ], const x8 (&fp)[kFP], const x8 (&fq)[kFQ], uint64_t those, float power, float scale) const {
 #pragma unroll
         for (uint32_t j = 0; j < kFQ; ++j) {
             const uint32_t rows = (uint32_t)(those >> (16u * j)) & 0xFFFFu;
@@ -173,10 +173,10 @@ struct LowRank {
             const float factor = of_row(power, j) * scale;
             const bool member  = rows >> (threadIdx.x & 15u) & 1u;
 #pragma unroll
-            for (uint32_t i = 0; i < kN; ++i) {
+            for (uint32_t i = 0; i < kFP; ++i) {
                 const floatx4 part = Vec<T>::mfma(fp[i], fq[j], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-                for (uint32_t r = 0; r < 4u; ++r) acc[i0 + i][j][r] = member ? acc[i0 + i][j][r] + factor * part[r] : acc[i0 + i][j][r];
+                for (uint32_t r = 0; r < 4u; ++r) acc[i][j][r] = member ? acc[i][j][r] + factor * part[r] : acc[i][j][r];
             }
         }
     }
@@ -206,14 +206,10 @@ struct LowRank {
                 const uint64_t those = __ballot(mine == g);
                 left &= ~those;
                 const float scale = scales ? scales[g] : 1.0f;
-                constexpr uint32_t kAtOnce = kTight ? 4u : kFP;
+                x8 fp[kFP];
 #pragma unroll
-                for (uint32_t i0 = 0; i0 < kFP; i0 += kAtOnce) {
-                    x8 fp[kAtOnce];
-#pragma unroll
-                    for (uint32_t i = 0; i < kAtOnce; ++i) fp[i] = wide_eight(g, p0 + 16u * (i0 + i) + (threadIdx.x & 15u), step.r0);
-                    add_group(acc, i0, fp, fq, those, power.value, scale);
-                }
+                for (uint32_t i = 0; i < kFP; ++i) fp[i] = wide_eight(g, p0 + 16u * i + (threadIdx.x & 15u), step.r0);
+                add_group(acc, fp, fq, those, power.value, scale);
             }
         }
     }
@@ -289,7 +285,7 @@ struct LowRank {
 #pragma unroll
                     for (uint32_t i = 0; i < kFP; ++i) fp[i] = wide_eight(g, p0 + 16u * i + (threadIdx.x & 15u), step.r0);
                 }
-                add_group(acc, 0u, fp, fq, those, a.power.value, scale);
+                add_group(acc, fp, fq, those, a.power.value, scale);
             });
         }
     }
