@@ -803,10 +803,10 @@ hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& mo
     const bool by_128 = A.np > 64u && A.nq > 64u && tiles(128u) >= cus;
     if (words) return by_128 ? launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kByWords, true, Out>, 128u, 128u, 256u) : launch(k_adapter<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
     // A tile of 256 takes a CU nearly as long as four of 128, so it needs full rounds: us of
-    // a call, 128 / 256, 2048 -> 2048 rank 16, 4096 rows (1 round for 2) 55 / 83, 8192 (1 for
-    // 4) 97 / 94; gradients of 4096 -> 2048, rank 64, 6144 rows (2 for 6) 294 / 323, 8192 (2 for
-    // 8) 374 / 357, 10240 (3 for 10) 445 / 467, 12288 rank 16 (3 for 12) 382 / 352; 512 -> 512,
-    // 65536 rows (2 for 8) 85 / 89.
+    // a call, 128 / 256, 2048 -> 2048 rank 16, 4096 rows (1 round for 2) 54 / 81, 8192 (1 for
+    // 4) 93-97 / 94-98; gradients of 4096 -> 2048, rank 64, 6144 rows (2 for 6) 265 / 291, 8192
+    // (2 for 8) 338 / 319, 10240 (3 for 10) 404 / 417, 12288 rank 16 (3 for 12) 364 / 338;
+    // 512 -> 512, 65536 rows (2 for 8) 85-90 / 89.
     if (A.np > 128u && A.nq > 128u && A.nk >= 1024u && 15u * ((tiles(256u) + cus - 1u) / cus) * cus <= 4u * tiles(128u))
         return gather ? launch(k_adapter<T, 256, 256, 2, 4, 2, kPT, kDirect, true, Out>, 256u, 256u, 512u) : launch(k_adapter<T, 256, 256, 2, 4, 2, kPT, kDirect, false, Out>, 256u, 256u, 512u);
     if (by_128) return gather ? launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kDirect, true, Out>, 128u, 128u, 256u) : launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kDirect, false, Out>, 128u, 128u, 256u);
