@@ -329,7 +329,6 @@ __global__ __launch_bounds__(kFewWaves * 64u) void k_adapter_few(GatheredOperand
 // value moves between lanes.  A workgroup has consecutive positions, group by group.
 // 262144 rows in 16 groups, rank 16, 256 -> 256 fp16, residual and pre: 138 us, 4.0
 // TB/s (tiles after a pass for m 199); its input gradient 156.
-constexpr uint32_t kStreamChunk = 1024u;  // positions whose rows are looked up at a time
 struct StreamRanks {
     const void* shrink;  // down [groups][rank][nk]; kPT: up [groups][nk][rank]
     float* low;          // m
@@ -821,7 +820,7 @@ hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& mo
 // 65536 rows 90 / 105, 32768 rows 60 / 60.
 template <typename T, bool kPT>
 bool streamed(const GatheredOperands& A, const LowRank<T, kPT>& more, const void* shrink, bool vec, const uint32_t* index, uint32_t count, uint64_t widest) {
-    return A.nk <= 256u && A.nk % 32u == 0u && A.np <= 512u && more.rank <= 64u && A.nq >= 65536u && vec && whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) && whole_chunks(A.q, A.ldq, A.nk) && aligned(shrink, 16u) && (!index || near(count, widest));
+    return A.nk <= 256u && A.nk % 32u == 0u && A.np <= 512u && more.rank <= 64u && A.nq >= 65536u && vec && whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) && whole_chunks(A.q, A.ldq, A.nk) && aligned(shrink, 16u) && stream_outputs_near(index != nullptr, count, widest);
 }
 
 template <typename T, bool kPT, typename Out>

@@ -16,6 +16,7 @@
 #pragma once
 
 #include "linear_device.hpp"
+#include "offsets.hpp"
 
 namespace nerf_hip {
 namespace grouped {
@@ -286,10 +287,6 @@ __device__ __forceinline__ uint64_t place_of(const Groups& G, const Part& part, 
 
 // ------------------------------------------------------------------- host
 constexpr uint32_t kMaxGroups = NERF_EXT_MAX_GROUPS;
-
-// Whether an operand whose lines an index names can go straight into LDS: by 32-bit
-// offsets from the array's start.
-inline bool near(uint64_t count, uint64_t ld) { return count * ld * 2u < 1ull << 31; }
 
 // What NerfExtRowGroups says, with its defaults filled in.
 NerfStatus check_groups(const NerfExtRowGroups* groups, const NerfExtLinearDesc& d, NerfExtRowGroups& out, const char* fn);
