@@ -473,6 +473,9 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_adapter_stream(GatheredO
                     for (uint32_t s = 0; s < kKS; ++s) m = Vec<T>::mfma(lds_shrink[(rb * kKS + s) * 64u + lane], __builtin_bit_cast(x8, c0.q[s]), m);
                     if constexpr (kPT) m *= scale;
                     const uint32_t position = pos + tile * 16u + l, r = 16u * rb + 4u * quarter;
+                    // Beyond the rank: an infinite input makes NaN of the zeros there.
+#pragma unroll
+                    for (uint32_t e = 0; e < 4u; ++e) m[e] = r + e < more.rank ? m[e] : 0.0f;
                     if (keeps_low && position < end) {
                         float* to = R.low + (uint64_t)position * more.rank + r;
                         if (more.vec_low) {
