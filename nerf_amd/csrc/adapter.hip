@@ -34,6 +34,20 @@ __device__ __forceinline__ Power power_of(float most) {
 }
 // What a rounding leaves of a value: nothing of an infinity or NaN.
 __device__ __forceinline__ float rest_of(float value, float rounded) { return fabsf(rounded) < __builtin_inff() ? value - rounded : 0.0f; }
+// The factors of a value's pieces: all of them for the first piece (first[e] = 1),
+// which has the value's sign; for the others, which may be zero or have the other
+// sign, with zeros in place of infinities and NaN.  So an infinite factor gives what it
+// gives with the value itself.
+template <uint32_t kCount>
+using u16s = unsigned short __attribute__((ext_vector_type(kCount)));
+typedef u16s<8> u16x8;
+template <typename T, typename V, typename First>
+__device__ __forceinline__ V factors_of(V v, First first) {
+    using Bits = u16s<sizeof(V) / 2u>;
+    constexpr unsigned short kExponent = std::is_same_v<T, half_t> ? 0x7C00u : 0x7F80u;
+    const Bits bits = __builtin_bit_cast(Bits, v), keep = (~bits & kExponent) | first;
+    return __builtin_bit_cast(V, bits & (0 - __builtin_elementwise_min(keep, (Bits)1)));
+}
 
 // The low-rank part of a wave's sums: low [rows][rank] times wide, which is
 // [groups][np][rank] (kPT: [groups][rank][np]).
@@ -67,7 +81,7 @@ struct LowRank {
         for (uint32_t e = 0; e < 8u; ++e) v[e] = r0 + e < rank ? v[e] : 0.0f;
         return v;
     }
-    // Eight of wide's values at p from r0, zeros outside.
+    // Eight of wide's values at p from r0; others of the array where those are outside.
     __device__ __forceinline__ x8 wide_eight(uint32_t g, uint32_t p, uint32_t r0) const {
         const uint32_t column = min(p, np - 1u);
         x8 v;
@@ -84,8 +98,6 @@ struct LowRank {
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) v[e] = at[(uint64_t)min(r0 + e, rank - 1u) * np];
         }
-#pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) v[e] = p < np && r0 + e < rank ? v[e] : (T)0.0f;
         return v;
     }
     // Piece `piece` of eight values.
@@ -133,6 +145,14 @@ struct LowRank {
     struct Step {
         uint32_t piece, r0;
     };
+    // Which of wide's eight values a step takes as they are: those of first pieces within
+    // the rank.  Of the others, m's are zeros or low pieces, factors_of() the finite ones.
+    __device__ __forceinline__ u16x8 as_they_are(const Step& step) const {
+        u16x8 first;
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) first[e] = step.piece == 0u && step.r0 + e < rank;
+        return first;
+    }
     __device__ __forceinline__ Step step_of(uint32_t s) const {
         const uint32_t chunks = (rank + 7u) / 8u, chunk = 4u * s + ((threadIdx.x & 63u) >> 4), piece = chunk / chunks;
         return {piece < pieces ? piece : 0u, piece < pieces ? 8u * (chunk - piece * chunks) : rank};
@@ -164,8 +184,8 @@ struct LowRank {
     static __device__ __forceinline__ float of_row(float v, uint32_t j) { return std::is_same_v<T, half_t> ? __shfl(v, (int)(16u * j + (threadIdx.x & 15u))) : 1.0f; }
     // acc[i][j] of group g's rows += factor times the product of one step.  Rows of
     // other groups keep theirs, whatever this group's weights hold.
-    template <uint32_t kFP, uint32_t kFQ>
-    __device__ __forceinline__ void add_group(floatx4 (&acc)[kFP][kFQ], const x8 (&fp)[kFP], const x8 (&fq)[kFQ], uint64_t those, float power, float scale) const {
+    template <uint32_t kFP, uint32_t kFQ, uint32_t kSome>
+    __device__ __forceinline__ void add_group(floatx4 (&acc)[kFP][kFQ], uint32_t from, const x8 (&fp)[kSome], const x8 (&fq)[kFQ], uint64_t those, float power, float scale) const {
 #pragma unroll
         for (uint32_t j = 0; j < kFQ; ++j) {
             const uint32_t rows = (uint32_t)(those >> (16u * j)) & 0xFFFFu;
@@ -173,10 +193,10 @@ struct LowRank {
             const float factor = of_row(power, j) * scale;
             const bool member  = rows >> (threadIdx.x & 15u) & 1u;
 #pragma unroll
-            for (uint32_t i = 0; i < kFP; ++i) {
+            for (uint32_t i = 0; i < kSome; ++i) {
                 const floatx4 part = Vec<T>::mfma(fp[i], fq[j], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-                for (uint32_t r = 0; r < 4u; ++r) acc[i][j][r] = member ? acc[i][j][r] + factor * part[r] : acc[i][j][r];
+                for (uint32_t r = 0; r < 4u; ++r) acc[from + i][j][r] = member ? acc[from + i][j][r] + factor * part[r] : acc[from + i][j][r];
             }
         }
     }
@@ -195,6 +215,7 @@ struct LowRank {
         const Power power = power_of_lane(q0);
         for (uint32_t s = 0; s < steps(); ++s) {
             const Step step = step_of(s);
+            const u16x8 first = as_they_are(step);
             x8 fq[kFQ];
             if (kTight) fetch(values, q0, s);
 #pragma unroll
@@ -206,10 +227,18 @@ struct LowRank {
                 const uint64_t those = __ballot(mine == g);
                 left &= ~those;
                 const float scale = scales ? scales[g] : 1.0f;
-                x8 fp[kFP];
+                // A few at a time in the widest tiles (8192 rows, rank 64, gradients of 4096 ->
+                // 2048: 305 us with four, 325 with all eight, some of them spilled).
+                constexpr uint32_t kSome = kTight ? 4u : kFP;
 #pragma unroll
-                for (uint32_t i = 0; i < kFP; ++i) fp[i] = wide_eight(g, p0 + 16u * i + (threadIdx.x & 15u), step.r0);
-                add_group(acc, fp, fq, those, power.value, scale);
+                for (uint32_t from = 0; from < kFP; from += kSome) {
+                    x8 fp[kSome];
+#pragma unroll
+                    for (uint32_t i = 0; i < kSome; ++i) fp[i] = wide_eight(g, p0 + 16u * (from + i) + (threadIdx.x & 15u), step.r0);
+#pragma unroll
+                    for (uint32_t i = 0; i < kSome; ++i) fp[i] = factors_of<T>(fp[i], first);
+                    add_group(acc, from, fp, fq, those, power.value, scale);
+                }
             }
         }
     }
@@ -264,6 +293,7 @@ struct LowRank {
         if (__ballot(a.mine != kNoRow) == 0ull) return;
         for (uint32_t s = 0; s < steps(); ++s) {
             const Step step = step_of(s);
+            const u16x8 first = as_they_are(step);
             floatx8 values[kFQ];
             x8 fq[kFQ];
             if (s) fetch(values, q0, s);
@@ -285,7 +315,9 @@ struct LowRank {
 #pragma unroll
                     for (uint32_t i = 0; i < kFP; ++i) fp[i] = wide_eight(g, p0 + 16u * i + (threadIdx.x & 15u), step.r0);
                 }
-                add_group(acc, fp, fq, those, a.power.value, scale);
+#pragma unroll
+                for (uint32_t i = 0; i < kFP; ++i) fp[i] = factors_of<T>(fp[i], first);
+                add_group(acc, 0u, fp, fq, those, a.power.value, scale);
             });
         }
     }
@@ -345,7 +377,7 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_adapter_stream(GatheredO
     __shared__ floatx4 lds_bias[Out::kBias ? kBP / 4u : 1u];
     __shared__ uint32_t x_rows[kStreamChunk], y_rows[kStreamChunk];
     __shared__ x8 lds_shrink[kRB * kKS * 64u];
-    __shared__ x4 lds_grow[kRB * kBP * 4u];
+    __shared__ x8 lds_grow[kRB * kBP * 4u];  // factors of high parts, then of low ones
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, l = lane & 15u, quarter = lane >> 4;
     const uint32_t wp = wave % p_waves * kSP, p0 = blockIdx.y * p_waves * kSP, waves_q = kStreamWaves / p_waves;
     const Groups& G = more.G;
@@ -420,7 +452,7 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_adapter_stream(GatheredO
                     const T w = more.wide[!inner ? 0ull : kPT ? ((uint64_t)g * more.rank + r + e) * A.np + at : ((uint64_t)g * A.np + at) * more.rank + r + e];
                     v[e] = inner ? w : (T)0.0f;
                 }
-                lds_grow[i] = v;
+                lds_grow[i] = __builtin_shufflevector(v, factors_of<T>(v, u16s<4>{0, 0, 0, 0}), 0, 1, 2, 3, 4, 5, 6, 7);
             }
         }
         const float scale = member && more.scales ? more.scales[g] : 1.0f;
@@ -508,10 +540,9 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_adapter_stream(GatheredO
                     }
 #pragma unroll
                     for (uint32_t i = 0; i < kFP; ++i) {
-                        const x4 w = lds_grow[(rb * (kBP / 16u) + wp / 16u + i) * 64u + lane];
-                        const x8 twice = __builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7);
-                        floatx4 part = Vec<T>::mfma(twice, pieces, floatx4{0.0f, 0.0f, 0.0f, 0.0f});
-                        if (more.pieces == 3u) part = Vec<T>::mfma(twice, third, part);
+                        const x8 w = lds_grow[(rb * (kBP / 16u) + wp / 16u + i) * 64u + lane];
+                        floatx4 part = Vec<T>::mfma(w, pieces, floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+                        if (more.pieces == 3u) part = Vec<T>::mfma(__builtin_shufflevector(w, w, 4, 5, 6, 7, 4, 5, 6, 7), third, part);
                         acc[i] += factor * part;
                     }
                 }

@@ -107,6 +107,30 @@ def backward_is(c, g, at, mid, ws, x_columns=(), d_columns=()):
 
 @pytest.mark.parametrize("kind,y_kind", TYPES)
 @pytest.mark.parametrize("n,i,o,r", SHAPES)
+def test_infinite_up(workspace, n, i, o, r, kind, y_kind):
+    announce(f"infinite up, {n} x {i} -> {o}, rank {r}, {kind} -> {y_kind}")
+    c, g, at = case(n, i, o, r, kind)
+    c.up[g][3, 0], c.up[g][5, r - 1], c.up[g][o - 1, r // 2] = np.inf, -np.inf, np.inf
+    c.x[c.xr()[at[1]]] = 0.0  # m of zeros, whose products with infinities are NaN
+    z = forward_is(c, g, at, y_kind, workspace)
+    assert np.isposinf(z).any() and np.isneginf(z).any() and np.isnan(z[1, 3])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n,i,o,r", SHAPES)
+def test_infinite_down(workspace, n, i, o, r, kind):
+    """In the forward pass m of that rank is infinite, in the backward pass an input's
+    gradient."""
+    announce(f"infinite down, {n} x {i} -> {o}, rank {r}, {kind}")
+    c, g, at = case(n, i, o, r, kind)
+    c.down[g][0, 3], c.down[g][r - 1, 5] = np.inf, -np.inf
+    forward_is(c, g, at, "f32", workspace)
+    mid = np.random.default_rng(1).normal(0, 1, (n, r)).astype(np.float32).astype(np.float64)
+    backward_is(c, g, at, mid, workspace)
+
+
+@pytest.mark.parametrize("kind,y_kind", TYPES)
+@pytest.mark.parametrize("n,i,o,r", SHAPES)
 def test_infinite_inputs(workspace, n, i, o, r, kind, y_kind):
     """An infinite input whose products all have the same sign: outputs of that row are
     infinite, at ranks that are no whole multiples of a tile's too."""
