@@ -328,8 +328,10 @@ struct LowRank {
 // adapters 170: what is added is the wait for the adapter's values at a tile's
 // start, once a group in it, which nothing hides with one tile a CU.  (A copy of down
 // with the ranks in a row, one load for eight, took as long.)
+// As many waves a SIMD as LDS holds: with three registers more than they leave, odd
+// rows' tiles of 128 ran one at a time (8192 rows of 1023 -> 2047, 214 us, so 138).
 template <typename T, uint32_t kBP, uint32_t kBQ, uint32_t kWP, uint32_t kWQ, uint32_t kDepth, bool kPT, Mode kMode, bool kGather, typename Out>
-__global__ __launch_bounds__(kWP * kWQ * 64u) void k_adapter(GatheredOperands A, Out out, LowRank<T, kPT> more) {
+__global__ __launch_bounds__(kWP * kWQ * 64u, kBP > 64u || kMode == kDirect ? 2u : 4u) void k_adapter(GatheredOperands A, Out out, LowRank<T, kPT> more) {
     __shared__ uint32_t rows[kBQ];
     const uint32_t block = block_number(), tiles = A.tiles_p * A.tiles_q;
     if (block >= tiles) return;
