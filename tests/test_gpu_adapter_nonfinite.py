@@ -158,3 +158,19 @@ def test_infinite_deltas(workspace, n, i, o, r, kind):
     mid = np.random.default_rng(1).normal(0, 1, (n, r)).astype(np.float32).astype(np.float64)
     got = backward_is(c, g, at, mid, workspace)
     assert np.isneginf(got["dx"][c.xr()[at[2]]]).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n,i,o,r", SHAPES)
+def test_infinite_rows_of_sums(workspace, n, i, o, r, kind):
+    """An infinite input and an infinite delta in the sums over a group's rows: an
+    infinity of the other factor's sign."""
+    announce(f"infinite rows of sums, {n} x {i} -> {o}, rank {r}, {kind}")
+    c, g, at = case(n, i, o, r, kind)
+    mid = np.random.default_rng(1).normal(0, 1, (n, r)).astype(np.float32).astype(np.float64)
+    c.x[c.xr()[at[2]], 7] = np.inf
+    got = backward_is(c, g, at, mid, workspace, x_columns=(6, 7))
+    assert np.isposinf(got["ddown"][g][:, 7]).any() and np.isinf(got["ddown"][g][:, 7]).all()
+    c.delta[c.yr()[at[3]], 7] = -np.inf
+    got = backward_is(c, g, at, mid, workspace, d_columns=(6, 7))
+    assert np.isposinf(got["dup"][g][7]).any() and np.isinf(got["dup"][g][7]).all()
