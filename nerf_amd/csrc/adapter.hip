@@ -23,13 +23,14 @@ using namespace nerf_hip::grouped;
 namespace {
 
 // The power of two that scales values of at most `most` to less than 2 (8), and its
-// inverse.
+// inverse.  Beside an infinity the largest one: the sum is an infinity or NaN then, and
+// what the finite values keep is that they are finite.
 struct Power {
     float value, inverse;
 };
 __device__ __forceinline__ Power power_of(float most) {
     const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 1u), 252u);
-    if (most > 0.0f && most < __builtin_inff()) return {__uint_as_float(exponent << 23), __uint_as_float((254u - exponent) << 23)};
+    if (most > 0.0f) return {__uint_as_float(exponent << 23), __uint_as_float((254u - exponent) << 23)};
     return {1.0f, 1.0f};
 }
 // What a rounding leaves of a value: nothing of an infinity or NaN.

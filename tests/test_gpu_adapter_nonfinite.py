@@ -174,3 +174,18 @@ def test_infinite_rows_of_sums(workspace, n, i, o, r, kind):
     c.delta[c.yr()[at[3]], 7] = -np.inf
     got = backward_is(c, g, at, mid, workspace, d_columns=(6, 7))
     assert np.isposinf(got["dup"][g][7]).any() and np.isinf(got["dup"][g][7]).all()
+
+
+@pytest.mark.parametrize("n,i,o,r", SHAPES)
+def test_large_values_beside_an_infinity(workspace, n, i, o, r):
+    """fp16: an infinite m, and others of the row beyond 65504 with factors of the other
+    sign, do not cancel."""
+    announce(f"large m beside an infinite one, {n} x {i} -> {o}, rank {r}")
+    c, g, at = case(n, i, o, r, "f16")
+    c.x = decode(encode(np.abs(c.x) * 3e3 + 1e3, "f16"), "f16")
+    c.down[g] = decode(encode(np.abs(c.down[g]) * 200.0 + 1.0, "f16"), "f16")
+    c.down[g][1, 3] = np.inf
+    c.up[g] = -np.abs(c.up[g]) - 0.125
+    c.up[g][:, 1] = 1.0
+    z = forward_is(c, g, at, "f32", workspace)
+    assert np.isposinf(z).all()
