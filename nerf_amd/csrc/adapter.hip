@@ -33,6 +33,13 @@ __device__ __forceinline__ Power power_of(float most) {
     if (most > 0.0f) return {__uint_as_float(exponent << 23), __uint_as_float((254u - exponent) << 23)};
     return {1.0f, 1.0f};
 }
+// What a value's first piece is rounded from (`scaled` by its row's power): one that is not
+// zero stays so, as the smallest number of fp16 at least, whose rest is taken off again.
+template <typename T>
+__device__ __forceinline__ float to_round(float scaled, float value) {
+    if constexpr (std::is_same_v<T, half_t>) return value != 0.0f && fabsf(scaled) < 0x1p-24f ? __builtin_copysignf(0x1p-24f, value) : scaled;
+    return scaled;
+}
 // What a rounding leaves of a value: nothing of an infinity or NaN.
 __device__ __forceinline__ float rest_of(float value, float rounded) { return fabsf(rounded) < __builtin_inff() ? value - rounded : 0.0f; }
 // The factors of a value's pieces: all of them for the first piece (first[e] = 1),
@@ -117,9 +124,13 @@ struct LowRank {
         }
         return v;
     }
-    // Piece `piece` of eight values.
-    static __device__ __forceinline__ x8 piece_of(floatx8 v, uint32_t piece) {
-        x8 h = __builtin_convertvector(v, x8);
+    // Piece `piece` of eight values, scaled by their row's power.
+    static __device__ __forceinline__ x8 piece_of(floatx8 v, float inverse, uint32_t piece) {
+        floatx8 first;
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) first[e] = to_round<T>(v[e] * inverse, v[e]);
+        v *= inverse;
+        x8 h = __builtin_convertvector(first, x8);
         for (uint32_t i = 0; i < piece; ++i) {
             const floatx8 back = __builtin_convertvector(h, floatx8);
 #pragma unroll
@@ -236,7 +247,7 @@ struct LowRank {
             x8 fq[kFQ];
             if (kTight) fetch(values, q0, s);
 #pragma unroll
-            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = piece_of(values[j] * of_row(power.inverse, j), step.piece);
+            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = piece_of(values[j], of_row(power.inverse, j), step.piece);
             if (!kTight && s + 1u < steps()) fetch(values, q0, s + 1u);
             // The groups of the wave's rows, one after another.
             for (uint64_t left = __ballot(mine != kNoRow); left;) {
@@ -315,7 +326,7 @@ struct LowRank {
             x8 fq[kFQ];
             if (s) fetch(values, q0, s);
 #pragma unroll
-            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = piece_of((s ? values[j] : a.values[j]) * of_row(a.power.inverse, j), step.piece);
+            for (uint32_t j = 0; j < kFQ; ++j) fq[j] = piece_of(s ? values[j] : a.values[j], of_row(a.power.inverse, j), step.piece);
             for_groups(a.mine, share, shares, [&](uint32_t n, uint32_t g, uint64_t those) {
                 x8 fp[kFP];
                 float scale;
@@ -538,19 +549,24 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_adapter_stream(GatheredO
                         }
                     }
                     float factor = kPT ? 1.0f : scale;
+                    floatx4 first;
                     if constexpr (std::is_same_v<T, half_t>) {
                         float most = fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3])));
                         most = fmaxf(most, __shfl_xor(most, 16));
                         most = fmaxf(most, __shfl_xor(most, 32));
                         const Power power = power_of(most);
+#pragma unroll
+                        for (uint32_t e = 0; e < 4u; ++e) first[e] = to_round<T>(m[e] * power.inverse, m[e]);
                         m *= power.inverse;
                         factor *= power.value;
+                    } else {
+#pragma unroll
+                        for (uint32_t e = 0; e < 4u; ++e) first[e] = to_round<T>(m[e], m[e]);
                     }
-                    const floatx8 both = {m[0], m[1], m[2], m[3], m[0], m[1], m[2], m[3]};
-                    const x8 high = __builtin_convertvector(both, x8);
+                    const x4 high = __builtin_convertvector(first, x4);
                     floatx8 rest;
 #pragma unroll
-                    for (uint32_t e = 0; e < 8u; ++e) rest[e] = e < 4u ? both[e] : rest_of(both[e], (float)high[e]);
+                    for (uint32_t e = 0; e < 8u; ++e) rest[e] = e < 4u ? first[e] : rest_of(m[e - 4u], (float)high[e - 4u]);
                     const x8 pieces = __builtin_convertvector(rest, x8);
                     x8 third;
                     if (more.pieces == 3u) {

@@ -189,3 +189,16 @@ def test_large_values_beside_an_infinity(workspace, n, i, o, r):
     c.up[g][:, 1] = 1.0
     z = forward_is(c, g, at, "f32", workspace)
     assert np.isposinf(z).all()
+
+
+@pytest.mark.parametrize("n,i,o,r", SHAPES)
+def test_small_values_beside_large_ones(workspace, n, i, o, r):
+    """fp16: an m far below the row's largest is still not zero where up is infinite."""
+    announce(f"small m beside large ones, {n} x {i} -> {o}, rank {r}")
+    c, g, at = case(n, i, o, r, "f16")
+    c.x = decode(encode(np.abs(c.x) * 3e3 + 1e3, "f16"), "f16")
+    c.down[g] = decode(encode(np.abs(c.down[g]) * 200.0 + 1.0, "f16"), "f16")
+    c.down[g][1], c.down[g][1, 3] = 0.0, 2.0**-24
+    c.up[g][4, 1], c.up[g][6, 1] = np.inf, -np.inf
+    z = forward_is(c, g, at, "f32", workspace)
+    assert np.isposinf(z[:, 4]).all() and np.isneginf(z[:, 6]).all()
