@@ -34,11 +34,12 @@ __device__ __forceinline__ Power power_of(float most) {
     return {1.0f, 1.0f};
 }
 // What a value's first piece is rounded from (`scaled` by its row's power): one that is not
-// zero stays so, as the smallest number of fp16 at least, whose rest is taken off again.
+// zero stays so, as the smallest number of fp16 at least, and one that is finite too, as
+// the largest of bf16 at most; the rest has the difference.
 template <typename T>
 __device__ __forceinline__ float to_round(float scaled, float value) {
     if constexpr (std::is_same_v<T, half_t>) return value != 0.0f && fabsf(scaled) < 0x1p-24f ? __builtin_copysignf(0x1p-24f, value) : scaled;
-    return scaled;
+    return fabsf(value) < __builtin_inff() ? __builtin_amdgcn_fmed3f(value, -0x1.FEp127f, 0x1.FEp127f) : value;
 }
 // What a rounding leaves of a value: nothing of an infinity or NaN.
 __device__ __forceinline__ float rest_of(float value, float rounded) { return fabsf(rounded) < __builtin_inff() ? value - rounded : 0.0f; }
@@ -741,10 +742,17 @@ __global__ __launch_bounds__(256) void k_rank_sums(RankSums A, Groups G, uint32_
             if constexpr (std::is_same_v<T, bf16_t>) {
 #pragma unroll
                 for (uint32_t piece = 0; piece < 3u; ++piece) {
-                    const typename Vec<T>::x8 h = __builtin_convertvector(m, typename Vec<T>::x8);
+                    // The first one towards zero, so that a finite value's is finite: the two
+                    // others hold the 16 bits that are left.
+                    floatx8 first = m;
+                    if (piece == 0u) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 8u; ++e) first[e] = __uint_as_float(__float_as_uint(m[e]) & 0xFFFF0000u);
+                    }
+                    const typename Vec<T>::x8 h = __builtin_convertvector(first, typename Vec<T>::x8);
 #pragma unroll
                     for (uint32_t i = 0; i < kFW; ++i) acc[i] = Vec<T>::mfma(w[i], h, acc[i]);
-                    const floatx8 back = __builtin_convertvector(h, floatx8);
+                    const floatx8 back = piece == 0u ? first : __builtin_convertvector(h, floatx8);
 #pragma unroll
                     for (uint32_t e = 0; e < 8u; ++e) m[e] = rest_of(m[e], back[e]);
                     // (For every step alike: 8192 rows of 4096 -> 2048, rank 64, 324 us, so 305.)

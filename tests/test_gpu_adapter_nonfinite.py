@@ -202,3 +202,25 @@ def test_small_values_beside_large_ones(workspace, n, i, o, r):
     c.up[g][4, 1], c.up[g][6, 1] = np.inf, -np.inf
     z = forward_is(c, g, at, "f32", workspace)
     assert np.isposinf(z[:, 4]).all() and np.isneginf(z[:, 6]).all()
+
+
+@pytest.mark.parametrize("y_kind", ["bf16", "f32"])
+@pytest.mark.parametrize("n,i,o,r", SHAPES)
+def test_values_beyond_the_largest_of_bf16(workspace, n, i, o, r, y_kind):
+    """m between bf16's largest number and 32 bits': finite, and so are its products."""
+    announce(f"m beyond bf16's largest, {n} x {i} -> {o}, rank {r}, {y_kind}")
+    c, g, at = case(n, i, o, r, "bf16")
+    largest = 255.0 * 2.0**120
+    rows = c.xr()[at]
+    c.x[rows] = 0.0
+    c.x[rows, 2], c.x[rows, 3] = largest, 2.0**119
+    c.w[:, 2:4] = 0.0
+    c.down[g][:, 2:4] = 1.0  # m = (255 + 1/2) 2^120, which rounds to an infinity
+    c.up[g] = decode(encode(c.up[g] * 2.0**-30, "bf16"), "bf16")
+    z = forward_is(c, g, at, y_kind, workspace)
+    assert np.isfinite(z).all()
+    mid = np.where(np.arange(n)[:, None] % 50 == 0, 255.5 * 2.0**120, np.ones((n, r)))
+    c.delta = decode(encode(c.delta * 2.0**-60, "bf16"), "bf16")
+    c.up[g] = decode(encode(c.up[g] * 2.0**30, "bf16"), "bf16")
+    got = backward_is(c, g, at, mid, workspace, d_columns=(0, o - 1))
+    assert np.isfinite(got["dup"][g]).all()
