@@ -894,15 +894,31 @@ hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& mo
     return gather ? launch(k_adapter<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_adapter<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
 }
 
-// Whether k_adapter_stream takes a layer: with so many rows that its start is small
-// beside them.  Streamed against by tiles with the low-rank products before them, in
-// us, fp16, residual and pre, 16 groups: 262144 x 256 -> 256 rank 16 168 / 209, rank
-// 64 310 / 316, -> 512 280 / 353; 65536 x 256 -> 256 49 / 52, 128 -> 256 35 / 39;
-// 32768 x 256 -> 256 32 / 27.  Gradients: 262144 rows 268 / 339, rank 64 536 / 589,
-// 65536 rows 90 / 105, 32768 rows 60 / 60.
+// Whether k_adapter_stream takes a layer: with so many rows that its start, and the
+// loading of an adapter at every group's first row, are small beside them.  Streamed /
+// by tiles with the low-rank products before them, us, fp16, residual and pre (gradients:
+// add, dx and both sums):
+//   256 -> 256, rank 16: 65536 rows in 16 groups 50 / 56, in 256 60 / 60, in 1024 87 / 68;
+//     131072 in 512 104 / 117, in 1024 120 / 120; 262144 in 16 146 / 206, in 1024 181 / 218,
+//     in 4096 262 / 245; 32768 in 16 32 / 27.  Gradients 65536 in 16 89 / 104, in 256 104 /
+//     111, in 1024 146 / 130; 262144 in 1024 298 / 364, in 4096 436 / 443.
+//   Rank 32: 65536 in 64 65 / 72, in 256 79 / 75; 131072 in 256 120 / 139, in 1024 164 / 144;
+//     262144 in 1024 233 / 264.
+//   Less work a group is less to load: 64 -> 64, rank 64, 65536 in 256 45 / 57, rank 16 in
+//     1024 44 / 36; 128 -> 128, rank 64, 65536 in 64 45 / 54, in 256 64 / 56.
+// Four blocks of ranks for more than 128 k spill, and several waves compute the same m
+// for more than 64 p: 256 -> 256, rank 64, 131072 rows in 1 group 173 / 173, in 64 183 / 176;
+// 262144 in 64 325 / 338, in 256 353 / 346; gradients 65536 in 16 212 / 207, 131072 in 64
+// 364 / 383, 262144 in 256 671 / 707, in 1024 747 / 722; 256 -> 128 65536 in 16 68 / 55, 262144
+// 189 / 201.  Rank 48, which takes as long: 262144 in 16 316 / 275, gradients 598 / 603, 256
+// -> 128 186 / 173.  256 -> 64, rank 64, 65536 in 16 52 / 54.
 template <typename T, bool kPT>
 bool streamed(const GatheredOperands& A, const LowRank<T, kPT>& more, const void* shrink, bool vec, const uint32_t* index, uint32_t count, uint64_t widest) {
-    return A.nk <= 256u && A.nk % 32u == 0u && A.np <= 512u && more.rank <= 64u && A.nq >= 65536u && vec && whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) && whole_chunks(A.q, A.ldq, A.nk) && aligned(shrink, 16u) && stream_outputs_near(index != nullptr, count, widest);
+    const uint32_t blocks = more.rank <= 16u ? 1u : more.rank <= 32u ? 2u : 4u;
+    const bool spills     = blocks == 4u && A.nk > 128u && A.np > 64u;
+    const uint64_t start  = !spills ? 32768u : kPT ? 98304u : 196608u, group = 48u + blocks * (A.nk + A.np) / 8u;
+    if (A.nq < 65536u || A.nq < start + more.G.count * group || (spills && more.rank <= 48u)) return false;
+    return A.nk <= 256u && A.nk % 32u == 0u && A.np <= 512u && more.rank <= 64u && vec && whole_chunks(A.p, A.ldp, kPT ? A.np : A.nk) && whole_chunks(A.q, A.ldq, A.nk) && aligned(shrink, 16u) && stream_outputs_near(index != nullptr, count, widest);
 }
 
 template <typename T, bool kPT, typename Out>
