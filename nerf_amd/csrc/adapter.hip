@@ -880,8 +880,10 @@ hipError_t launch_adapter(GatheredOperands A, Out out, const LowRank<T, kPT>& mo
         if (tiles(32u) <= cus) return few(Two{}, Two{});
     }
     // us, tiles of 64 / of 128: 2048 -> 2048, 2048 rows (1024, 256 tiles) 44 / 39, 8192 rows
-    // 150 / 97; 256 -> 256, 16384 rows (1024, 256) 20.7 / 20.2.
-    const bool by_128 = A.np > 64u && A.nq > 64u && tiles(128u) >= cus;
+    // 150 / 97; 256 -> 256, 16384 rows (1024, 256) 20.7 / 20.2.  By words, one buffer and two
+    // barriers a step: 255 -> 255, 16384 rows (256 of 128) 34 / 39, 32768 54 / 47, 1023 -> 1023,
+    // 4096 rows (256) 57 / 64, 8192 109 / 93.
+    const bool by_128 = A.np > 64u && A.nq > 64u && tiles(128u) >= (words ? 2u : 1u) * cus;
     if (words) return by_128 ? launch(k_adapter<T, 128, 128, 2, 2, 2, kPT, kByWords, true, Out>, 128u, 128u, 256u) : launch(k_adapter<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
     // A tile of 256 takes a CU nearly as long as four of 128, so it needs full rounds: us of
     // a call, 128 / 256, 2048 -> 2048 rank 16, 4096 rows (1 round for 2) 54 / 81, 8192 (1 for

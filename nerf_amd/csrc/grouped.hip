@@ -184,9 +184,16 @@ hipError_t launch_grouped(GatheredOperands A, Out out, const Groups& G, hipStrea
         return gather ? launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, true, Out>, 64u, 64u, 256u) : launch(k_grouped<T, 64, 64, 2, 2, 4, kPT, kDirect, false, Out>, 64u, 64u, 256u);
     } else {
         // us, tiles of 64 / of 128, fp16 256 -> 256: 4096 rows in 64 groups 7.3 / 10.5, 8192
-        // 11.9 / 12.0, 16384 17 / 14, 131072 in 16 108 / 69; bf16 2048 -> 2048: 2048 rows in
-        // 8 groups 44 / 36.
-        const bool by_128 = A.np > 64u && mean >= 128u && tiles(128u) >= cus;
+        // 11.9 / 12.0, in 128 13.5 / 13.7, 16384 in 64 17 / 14, 131072 in 16 108 / 69; bf16
+        // 2048 -> 2048: 2048 rows in 8 groups 44 / 36, 1024 in 32 67 / 90, 2048 83 / 90, 3072
+        // 103 / 96.  Where there may be so many tiles that most have no rows, fewer numbers
+        // count for more than full tiles: 4096 rows in 1024 groups 35 / 34, 16384 in 4096 153 /
+        // 137, 262144 in 4096 317 / 245, the same if 8 of them have all the rows 388 / 281.
+        // By words a tile of 128 waits for its one buffer, and pays with many products only:
+        // 255 -> 255, 65536 rows in 512 groups 81 / 97, 262144 246 / 245; 1023 -> 1023, 8192 in 16
+        // 77 / 90, 16384 147 / 141, in 128 207 / 209, 65536 in 64 542 / 452, 32768 in 512 498 / 562.
+        const uint64_t products = (uint64_t)G.rows * A.np * A.nk;
+        const bool by_128 = A.np > 64u && tiles(128u) >= cus && (words ? mean >= 128u && products >= 1ull << 34 : mean >= 64u || tiles(128u) >= 8u * cus);
         if (words) return by_128 ? launch(k_grouped<T, 128, 128, 2, 2, 2, kPT, kByWords, true, Out>, 128u, 128u, 256u) : launch(k_grouped<T, 64, 64, 2, 2, 2, kPT, kByWords, true, Out>, 64u, 64u, 256u);
         // A CU has one tile of 256 at a time, as long as 2.75 of 128 take it, and the last
         // round of them is seldom full.  us, 128 / 256, bf16: 4096 -> 4096, 16384 rows in 8
@@ -227,12 +234,14 @@ hipError_t launch_sums(GatheredOperands A, const Groups& G, float* dw, float* db
     const bool words  = !whole_chunks(A.p, A.ldp, A.np) || !whole_chunks(A.q, A.ldq, A.nq) || (gather && !(near(A.p_count, A.ldp) && near(A.q_count, A.ldq)));
     // us of a backward pass, sums by tiles of 64 / of 128, fp16: 16384 rows in 16 groups,
     // 256 x 256 (2^30) 30 / 35, 512 x 512 (2^32) 66 / 61; 65536 rows, 256 x 256 (2^32) 82 / 72;
+    // by words 255 x 255, 8192 rows 37 / 38, 16384 64 / 54, 65536 188 / 132, 511 x 511, 2048 39 /
+    // 43, 4096 55 / 53, 95 x 95, 8192 23 / 28, 32768 41 / 40;
     // 128 / 256: 2048 x 2048, 16384 rows in 8 (2^36) 381 / 409, bf16 4096 x 2048 (2^37) 725 /
     // 688, in 32 groups 965 / 913, 4096 x 4096 (2^38) 1390 / 1239.  Parts enough for one
     // workgroup a CU, for half, one, two and four: 262144 rows in 64 groups 279, 224, 234, 234;
     // 16384 rows in 8 groups, 1024 x 1024, 180, 168, 172, 187.
     const uint64_t work = length * G.rows;
-    const bool by_128   = A.np > 64u && A.nq > 64u && work >= 1ull << 32;
+    const bool by_128   = A.np > 64u && A.nq > 64u && work >= (words ? 3ull << 28 : 1ull << 32);
     if (words) return by_128 ? launch(k_grouped_sums<T, 128, 128, 2, 2, kByWords, true>, 128u, 128u, 256u) : launch(k_grouped_sums<T, 64, 64, 2, 2, kByWords, true>, 64u, 64u, 256u);
     if (A.np > 128u && A.nq > 128u && work >= 1ull << 37)
         return gather ? launch(k_grouped_sums<T, 256, 256, 2, 4, kDirect, true>, 256u, 256u, 512u) : launch(k_grouped_sums<T, 256, 256, 2, 4, kDirect, false>, 256u, 256u, 512u);

@@ -29,3 +29,14 @@ def test_streamed_wide_layers(workspace, n, rank, kind, index):  # noqa: F811
     c = G.Case(n, 4, 256, 256, kind, seed=rank, rank=rank, whole=True, **INDEXES[index])
     forward_equal(c, "relu", "f32" if kind == "bf16" else kind, workspace)
     backward_equal(c, "relu", workspace)
+
+
+# Rows of odd length in tiles of 128, which few products do not take; the same in
+# groups of fewer rows, and so many groups of whole chunks that most tiles are empty.
+@pytest.mark.parametrize("n,groups,i,o", [(17000, 5, 1021, 1001), (17000, 200, 1021, 1001), (9000, 3000, 96, 136), (70000, 1000, 264, 128)])
+@pytest.mark.parametrize("kind,index", [("f16", 1), ("bf16", 0)])
+def test_grouped_tiles_by_rows_and_groups(workspace, n, groups, i, o, kind, index):  # noqa: F811
+    announce(f"grouped {n} x {i} -> {o}, {groups} groups, {kind}")
+    c = G.Case(n, groups, i, o, kind, seed=n, whole=True, **INDEXES[index])
+    forward_equal(c, "relu", "f32" if kind == "bf16" else kind, workspace)
+    backward_equal(c, "relu", workspace)
