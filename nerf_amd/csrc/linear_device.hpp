@@ -237,9 +237,6 @@ __device__ __forceinline__ floatx8 bias8(const float* lds, uint32_t at) {
 
 // Each epilogue gets eight consecutive p of one row q0 + row at a time, n of
 // them inside the output (0 for a row outside), with their biases, and first
-
-// Each epilogue gets eight consecutive p of one row q0 + row at a time, n of
-// them inside the output (0 for a row outside), with their biases, and first
 // loads what else it needs, so that a caller can have that under way early.
 template <typename T>
 struct ForwardOut {
@@ -359,7 +356,6 @@ struct Place {
 template <uint32_t kB, bool kT>
 __device__ __forceinline__ constexpr uint32_t chunk_key(uint32_t line) {
     if (!kT) return line & 7u;
-    if (kB == 32u) return ((line >> 1 ^ line >> 3) & 1u) << 1;  // as all of them, the same for k 4 on
     if (kB >= 128u) return ((line & 3u) | ((line >> 3) & 1u) << 2) << 1;
     return (((line >> 1) & 1u) | ((line >> 3) & 1u) << 1) << 1;
 }
