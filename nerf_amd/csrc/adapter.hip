@@ -414,28 +414,7 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_adapter_stream(GatheredO
     const Groups& G = more.G;
 
     x8 fp[kKS][kFP];
-    {
-        const float bias = thread_bias<kBP>(out, p0);
-        Stager<T, kBP, kPT, kThreads, true> stager;
-        stager.fetch((const T*)A.p, A.ldp, A.np, p0, 0u, A.nk);
-        if (Out::kBias && threadIdx.x < kBP) reinterpret_cast<float*>(lds_bias)[threadIdx.x] = bias;
-        const uint32_t base = fragment_base<kBP, kPT>(wp & ~127u);
-#pragma unroll
-        for (uint32_t s = 0; s < kKS; s += 2u) {
-            stager.keep(lds, (const T*)A.p, A.ldp, A.np, p0, 32u * s, A.nk);
-            __syncthreads();
-            if (s + 2u < kKS) stager.fetch((const T*)A.p, A.ldp, A.np, p0, 32u * (s + 2u), A.nk);
-#pragma unroll
-            for (uint32_t i = 0; i < kFP; ++i)
-#pragma unroll
-                for (uint32_t h = 0; h < 2u; ++h)
-                    if (s + h < kKS) {
-                        fp[s + h][i] = fragment<T, kBP, kPT>(lds, base, (wp & 127u) / 16u + i, h);
-                        settle_here(fp[s + h][i]);
-                    }
-            __syncthreads();
-        }
-    }
+    hold_weights<T, kBP, kPT>(A, out, p0, wp, lds, lds_bias, fp);
 
     const uint32_t row = lane / kLanes, col = 8u * (lane % kLanes), p = p0 + wp + col;
     const uint32_t n = p < A.np ? min(8u, A.np - p) : 0u;

@@ -55,7 +55,7 @@ template <typename T, uint32_t kKS, uint32_t kFP, bool kPT, bool kRagged, bool k
 __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out out, uint32_t p_waves) {
     // Where P takes half of the registers, the outputs' edges have to do without any.
     if constexpr (kKS * kFP == 32u) out.vec = true;
-    constexpr uint32_t kThreads = kStreamWaves * 64u, kSP = 16u * kFP, kBP = 256u;
+    constexpr uint32_t kSP = 16u * kFP, kBP = 256u;
     constexpr uint32_t kLanes = kSP / 8u, kPasses = 16u * kLanes / 64u;
     using x8 = typename Vec<T>::x8;
     __shared__ uint4 lds[kBP * 8u];
@@ -65,28 +65,7 @@ __global__ __launch_bounds__(kStreamWaves * 64u) void k_stream(Operands A, Out o
     const uint32_t wp = wave % p_waves * kSP, p0 = blockIdx.y * p_waves * kSP;
 
     x8 fp[kKS][kFP];
-    {
-        const float bias = thread_bias<kBP>(out, p0);
-        Stager<T, kBP, kPT, kThreads, true> stager;
-        stager.fetch((const T*)A.p, A.ldp, A.np, p0, 0u, A.nk);
-        if (Out::kBias && threadIdx.x < kBP) reinterpret_cast<float*>(lds_bias)[threadIdx.x] = bias;
-        const uint32_t base = fragment_base<kBP, kPT>(wp & ~127u);
-#pragma unroll
-        for (uint32_t s = 0; s < kKS; s += 2u) {
-            stager.keep(lds, (const T*)A.p, A.ldp, A.np, p0, 32u * s, A.nk);
-            __syncthreads();
-            if (s + 2u < kKS) stager.fetch((const T*)A.p, A.ldp, A.np, p0, 32u * (s + 2u), A.nk);
-#pragma unroll
-            for (uint32_t i = 0; i < kFP; ++i)
-#pragma unroll
-                for (uint32_t h = 0; h < 2u; ++h)
-                    if (s + h < kKS) {
-                        fp[s + h][i] = fragment<T, kBP, kPT>(lds, base, (wp & 127u) / 16u + i, h);
-                        settle_here(fp[s + h][i]);
-                    }
-            __syncthreads();
-        }
-    }
+    hold_weights<T, kBP, kPT>(A, out, p0, wp, lds, lds_bias, fp);
 
     // Rows: lane l has k 8 (l / 16) + 0..7 of every 32 of row l % 16.
     const uint32_t groups = kStreamWaves / p_waves, tiles = (A.nq + 15u) / 16u, stride = gridDim.x * groups;

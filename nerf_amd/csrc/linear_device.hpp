@@ -629,6 +629,33 @@ __device__ __forceinline__ void settle_here(V& v) {
     asm volatile("" : "+v"(v)::"memory");
 }
 
+// What the kernels that stream rows begin with: the workgroup's kBP rows of P from p0, 64 k
+// at a time, through LDS (kBP * 8 chunks) into the registers of the waves, each of which
+// holds 16 kFP of them from wp on for all k; their biases into LDS.
+template <typename T, uint32_t kBP, bool kPT, uint32_t kKS, uint32_t kFP, typename Ops, typename Out>
+__device__ __forceinline__ void hold_weights(const Ops& A, const Out& out, uint32_t p0, uint32_t wp, uint4* lds, floatx4* lds_bias, typename Vec<T>::x8 (&fp)[kKS][kFP]) {
+    const float bias = thread_bias<kBP>(out, p0);
+    Stager<T, kBP, kPT, kStreamWaves * 64u, true> stager;
+    stager.fetch((const T*)A.p, A.ldp, A.np, p0, 0u, A.nk);
+    if (Out::kBias && threadIdx.x < kBP) reinterpret_cast<float*>(lds_bias)[threadIdx.x] = bias;
+    const uint32_t base = fragment_base<kBP, kPT>(wp & ~127u);
+#pragma unroll
+    for (uint32_t s = 0; s < kKS; s += 2u) {
+        stager.keep(lds, (const T*)A.p, A.ldp, A.np, p0, 32u * s, A.nk);
+        __syncthreads();
+        if (s + 2u < kKS) stager.fetch((const T*)A.p, A.ldp, A.np, p0, 32u * (s + 2u), A.nk);
+#pragma unroll
+        for (uint32_t i = 0; i < kFP; ++i)
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; ++h)
+                if (s + h < kKS) {
+                    fp[s + h][i] = fragment<T, kBP, kPT>(lds, base, (wp & 127u) / 16u + i, h);
+                    settle_here(fp[s + h][i]);
+                }
+        __syncthreads();
+    }
+}
+
 // Waits until at most `kLater` of the wave's own loads are on their way, and
 // then for the workgroup.
 template <uint32_t kLater>
