@@ -350,7 +350,11 @@ typedef struct NerfExtAdapters {
 /* mid = down x, z = weight x + bias + scale up mid, y = act(z) + residual: weight
  * [out][in] and bias [out] are shared, mid is fp32 [rows][rank] by position (for
  * the backward pass).  Rows in no group have no adapter: z = weight x + bias, and
- * mid keeps what it holds there. */
+ * mid keeps what it holds there.
+ * mid is summed in 32 bits.  Its product with up is of 16-bit operands summed in 32
+ * bits, mid as two of them (three for fp32 y of bf16), which keep 2^-16 (2^-24) of
+ * each value in bf16, 2^-22 of a row's largest in fp16: where scale up mid and
+ * weight x + bias cancel, z is off by that much of the terms. */
 NERF_API NerfStatus nerf_ext_adapter_linear_forward(const NerfExtLinearDesc* desc, const NerfExtRowGroups* groups, const NerfExtAdapters* adapters, const void* x, const void* weight, const float* bias, const void* residual, void* y, void* pre,
                                                    float* mid, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Gradients from delta, the shared weights held (theirs are
@@ -360,7 +364,9 @@ NERF_API NerfStatus nerf_ext_adapter_linear_forward(const NerfExtLinearDesc* des
  *   ddown = dmid^T x, dup = scale delta^T mid    fp32 [groups][rank][in] and
  *                                [groups][out][rank], sums over the group's rows
  * Outputs may be NULL, and what no output needs too.  Rows in no group: dmid keeps
- * what it holds, g = delta weight + add. */
+ * what it holds, g = delta weight + add.  dmid meets down as mid meets up, in two
+ * operands; ddown and dup take all of dmid's and mid's 32 bits (in bf16 as three
+ * operands, whose last bits are lost below 2^-110). */
 NERF_API NerfStatus nerf_ext_adapter_linear_backward(const NerfExtLinearDesc* desc, const NerfExtRowGroups* groups, const NerfExtAdapters* adapters, const void* x, const void* weight, const void* delta, const float* mid, const void* pre,
                                                     const void* add, void* dx, void* dpre, float* dmid, float* ddown, float* dup, void* workspace, uint64_t workspace_bytes, void* stream);
 

@@ -14,7 +14,9 @@
 // of that type (three where fp32 outputs of bf16 values keep more), high and low
 // part, whose products are as if the rank were two or three times as large.  For
 // fp16 a row's m are first scaled by a power of two to less than 2 (8 at the end
-// of 32 bits' range), which keeps them and their low parts in its range.
+// of 32 bits' range), which keeps them and their low parts in its range.  Infinite and
+// zero m and factors give what they give unsplit: a finite m's parts are finite, the
+// high part of one that is not zero is not zero, and only high parts meet infinities.
 #include "grouped_device.hpp"
 
 using namespace nerf_hip;
@@ -390,8 +392,8 @@ __global__ __launch_bounds__(kFewWaves * 64u) void k_adapter_few(GatheredOperand
 // ends with ranks 4 g .. 4 g + 3 of row l, and their high and low parts are what it
 // has to hold for the next product, if that counts its k as (g, part, rank): no
 // value moves between lanes.  A workgroup has consecutive positions, group by group.
-// 262144 rows in 16 groups, rank 16, 256 -> 256 fp16, residual and pre: 138 us, 4.0
-// TB/s (tiles after a pass for m 199); its input gradient 156.
+// 262144 rows in 16 groups, rank 16, 256 -> 256 fp16, residual and pre: 140-145 us,
+// 3.9 TB/s (tiles after a pass for m 206); its input gradient 156.
 struct StreamRanks {
     const void* shrink;  // down [groups][rank][nk]; kPT: up [groups][nk][rank]
     float* low;          // m
@@ -643,9 +645,9 @@ __global__ __launch_bounds__(64) void k_adapter_tiny(GatheredOperands A, Out out
 // their last ones are lost), whose products take three sixteenths of the
 // 32-bit instruction's time.  fp16 values would need a scale a row for that, which a
 // sum over rows cannot take out again: the 32-bit instruction, four positions at a
-// time.  8192 rows in 8 groups, rank 64, 4096 values: 45 us in bf16 (by the 32-bit
+// time.  8192 rows in 8 groups, rank 64, 4096 values: 46 us in bf16 (by the 32-bit
 // instruction, each wave with all of r, 72; split so, 63; one wave for 16 of r, as it
-// is now, reads and splits a value once), 2048 values 28.  What is left is the waits for
+// is now, reads and splits a value once), 2048 values 30.  What is left is the waits for
 // gathered rows, two loads after each other, in parts of a few tiles; memory
 // alone would take 13.  262144 rows, rank 16, 256 values, fp16: 45 us, 3.3 TB/s.
 struct RankSums {
