@@ -185,8 +185,8 @@ hipError_t launch_grouped(GatheredOperands A, Out out, const Groups& G, hipStrea
     } else {
         // us, tiles of 64 / of 128, fp16 256 -> 256: 4096 rows in 64 groups 7.3 / 10.5, 8192
         // 11.9 / 12.0, in 128 13.5 / 13.7, 16384 in 64 17 / 14, 131072 in 16 108 / 69; bf16
-        // 2048 -> 2048: 2048 rows in 8 groups 44 / 36, 1024 in 32 67 / 90, 2048 83 / 90, 3072
-        // 103 / 96.  Where there may be so many tiles that most have no rows, fewer numbers
+        // 2048 -> 2048: 2048 rows in 8 groups 44 / 36, 1024 in 32 67 / 90, 2048 83 / 90,
+        // 4096 123 / 100.  Where there may be so many tiles that most have no rows, fewer numbers
         // count for more than full tiles: 4096 rows in 1024 groups 35 / 34, 16384 in 4096 153 /
         // 137, 262144 in 4096 317 / 245, the same if 8 of them have all the rows 388 / 281.
         // By words a tile of 128 waits for its one buffer, and pays with many products only:
